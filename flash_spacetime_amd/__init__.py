@@ -32,6 +32,8 @@ __all__ = [
     "flash_spacetime_attention_qkv",
     "flash_spacetime_forward",
     "flash_spacetime_backward",
+    "flash_layer_norm",
+    "flash_gated_feed_forward",
     "spacetime_attention_reference",
     "spacetime_pair_features",
     "sinusoidal_frequencies",
@@ -54,6 +56,8 @@ _OPS = {
     "flash_spacetime_attention_qkv": "forward",
     "flash_spacetime_forward": "forward",
     "flash_spacetime_backward": "backward",
+    "flash_layer_norm": "norm",
+    "flash_gated_feed_forward": "feed_forward",
 }
 
 

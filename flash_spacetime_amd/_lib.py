@@ -18,6 +18,10 @@ LIB_PATH = Path(__file__).resolve().parent / "libflash_spacetime.so"
 
 FST_BF16 = 0
 FST_F32 = 1
+FST_F16 = 2
+FST_SILU = 0
+FST_GELU = 1
+FST_GELU_TANH = 2
 FST_ATTN_BIAS = 1
 FST_ACT_BIAS = 2
 FST_PACKED = 4
@@ -66,6 +70,7 @@ FST_ELAUNCH = -4
 
 # Every symbol the C header declares, with its ctypes signature.
 _vp, _i, _f, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
+_l = ctypes.c_int64
 SIGNATURES = {
     "fst_supported": (_i, [_i, _i, _i, _i]),
     "fst_plans": (_i, [_i, _i, _i, _i]),
@@ -93,6 +98,22 @@ SIGNATURES = {
         _i,
         [_i, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _f,
          _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp],
+    ),
+    "fst_layer_norm_forward": (_i, [_i, _i, _i, _i, _i, _vp, _l, _vp, _l, _vp, _vp, _vp, _f, _vp, _vp, _vp, _vp]),
+    "fst_layer_norm_backward_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "fst_layer_norm_backward": (
+        _i,
+        [_i, _i, _i, _i, _i, _vp, _l, _vp, _vp, _vp, _vp, _l, _vp, _l, _vp, _vp, _vp, _vp, _sz, _vp],
+    ),
+    "fst_ffn_forward": (
+        _i,
+        [_i, _i, _i, _i, _i, _i, _vp, _l, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    ),
+    "fst_ffn_backward_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "fst_ffn_backward": (
+        _i,
+        [_i, _i, _i, _i, _i, _i, _vp, _l, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _l,
+         _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp],
     ),
     "fst_max_event_len": (_i, [_i, _i, _i, _i, _i]),
     "fst_frequencies": (None, [_i, ctypes.POINTER(ctypes.c_float)]),

@@ -39,6 +39,7 @@ FLAGS = [
 ]
 
 DTYPES = {"bf16": "bf16", "f32": "float"}
+FFN_DTYPES = {"bf16": "bf16", "f16": "f16", "f32": "float"}
 HEAD_DIMS = (16, 32, 48, 64)
 
 
@@ -63,7 +64,10 @@ def source_hash() -> str:
 
 
 def _units():
-    units = [("capi", CSRC / "fst_capi.hip", [f'-DFST_BUILD_ID="{source_hash()}"'])]
+    units = [("capi", CSRC / "fst_capi.hip", [f'-DFST_BUILD_ID="{source_hash()}"']),
+             ("norm", CSRC / "fst_norm.hip", []), ("ffn", CSRC / "fst_ffn.hip", [])]
+    for tag, ctype in FFN_DTYPES.items():
+        units.append((f"ffn_{tag}", CSRC / "fst_ffn_inst.hip", [f"-DFST_T={ctype}", f"-DFST_NAME={tag}"]))
     for tag, ctype in DTYPES.items():
         for d in HEAD_DIMS:
             name = f"{tag}_{d}"

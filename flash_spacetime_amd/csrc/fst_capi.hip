@@ -14,14 +14,16 @@ namespace fst {
 
 static thread_local char g_last_error[512] = "";
 
-static int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
-static int fail(int code, const char* fmt, ...) {
+int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+int fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
   va_end(ap);
   return code;
 }
+
+void clear_error() { g_last_error[0] = 0; }
 
 static size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 

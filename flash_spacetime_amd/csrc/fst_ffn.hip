@@ -1,0 +1,375 @@
+// Gated feed-forward block: C ABI, and the small kernels around its matrix
+// products (fst_ffn_inst.hip).
+//
+//   a = x Wg^T + bg,  u = x Wu^T + bu,  h = act(a) u,  y = h Wd^T + bd;
+//   dh = dy Wd,  da = dh u act'(a),  du = dh act(a),  dx = da Wg + du Wu,
+//   dWg = da^T x,  dWu = du^T x,  dWd = dy^T h,  biases: column sums of da, du, dy.
+//
+// Forward: gate and up projections with the activation in one product, then the
+// output product. Backward: da and du (side by side in one row, so that the
+// products after them are one each) from dy and the forward's a and u, dx, and
+// the three weights' gradients in one launch, summed over its token runs in
+// order. a, u and h are kept from the forward: forming a and u again would add 4
+// T F D operations to the 12 T F D of the backward, against 2 T F elements
+// written and read; where D is 1024 the products are several times dearer, at
+// D = 384 about equal. Padded batches are gathered on the way: a list of the
+// valid rows is the products' token axis, so padding costs nothing but its zeros.
+#include "fst_ffn.h"
+
+namespace fst {
+
+namespace {
+
+// Valid rows of a padded batch in order (map[0]: their number, map[1 ..]: the
+// rows; or map null), and zeros into the padding rows of out. Workgroup x takes
+// `per` consecutive events, its y-th slice of their rows.
+__global__ __launch_bounds__(256) void ffn_rows(const int32_t* seqlens, int B, int L, int per, int32_t* map,
+                                                unsigned char* out, long row_bytes) {
+  __shared__ int red[256];
+  const int e0 = blockIdx.x * per, e1 = min(e0 + per, B), tid = threadIdx.x;
+  int off = 0;
+  if (map) {
+    int sum = 0;
+    for (int e = tid; e < e0; e += 256) sum += event_len(seqlens, e, L);
+    red[tid] = sum;
+    __syncthreads();
+    for (int h = 128; h > 0; h >>= 1) {
+      if (tid < h) red[tid] += red[tid + h];
+      __syncthreads();
+    }
+    off = red[0];
+  }
+  const long at = (long)blockIdx.y * 256 + tid, step = (long)gridDim.y * 256;
+  for (int e = e0; e < e1; ++e) {
+    const int len = event_len(seqlens, e, L);
+    const long row = (long)e * L;
+    if (map)
+      for (long l = at; l < len; l += step) map[1 + off + l] = (int32_t)(row + l);
+    u32x4* pad = reinterpret_cast<u32x4*>(out + (row + len) * row_bytes);
+    const long parts = (L - len) * (row_bytes / 16);
+    for (long i = at; i < parts; i += step) pad[i] = u32x4{0, 0, 0, 0};
+    off += len;
+  }
+  if (map && e1 == B && e0 < B && at == 0) map[0] = off;
+}
+
+// out[c * ldo + r] = in[r * C + c] for up to three matrices [R, C] of E-byte elements.
+struct Transposes {
+  const void* in[3];
+  void* out[3];
+  long ldo[3];
+  int R[3], C[3], first[3];  // workgroups before the next matrix
+};
+
+template <typename E>
+__global__ __launch_bounds__(256) void ffn_transpose(Transposes p) {
+  __shared__ E tile[64][65];
+  const int k = (int)blockIdx.x >= p.first[0] ? ((int)blockIdx.x >= p.first[1] ? 2 : 1) : 0;
+  const int wg = (int)blockIdx.x - (k ? p.first[k - 1] : 0);
+  const int R = p.R[k], C = p.C[k], nc = (C + 63) / 64;
+  const int r0 = wg / nc * 64, c0 = wg % nc * 64;
+  const E* in = static_cast<const E*>(p.in[k]);
+  E* out = static_cast<E*>(p.out[k]);
+  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = r0 + y + 4 * i;
+    if (r < R && c0 + x < C) tile[y + 4 * i][x] = in[(long)r * C + c0 + x];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int c = c0 + y + 4 * i;
+    if (c < C && r0 + x < R) out[c * p.ldo[k] + r0 + x] = tile[x][y + 4 * i];
+  }
+}
+
+// Gradients = the sums of their partials over the token runs, in order.
+struct GradSums {
+  const float* part[6];
+  void* out[6];
+  long stride[6];  // between the runs' partials
+  long count[6];   // elements, a multiple of 4
+  int splits[6], first[6];
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void ffn_grad_sum(GradSums p) {
+  int k = 0;
+#pragma unroll
+  for (int i = 0; i < 5; ++i) k += (int)blockIdx.x >= p.first[i];
+  const long e = ((long)((int)blockIdx.x - (k ? p.first[k - 1] : 0)) * 256 + threadIdx.x) * 4;
+  if (e >= p.count[k]) return;
+  const float* in = p.part[k] + e;
+  f32x4 sum = *reinterpret_cast<const f32x4*>(in);
+  for (int s = 1; s < p.splits[k]; ++s) sum += *reinterpret_cast<const f32x4*>(in + s * p.stride[k]);
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  T4 o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = (T)sum[i];
+  *reinterpret_cast<T4*>(static_cast<T*>(p.out[k]) + e) = o;
+}
+
+int check_ffn(int dtype, int activation, int B, int L, int D, int F) {
+  if (dtype != FST_BF16 && dtype != FST_F32 && dtype != FST_F16)
+    return fail(FST_EINVAL, "dtype must be FST_BF16, FST_F16 or FST_F32, got %d", dtype);
+  if (activation != FST_SILU && activation != FST_GELU && activation != FST_GELU_TANH)
+    return fail(FST_EINVAL, "unknown activation %d", activation);
+  if (B < 0 || L < 0) return fail(FST_EINVAL, "negative size (B=%d, L=%d)", B, L);
+  if (D < 8 || F < 8 || D % 8 || F % 8)
+    return fail(FST_EUNSUPPORTED, "features must be multiples of 8, got D=%d, F=%d", D, F);
+  if (D > 65536 || F > 65536 || (long)D * F >= 1l << 28)
+    return fail(FST_EUNSUPPORTED, "a weight of D=%d by F=%d: at most 65536 each and 2^28 - 1 elements", D, F);
+  if ((long)B * L > 0x7fffffffL - 65536) return fail(FST_EUNSUPPORTED, "too many rows (B=%d, L=%d)", B, L);
+  return FST_OK;
+}
+
+bool misaligned(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if (reinterpret_cast<uintptr_t>(p) % 16) return true;
+  return false;
+}
+
+ffn_product_fn product_of(int dtype) {
+  return dtype == FST_BF16 ? ffn_product_bf16 : dtype == FST_F16 ? ffn_product_f16 : ffn_product_f32;
+}
+ffn_outer_fn outer_of(int dtype) {
+  return dtype == FST_BF16 ? ffn_outer_bf16 : dtype == FST_F16 ? ffn_outer_f16 : ffn_outer_f32;
+}
+
+// rows: valid rows listed in map (null: only the zeros of out's padding rows).
+void launch_rows(const int32_t* seqlens, int B, int L, int32_t* map, void* out, int D, size_t es, hipStream_t st) {
+  const int wgs = B < 1024 ? B : 1024, per = (B + wgs - 1) / wgs;
+  int slices = 1024 / wgs;
+  const int most = (L + 31) / 32;
+  slices = slices > most ? most : slices;
+  ffn_rows<<<dim3((B + per - 1) / per, slices), 256, 0, st>>>(seqlens, B, L, per, map,
+                                                             static_cast<unsigned char*>(out), (long)D * es);
+}
+
+int tiles_of(int M, int N) { return ((M + kOuterM - 1) / kOuterM) * ((N + kOuterN - 1) / kOuterN); }
+
+// Token runs of the weights' gradients: a workgroup holds two tiles a CU (512 at
+// a time); more runs shorten the rounds, and write and read their partials.
+int outer_splits(int dtype, long tokens, int D, int F) {
+  const int tiles = tiles_of(D, 2 * F) + tiles_of(F, D);
+  const double tile_s = (double)tokens * 2 * kOuterM * kOuterN / (dtype == FST_F32 ? 0.2e12 : 1.5e12);
+  const double part_s = 3.0 * D * F * 8 / 4e12;
+  int best = 1;
+  double least = 0;
+  for (int s = 1; s <= 64 && (s == 1 || s * 256l <= tokens); ++s) {
+    const double t = (double)((tiles * s + 511) / 512) / s * tile_s + s * part_s;
+    if (s == 1 || t < least) best = s, least = t;
+  }
+  return best;
+}
+
+struct GradLayout {
+  size_t wdt, w2t, dadu, part0, part1, bias0, bias1, total;
+  int splits;
+};
+
+GradLayout grad_layout(int dtype, long rows, int D, int F) {
+  GradLayout l;
+  const size_t es = elem_size(dtype), df = (size_t)D * F;
+  l.splits = outer_splits(dtype, rows, D, F);
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = off;
+    off += align256(bytes);
+    return at;
+  };
+  l.wdt = take(df * es);
+  l.w2t = take(2 * df * es);
+  l.dadu = take((size_t)rows * 2 * F * es);
+  l.part0 = take(l.splits * 2 * df * 4);
+  l.part1 = take(l.splits * df * 4);
+  l.bias0 = take((size_t)l.splits * 2 * F * 4);
+  l.bias1 = take((size_t)l.splits * D * 4);
+  l.total = off;
+  return l;
+}
+
+}  // namespace
+
+}  // namespace fst
+
+using namespace fst;
+
+extern "C" {
+
+int fst_ffn_forward(int dtype, int activation, int B, int L, int D, int F, const void* x, int64_t x_stride,
+                    const void* w_gate, const void* w_up, const void* w_down, const void* b_gate, const void* b_up,
+                    const void* b_down, const int32_t* seqlens, void* hidden, void* gate, void* up, int32_t* rowmap,
+                    void* y, void* stream) {
+  clear_error();
+  int rc = check_ffn(dtype, activation, B, L, D, F);
+  if (rc != FST_OK) return rc;
+  const long rows = (long)B * L;
+  if (rows == 0) return FST_OK;
+  if (!x || !w_gate || !w_up || !w_down || !hidden || !y || (seqlens && !rowmap) || !gate != !up)
+    return fail(FST_EINVAL, "null tensor pointer");
+  const size_t es = elem_size(dtype);
+  if (x_stride < D || x_stride * es % 16) return fail(FST_EINVAL, "x's row stride must be at least D and whole 16 bytes");
+  if (misaligned({x, w_gate, w_up, w_down, b_gate, b_up, b_down, hidden, gate, up, y}))
+    return fail(FST_EINVAL, "pointers must be multiples of 16 bytes");
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (seqlens) launch_rows(seqlens, B, L, rowmap, y, D, es, st);
+  FfnProduct p{};
+  p.count = seqlens ? rowmap : nullptr;
+  p.tokens = (int)rows;
+  p.act = activation;
+  p.w[0] = w_gate;
+  p.w[1] = w_up;
+  p.bias[0] = b_gate;
+  p.bias[1] = b_up;
+  p.x = x;
+  p.ldx = x_stride;
+  p.rows_in = seqlens ? rowmap + 1 : nullptr;
+  p.out[0] = hidden;
+  p.out[1] = gate;
+  p.out[2] = up;
+  p.ldo = F;
+  p.ldw = p.K = D;
+  p.F = F;
+  rc = product_of(dtype)(kFfnGate, p, st);
+  if (rc == FST_OK) {
+    p.w[0] = w_down;
+    p.bias[0] = b_down;
+    p.x = hidden;
+    p.rows_in = nullptr;
+    p.rows_out = seqlens ? rowmap + 1 : nullptr;
+    p.out[0] = y;
+    p.ldo = D;
+    p.ldx = p.ldw = p.K = F;
+    p.F = D;
+    rc = product_of(dtype)(kFfnOut, p, st);
+  }
+  if (rc != FST_OK) return fail(rc, "feed-forward launch failed");
+  return FST_OK;
+}
+
+size_t fst_ffn_backward_workspace_bytes(int dtype, int B, int L, int D, int F) {
+  if (check_ffn(dtype, FST_SILU, B, L, D, F) != FST_OK) return 0;
+  return grad_layout(dtype, (long)B * L, D, F).total;
+}
+
+int fst_ffn_backward(int dtype, int activation, int B, int L, int D, int F, const void* x, int64_t x_stride,
+                     const void* w_gate, const void* w_up, const void* w_down, const int32_t* seqlens,
+                     const void* hidden, const void* gate, const void* up, const int32_t* rowmap, const void* dy,
+                     int64_t dy_stride, void* dx, void* dw_gate, void* dw_up, void* dw_down, void* db_gate,
+                     void* db_up, void* db_down, void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  int rc = check_ffn(dtype, activation, B, L, D, F);
+  if (rc != FST_OK) return rc;
+  const long rows = (long)B * L;
+  const bool first = dw_gate || dw_up || db_gate || db_up, second = dw_down || db_down;
+  if (!first && !second && !dx) return FST_OK;
+  const size_t es = elem_size(dtype);
+  if (rows > 0) {
+    if (!x || !w_gate || !w_up || !w_down || !hidden || !gate || !up || !dy || (seqlens && !rowmap))
+      return fail(FST_EINVAL, "null tensor pointer");
+    if (x_stride < D || x_stride * es % 16 || dy_stride < D || dy_stride * es % 16)
+      return fail(FST_EINVAL, "row strides of x and dy must be at least D and whole 16 bytes");
+  }
+  if (misaligned({x, w_gate, w_up, w_down, hidden, gate, up, dy, dx, dw_gate, dw_up, dw_down, db_gate, db_up, db_down,
+                  workspace}))
+    return fail(FST_EINVAL, "pointers must be multiples of 16 bytes");
+  const GradLayout l = grad_layout(dtype, rows, D, F);
+  if (!workspace || workspace_bytes < l.total)
+    return fail(FST_EWORKSPACE, "workspace of %zu bytes is smaller than the %zu required", workspace_bytes, l.total);
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const int32_t* map = seqlens ? rowmap + 1 : nullptr;
+
+  if (rows > 0 && (first || dx)) {
+    Transposes t{};
+    int grid = 0;
+    auto add = [&](int k, const void* in, size_t out, int R, int C, long ldo) {
+      t.in[k] = in;
+      t.out[k] = ws + out;
+      t.R[k] = R;
+      t.C[k] = C;
+      t.ldo[k] = ldo;
+      if (in) grid += ((R + 63) / 64) * ((C + 63) / 64);
+      t.first[k] = grid;
+    };
+    add(0, w_down, l.wdt, D, F, D);
+    add(1, dx ? w_gate : nullptr, l.w2t, F, D, 2l * F);
+    add(2, dx ? w_up : nullptr, l.w2t + F * es, F, D, 2l * F);
+    if (es == 2)
+      ffn_transpose<uint16_t><<<grid, 256, 0, st>>>(t);
+    else
+      ffn_transpose<uint32_t><<<grid, 256, 0, st>>>(t);
+    FfnProduct p{};
+    p.count = seqlens ? rowmap : nullptr;
+    p.tokens = (int)rows;
+    p.act = activation;
+    p.w[0] = ws + l.wdt;
+    p.x = dy;
+    p.ldx = dy_stride;
+    p.rows_in = map;
+    p.gate = gate;
+    p.up = up;
+    p.out[0] = ws + l.dadu;
+    p.ldo = 2l * F;
+    p.ldw = p.K = D;
+    p.F = F;
+    rc = product_of(dtype)(kFfnGrad, p, st);
+    if (rc == FST_OK && dx) {
+      if (seqlens) launch_rows(seqlens, B, L, nullptr, dx, D, es, st);
+      p.w[0] = ws + l.w2t;
+      p.x = ws + l.dadu;
+      p.rows_in = nullptr;
+      p.rows_out = map;
+      p.out[0] = dx;
+      p.ldo = D;
+      p.ldx = p.ldw = p.K = 2 * F;
+      p.F = D;
+      rc = product_of(dtype)(kFfnOut, p, st);
+    }
+    if (rc != FST_OK) return fail(rc, "feed-forward backward launch failed");
+  }
+  if (first || second) {
+    FfnOuters o{};
+    o.count = seqlens ? rowmap : nullptr;
+    o.tokens = (int)rows;
+    o.splits[0] = first ? l.splits : 0;
+    o.splits[1] = second ? l.splits : 0;
+    o.p[0] = FfnOuter{x, ws + l.dadu, map, nullptr, (long)x_stride, 2l * F, D, 2 * F,
+                      reinterpret_cast<float*>(ws + l.part0),
+                      db_gate || db_up ? reinterpret_cast<float*>(ws + l.bias0) : nullptr};
+    o.p[1] = FfnOuter{hidden, dy, nullptr, map, F, (long)dy_stride, F, D, reinterpret_cast<float*>(ws + l.part1),
+                      db_down ? reinterpret_cast<float*>(ws + l.bias1) : nullptr};
+    rc = outer_of(dtype)(o, st);
+    if (rc != FST_OK) return fail(rc, "feed-forward weight gradient launch failed");
+    const long df = (long)D * F;
+    const float *p0 = o.p[0].part, *p1 = o.p[1].part;
+    const float *b0 = reinterpret_cast<float*>(ws + l.bias0), *b1 = reinterpret_cast<float*>(ws + l.bias1);
+    const float* part[6] = {p0, p0 + df, p1, b0, b0 + F, b1};
+    void* out[6] = {dw_gate, dw_up, dw_down, db_gate, db_up, db_down};
+    const long stride[6] = {2 * df, 2 * df, df, 2l * F, 2l * F, D}, count[6] = {df, df, df, F, F, D};
+    GradSums s{};
+    int grid = 0;
+    for (int k = 0; k < 6; ++k) {
+      s.part[k] = part[k];
+      s.out[k] = out[k];
+      s.stride[k] = stride[k];
+      s.count[k] = count[k];
+      s.splits[k] = l.splits;
+      if (out[k]) grid += (int)((count[k] + 1023) / 1024);
+      s.first[k] = grid;
+    }
+    if (dtype == FST_BF16)
+      ffn_grad_sum<bf16><<<grid, 256, 0, st>>>(s);
+    else if (dtype == FST_F16)
+      ffn_grad_sum<f16><<<grid, 256, 0, st>>>(s);
+    else
+      ffn_grad_sum<float><<<grid, 256, 0, st>>>(s);
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(FST_ELAUNCH, "feed-forward backward launch failed (%s)", hipGetErrorString(e));
+  return FST_OK;
+}
+
+}  // extern "C"

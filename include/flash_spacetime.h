@@ -55,7 +55,13 @@
 extern "C" {
 #endif
 
-enum fst_dtype { FST_BF16 = 0, FST_F32 = 1 };
+/* FST_F16: layer norm and the feed-forward block only. */
+enum fst_dtype { FST_BF16 = 0, FST_F32 = 1, FST_F16 = 2 };
+
+/* The gate's activation in fst_ffn_*: a sigmoid(a); a Phi(a) with the normal
+ * distribution function Phi; and its tanh form
+ * a / 2 (1 + tanh(sqrt(2 / pi) (a + 0.044715 a^3))). */
+enum fst_activation { FST_SILU = 0, FST_GELU = 1, FST_GELU_TANH = 2 };
 
 enum fst_flags {
   FST_ATTN_BIAS = 1, /* add qt_i . R_ij to the logits (use_attn_bias)        */
@@ -267,6 +273,68 @@ int fst_backward_phases(int phases, int dtype, int flags, int B, int H, int L, i
  * less than 2^31 bytes. Host-only, no GPU call. No reference counterpart
  * (the reference's Triton kernels state no bound). */
 int fst_max_event_len(int dtype, int flags, int H, int D, int C);
+
+/* ---------------------------------------------------------------------------
+ * The transformer block beside its attention: layer norm and the gated
+ * feed-forward block (graphnet's Block_rel runs both around the reference's
+ * operator; the reference itself has no counterpart).
+ *
+ * Rows are tokens: B * L of them, L to an event. seqlens [B] int32 (nullable:
+ * every row is a token; packed tokens are B = T events of L = 1, or the
+ * other way round) gives padded events' lengths, taken within [0, L]: rows past
+ * them are not read, are zeros in every row-shaped output, and add nothing
+ * to the gradients of weights and biases. Row strides are in elements;
+ * outputs are dense. B * L is at most 2^31 - 1. dtype is FST_BF16, FST_F16 or
+ * FST_F32; sums and statistics are float32, every output is rounded once.
+ * Results are bitwise deterministic. As above nothing is allocated or
+ * synchronised. */
+
+/* y = (s - mean(s)) / sqrt(var(s) + eps) * weight + bias over the N features of
+ * a row, s = x, or with residual (nullable) s = x + residual rounded to dtype
+ * and written to sum. weight and bias (each nullable: 1, 0) are float32 or of
+ * dtype (param_dtype). stats (nullable) receives the rows' mean and
+ * 1 / sqrt(var + eps), [B * L, 2], for the backward. N is at most 16384; any
+ * address and stride alignment of whole elements. */
+int fst_layer_norm_forward(int dtype, int param_dtype, int B, int L, int N, const void* x, int64_t x_stride,
+                           const void* residual, int64_t residual_stride, const void* weight, const void* bias,
+                           const int32_t* seqlens, float eps, void* y, void* sum, float* stats, void* stream);
+
+/* Scratch bytes fst_layer_norm_backward needs (when dweight or dbias is asked for). */
+size_t fst_layer_norm_backward_workspace_bytes(int dtype, int B, int L, int N);
+
+/* From s (x, or the forward's sum), its stats, and the gradients dy of y and
+ * dsum (nullable) of sum: dx, the gradient of x and of residual alike, and
+ * dweight, dbias in param_dtype. Each of the three is nullable. */
+int fst_layer_norm_backward(int dtype, int param_dtype, int B, int L, int N, const void* s, int64_t s_stride,
+                            const void* weight, const int32_t* seqlens, const float* stats, const void* dy,
+                            int64_t dy_stride, const void* dsum, int64_t dsum_stride, void* dx, void* dweight,
+                            void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+
+/* y = h Wd^T + bd with h = act(a) u, a = x Wg^T + bg, u = x Wu^T + bu, for rows
+ * x of D features and F hidden ones: w_gate, w_up [F, D], w_down [D, F], all of
+ * dtype and dense, as the biases (b_gate, b_up [F], b_down [D]; each
+ * nullable). D and F are multiples of 8, at most 65536, and their product less
+ * than 2^28; every pointer, and the row strides of x and dy in bytes, are
+ * multiples of 16.
+ * hidden [B * L, F] receives h, and gate, up of the same size (both or neither;
+ * the backward needs them) a and u, rounded to dtype; with seqlens the rows
+ * of all three are the valid tokens in order, and rowmap (B * L + 1 ints, needed
+ * with seqlens, else unused) receives their number and their rows. */
+int fst_ffn_forward(int dtype, int activation, int B, int L, int D, int F, const void* x, int64_t x_stride,
+                    const void* w_gate, const void* w_up, const void* w_down, const void* b_gate, const void* b_up,
+                    const void* b_down, const int32_t* seqlens, void* hidden, void* gate, void* up, int32_t* rowmap,
+                    void* y, void* stream);
+
+/* Scratch bytes fst_ffn_backward needs. */
+size_t fst_ffn_backward_workspace_bytes(int dtype, int B, int L, int D, int F);
+
+/* The gradients, from the forward's operands, its hidden, gate, up and rowmap,
+ * and dy. Each gradient is nullable. */
+int fst_ffn_backward(int dtype, int activation, int B, int L, int D, int F, const void* x, int64_t x_stride,
+                     const void* w_gate, const void* w_up, const void* w_down, const int32_t* seqlens,
+                     const void* hidden, const void* gate, const void* up, const int32_t* rowmap, const void* dy,
+                     int64_t dy_stride, void* dx, void* dw_gate, void* dw_up, void* dw_down, void* db_gate,
+                     void* db_up, void* db_down, void* workspace, size_t workspace_bytes, void* stream);
 
 /* The fp32 frequency ladder exp(-i ln(1e4) / (C/2)), i < C/2, that the kernels
  * embed with, written to out[0 .. C/2). Counterpart of sinusoidal_frequencies
