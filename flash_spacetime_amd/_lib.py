@@ -112,7 +112,7 @@ SIGNATURES = {
     "fst_ffn_backward_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "fst_ffn_backward": (
         _i,
-        [_i, _i, _i, _i, _i, _i, _vp, _l, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _l,
+        [_i, _i, _i, _i, _i, _i, _vp, _l, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _l,
          _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp],
     ),
     "fst_max_event_len": (_i, [_i, _i, _i, _i, _i]),

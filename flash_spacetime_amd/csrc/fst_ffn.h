@@ -10,57 +10,59 @@ namespace fst {
 enum FfnMode {
   kFfnGate = 0,  // a = x Wg^T + bg, u = x Wu^T + bu: h = act(a) u (and a, u)
   kFfnOut = 1,   // x W^T + b
-  kFfnGrad = 2,  // dh = x W^T: da = dh u act'(a), du = dh act(a), one row of 2 F
+  kFfnGrad = 2,  // dh = x W^T: da = dh u act'(a), du = dh act(a), one row of 2 F, from a and u as kept
+  kFfnRedo = 3,  // the same with a and u formed again (x Wg^T + bg, x Wu^T + bu; dh = dy W^T)
 };
+
+// Whether the backward forms a and u again: rounded to 16 bits they would move
+// every gradient by as much as its own rounding does. float32 keeps them.
+inline bool ffn_redo(int dtype) { return dtype != FST_F32; }
 
 // C[token, f] = sum_k x[token, k] w[f, k]: both operands contiguous along k.
 struct FfnProduct {
-  const void* w[2];        // [F, K], rows ldw apart; w[1] with kFfnGate
+  const void* w[3];        // [F, K], rows ldw apart; w[1]: up, w[2]: dh's (kFfnRedo)
   const void* bias[2];     // [F] or null
-  const void* x;           // rows of K, ldx apart
+  const void *x, *dy;      // rows of K, ldx, lddy apart; dy with kFfnRedo
   void* out[3];            // kFfnGate: h, a, u (a, u may be null); else out[0]
   const void *gate, *up;   // kFfnGrad: a, u [tokens, F]
   const int32_t* count;    // tokens, on the device (seqlens given); or null
-  const int32_t* rows_in;  // row of x of each token, or null (the token's own)
+  const int32_t* rows_in;  // row of x (and dy) of each token, or null (the token's own)
   const int32_t* rows_out; // row of out[0] of each token (kFfnOut), or null
-  long ldx, ldo, ldw;      // elements
+  long ldx, lddy, ldo, ldw;  // elements
   int tokens;              // tokens, or the most there can be
   int F, K, act;
 };
 
 // C[n, m] = sum_token b[token, n] a[token, m], and sum_token b[token, n]: the
-// gradient of a weight (and of the bias beside it), m contiguous in C.
-// Workgroups with part >= 0 rows take `splits` equal runs of the tokens; each
-// writes its own partial, summed in order afterwards.
+// gradient of a weight (and of the bias beside it), m contiguous in C. The tokens
+// are taken in `splits` equal runs, each with a partial of its own, summed in
+// order afterwards.
 struct FfnOuter {
   const void *a, *b;
-  const int32_t *rows_a, *rows_b;  // rows of the tokens, or null
-  long lda, ldb;
-  int M, N;
-  float* part;     // [splits][N][M]
-  float* bias;     // [splits][N]
-};
-
-struct FfnOuters {
-  FfnOuter p[2];
-  int first[2];    // workgroups of the problems: [0, first[0]), [first[0], first[1])
-  int splits[2];
+  const int32_t *rows_a, *rows_b;  // rows of the tokens (one of them at most), or null
   const int32_t* count;
-  int tokens;
+  long lda, ldb;   // elements; in bytes below 2^32
+  int M, N, tokens, splits;
+  float* part;     // [splits][N][M]
+  float* bias;     // [splits][N], or null
 };
 
 typedef int (*ffn_product_fn)(int mode, const FfnProduct&, hipStream_t);
-typedef int (*ffn_outer_fn)(FfnOuters&, hipStream_t);
+typedef int (*ffn_outer_fn)(const FfnOuter&, int shape, hipStream_t);
 
 #define FST_FFN_DECL(name)                                      \
   int ffn_product_##name(int mode, const FfnProduct&, hipStream_t); \
-  int ffn_outer_##name(FfnOuters&, hipStream_t);
+  int ffn_outer_##name(const FfnOuter&, int shape, hipStream_t);
 FST_FFN_DECL(bf16)
 FST_FFN_DECL(f16)
 FST_FFN_DECL(f32)
 #undef FST_FFN_DECL
 
-// Tile of an outer product, in elements of M and N.
-constexpr int kOuterM = 128, kOuterN = 256;
+// Tiles of an outer product (shape of ffn_outer_*): M and N of a workgroup, and
+// workgroups a CU holds.
+struct OuterTile {
+  int m, n, per_cu;
+};
+constexpr OuterTile kOuterTiles[] = {{128, 128, 2}, {256, 256, 1}, {192, 256, 1}, {256, 192, 1}};
 
 }  // namespace fst

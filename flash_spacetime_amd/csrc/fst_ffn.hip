@@ -7,13 +7,14 @@
 //
 // Forward: gate and up projections with the activation in one product, then the
 // output product. Backward: da and du (side by side in one row, so that the
-// products after them are one each) from dy and the forward's a and u, dx, and
-// the three weights' gradients in one launch, summed over its token runs in
-// order. a, u and h are kept from the forward: forming a and u again would add 4
-// T F D operations to the 12 T F D of the backward, against 2 T F elements
-// written and read; where D is 1024 the products are several times dearer, at
-// D = 384 about equal. Padded batches are gathered on the way: a list of the
-// valid rows is the products' token axis, so padding costs nothing but its zeros.
+// products after them are one each), dx, and the weights' gradients, summed over
+// runs of the tokens in order. h is kept from the forward; a and u are formed
+// again (4 T F D operations beside the backward's 12) except in float32, which
+// keeps them: rounded to 16 bits they had moved the gradients to twice the
+// distance from 64 bits (bf16 0.0031 of their norm against 0.0024), and at D =
+// 384 writing and reading them took as long as the products do.
+// Padded batches are gathered on the way: a list of the valid rows is the
+// products' token axis, so padding costs nothing but its zeros.
 #include "fst_ffn.h"
 
 namespace fst {
@@ -124,6 +125,9 @@ int check_ffn(int dtype, int activation, int B, int L, int D, int F) {
   return FST_OK;
 }
 
+// A row stride in elements that the kernels do not take.
+bool bad_stride(int64_t stride, int n, size_t es) { return stride < n || stride * es % 16 || stride >= (int64_t)(1ul << 32) / (int64_t)es; }
+
 bool misaligned(std::initializer_list<const void*> ps) {
   for (const void* p : ps)
     if (reinterpret_cast<uintptr_t>(p) % 16) return true;
@@ -147,32 +151,39 @@ void launch_rows(const int32_t* seqlens, int B, int L, int32_t* map, void* out, 
                                                              static_cast<unsigned char*>(out), (long)D * es);
 }
 
-int tiles_of(int M, int N) { return ((M + kOuterM - 1) / kOuterM) * ((N + kOuterN - 1) / kOuterN); }
+// Tile and token runs of a weight's gradient [N, M]: the least of the rounds of
+// workgroups over the chip at the tiles' rates (PFLOP/s of a full chip measured:
+// bf16 1.0 and, in the small tiles, 0.8) plus the runs' partials written and read.
+struct OuterPlan {
+  int shape, splits;
+};
 
-// Token runs of the weights' gradients: a workgroup holds two tiles a CU (512 at
-// a time); more runs shorten the rounds, and write and read their partials.
-int outer_splits(int dtype, long tokens, int D, int F) {
-  const int tiles = tiles_of(D, 2 * F) + tiles_of(F, D);
-  const double tile_s = (double)tokens * 2 * kOuterM * kOuterN / (dtype == FST_F32 ? 0.2e12 : 1.5e12);
-  const double part_s = 3.0 * D * F * 8 / 4e12;
-  int best = 1;
+OuterPlan plan_outer(int dtype, long tokens, int M, int N) {
+  OuterPlan best{0, 1};
   double least = 0;
-  for (int s = 1; s <= 64 && (s == 1 || s * 256l <= tokens); ++s) {
-    const double t = (double)((tiles * s + 511) / 512) / s * tile_s + s * part_s;
-    if (s == 1 || t < least) best = s, least = t;
+  for (int k = 0; k < 4; ++k) {
+    const OuterTile& o = kOuterTiles[k];
+    const long tiles = (long)((M + o.m - 1) / o.m) * ((N + o.n - 1) / o.n), slots = 256l * o.per_cu;
+    const double rate = (dtype == FST_F32 ? 0.12e15 : k ? 1.0e15 : 0.8e15) / slots;
+    for (int s = 1; s <= 64 && (s == 1 || s * 256l <= tokens); ++s) {
+      const double work = (double)tokens / s * 2 * o.m * o.n / rate;
+      const double t = (double)((tiles * s + slots - 1) / slots) * work + s * 8.0 * M * N / 4e12;
+      if ((k == 0 && s == 1) || t < least) best = OuterPlan{k, s}, least = t;
+    }
   }
   return best;
 }
 
 struct GradLayout {
   size_t wdt, w2t, dadu, part0, part1, bias0, bias1, total;
-  int splits;
+  OuterPlan first, second;
 };
 
 GradLayout grad_layout(int dtype, long rows, int D, int F) {
   GradLayout l;
   const size_t es = elem_size(dtype), df = (size_t)D * F;
-  l.splits = outer_splits(dtype, rows, D, F);
+  l.first = plan_outer(dtype, rows, D, 2 * F);
+  l.second = plan_outer(dtype, rows, F, D);
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const size_t at = off;
@@ -182,10 +193,10 @@ GradLayout grad_layout(int dtype, long rows, int D, int F) {
   l.wdt = take(df * es);
   l.w2t = take(2 * df * es);
   l.dadu = take((size_t)rows * 2 * F * es);
-  l.part0 = take(l.splits * 2 * df * 4);
-  l.part1 = take(l.splits * df * 4);
-  l.bias0 = take((size_t)l.splits * 2 * F * 4);
-  l.bias1 = take((size_t)l.splits * D * 4);
+  l.part0 = take(l.first.splits * 2 * df * 4);
+  l.part1 = take(l.second.splits * df * 4);
+  l.bias0 = take((size_t)l.first.splits * 2 * F * 4);
+  l.bias1 = take((size_t)l.second.splits * D * 4);
   l.total = off;
   return l;
 }
@@ -209,8 +220,9 @@ int fst_ffn_forward(int dtype, int activation, int B, int L, int D, int F, const
   if (rows == 0) return FST_OK;
   if (!x || !w_gate || !w_up || !w_down || !hidden || !y || (seqlens && !rowmap) || !gate != !up)
     return fail(FST_EINVAL, "null tensor pointer");
+  if (gate && ffn_redo(dtype)) return fail(FST_EINVAL, "gate and up are kept in float32 only");
   const size_t es = elem_size(dtype);
-  if (x_stride < D || x_stride * es % 16) return fail(FST_EINVAL, "x's row stride must be at least D and whole 16 bytes");
+  if (bad_stride(x_stride, D, es)) return fail(FST_EINVAL, "x's row stride must be at least D, whole 16 bytes and below 2^32");
   if (misaligned({x, w_gate, w_up, w_down, b_gate, b_up, b_down, hidden, gate, up, y}))
     return fail(FST_EINVAL, "pointers must be multiples of 16 bytes");
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -255,9 +267,9 @@ size_t fst_ffn_backward_workspace_bytes(int dtype, int B, int L, int D, int F) {
 }
 
 int fst_ffn_backward(int dtype, int activation, int B, int L, int D, int F, const void* x, int64_t x_stride,
-                     const void* w_gate, const void* w_up, const void* w_down, const int32_t* seqlens,
-                     const void* hidden, const void* gate, const void* up, const int32_t* rowmap, const void* dy,
-                     int64_t dy_stride, void* dx, void* dw_gate, void* dw_up, void* dw_down, void* db_gate,
+                     const void* w_gate, const void* w_up, const void* w_down, const void* b_gate, const void* b_up,
+                     const int32_t* seqlens, const void* hidden, const void* gate, const void* up,
+                     const int32_t* rowmap, const void* dy, int64_t dy_stride, void* dx, void* dw_gate, void* dw_up, void* dw_down, void* db_gate,
                      void* db_up, void* db_down, void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
   int rc = check_ffn(dtype, activation, B, L, D, F);
@@ -267,12 +279,12 @@ int fst_ffn_backward(int dtype, int activation, int B, int L, int D, int F, cons
   if (!first && !second && !dx) return FST_OK;
   const size_t es = elem_size(dtype);
   if (rows > 0) {
-    if (!x || !w_gate || !w_up || !w_down || !hidden || !gate || !up || !dy || (seqlens && !rowmap))
+    if (!x || !w_gate || !w_up || !w_down || !hidden || !dy || (seqlens && !rowmap) || (!ffn_redo(dtype) && !(gate && up)))
       return fail(FST_EINVAL, "null tensor pointer");
-    if (x_stride < D || x_stride * es % 16 || dy_stride < D || dy_stride * es % 16)
-      return fail(FST_EINVAL, "row strides of x and dy must be at least D and whole 16 bytes");
+    if (bad_stride(x_stride, D, es) || bad_stride(dy_stride, D, es))
+      return fail(FST_EINVAL, "row strides of x and dy must be at least D, whole 16 bytes and below 2^32");
   }
-  if (misaligned({x, w_gate, w_up, w_down, hidden, gate, up, dy, dx, dw_gate, dw_up, dw_down, db_gate, db_up, db_down,
+  if (misaligned({x, w_gate, w_up, w_down, b_gate, b_up, hidden, gate, up, dy, dx, dw_gate, dw_up, dw_down, db_gate, db_up, db_down,
                   workspace}))
     return fail(FST_EINVAL, "pointers must be multiples of 16 bytes");
   const GradLayout l = grad_layout(dtype, rows, D, F);
@@ -305,20 +317,33 @@ int fst_ffn_backward(int dtype, int activation, int B, int L, int D, int F, cons
     p.count = seqlens ? rowmap : nullptr;
     p.tokens = (int)rows;
     p.act = activation;
-    p.w[0] = ws + l.wdt;
-    p.x = dy;
-    p.ldx = dy_stride;
+    if (ffn_redo(dtype)) {
+      p.w[0] = w_gate;
+      p.w[1] = w_up;
+      p.w[2] = ws + l.wdt;
+      p.bias[0] = b_gate;
+      p.bias[1] = b_up;
+      p.x = x;
+      p.ldx = x_stride;
+      p.dy = dy;
+      p.lddy = dy_stride;
+    } else {
+      p.w[0] = ws + l.wdt;
+      p.x = dy;
+      p.ldx = dy_stride;
+      p.gate = gate;
+      p.up = up;
+    }
     p.rows_in = map;
-    p.gate = gate;
-    p.up = up;
     p.out[0] = ws + l.dadu;
     p.ldo = 2l * F;
     p.ldw = p.K = D;
     p.F = F;
-    rc = product_of(dtype)(kFfnGrad, p, st);
+    rc = product_of(dtype)(ffn_redo(dtype) ? kFfnRedo : kFfnGrad, p, st);
     if (rc == FST_OK && dx) {
       if (seqlens) launch_rows(seqlens, B, L, nullptr, dx, D, es, st);
       p.w[0] = ws + l.w2t;
+      p.bias[0] = nullptr;
       p.x = ws + l.dadu;
       p.rows_in = nullptr;
       p.rows_out = map;
@@ -331,21 +356,41 @@ int fst_ffn_backward(int dtype, int activation, int B, int L, int D, int F, cons
     if (rc != FST_OK) return fail(rc, "feed-forward backward launch failed");
   }
   if (first || second) {
-    FfnOuters o{};
+    FfnOuter o{};
     o.count = seqlens ? rowmap : nullptr;
     o.tokens = (int)rows;
-    o.splits[0] = first ? l.splits : 0;
-    o.splits[1] = second ? l.splits : 0;
-    o.p[0] = FfnOuter{x, ws + l.dadu, map, nullptr, (long)x_stride, 2l * F, D, 2 * F,
-                      reinterpret_cast<float*>(ws + l.part0),
-                      db_gate || db_up ? reinterpret_cast<float*>(ws + l.bias0) : nullptr};
-    o.p[1] = FfnOuter{hidden, dy, nullptr, map, F, (long)dy_stride, F, D, reinterpret_cast<float*>(ws + l.part1),
-                      db_down ? reinterpret_cast<float*>(ws + l.bias1) : nullptr};
-    rc = outer_of(dtype)(o, st);
+    float *p0 = reinterpret_cast<float*>(ws + l.part0), *p1 = reinterpret_cast<float*>(ws + l.part1);
+    float *b0 = reinterpret_cast<float*>(ws + l.bias0), *b1 = reinterpret_cast<float*>(ws + l.bias1);
+    rc = FST_OK;
+    if (first) {
+      o.a = x;
+      o.rows_a = map;
+      o.lda = x_stride;
+      o.b = ws + l.dadu;
+      o.ldb = 2l * F;
+      o.M = D;
+      o.N = 2 * F;
+      o.splits = l.first.splits;
+      o.part = p0;
+      o.bias = db_gate || db_up ? b0 : nullptr;
+      rc = outer_of(dtype)(o, l.first.shape, st);
+    }
+    if (second && rc == FST_OK) {
+      o.a = hidden;
+      o.rows_a = nullptr;
+      o.lda = F;
+      o.b = dy;
+      o.rows_b = map;
+      o.ldb = dy_stride;
+      o.M = F;
+      o.N = D;
+      o.splits = l.second.splits;
+      o.part = p1;
+      o.bias = db_down ? b1 : nullptr;
+      rc = outer_of(dtype)(o, l.second.shape, st);
+    }
     if (rc != FST_OK) return fail(rc, "feed-forward weight gradient launch failed");
     const long df = (long)D * F;
-    const float *p0 = o.p[0].part, *p1 = o.p[1].part;
-    const float *b0 = reinterpret_cast<float*>(ws + l.bias0), *b1 = reinterpret_cast<float*>(ws + l.bias1);
     const float* part[6] = {p0, p0 + df, p1, b0, b0 + F, b1};
     void* out[6] = {dw_gate, dw_up, dw_down, db_gate, db_up, db_down};
     const long stride[6] = {2 * df, 2 * df, df, 2l * F, 2l * F, D}, count[6] = {df, df, df, F, F, D};
@@ -356,7 +401,7 @@ int fst_ffn_backward(int dtype, int activation, int B, int L, int D, int F, cons
       s.out[k] = out[k];
       s.stride[k] = stride[k];
       s.count[k] = count[k];
-      s.splits[k] = l.splits;
+      s.splits[k] = k == 2 || k == 5 ? l.second.splits : l.first.splits;
       if (out[k]) grid += (int)((count[k] + 1023) / 1024);
       s.first[k] = grid;
     }

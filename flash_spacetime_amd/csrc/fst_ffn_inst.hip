@@ -93,11 +93,12 @@ __device__ __forceinline__ float activate(int kind, float a, float& slope) {
   return a * g;
 }
 
-// 16 consecutive elements: loads and stores of `n` of them (a multiple of 8).
-__device__ __forceinline__ void load16(const T* p, int n, float* v) {
+// N consecutive elements: loads and stores of `n` of them (a multiple of 8).
+template <int N>
+__device__ __forceinline__ void load_run(const T* p, int n, float* v) {
   constexpr int V = kVec<T>;
 #pragma unroll
-  for (int q = 0; q < 16 / V; ++q) {
+  for (int q = 0; q < N / V; ++q) {
     typename Piece<T>::V x;
 #pragma unroll
     for (int i = 0; i < V; ++i) x[i] = (T)0.f;
@@ -106,10 +107,11 @@ __device__ __forceinline__ void load16(const T* p, int n, float* v) {
     for (int i = 0; i < V; ++i) v[q * V + i] = (float)x[i];
   }
 }
-__device__ __forceinline__ void store16(T* p, int n, const float* v) {
+template <int N>
+__device__ __forceinline__ void store_run(T* p, int n, const float* v) {
   constexpr int V = kVec<T>;
 #pragma unroll
-  for (int q = 0; q < 16 / V; ++q)
+  for (int q = 0; q < N / V; ++q)
     if (q * V < n) *reinterpret_cast<typename Piece<T>::V*>(p + q * V) = pack_piece<T>(v + q * V);
 }
 
@@ -128,28 +130,40 @@ __device__ __forceinline__ bool pick_tile(int wg, int nf, int nt, int& f, int& t
   return true;
 }
 
-// Workgroups of 256 threads: WF x WT waves of NI x NJ subtiles of 16 features by
-// 16 tokens. The weight is the matrix core's row operand, so a lane ends up
-// with the same 16 consecutive features (of each 64) of its tokens: slot m =
-// 4 a + r of subtile s of a group holds feature 16 a + 4 s + r, which the
-// loads into LDS arrange. LDS rows are 64 bytes of k; 16-byte part c of row r
-// sits at c ^ ((r >> 2) & 3), so that the 16 rows of a read pass cover the
-// banks once. Three stages: the loads of two k steps are in flight while a
-// third is multiplied, one barrier a step.
+// WF x WT waves of NI x NJ subtiles of 16 features by 16 tokens. The weight is
+// the matrix core's row operand, so a lane ends up with 4 GS consecutive
+// features of its tokens: slot m = 4 a + r of subtile s of a group of GS holds
+// feature 4 GS a + 4 s + r, which the loads into LDS arrange. LDS rows are 128
+// bytes of k (whole lines of memory: 64-byte rows measured a fifth slower);
+// 16-byte part c of row r sits at c ^ ((r >> 1) & 7), so that the 16 rows of a
+// read pass cover the banks once. Two stages: the loads of a k step run while
+// the step before is multiplied, one barrier a step.
+//
+// kFfnRedo runs two contractions after each other, a and u from x and then dh
+// from dy, and holds all three.
 template <int MODE, int WF, int WT, int NI, int NJ>
 struct Product {
-  static constexpr int BF = 16 * NI * WF, BT = 16 * NJ * WT, ROWS = BF + BT;
-  static constexpr int FEATURES = MODE == kFfnGate ? BF / 2 : BF;  // of the output
-  static constexpr int LW = BF / 64, LT = BT / 64;
-  static constexpr int STAGE = ROWS * 64;
-  static constexpr int KE = 64 / ES;  // k of a step
+  static constexpr int WAVES = WF * WT;
+  // Weights whose rows share a stage's feature rows, side by side in each wave's NI.
+  static constexpr int MATS = MODE == kFfnGate || MODE == kFfnRedo ? 2 : 1;
+  static constexpr int NF = NI / MATS;             // feature subtiles of a wave
+  static constexpr int GS = NF % 4 == 0 ? 4 : 2;   // subtiles of a group
+  static constexpr int FEATURES = 16 * NF * WF;    // of the output, a workgroup
+  static constexpr int BF = 16 * NI * WF, BT = 16 * NJ * WT;
+  static constexpr int LW = BF / (8 * WAVES), LT = BT / (8 * WAVES), LD = FEATURES / (8 * WAVES);
+  static constexpr int STAGE = (BF + BT) * 128;
+  static constexpr int KE = 128 / ES;              // k of a step
+  static_assert(NF % 2 == 0 && BF % (8 * WAVES) == 0 && BT % (8 * WAVES) == 0 && FEATURES % (8 * WAVES) == 0, "tile");
 };
 
-template <int MODE, int WF, int WT, int NI, int NJ>
-__global__ __launch_bounds__(256, 2) void ffn_product(FfnProduct p) {
+__device__ __forceinline__ u32x4 read16(const unsigned char* p) { return *reinterpret_cast<const u32x4*>(p); }
+
+template <int MODE, int WF, int WT, int NI, int NJ, int OCC>
+__global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
   typedef Product<MODE, WF, WT, NI, NJ> C;
-  static_assert(WF * WT == 4 && NI % (MODE == kFfnGate ? 8 : 4) == 0, "waves and feature groups");
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[3][C::STAGE];
+  constexpr int NF = C::NF, GS = C::GS, NE = 4 * GS, WAVES = C::WAVES;
+  constexpr bool REDO = MODE == kFfnRedo;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2][C::STAGE];
   const int tokens = p.count ? *p.count : p.tokens;
   const int nf = (p.F + C::FEATURES - 1) / C::FEATURES, nt = (tokens + C::BT - 1) / C::BT;
   int ft, tt;
@@ -158,130 +172,171 @@ __global__ __launch_bounds__(256, 2) void ffn_product(FfnProduct p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wf = wave % WF, wt = wave / WF, g = lane >> 4, n = lane & 15;
 
-  // Loads: wave w fills subtile w of each group of 64 rows, lane l the 16 bytes
-  // at 16 l of it: row l / 4, part (l & 3) of the layout above.
-  const int row = lane >> 2, part = (lane & 3) ^ ((row >> 2) & 3);
-  const int wrow = 16 * (row >> 2) + 4 * wave + (row & 3);
+  // Loads: each fills 8 rows, lane l the 16 bytes at 16 l: row l / 8, part l & 7
+  // of the layout above. Load i of a wave takes the rows 8 (i WAVES + wave) ..
+  const int row8 = lane >> 3, m = 8 * (wave & 1) + row8;  // row of its subtile: WAVES is even
+  const int part = (lane & 7) ^ ((m >> 1) & 7);
   const int row_bytes = (int)p.ldw * ES;
-  // The scalar offset moves along k only and stays inside a row: the range
-  // check subtracts it from the buffer's size.
-  int voff[C::LW];
+  // The feature of row m of feature subtile i (of a workgroup).
+  auto feature = [&](int i) { return (i / GS) * 16 * GS + NE * (m >> 2) + 4 * (i % GS) + (m & 3); };
+  int voff[C::LW], mat[C::LW];
 #pragma unroll
-  for (int i = 0; i < C::LW; ++i) voff[i] = (wrow + 64 * (MODE == kFfnGate ? i >> 1 : i)) * row_bytes + part * 16;
-  // Rows of the weight past F read as zeros (range of the buffer).
+  for (int i = 0; i < C::LW; ++i) {
+    const int sub = (i * WAVES + wave) >> 1, of = sub % NI;
+    mat[i] = of / NF;
+    voff[i] = feature(sub / NI * NF + of % NF) * row_bytes + part * 16;
+  }
+  // Rows of the weights past F read as zeros (range of the buffer; the scalar
+  // offset moves along k only and stays inside a row, as the range check
+  // subtracts it from the buffer's size).
   const int range = (p.F - f0) * row_bytes;
-  const __amdgpu_buffer_rsrc_t wr0 = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<char*>(static_cast<const char*>(p.w[0]) + (long)f0 * row_bytes), (short)0, range, 0x00020000);
-  const __amdgpu_buffer_rsrc_t wr1 = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<char*>(static_cast<const char*>(p.w[MODE == kFfnGate]) + (long)f0 * row_bytes), (short)0, range, 0x00020000);
-  const char* xp[C::LT];
+  auto weight = [&](int k) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(p.w[k]) + (long)f0 * row_bytes),
+                                             (short)0, range, 0x00020000);
+  };
+  const __amdgpu_buffer_rsrc_t wr0 = weight(0), wr1 = weight(C::MATS - 1), wr2 = weight(REDO ? 2 : 0);
+  const char *xp[C::LT], *yp[REDO ? C::LT : 1];
 #pragma unroll
   for (int i = 0; i < C::LT; ++i) {
     // Tokens past the last repeat it; their columns are not stored.
-    const int t = min(t0 + 64 * i + 16 * wave + row, tokens - 1);
+    const int t = min(t0 + 8 * (i * WAVES + wave) + row8, tokens - 1);
     const long r = p.rows_in ? p.rows_in[t] : t;
     xp[i] = static_cast<const char*>(p.x) + (r * p.ldx) * ES + part * 16;
+    if constexpr (REDO) yp[i] = static_cast<const char*>(p.dy) + (r * p.lddy) * ES + part * 16;
   }
   const int steps = (p.K + C::KE - 1) / C::KE;
   const int tail = p.K % C::KE * ES;  // bytes of the last step, 0: all
 
-  auto issue = [&](int s, int b) __attribute__((always_inline)) {
+  // Loads of k step s into stage b; second: of dh's contraction.
+  auto issue = [&](int s, int b, bool second) __attribute__((always_inline)) {
     unsigned char* base = lds[b] + wave * 1024;
     // Parts past K are zeros in both operands.
     const bool cut = tail != 0 && s == steps - 1 && part * 16 >= tail;
+    if (!REDO || !second) {
 #pragma unroll
-    for (int i = 0; i < C::LW; ++i) {
-      load_to_lds(MODE == kFfnGate && (i & 1) ? wr1 : wr0, base + i * 4096, cut ? (int)0x80000000 : voff[i], s * 64);
+      for (int i = 0; i < C::LW; ++i)
+        load_to_lds(C::MATS == 2 && mat[i] ? wr1 : wr0, base + i * WAVES * 1024, cut ? (int)0x80000000 : voff[i], s * 128);
+    } else {
+#pragma unroll
+      for (int i = 0; i < C::LD; ++i)
+        load_to_lds(wr2, base + i * WAVES * 1024,
+                    cut ? (int)0x80000000 : feature((i * WAVES + wave) >> 1) * row_bytes + part * 16, s * 128);
     }
 #pragma unroll
     for (int i = 0; i < C::LT; ++i) {
-      const char* q = cut ? reinterpret_cast<const char*>(&kZero16) : xp[i];
-      __builtin_amdgcn_global_load_lds((glb_ptr)q, (lds_ptr)(base + (C::LW + i) * 4096), 16, 0, 0);
-      xp[i] += 64;
+      const char* from = (REDO && second ? yp[REDO ? i : 0] : xp[i]) + s * 128l;
+      const char* q = cut ? reinterpret_cast<const char*>(&kZero16) : from;
+      __builtin_amdgcn_global_load_lds((glb_ptr)q, (lds_ptr)(base + C::BF * 128 + i * WAVES * 1024), 16, 0, 0);
     }
   };
 
-  f32x4 acc[NI][NJ];
+  f32x4 acc[NI][NJ], dh[REDO ? NF : 1][REDO ? NJ : 1];
 #pragma unroll
-  for (int i = 0; i < NI; ++i)
+  for (int j = 0; j < NJ; ++j) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  issue(0, 0);
-  if (steps > 1) issue(1, 1);
-  int b = 0;
-  const int rd = n * 64 + ((g ^ ((n >> 2) & 3)) << 4);
+    for (int i = 0; i < NI; ++i) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if constexpr (REDO) {
+#pragma unroll
+      for (int i = 0; i < NF; ++i) dh[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  const int rd = n * 128, swz = (n >> 1) & 7;
+  issue(0, 0, false);
   for (int s = 0; s < steps; ++s) {
+    const int b = s & 1;
+    stage_wait<0>();
     if (s + 1 < steps)
-      stage_wait<C::LW + C::LT>();
-    else
+      issue(s + 1, b ^ 1, false);
+    else if constexpr (REDO)
+      issue(0, b ^ 1, true);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const unsigned char* base = lds[b] + rd + (((4 * k + g) ^ swz) << 4);
+      u32x4 fw[NI], fx[NJ];
+#pragma unroll
+      for (int i = 0; i < NI; ++i) fw[i] = read16(base + (wf * NI + i) * 2048);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) fx[j] = read16(base + C::BF * 128 + (wt * NJ + j) * 2048);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int i = 0; i < NI; ++i) acc[i][j] = Mma<T>::run(fw[i], fx[j], acc[i][j]);
+    }
+  }
+  if constexpr (REDO) {
+    for (int s = 0; s < steps; ++s) {
+      const int b = (steps + s) & 1;
       stage_wait<0>();
-    if (s + 2 < steps) issue(s + 2, b == 0 ? 2 : b - 1);
-    const unsigned char* base = lds[b] + rd;
-    u32x4 fw[NI], fx[NJ];
+      if (s + 1 < steps) issue(s + 1, b ^ 1, true);
 #pragma unroll
-    for (int i = 0; i < NI; ++i) fw[i] = *reinterpret_cast<const u32x4*>(base + (wf * NI + i) * 1024);
+      for (int k = 0; k < 2; ++k) {
+        const unsigned char* base = lds[b] + rd + (((4 * k + g) ^ swz) << 4);
+        u32x4 fw[NF], fx[NJ];
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) fx[j] = *reinterpret_cast<const u32x4*>(base + (WF * NI + wt * NJ + j) * 1024);
+        for (int i = 0; i < NF; ++i) fw[i] = read16(base + (wf * NF + i) * 2048);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
+        for (int j = 0; j < NJ; ++j) fx[j] = read16(base + C::BF * 128 + (wt * NJ + j) * 2048);
 #pragma unroll
-      for (int i = 0; i < NI; ++i) acc[i][j] = Mma<T>::run(fw[i], fx[j], acc[i][j]);
-    b = b == 2 ? 0 : b + 1;
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int i = 0; i < NF; ++i) dh[i][j] = Mma<T>::run(fw[i], fx[j], dh[i][j]);
+      }
+    }
   }
 
-  // Epilogue: 16 features of one token at a time.
-  constexpr int GROUPS = MODE == kFfnGate ? NI / 8 : NI / 4;
+  // Epilogue: NE features of one token at a time.
   float unused;
 #pragma unroll
-  for (int q = 0; q < GROUPS; ++q) {
-    const int f = f0 + (wf * GROUPS + q) * 64 + 16 * g;
-    const int left = min(16, p.F - f);
+  for (int q = 0; q < NF / GS; ++q) {
+    const int f = f0 + (wf * (NF / GS) + q) * 16 * GS + NE * g;
+    const int left = min(NE, p.F - f);
     if (left <= 0) continue;
-    float b0[16], b1[16];
+    float b0[NE], b1[NE];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) b0[e] = b1[e] = 0.f;
-    if (MODE != kFfnGrad && p.bias[0]) load16(static_cast<const T*>(p.bias[0]) + f, left, b0);
-    if (MODE == kFfnGate && p.bias[1]) load16(static_cast<const T*>(p.bias[1]) + f, left, b1);
+    for (int e = 0; e < NE; ++e) b0[e] = b1[e] = 0.f;
+    if (MODE != kFfnGrad && p.bias[0]) load_run<NE>(static_cast<const T*>(p.bias[0]) + f, left, b0);
+    if (C::MATS == 2 && p.bias[1]) load_run<NE>(static_cast<const T*>(p.bias[1]) + f, left, b1);
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int t = t0 + (wt * NJ + j) * 16 + n;
       if (t >= tokens) continue;
-      float v[16];
+      float v[NE], u[NE];
+#pragma unroll
+      for (int e = 0; e < NE; ++e) {
+        v[e] = acc[GS * q + (e >> 2)][j][e & 3];
+        if constexpr (MODE != kFfnGrad) v[e] += b0[e];
+        if constexpr (C::MATS == 2) u[e] = acc[NF + GS * q + (e >> 2)][j][e & 3] + b1[e];
+      }
       if constexpr (MODE == kFfnGate) {
-        float u[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          v[e] = acc[8 * q + (e >> 2)][j][e & 3] + b0[e];
-          u[e] = acc[8 * q + 4 + (e >> 2)][j][e & 3] + b1[e];
-        }
         const long at = (long)t * p.ldo + f;
-        if (p.out[1]) {
-          store16(static_cast<T*>(p.out[1]) + at, left, v);
-          store16(static_cast<T*>(p.out[2]) + at, left, u);
+        if (F32 && p.out[1]) {
+          store_run<NE>(static_cast<T*>(p.out[1]) + at, left, v);
+          store_run<NE>(static_cast<T*>(p.out[2]) + at, left, u);
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = activate<false>(p.act, v[e], unused) * u[e];
-        store16(static_cast<T*>(p.out[0]) + at, left, v);
+        for (int e = 0; e < NE; ++e) v[e] = activate<false>(p.act, v[e], unused) * u[e];
+        store_run<NE>(static_cast<T*>(p.out[0]) + at, left, v);
       } else if constexpr (MODE == kFfnOut) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) v[e] = acc[4 * q + (e >> 2)][j][e & 3] + b0[e];
         const long r = p.rows_out ? p.rows_out[t] : t;
-        store16(static_cast<T*>(p.out[0]) + r * p.ldo + f, left, v);
+        store_run<NE>(static_cast<T*>(p.out[0]) + r * p.ldo + f, left, v);
       } else {
-        float u[16];
-        load16(static_cast<const T*>(p.gate) + (long)t * p.F + f, left, v);
-        load16(static_cast<const T*>(p.up) + (long)t * p.F + f, left, u);
+        float d[NE];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float dh = acc[4 * q + (e >> 2)][j][e & 3];
+        for (int e = 0; e < NE; ++e) d[e] = REDO ? dh[REDO ? GS * q + (e >> 2) : 0][REDO ? j : 0][e & 3] : v[e];
+        if constexpr (!REDO) {
+          load_run<NE>(static_cast<const T*>(p.gate) + (long)t * p.F + f, left, v);
+          load_run<NE>(static_cast<const T*>(p.up) + (long)t * p.F + f, left, u);
+        }
+#pragma unroll
+        for (int e = 0; e < NE; ++e) {
           float slope;
           const float act = activate<true>(p.act, v[e], slope);
-          v[e] = dh * u[e] * slope;
-          u[e] = dh * act;
+          v[e] = d[e] * u[e] * slope;
+          u[e] = d[e] * act;
         }
         T* out = static_cast<T*>(p.out[0]) + (long)t * p.ldo + f;
-        store16(out, left, v);
-        store16(out + p.F, left, u);
+        store_run<NE>(out, left, v);
+        store_run<NE>(out + p.F, left, u);
       }
     }
   }
@@ -290,105 +345,108 @@ __global__ __launch_bounds__(256, 2) void ffn_product(FfnProduct p) {
 // ---------------------------------------------------------------------------
 // Weights' gradients. LDS holds rows of tokens, features along them: 16-bit
 // types read them transposed (ds_read_tr16), float32 element by element. A
-// stage is KT tokens of kOuterM features of a and kOuterN of b: 8 + 16 KB.
-// 32-byte (float32: 64-byte) slices of 16 features are stored in the order
-// slice ^ (row & 7) (float32: ^ (row & 3)), so that the rows of a read pass
-// cover the banks once.
+// stage is 64 tokens (float32: 32) of the tile's M features of a and N of b. 32-byte
+// (float32: 64-byte) slices of 16 features are stored in an order that depends
+// on the row, so that the rows of a read pass cover the banks once.
 // ---------------------------------------------------------------------------
-constexpr int KT = F32 ? 16 : 32;
+constexpr int KT = 128 / ES;
 
-template <int FEATS>
+// One operand's side: FEATS features, loaded by NT threads. MAP: the tokens' rows
+// come from a list, read a stage ahead so that no load waits for it.
+template <int FEATS, int NT, bool MAP>
 struct OuterSide {
-  static constexpr int ROW = FEATS * ES;           // bytes of a token's row
-  static constexpr int PARTS = ROW / 16;           // 16-byte parts of it
-  static constexpr int ROWS_PER_LOAD = 256 / PARTS;
-  static constexpr int LOADS = KT / ROWS_PER_LOAD;
-  static __device__ __forceinline__ int swizzle(int row) { return F32 ? (row & 3) << 2 : (row & 7) << 1; }
+  static constexpr int ROW = FEATS * ES;  // bytes of a token's row
+  static constexpr int PARTS = ROW / 16;
+  static constexpr int LOADS = KT * PARTS / NT;
+  static_assert(KT * PARTS % NT == 0, "whole loads");
 
-  const char* base;        // this lane's part of row 0
+  const char* base[LOADS];  // this lane's part of row 0 in each load
+  unsigned ld[LOADS];       // row stride in bytes; 0 where the features do not exist
+  int r[LOADS];             // its row of the stage
+  int next[MAP ? LOADS : 1];
   const int32_t* rows;
-  long ld;                 // bytes
-  bool in;                 // its features exist
-  int r0;                  // its row of a load
 
-  __device__ __forceinline__ void init(const void* p, const int32_t* map, long ld_elems, int f0, int count, int tid) {
-    r0 = tid / PARTS;
-    // ROWS_PER_LOAD is a multiple of the swizzle's period or the row's low
-    // bits are those of r0 in every load.
-    const int part = (tid % PARTS) ^ swizzle(r0);
-    const int f = f0 + part * kVec<T>;
-    in = f < count;
-    base = static_cast<const char*>(p) + (in ? (long)f * ES : 0);
-    rows = map;
-    ld = ld_elems * ES;
+  // Order of the slices of row r, in 16-byte parts.
+  static __device__ __forceinline__ int swizzle(int r) {
+    return F32 ? (r & 3) << 2 : ROW % 256 ? ((r >> 1) & 3) << 1 : (r & 7) << 1;
   }
-  __device__ __forceinline__ void issue(int t0, int t1, unsigned char* dst, int wave) const {
+  __device__ __forceinline__ void init(const void* p, const int32_t* map, long ld_elems, int f0, int count, int tid) {
+    rows = map;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int t = t0 + i * ROWS_PER_LOAD + r0;
-      const bool ok = in && t < t1;
-      const long r = ok ? (rows ? rows[t] : t) : 0;
-      const char* q = ok ? base + r * ld : reinterpret_cast<const char*>(&kZero16);
-      __builtin_amdgcn_global_load_lds((glb_ptr)q, (lds_ptr)(dst + i * 4096 + wave * 1024), 16, 0, 0);
+      const int at = i * NT + tid;
+      r[i] = at / PARTS;
+      const int f = f0 + ((at % PARTS) ^ swizzle(r[i])) * kVec<T>;
+      const bool in = f < count;
+      base[i] = in ? static_cast<const char*>(p) + (long)f * ES : reinterpret_cast<const char*>(&kZero16);
+      ld[i] = in ? (unsigned)(ld_elems * ES) : 0;
     }
   }
-  // Subtile `sub` (16 features) as a matrix-core operand. 16-bit: tokens 4 g +
-  // .., 16 + 4 g + .. in the lane's eight slots; float32: step e (of four)
-  // holds token 4 e + g.
-  static __device__ __forceinline__ u32x4 frag(const unsigned char* tile, int sub, int g, int n) {
+  __device__ __forceinline__ void prefetch(int t0, int t1) {
+    if constexpr (MAP) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) next[i] = rows[min(t0 + r[i], t1 - 1)];
+    }
+  }
+  __device__ __forceinline__ void issue(int t0, int t1, unsigned char* dst, int wave) const {
+    const bool whole = t0 + KT <= t1;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const unsigned row = MAP ? next[MAP ? i : 0] : t0 + r[i];
+      const char* q = base[i] + (uint64_t)row * ld[i];
+      if (!whole) q = t0 + r[i] < t1 ? q : reinterpret_cast<const char*>(&kZero16);
+      __builtin_amdgcn_global_load_lds((glb_ptr)q, (lds_ptr)(dst + i * NT * 16 + wave * 1024), 16, 0, 0);
+    }
+  }
+  // Subtile `sub` (16 features) of half k of the stage's tokens as a matrix-core
+  // operand. 16-bit: tokens 4 g + .., 16 + 4 g + .. of the half in the lane's
+  // eight slots; float32: step e (of four) holds token 4 e + g.
+  static __device__ __forceinline__ u32x4 frag(const unsigned char* tile, int k, int sub, int g, int n) {
     if constexpr (F32) {
       u32x4 v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int r = 4 * e + g;
-        v[e] = *reinterpret_cast<const unsigned*>(tile + r * ROW + (((sub << 2) ^ swizzle(r)) << 4) + 4 * n);
+        const int r = 16 * k + 4 * e + g;
+        v[e] = *reinterpret_cast<const unsigned*>(tile + r * ROW + (((sub << 2) ^ swizzle(g)) << 4) + 4 * n);
       }
       return v;
     } else {
       typedef short s16x4 __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
       const int r = 4 * g + (n >> 2), at = (((sub << 1) ^ swizzle(r)) << 4) + 8 * (n & 3);
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(tile + r * ROW + at));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(tile + (r + 16) * ROW + at));
+      const unsigned char* p = tile + (32 * k + r) * ROW + at;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)p);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p + 16 * ROW));
       const u32x2 a = __builtin_bit_cast(u32x2, lo), c = __builtin_bit_cast(u32x2, hi);
       return u32x4{a[0], a[1], c[0], c[1]};
     }
   }
 };
 
-__global__ __launch_bounds__(256, 2) void ffn_outer(FfnOuters ps) {
-  typedef OuterSide<kOuterM> SideA;
-  typedef OuterSide<kOuterN> SideB;
-  constexpr int NI = 4, NJ = 8, A_BYTES = KT * SideA::ROW, STAGE = A_BYTES + KT * SideB::ROW;
-  constexpr int LOADS = SideA::LOADS + SideB::LOADS;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[3][STAGE];
-  const int k = (int)blockIdx.x >= ps.first[0];
-  const FfnOuter& p = ps.p[k];
-  const int splits = ps.splits[k];
-  const int nm = (p.M + kOuterM - 1) / kOuterM, nn = (p.N + kOuterN - 1) / kOuterN;
-  int at = (int)blockIdx.x - (k ? ps.first[0] : 0);
+template <int WM, int WN, int NI, int NJ, bool MA, bool MB, int OCC>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void ffn_outer(FfnOuter p) {
+  constexpr int TM = 16 * NI * WM, TN = 16 * NJ * WN, NT = 64 * WM * WN;
+  typedef OuterSide<TM, NT, MA> SideA;
+  typedef OuterSide<TN, NT, MB> SideB;
+  constexpr int A_BYTES = KT * SideA::ROW, STAGE = A_BYTES + KT * SideB::ROW;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2][STAGE];
+  const int nm = (p.M + TM - 1) / TM, nn = (p.N + TN - 1) / TN;
   // Consecutive workgroups of an XCD take the tiles of one run of tokens.
-  const int total = nm * nn * splits, per = (total + 7) >> 3;
-  const int i8 = at >> 3;
-  at = (at & 7) * per + i8;
+  const int total = nm * nn * p.splits, per = (total + 7) >> 3;
+  const int i8 = blockIdx.x >> 3, at = (blockIdx.x & 7) * per + i8;
   if (i8 >= per || at >= total) return;
   const int split = at / (nm * nn), tile = at - split * nm * nn;
-  const int m0 = tile % nm * kOuterM, n0 = tile / nm * kOuterN;
-  const int tokens = ps.count ? *ps.count : ps.tokens;
-  const int run = ((tokens + splits - 1) / splits + KT - 1) / KT * KT;
-  const long ta = min((long)split * run, (long)tokens), tb = min(ta + run, (long)tokens);
-  const int t0 = (int)ta, t1 = (int)tb;
+  const int m0 = tile % nm * TM, n0 = tile / nm * TN;
+  const int tokens = p.count ? *p.count : p.tokens;
+  const int run = ((tokens + p.splits - 1) / p.splits + KT - 1) / KT * KT;
+  const int t0 = (int)min((long)split * run, (long)tokens), t1 = (int)min((long)t0 + run, (long)tokens);
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave & 1, wn = wave >> 1, g = lane >> 4, n = lane & 15;
+  const int wm = wave % WM, wn = wave / WM, g = lane >> 4, n = lane & 15;
   SideA a;
   SideB bb;
   a.init(p.a, p.rows_a, p.lda, m0, p.M, tid);
   bb.init(p.b, p.rows_b, p.ldb, n0, p.N, tid);
-  auto issue = [&](int s, int buf) __attribute__((always_inline)) {
-    a.issue(t0 + s * KT, t1, lds[buf], wave);
-    bb.issue(t0 + s * KT, t1, lds[buf] + A_BYTES, wave);
-  };
   // The bias' gradient: the columns of b against a row of ones, in the first
   // waves of the first tile of m.
   const bool sums = p.bias && m0 == 0 && wm == 0;
@@ -401,30 +459,39 @@ __global__ __launch_bounds__(256, 2) void ffn_outer(FfnOuters ps) {
 #pragma unroll
     for (int i = 0; i < NI; ++i) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const int steps = (t1 - t0 + KT - 1) / KT;
-  if (steps > 0) issue(0, 0);
-  if (steps > 1) issue(1, 1);
+  if (t0 < t1) {
+    a.prefetch(t0, t1);
+    bb.prefetch(t0, t1);
+    a.issue(t0, t1, lds[0], wave);
+    bb.issue(t0, t1, lds[0] + A_BYTES, wave);
+    a.prefetch(t0 + KT, t1);
+    bb.prefetch(t0 + KT, t1);
+  }
   int b = 0;
-  for (int s = 0; s < steps; ++s) {
-    if (s + 1 < steps)
-      stage_wait<LOADS>();
-    else
-      stage_wait<0>();
-    if (s + 2 < steps) issue(s + 2, b == 0 ? 2 : b - 1);
-    u32x4 fa[NI], fb[NJ];
-#pragma unroll
-    for (int i = 0; i < NI; ++i) fa[i] = SideA::frag(lds[b], wm * NI + i, g, n);
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) fb[j] = SideB::frag(lds[b] + A_BYTES, wn * NJ + j, g, n);
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int i = 0; i < NI; ++i) acc[i][j] = Mma<T>::run(fa[i], fb[j], acc[i][j]);
-    if (sums) {
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) sum[j] = Mma<T>::run(ones, fb[j], sum[j]);
+  for (int t = t0; t < t1; t += KT, b ^= 1) {
+    stage_wait<0>();
+    if (t + KT < t1) {
+      a.issue(t + KT, t1, lds[b ^ 1], wave);
+      bb.issue(t + KT, t1, lds[b ^ 1] + A_BYTES, wave);
+      a.prefetch(t + 2 * KT, t1);
+      bb.prefetch(t + 2 * KT, t1);
     }
-    b = b == 2 ? 0 : b + 1;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      u32x4 fa[NI], fb[NJ];
+#pragma unroll
+      for (int i = 0; i < NI; ++i) fa[i] = SideA::frag(lds[b], k, wm * NI + i, g, n);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) fb[j] = SideB::frag(lds[b] + A_BYTES, k, wn * NJ + j, g, n);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int i = 0; i < NI; ++i) acc[i][j] = Mma<T>::run(fa[i], fb[j], acc[i][j]);
+      if (sums) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) sum[j] = Mma<T>::run(ones, fb[j], sum[j]);
+      }
+    }
   }
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
@@ -440,11 +507,34 @@ __global__ __launch_bounds__(256, 2) void ffn_outer(FfnOuters ps) {
   }
 }
 
-template <int MODE, int WF, int WT, int NI, int NJ>
+template <int MODE, int WF, int WT, int NI, int NJ, int OCC>
 void launch(const FfnProduct& p, hipStream_t st) {
   typedef Product<MODE, WF, WT, NI, NJ> C;
   const long tiles = (long)((p.F + C::FEATURES - 1) / C::FEATURES) * ((p.tokens + C::BT - 1) / C::BT);
-  ffn_product<MODE, WF, WT, NI, NJ><<<(unsigned)((tiles + 7) / 8 * 8), 256, 0, st>>>(p);
+  ffn_product<MODE, WF, WT, NI, NJ, OCC><<<(unsigned)((tiles + 7) / 8 * 8), 64 * WF * WT, 0, st>>>(p);
+}
+
+// Whether tiles of `big` features by `bt` tokens, one workgroup a CU, beat tiles
+// of a quarter of the area, two a CU: their rounds over the chip, at the rates
+// the two reach (1.2 and 0.9 PFLOP/s of a full chip in bf16).
+bool big_tiles(const FfnProduct& p, int big, int bt) {
+  auto tiles = [&](int f, int t) { return (long)((p.F + f - 1) / f) * ((p.tokens + t - 1) / t); };
+  const double rb = (double)((tiles(big, bt) + 255) / 256) * big * bt;
+  const double rs = (double)((tiles(big / 2, bt / 2) + 511) / 512) * big * bt / 4 * 2 * 1.33;
+  return rb <= rs;
+}
+
+template <int WM, int WN, int NI, int NJ, int OCC>
+void launch_outer(const FfnOuter& p, hipStream_t st) {
+  constexpr int TM = 16 * NI * WM, TN = 16 * NJ * WN;
+  const int total = p.splits * ((p.M + TM - 1) / TM) * ((p.N + TN - 1) / TN), grid = (total + 7) / 8 * 8;
+  constexpr int NT = 64 * WM * WN;
+  if (p.rows_a)
+    ffn_outer<WM, WN, NI, NJ, true, false, OCC><<<grid, NT, 0, st>>>(p);
+  else if (p.rows_b)
+    ffn_outer<WM, WN, NI, NJ, false, true, OCC><<<grid, NT, 0, st>>>(p);
+  else
+    ffn_outer<WM, WN, NI, NJ, false, false, OCC><<<grid, NT, 0, st>>>(p);
 }
 
 }  // namespace
@@ -453,25 +543,37 @@ void launch(const FfnProduct& p, hipStream_t st) {
 #define FST_CAT(a, b) FST_CAT2(a, b)
 
 int FST_CAT(ffn_product_, FST_NAME)(int mode, const FfnProduct& p, hipStream_t st) {
-  if (mode == kFfnGate)
-    launch<kFfnGate, 2, 2, 8, 4>(p, st);
-  else if (mode == kFfnOut)
-    launch<kFfnOut, 2, 2, 4, 8>(p, st);
-  else
-    launch<kFfnGrad, 2, 2, 4, 8>(p, st);
+  if (mode == kFfnGate) {
+    if (big_tiles(p, 128, 256))
+      launch<kFfnGate, 2, 4, 8, 4, 1>(p, st);
+    else
+      launch<kFfnGate, 2, 2, 4, 4, 2>(p, st);
+  } else if (mode == kFfnOut) {
+    if (big_tiles(p, 256, 256))
+      launch<kFfnOut, 2, 4, 8, 4, 1>(p, st);
+    else
+      launch<kFfnOut, 2, 2, 4, 4, 2>(p, st);
+  } else if constexpr (F32) {
+    if (big_tiles(p, 256, 256))
+      launch<kFfnGrad, 2, 4, 8, 4, 1>(p, st);
+    else
+      launch<kFfnGrad, 2, 2, 4, 4, 2>(p, st);
+  } else {
+    if (big_tiles(p, 128, 192))
+      launch<kFfnRedo, 2, 4, 8, 3, 1>(p, st);
+    else
+      launch<kFfnRedo, 2, 2, 4, 2, 2>(p, st);
+  }
   return hipGetLastError() == hipSuccess ? FST_OK : FST_ELAUNCH;
 }
 
-int FST_CAT(ffn_outer_, FST_NAME)(FfnOuters& ps, hipStream_t st) {
-  int grid = 0;
-  for (int k = 0; k < 2; ++k) {
-    const FfnOuter& p = ps.p[k];
-    const int tiles = ps.splits[k] * ((p.M + kOuterM - 1) / kOuterM) * ((p.N + kOuterN - 1) / kOuterN);
-    grid += (tiles + 7) / 8 * 8;
-    ps.first[k] = grid;
+int FST_CAT(ffn_outer_, FST_NAME)(const FfnOuter& p, int shape, hipStream_t st) {
+  switch (shape) {
+    case 0: launch_outer<2, 2, 4, 4, 2>(p, st); break;
+    case 1: launch_outer<2, 4, 8, 4, 1>(p, st); break;
+    case 2: launch_outer<2, 4, 6, 4, 1>(p, st); break;
+    default: launch_outer<2, 4, 8, 3, 1>(p, st); break;
   }
-  if (grid == 0) return FST_OK;
-  ffn_outer<<<grid, 256, 0, st>>>(ps);
   return hipGetLastError() == hipSuccess ? FST_OK : FST_ELAUNCH;
 }
 

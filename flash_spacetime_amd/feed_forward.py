@@ -30,8 +30,8 @@ def _dense(t: Optional[Tensor]) -> Optional[Tensor]:
 
 
 class _GatedFeedForward(torch.autograd.Function):
-    """Fused forward and deterministic backward; keeps x and, in x's dtype, both
-    projections and the hidden rows."""
+    """Fused forward and deterministic backward; keeps x, the hidden rows and, in
+    float32, both projections (16-bit types form them again, unrounded)."""
 
     @staticmethod
     def forward(ctx: Any, x, w_gate, w_up, w_down, b_gate, b_up, b_down, activation, seqlens):  # type: ignore[override]
@@ -44,7 +44,7 @@ class _GatedFeedForward(torch.autograd.Function):
         like = {"device": x.device, "dtype": x.dtype}
         y = torch.empty(x.shape, **like)
         hidden = torch.empty(b * length, f, **like)
-        gate, up = (torch.empty_like(hidden), torch.empty_like(hidden)) if keep else (None, None)
+        gate, up = (torch.empty_like(hidden), torch.empty_like(hidden)) if keep and dtype == _lib.FST_F32 else (None, None)
         rowmap = None if lens is None else torch.empty(b * length + 1, device=x.device, dtype=torch.int32)
         P = _lib.ptr
         with torch.cuda.device(x.device):
@@ -53,14 +53,14 @@ class _GatedFeedForward(torch.autograd.Function):
                 P(hidden), P(gate), P(up), P(rowmap), P(y), _lib.stream_handle(x.device))
         _lib.check(rc, "flash_gated_feed_forward")
         if keep:
-            ctx.save_for_backward(xr, wg, wu, wd, lens, hidden, gate, up, rowmap)
+            ctx.save_for_backward(xr, wg, wu, wd, bg, bu, lens, hidden, gate, up, rowmap)
             ctx.meta = (dtype, act, b, length, d, f, x_stride, x.shape)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, dy: Tensor):  # type: ignore[override]
-        x, wg, wu, wd, lens, hidden, gate, up, rowmap = ctx.saved_tensors
+        x, wg, wu, wd, bg, bu, lens, hidden, gate, up, rowmap = ctx.saved_tensors
         dtype, act, b, length, d, f, x_stride, shape = ctx.meta
         need = ctx.needs_input_grad[:7]
         like = {"device": x.device, "dtype": x.dtype}
@@ -73,8 +73,8 @@ class _GatedFeedForward(torch.autograd.Function):
         P = _lib.ptr
         with torch.cuda.device(x.device):
             rc = lib.fst_ffn_backward(
-                dtype, act, b, length, d, f, P(x), x_stride, P(wg), P(wu), P(wd), P(lens), P(hidden), P(gate), P(up),
-                P(rowmap), P(dyr), dy_stride, *(P(g) for g in grads), P(ws), nbytes, _lib.stream_handle(x.device))
+                dtype, act, b, length, d, f, P(x), x_stride, P(wg), P(wu), P(wd), P(bg), P(bu), P(lens), P(hidden),
+                P(gate), P(up), P(rowmap), P(dyr), dy_stride, *(P(g) for g in grads), P(ws), nbytes, _lib.stream_handle(x.device))
         _lib.check(rc, "flash_gated_feed_forward backward")
         return (*grads, None, None)
 

@@ -315,11 +315,12 @@ int fst_layer_norm_backward(int dtype, int param_dtype, int B, int L, int N, con
  * dtype and dense, as the biases (b_gate, b_up [F], b_down [D]; each
  * nullable). D and F are multiples of 8, at most 65536, and their product less
  * than 2^28; every pointer, and the row strides of x and dy in bytes, are
- * multiples of 16.
- * hidden [B * L, F] receives h, and gate, up of the same size (both or neither;
- * the backward needs them) a and u, rounded to dtype; with seqlens the rows
- * of all three are the valid tokens in order, and rowmap (B * L + 1 ints, needed
- * with seqlens, else unused) receives their number and their rows. */
+ * multiples of 16 (and less than 2^32).
+ * hidden [B * L, F] receives h, rounded to dtype. gate, up of the same size (FST_F32
+ * only, both or null; its backward needs them) receive a and u: the 16-bit
+ * types' backward forms them again, unrounded. With seqlens the rows of all
+ * three are the valid tokens in order, and rowmap (B * L + 1 ints, needed with
+ * seqlens, else unused) receives their number and their rows. */
 int fst_ffn_forward(int dtype, int activation, int B, int L, int D, int F, const void* x, int64_t x_stride,
                     const void* w_gate, const void* w_up, const void* w_down, const void* b_gate, const void* b_up,
                     const void* b_down, const int32_t* seqlens, void* hidden, void* gate, void* up, int32_t* rowmap,
@@ -331,10 +332,11 @@ size_t fst_ffn_backward_workspace_bytes(int dtype, int B, int L, int D, int F);
 /* The gradients, from the forward's operands, its hidden, gate, up and rowmap,
  * and dy. Each gradient is nullable. */
 int fst_ffn_backward(int dtype, int activation, int B, int L, int D, int F, const void* x, int64_t x_stride,
-                     const void* w_gate, const void* w_up, const void* w_down, const int32_t* seqlens,
-                     const void* hidden, const void* gate, const void* up, const int32_t* rowmap, const void* dy,
-                     int64_t dy_stride, void* dx, void* dw_gate, void* dw_up, void* dw_down, void* db_gate,
-                     void* db_up, void* db_down, void* workspace, size_t workspace_bytes, void* stream);
+                     const void* w_gate, const void* w_up, const void* w_down, const void* b_gate, const void* b_up,
+                     const int32_t* seqlens, const void* hidden, const void* gate, const void* up,
+                     const int32_t* rowmap, const void* dy, int64_t dy_stride, void* dx, void* dw_gate, void* dw_up,
+                     void* dw_down, void* db_gate, void* db_up, void* db_down, void* workspace,
+                     size_t workspace_bytes, void* stream);
 
 /* The fp32 frequency ladder exp(-i ln(1e4) / (C/2)), i < C/2, that the kernels
  * embed with, written to out[0 .. C/2). Counterpart of sinusoidal_frequencies

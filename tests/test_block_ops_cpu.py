@@ -78,17 +78,20 @@ def test_feed_forward_refusals():
     assert fwd(d=32768, f=8192, xs=32768) == _lib.FST_EUNSUPPORTED and "elements" in _lib.last_error()
     assert fwd(b=65536, l=32768) == _lib.FST_EUNSUPPORTED and "rows" in _lib.last_error()
     assert fwd(xs=8) == _lib.FST_EINVAL and "stride" in _lib.last_error()
+    assert fwd(xs=1 << 31) == _lib.FST_EINVAL and "stride" in _lib.last_error()
     assert fwd(xs=20) == _lib.FST_EINVAL and "stride" in _lib.last_error()
     assert fwd(x=8) == _lib.FST_EINVAL and "16 bytes" in _lib.last_error()
     assert fwd(wg=None) == _lib.FST_EINVAL and "null" in _lib.last_error()
-    assert fwd(gate=16) == _lib.FST_EINVAL and fwd(lens=16) == _lib.FST_EINVAL and "null" in _lib.last_error()
+    assert fwd(gate=16, up=16) == _lib.FST_EINVAL and "float32" in _lib.last_error()
+    assert fwd(dt=1, gate=16) == _lib.FST_EINVAL and fwd(lens=16) == _lib.FST_EINVAL and "null" in _lib.last_error()
     assert fwd(b=0) == _lib.FST_OK
 
-    def bwd(ws=16, nbytes=1 << 40, dy=16, dys=16, dx=16, dw=16):
-        return lib.fst_ffn_backward(0, 0, 2, 3, 16, 32, 16, 16, 16, 16, 16, None, 16, 16, 16, None, dy, dys, dx, dw, None,
-                                    None, None, None, None, ws, nbytes, None)
+    def bwd(ws=16, nbytes=1 << 40, dy=16, dys=16, dx=16, dw=16, dt=0):
+        return lib.fst_ffn_backward(dt, 0, 2, 3, 16, 32, 16, 16, 16, 16, 16, None, None, None, 16, None, None, None, dy, dys,
+                                    dx, dw, None, None, None, None, None, ws, nbytes, None)
 
     assert bwd(dy=None) == _lib.FST_EINVAL and "null" in _lib.last_error()
+    assert bwd(dt=1) == _lib.FST_EINVAL and "null" in _lib.last_error()  # float32 needs gate and up
     assert bwd(dys=12) == _lib.FST_EINVAL and "stride" in _lib.last_error()
     assert bwd(dx=8) == _lib.FST_EINVAL and "16 bytes" in _lib.last_error()
     need = lib.fst_ffn_backward_workspace_bytes(0, 2, 3, 16, 32)
