@@ -48,21 +48,18 @@ struct FfnOuter {
 };
 
 typedef int (*ffn_product_fn)(int mode, const FfnProduct&, hipStream_t);
-typedef int (*ffn_outer_fn)(const FfnOuter&, int shape, hipStream_t);
+typedef int (*ffn_outer_fn)(const FfnOuter&, bool large, hipStream_t);
 
 #define FST_FFN_DECL(name)                                      \
   int ffn_product_##name(int mode, const FfnProduct&, hipStream_t); \
-  int ffn_outer_##name(const FfnOuter&, int shape, hipStream_t);
+  int ffn_outer_##name(const FfnOuter&, bool large, hipStream_t);
 FST_FFN_DECL(bf16)
 FST_FFN_DECL(f16)
 FST_FFN_DECL(f32)
 #undef FST_FFN_DECL
 
-// Tiles of an outer product (shape of ffn_outer_*): M and N of a workgroup, and
-// workgroups a CU holds.
-struct OuterTile {
-  int m, n, per_cu;
-};
-constexpr OuterTile kOuterTiles[] = {{128, 128, 2}, {256, 256, 1}, {192, 256, 1}, {256, 192, 1}};
+// Tile of an outer product: features of M and of N a workgroup takes; two small
+// ones or one large one a CU.
+constexpr int kOuterSmall = 128, kOuterLarge = 256;
 
 }  // namespace fst

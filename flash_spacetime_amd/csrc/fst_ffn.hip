@@ -152,23 +152,27 @@ void launch_rows(const int32_t* seqlens, int B, int L, int32_t* map, void* out, 
 }
 
 // Tile and token runs of a weight's gradient [N, M]: the least of the rounds of
-// workgroups over the chip at the tiles' rates (PFLOP/s of a full chip measured:
-// bf16 1.0 and, in the small tiles, 0.8) plus the runs' partials written and read.
+// workgroups over the chip, at the rates of large and small tiles (a full chip in
+// bf16: 65536 tokens, M = 1024, N = 5504 920 against 1003 us; M = 2752, N = 1024
+// 474 / 538), plus the runs' partials written and read. float32 is as fast in
+// small tiles and has only those.
 struct OuterPlan {
-  int shape, splits;
+  bool large;
+  int splits;
 };
 
 OuterPlan plan_outer(int dtype, long tokens, int M, int N) {
-  OuterPlan best{0, 1};
-  double least = 0;
-  for (int k = 0; k < 4; ++k) {
-    const OuterTile& o = kOuterTiles[k];
-    const long tiles = (long)((M + o.m - 1) / o.m) * ((N + o.n - 1) / o.n), slots = 256l * o.per_cu;
-    const double rate = (dtype == FST_F32 ? 0.12e15 : k ? 1.0e15 : 0.8e15) / slots;
+  OuterPlan best{false, 1};
+  double least = -1;
+  for (const bool large : {false, true}) {
+    if (large && dtype == FST_F32) continue;
+    const int e = large ? kOuterLarge : kOuterSmall;
+    const long tiles = (long)((M + e - 1) / e) * ((N + e - 1) / e), slots = large ? 256 : 512;
+    const double rate = (dtype == FST_F32 ? 0.12e15 : large ? 0.8e15 : 0.72e15) / slots;
     for (int s = 1; s <= 64 && (s == 1 || s * 256l <= tokens); ++s) {
-      const double work = (double)tokens / s * 2 * o.m * o.n / rate;
+      const double work = (double)tokens / s * 2 * e * e / rate;
       const double t = (double)((tiles * s + slots - 1) / slots) * work + s * 8.0 * M * N / 4e12;
-      if ((k == 0 && s == 1) || t < least) best = OuterPlan{k, s}, least = t;
+      if (least < 0 || t < least) best = OuterPlan{large, s}, least = t;
     }
   }
   return best;
@@ -373,7 +377,7 @@ int fst_ffn_backward(int dtype, int activation, int B, int L, int D, int F, cons
       o.splits = l.first.splits;
       o.part = p0;
       o.bias = db_gate || db_up ? b0 : nullptr;
-      rc = outer_of(dtype)(o, l.first.shape, st);
+      rc = outer_of(dtype)(o, l.first.large, st);
     }
     if (second && rc == FST_OK) {
       o.a = hidden;
@@ -387,7 +391,7 @@ int fst_ffn_backward(int dtype, int activation, int B, int L, int D, int F, cons
       o.splits = l.second.splits;
       o.part = p1;
       o.bias = db_down ? b1 : nullptr;
-      rc = outer_of(dtype)(o, l.second.shape, st);
+      rc = outer_of(dtype)(o, l.second.large, st);
     }
     if (rc != FST_OK) return fail(rc, "feed-forward weight gradient launch failed");
     const long df = (long)D * F;

@@ -514,14 +514,23 @@ void launch(const FfnProduct& p, hipStream_t st) {
   ffn_product<MODE, WF, WT, NI, NJ, OCC><<<(unsigned)((tiles + 7) / 8 * 8), 64 * WF * WT, 0, st>>>(p);
 }
 
-// Whether tiles of `big` features by `bt` tokens, one workgroup a CU, beat tiles
-// of a quarter of the area, two a CU: their rounds over the chip, at the rates
-// the two reach (1.2 and 0.9 PFLOP/s of a full chip in bf16).
-bool big_tiles(const FfnProduct& p, int big, int bt) {
-  auto tiles = [&](int f, int t) { return (long)((p.F + f - 1) / f) * ((p.tokens + t - 1) / t); };
-  const double rb = (double)((tiles(big, bt) + 255) / 256) * big * bt;
-  const double rs = (double)((tiles(big / 2, bt / 2) + 511) / 512) * big * bt / 4 * 2 * 1.33;
-  return rb <= rs;
+// Whether tiles of `f` features by `t` tokens, one workgroup a CU, beat tiles of a
+// quarter of the area, two a CU: their rounds over the chip. A full chip of small
+// tiles takes 1.05 to 1.2 times as long as one of large ones in 16-bit types
+// (65536 tokens, D = 1024, F = 2752 bf16: gate 761 against 706 us, output 365 / 308;
+// 100500 tokens, D = 384, F = 1024: gate 250 / 236, output 107 / 128 us, where
+// three large tiles take two rounds' time); float32, bound by the matrix cores, is
+// as fast in small ones and runs only those.
+bool large_tiles(const FfnProduct& p, int f, int t) {
+  auto tiles = [&](int ff, int tt) { return (long)((p.F + ff - 1) / ff) * ((p.tokens + tt - 1) / tt); };
+  const double large = (double)((tiles(f, t) + 255) / 256) * f * t;
+  const double small = (double)((tiles(f / 2, t / 2) + 511) / 512) * (f / 2) * (t / 2) * 2 * 1.15;
+  return large <= small;
+}
+
+template <int MODE>
+void launch_small(const FfnProduct& p, hipStream_t st) {
+  launch<MODE, 2, 2, 4, MODE == kFfnRedo ? 2 : 4, 2>(p, st);
 }
 
 template <int WM, int WN, int NI, int NJ, int OCC>
@@ -543,37 +552,37 @@ void launch_outer(const FfnOuter& p, hipStream_t st) {
 #define FST_CAT(a, b) FST_CAT2(a, b)
 
 int FST_CAT(ffn_product_, FST_NAME)(int mode, const FfnProduct& p, hipStream_t st) {
-  if (mode == kFfnGate) {
-    if (big_tiles(p, 128, 256))
+  if constexpr (F32) {
+    if (mode == kFfnGate)
+      launch_small<kFfnGate>(p, st);
+    else if (mode == kFfnOut)
+      launch_small<kFfnOut>(p, st);
+    else
+      launch_small<kFfnGrad>(p, st);
+  } else if (mode == kFfnGate) {
+    if (large_tiles(p, 128, 256))
       launch<kFfnGate, 2, 4, 8, 4, 1>(p, st);
     else
-      launch<kFfnGate, 2, 2, 4, 4, 2>(p, st);
+      launch_small<kFfnGate>(p, st);
   } else if (mode == kFfnOut) {
-    if (big_tiles(p, 256, 256))
+    if (large_tiles(p, 256, 256))
       launch<kFfnOut, 2, 4, 8, 4, 1>(p, st);
     else
-      launch<kFfnOut, 2, 2, 4, 4, 2>(p, st);
-  } else if constexpr (F32) {
-    if (big_tiles(p, 256, 256))
-      launch<kFfnGrad, 2, 4, 8, 4, 1>(p, st);
-    else
-      launch<kFfnGrad, 2, 2, 4, 4, 2>(p, st);
+      launch_small<kFfnOut>(p, st);
   } else {
-    if (big_tiles(p, 128, 192))
+    if (large_tiles(p, 128, 192))
       launch<kFfnRedo, 2, 4, 8, 3, 1>(p, st);
     else
-      launch<kFfnRedo, 2, 2, 4, 2, 2>(p, st);
+      launch_small<kFfnRedo>(p, st);
   }
   return hipGetLastError() == hipSuccess ? FST_OK : FST_ELAUNCH;
 }
 
-int FST_CAT(ffn_outer_, FST_NAME)(const FfnOuter& p, int shape, hipStream_t st) {
-  switch (shape) {
-    case 0: launch_outer<2, 2, 4, 4, 2>(p, st); break;
-    case 1: launch_outer<2, 4, 8, 4, 1>(p, st); break;
-    case 2: launch_outer<2, 4, 6, 4, 1>(p, st); break;
-    default: launch_outer<2, 4, 8, 3, 1>(p, st); break;
+int FST_CAT(ffn_outer_, FST_NAME)(const FfnOuter& p, bool large, hipStream_t st) {
+  if constexpr (!F32) {
+    if (large) launch_outer<2, 4, 8, 4, 1>(p, st);
   }
+  if (F32 || !large) launch_outer<2, 2, 4, 4, 2>(p, st);
   return hipGetLastError() == hipSuccess ? FST_OK : FST_ELAUNCH;
 }
 
