@@ -75,60 +75,75 @@ __device__ __forceinline__ float group_sum(float x, float* red) {
   return x;
 }
 
-// Lane l's pieces of a row: elements (l + LPR i) V .. + V - 1, i < NC. EDGE:
-// the row's length is no whole number of pieces or rows start off 16 bytes;
-// pieces are then read at element alignment and the last one by elements.
-template <typename T, bool EDGE>
-__device__ __forceinline__ void load_piece(const T* row, int c, int n, float* v) {
-  constexpr int V = kVec<T>;
-  if constexpr (!EDGE) {
-    if (c < n) {
-      const typename Piece<T>::V p = *reinterpret_cast<const typename Piece<T>::V*>(row + c);
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = (float)p[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = 0.f;
-    }
-  } else {
-    if (c + V <= n) {
-      const typename Piece<T>::V p = *reinterpret_cast<const typename Piece<T>::VU*>(row + c);
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = (float)p[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = c + i < n ? (float)row[c + i] : 0.f;
-    }
-  }
-}
+// Lane l's pieces of a row: elements (l + LPR i) V .. + V - 1, i < NC, zeros past
+// its end. EDGE: the row's length is no whole number of pieces or rows start
+// off 16 bytes; pieces are then read at element alignment and the last one by
+// elements.
+template <typename T, int LPR, int NC, bool EDGE>
+struct Pieces {
+  static constexpr int V = kVec<T>, E = NC * V;
+  typename Piece<T>::V p[NC];
 
-template <typename T, bool EDGE>
-__device__ __forceinline__ void store_piece(T* row, int c, int n, const float* v) {
-  constexpr int V = kVec<T>;
-  const typename Piece<T>::V p = pack_piece<T>(v);
-  if constexpr (!EDGE) {
-    if (c < n) *reinterpret_cast<typename Piece<T>::V*>(row + c) = p;
-  } else {
-    if (c + V <= n) {
-      *reinterpret_cast<typename Piece<T>::VU*>(row + c) = p;
-    } else {
+  static __device__ __forceinline__ int at(int l, int i) { return (l + LPR * i) * V; }
+  __device__ __forceinline__ void load(const T* row, int l, int n) {
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (c + i < n) row[c + i] = p[i];
+    for (int i = 0; i < NC; ++i) {
+      const int c = at(l, i);
+      if (EDGE ? c + V <= n : c < n) {
+        p[i] = EDGE ? *reinterpret_cast<const typename Piece<T>::VU*>(row + c)
+                    : *reinterpret_cast<const typename Piece<T>::V*>(row + c);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) p[i][j] = EDGE && c + j < n ? row[c + j] : (T)0.f;
+      }
     }
   }
-}
+  __device__ __forceinline__ void get(float* v) const {
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = (float)p[i / V][i % V];
+  }
+  static __device__ __forceinline__ void store(T* row, int l, int n, const float* v) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = at(l, i);
+      const typename Piece<T>::V q = pack_piece<T>(v + i * V);
+      if (EDGE ? c + V <= n : c < n) {
+        if constexpr (EDGE)
+          *reinterpret_cast<typename Piece<T>::VU*>(row + c) = q;
+        else
+          *reinterpret_cast<typename Piece<T>::V*>(row + c) = q;
+      } else if (EDGE) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (c + j < n) row[c + j] = q[j];
+      }
+    }
+  }
+};
 
 // Parameters may be float32 or of the rows' type; null stands for `fill`.
+// Elements past the row's end are 0. Whole pieces come in 16-byte loads (by
+// elements, a workgroup's first microseconds were these loads: one event of 187
+// rows of 384 took 8.0 us).
 template <typename T>
 __device__ __forceinline__ void load_param(const void* p, bool f32, int c, int n, float fill, float* v) {
   constexpr int V = kVec<T>;
+  typedef f32x4 f32x4u __attribute__((aligned(4)));
+  if (!p || c + V > n) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const int k = c + i;
-    v[i] = (k >= n || !p) ? (k < n ? fill : 0.f)
-           : f32          ? static_cast<const float*>(p)[k]
-                          : (float)static_cast<const T*>(p)[k];
+    for (int i = 0; i < V; ++i)
+      v[i] = c + i >= n ? 0.f : !p ? fill : f32 ? static_cast<const float*>(p)[c + i] : (float)static_cast<const T*>(p)[c + i];
+  } else if (f32) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      const f32x4 q = *reinterpret_cast<const f32x4u*>(static_cast<const float*>(p) + c + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i + j] = q[j];
+    }
+  } else {
+    const typename Piece<T>::V q = *reinterpret_cast<const typename Piece<T>::VU*>(static_cast<const T*>(p) + c);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = (float)q[i];
   }
 }
 
@@ -138,138 +153,154 @@ __device__ __forceinline__ bool row_valid(const int32_t* lens, long row, int L) 
   return (int)((unsigned)row - b * (unsigned)L) < event_len(lens, (int)b, L);
 }
 
+// Both kernels walk the rows a group at a time, with the next row's pieces in
+// flight while a row is worked on, and the length that says whether the row after
+// it is a token before those.
 template <typename T, int LPR, int NC, bool EDGE>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_fwd(NormArgs a, int w_f32) {
-  constexpr int V = kVec<T>, NT = LPR > 256 ? LPR : 256, G = NT / LPR;
+  typedef Pieces<T, LPR, NC, EDGE> P;
+  constexpr int V = P::V, E = P::E, NT = LPR > 256 ? LPR : 256, G = NT / LPR;
   __shared__ float red[LPR > 64 ? LPR / 64 : 1];
   const int l = threadIdx.x % LPR, grp = threadIdx.x / LPR;
   const int n = a.n;
   const float inv_n = 1.f / (float)n;
-  float w[NC * V], b[NC * V];
+  const long step = (long)gridDim.x * G;
+  long row = (long)blockIdx.x * G + grp;
+  auto is_token = [&](long r) { return r < a.rows && row_valid(a.lens, r, a.L); };
+  P x0, x1, r0, r1;
+  auto fetch = [&](long r, P& x, P& q) {
+    x.load(static_cast<const T*>(a.x) + r * a.ldx, l, n);
+    if (a.r) q.load(static_cast<const T*>(a.r) + r * a.ldr, l, n);
+  };
+  bool now = is_token(row), next = is_token(row + step);
+  if (now) fetch(row, x0, r0);
+  float w[E], b[E];
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
-    const int c = (l + LPR * i) * V;
-    load_param<T>(a.w, w_f32, c, n, 1.f, w + i * V);
-    load_param<T>(a.b, w_f32, c, n, 0.f, b + i * V);
+    load_param<T>(a.w, w_f32, P::at(l, i), n, 1.f, w + i * V);
+    load_param<T>(a.b, w_f32, P::at(l, i), n, 0.f, b + i * V);
   }
-  for (long row = (long)blockIdx.x * G + grp; row < a.rows; row += (long)gridDim.x * G) {
+  for (; row < a.rows; row += step) {
+    const bool later = is_token(row + 2 * step);
+    if (next) fetch(row + step, x1, r1);
     T* y = static_cast<T*>(a.y) + row * n;
     T* so = static_cast<T*>(a.s) + row * n;
-    float v[NC * V];
-    if (!row_valid(a.lens, row, a.L)) {
+    float v[E];
+    float2 st = make_float2(0.f, 0.f);
+    if (now) {
+      x0.get(v);
+      if (a.r) {
+        float q[E];
+        r0.get(q);
+        // The norm is of the sum as it is returned, so that the backward, which
+        // has only that, differentiates the same function.
 #pragma unroll
-      for (int i = 0; i < NC * V; ++i) v[i] = 0.f;
-#pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const int c = (l + LPR * i) * V;
-        store_piece<T, EDGE>(y, c, n, v + i * V);
-        if (a.r) store_piece<T, EDGE>(so, c, n, v + i * V);
+        for (int i = 0; i < E; ++i) v[i] = (float)(T)(v[i] + q[i]);
+        P::store(so, l, n, v);
       }
-      if (a.stats && l == 0) a.stats[row] = make_float2(0.f, 0.f);
-      continue;
-    }
-    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+      float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < NC; ++i) load_piece<T, EDGE>(x, (l + LPR * i) * V, n, v + i * V);
-    if (a.r) {
-      const T* r = static_cast<const T*>(a.r) + row * a.ldr;
-      float q[NC * V];
+      for (int i = 0; i < E; ++i) sum += v[i];
+      const float m = group_sum<LPR>(sum, red) * inv_n;
+      // Second pass in registers: the deviations' own mean corrects m's rounding
+      // (rows whose mean is large beside their spread), their squares give the
+      // variance.
+      float d1 = 0.f, d2 = 0.f;
 #pragma unroll
-      for (int i = 0; i < NC; ++i) load_piece<T, EDGE>(r, (l + LPR * i) * V, n, q + i * V);
-      // The norm is of the sum as it is returned, so that the backward, which
-      // has only that, differentiates the same function.
-#pragma unroll
-      for (int i = 0; i < NC * V; ++i) v[i] = (float)(T)(v[i] + q[i]);
-#pragma unroll
-      for (int i = 0; i < NC; ++i) store_piece<T, EDGE>(so, (l + LPR * i) * V, n, v + i * V);
-    }
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < NC * V; ++i) sum += v[i];
-    const float m = group_sum<LPR>(sum, red) * inv_n;
-    // Second pass in registers: the deviations' own mean corrects m's rounding
-    // (rows whose mean is large beside their spread), their squares give the
-    // variance.
-    float d1 = 0.f, d2 = 0.f;
-#pragma unroll
-    for (int i = 0; i < NC; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float d = (l + LPR * i) * V + j < n ? v[i * V + j] - m : 0.f;
-        v[i * V + j] = d;
+      for (int i = 0; i < E; ++i) {
+        const float d = P::at(l, i / V) + i % V < n ? v[i] - m : 0.f;
+        v[i] = d;
         d1 += d;
         d2 = fmaf(d, d, d2);
       }
-    d1 = group_sum<LPR>(d1, red) * inv_n;
-    d2 = group_sum<LPR>(d2, red) * inv_n;
-    const float var = fmaxf(fmaf(-d1, d1, d2), 0.f);
-    const float rstd = 1.f / sqrtf(var + a.eps);
+      d1 = group_sum<LPR>(d1, red) * inv_n;
+      d2 = group_sum<LPR>(d2, red) * inv_n;
+      const float rstd = 1.f / sqrtf(fmaxf(fmaf(-d1, d1, d2), 0.f) + a.eps);
+      st = make_float2(m + d1, rstd);
 #pragma unroll
-    for (int i = 0; i < NC * V; ++i) v[i] = fmaf((v[i] - d1) * rstd, w[i], b[i]);
+      for (int i = 0; i < E; ++i) v[i] = fmaf((v[i] - d1) * rstd, w[i], b[i]);
+    } else {
 #pragma unroll
-    for (int i = 0; i < NC; ++i) store_piece<T, EDGE>(y, (l + LPR * i) * V, n, v + i * V);
-    if (a.stats && l == 0) a.stats[row] = make_float2(m + d1, rstd);
+      for (int i = 0; i < E; ++i) v[i] = 0.f;
+      if (a.r) P::store(so, l, n, v);
+    }
+    P::store(y, l, n, v);
+    if (a.stats && l == 0) a.stats[row] = st;
+    x0 = x1;
+    r0 = r1;
+    now = next;
+    next = later;
   }
 }
 
 template <typename T, int LPR, int NC, bool EDGE>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_bwd(NormGradArgs a, int w_f32) {
-  constexpr int V = kVec<T>, NT = LPR > 256 ? LPR : 256, G = NT / LPR, E = NC * V;
+  typedef Pieces<T, LPR, NC, EDGE> P;
+  constexpr int V = P::V, E = P::E, NT = LPR > 256 ? LPR : 256, G = NT / LPR;
   __shared__ float red[LPR > 64 ? LPR / 64 : 1];
   // Partial sums of the workgroup's row groups (G > 1): [G][E][LPR].
   __shared__ float acc[G > 1 ? NT * E : 1];
   const int l = threadIdx.x % LPR, grp = threadIdx.x / LPR;
   const int n = a.n;
   const float inv_n = 1.f / (float)n;
+  const long step = (long)gridDim.x * G;
+  long row = (long)blockIdx.x * G + grp;
+  auto is_token = [&](long r) { return r < a.rows && row_valid(a.lens, r, a.L); };
+  struct Row {
+    P s, dy, ds;
+    float2 st;
+  } r0, r1;
+  auto fetch = [&](long r, Row& q) {
+    q.st = a.stats[r];
+    q.s.load(static_cast<const T*>(a.s) + r * a.lds_, l, n);
+    q.dy.load(static_cast<const T*>(a.dy) + r * a.lddy, l, n);
+    if (a.ds) q.ds.load(static_cast<const T*>(a.ds) + r * a.ldds, l, n);
+  };
+  bool now = is_token(row), next = is_token(row + step);
+  if (now) fetch(row, r0);
   float w[E], dw[E], db[E];
 #pragma unroll
-  for (int i = 0; i < NC; ++i) load_param<T>(a.w, w_f32, (l + LPR * i) * V, n, 1.f, w + i * V);
+  for (int i = 0; i < NC; ++i) load_param<T>(a.w, w_f32, P::at(l, i), n, 1.f, w + i * V);
 #pragma unroll
   for (int i = 0; i < E; ++i) dw[i] = db[i] = 0.f;
-  for (long row = (long)blockIdx.x * G + grp; row < a.rows; row += (long)gridDim.x * G) {
-    T* dx = static_cast<T*>(a.dx) + row * n;
-    if (!row_valid(a.lens, row, a.L)) {
-      float z[V];
+  for (; row < a.rows; row += step) {
+    const bool later = is_token(row + 2 * step);
+    if (next) fetch(row + step, r1);
+    float g[E];
+    if (now) {
+      float v[E];
+      r0.s.get(v);
+      r0.dy.get(g);
+      const float2 st = r0.st;
+      float c1 = 0.f, c2 = 0.f;
 #pragma unroll
-      for (int i = 0; i < V; ++i) z[i] = 0.f;
-      if (a.dx) {
-#pragma unroll
-        for (int i = 0; i < NC; ++i) store_piece<T, EDGE>(dx, (l + LPR * i) * V, n, z);
+      for (int i = 0; i < E; ++i) {
+        v[i] = (v[i] - st.x) * st.y;  // xhat; past the row's end its dy is 0
+        dw[i] = fmaf(g[i], v[i], dw[i]);
+        db[i] += g[i];
+        g[i] *= w[i];
+        c1 += g[i];
+        c2 = fmaf(g[i], v[i], c2);
       }
-      continue;
+      if (a.dx) {
+        c1 = group_sum<LPR>(c1, red) * inv_n;
+        c2 = group_sum<LPR>(c2, red) * inv_n;
+#pragma unroll
+        for (int i = 0; i < E; ++i) g[i] = st.y * (g[i] - c1 - v[i] * c2);
+        if (a.ds) {
+          r0.ds.get(v);
+#pragma unroll
+          for (int i = 0; i < E; ++i) g[i] += v[i];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) g[i] = 0.f;
     }
-    const T* s = static_cast<const T*>(a.s) + row * a.lds_;
-    const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
-    float v[E], g[E];
-#pragma unroll
-    for (int i = 0; i < NC; ++i) load_piece<T, EDGE>(s, (l + LPR * i) * V, n, v + i * V);
-#pragma unroll
-    for (int i = 0; i < NC; ++i) load_piece<T, EDGE>(dy, (l + LPR * i) * V, n, g + i * V);
-    const float2 st = a.stats[row];
-    float c1 = 0.f, c2 = 0.f;
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      v[i] = (v[i] - st.x) * st.y;  // xhat; past the row's end its dy is 0
-      dw[i] = fmaf(g[i], v[i], dw[i]);
-      db[i] += g[i];
-      g[i] *= w[i];
-      c1 += g[i];
-      c2 = fmaf(g[i], v[i], c2);
-    }
-    if (!a.dx) continue;
-    c1 = group_sum<LPR>(c1, red) * inv_n;
-    c2 = group_sum<LPR>(c2, red) * inv_n;
-#pragma unroll
-    for (int i = 0; i < E; ++i) g[i] = st.y * (g[i] - c1 - v[i] * c2);
-    if (a.ds) {
-      const T* ds = static_cast<const T*>(a.ds) + row * a.ldds;
-#pragma unroll
-      for (int i = 0; i < NC; ++i) load_piece<T, EDGE>(ds, (l + LPR * i) * V, n, v + i * V);
-#pragma unroll
-      for (int i = 0; i < E; ++i) g[i] += v[i];
-    }
-#pragma unroll
-    for (int i = 0; i < NC; ++i) store_piece<T, EDGE>(dx, (l + LPR * i) * V, n, g + i * V);
+    if (a.dx) P::store(static_cast<T*>(a.dx) + row * n, l, n, g);
+    r0 = r1;
+    now = next;
+    next = later;
   }
   if (!a.part) return;
   float* out = a.part + (long)blockIdx.x * 2 * n;
@@ -299,22 +330,32 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_bwd(NormGradArgs a
   }
 }
 
-// dw | db = the column sums of part [blocks][2 n], in a fixed order: 16
-// columns a workgroup, 16 threads a column.
+// dw | db = the column sums of part [blocks][2 n], in a fixed order: 32 columns a
+// workgroup, 32 threads a column, eight loads of each in flight.
 template <typename T>
-__global__ __launch_bounds__(256) void norm_grad_sum(const float* part, int blocks, int n, void* dw, void* db,
-                                                     int w_f32) {
-  __shared__ float red[16][17];
-  const int c = threadIdx.x & 15, k = threadIdx.x >> 4;
-  const int col = blockIdx.x * 16 + c;
+__global__ __launch_bounds__(1024) void norm_grad_sum(const float* part, int blocks, int n, void* dw, void* db,
+                                                      int w_f32) {
+  __shared__ float red[32][33];
+  const int c = threadIdx.x & 31, k = threadIdx.x >> 5;
+  const int col = blockIdx.x * 32 + c;
   float sum = 0.f;
-  if (col < 2 * n)
-    for (int i = k; i < blocks; i += 16) sum += part[(long)i * 2 * n + col];
+  if (col < 2 * n) {
+    const float* in = part + col;
+    int i = k;
+    for (; i + 224 < blocks; i += 256) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = in[(long)(i + 32 * j) * 2 * n];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum += v[j];
+    }
+    for (; i < blocks; i += 32) sum += in[(long)i * 2 * n];
+  }
   red[k][c] = sum;
   __syncthreads();
   if (k == 0 && col < 2 * n) {
 #pragma unroll
-    for (int i = 1; i < 16; ++i) sum += red[i][c];
+    for (int i = 1; i < 32; ++i) sum += red[i][c];
     void* out = col < n ? dw : db;
     const int at = col < n ? col : col - n;
     if (out) {
@@ -327,8 +368,11 @@ __global__ __launch_bounds__(256) void norm_grad_sum(const float* part, int bloc
 }
 
 // The lanes a row takes: the fewest whose share is at most three 16-byte
-// pieces a lane (four in float32: half as many elements), which the backward
-// holds six times over (s, dy, w, dw, db and what is loaded) without spilling.
+// pieces a lane (four in float32: half as many elements), of which the backward
+// holds s, dy, w, dw, db and the next row's three without spilling (but for
+// float32 rows of more than 8192). Fewer lanes leave fewer idle: 256 x 768 rows
+// of 384 bf16, padded, by 16 / 32 / 64 lanes: forward 96 / 99 / 106 us, backward
+// 97 / 123 / 182.
 struct NormPlan {
   int lpr, nc;
   bool edge;
@@ -358,7 +402,11 @@ bool plan_norm(int dtype, int n, NormPlan& p) {
   return false;
 }
 
-constexpr int kNormBlocks = 512;  // workgroups of the backward, each with one partial of dw and db
+// Most workgroups. The forward's stay at work on rows of their own (one a row
+// group had taken 2 to 5 times as long: each loads the parameters). The
+// backward's each write one partial of dw and db; two a CU keep enough rows in
+// flight (768 or 1024 are slower by what the partials cost).
+constexpr int kNormForward = 2048, kNormBlocks = 512;
 
 int norm_rows_per_block(const NormPlan& p) { return p.lpr > 256 ? 1 : 256 / p.lpr; }
 
@@ -371,7 +419,7 @@ bool aligned16(const void* p, long ld, size_t es) { return reinterpret_cast<uint
 
 template <typename T>
 void launch_fwd(const NormPlan& p, const NormArgs& a, int w_f32, hipStream_t st) {
-  const int blocks = norm_blocks(p, a.rows, 2048), threads = p.lpr > 256 ? p.lpr : 256;
+  const int blocks = norm_blocks(p, a.rows, kNormForward), threads = p.lpr > 256 ? p.lpr : 256;
 #define FST_CASE(L, C)                                                                   \
   if constexpr (planned<T>(L, C)) {                                                      \
     if (p.lpr == L && p.nc == C) {                                                        \
@@ -506,13 +554,13 @@ int fst_layer_norm_backward(int dtype, int param_dtype, int B, int L, int N, con
       launch_bwd<float>(p, a, blocks, w_f32, st);
   }
   if (sums) {
-    const int grid = (2 * N + 15) / 16;
+    const int grid = (2 * N + 31) / 32;
     if (dtype == FST_BF16)
-      norm_grad_sum<bf16><<<grid, 256, 0, st>>>(part, blocks, N, dweight, dbias, w_f32);
+      norm_grad_sum<bf16><<<grid, 1024, 0, st>>>(part, blocks, N, dweight, dbias, w_f32);
     else if (dtype == FST_F16)
-      norm_grad_sum<f16><<<grid, 256, 0, st>>>(part, blocks, N, dweight, dbias, w_f32);
+      norm_grad_sum<f16><<<grid, 1024, 0, st>>>(part, blocks, N, dweight, dbias, w_f32);
     else
-      norm_grad_sum<float><<<grid, 256, 0, st>>>(part, blocks, N, dweight, dbias, w_f32);
+      norm_grad_sum<float><<<grid, 1024, 0, st>>>(part, blocks, N, dweight, dbias, w_f32);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(FST_ELAUNCH, "layer norm backward launch failed (%s)", hipGetErrorString(e));
