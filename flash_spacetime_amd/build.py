@@ -83,24 +83,37 @@ def _units():
     return [u for u in units if u[1].exists()]
 
 
+HOST_SOURCES = ("fst_host.cpp", "fst_block_host.cpp")
+
+
 def _build_host():
-    """Compile csrc/fst_host.cpp, the operators' host path (a Python extension
-    against torch's C++ API; no device code). It records the build id and the
-    torch it was compiled for, which _lib.host compares."""
+    """Compile the operators' host path (a Python extension against torch's C++
+    API; no device code). It records the build id and the torch it was compiled
+    for, which _lib.host compares."""
     import torch
     from torch.utils import cpp_extension
 
+    cxx = os.environ.get("CXX", "g++")
+    flags = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-DTORCH_EXTENSION_NAME=_fst_host",
+             f'-DFST_BUILD_ID="{source_hash()}"', f'-DFST_TORCH_VERSION="{torch.__version__}"',
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+             # torch's stream header, and the runtime's beside the compiler
+             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1"]
+    rocm = Path(shutil.which(HIPCC) or HIPCC).resolve().parents[1]
+    for inc in (*cpp_extension.include_paths(), sysconfig.get_paths()["include"], rocm / "include"):
+        flags += ["-isystem", str(inc)]
+    objs = [BUILD / f"{Path(src).stem}.o" for src in HOST_SOURCES]
+
+    def run(cmd):
+        res = subprocess.run([cxx, *cmd], capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError("host extension failed:\n" + res.stdout + res.stderr)
+
+    with ThreadPoolExecutor(max_workers=len(objs)) as pool:
+        list(pool.map(lambda so: run([*flags, "-c", str(CSRC / so[0]), "-o", str(so[1])]), zip(HOST_SOURCES, objs)))
     tmp = HOST_LIB.with_suffix(".so.tmp")
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall",
-           "-DTORCH_EXTENSION_NAME=_fst_host", f'-DFST_BUILD_ID="{source_hash()}"',
-           f'-DFST_TORCH_VERSION="{torch.__version__}"', f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
-    for inc in (*cpp_extension.include_paths(), sysconfig.get_paths()["include"]):
-        cmd += ["-isystem", str(inc)]
-    cmd += [str(CSRC / "fst_host.cpp"), "-o", str(tmp)]
-    cmd += [f"-L{p}" for p in cpp_extension.library_paths()] + ["-lc10", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError("host extension failed:\n" + res.stdout + res.stderr)
+    run(["-shared", *map(str, objs), "-o", str(tmp), *(f"-L{p}" for p in cpp_extension.library_paths()),
+         "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python"])
     os.replace(tmp, HOST_LIB)
     (PKG / "_fst_host.so").unlink(missing_ok=True)  # the untagged file of earlier builds
 

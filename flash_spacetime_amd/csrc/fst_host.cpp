@@ -23,7 +23,7 @@
 #include <stdexcept>
 #include <string>
 
-#include "../../include/flash_spacetime.h"
+#include "fst_block_host.h"
 
 namespace {
 
@@ -39,7 +39,9 @@ struct Library {
   decltype(&fst_last_error) last_error = nullptr;
 } lib;
 
-void bind_library(size_t supported, size_t fwd_ws, size_t fwd, size_t bwd_ws, size_t bwd, size_t last_error) {
+void bind_library(size_t supported, size_t fwd_ws, size_t fwd, size_t bwd_ws, size_t bwd, size_t last_error,
+                  size_t norm_fwd, size_t norm_ws, size_t norm_bwd, size_t ffn_fwd, size_t ffn_ws, size_t ffn_bwd) {
+  bind_block_library(norm_fwd, norm_ws, norm_bwd, ffn_fwd, ffn_ws, ffn_bwd, last_error);
   lib.supported = reinterpret_cast<decltype(lib.supported)>(supported);
   lib.forward_workspace_bytes = reinterpret_cast<decltype(lib.forward_workspace_bytes)>(fwd_ws);
   lib.forward = reinterpret_cast<decltype(lib.forward)>(fwd);
@@ -278,4 +280,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("bind_library", &bind_library);
   m.def("forward", &forward);
   m.def("backward", &backward);
+  define_block_operators(m);
 }

@@ -16,7 +16,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .norm import BLOCK_DTYPES, batch_of_rows, check_rows, token_rows
+from .norm import BLOCK_DTYPES, PLAIN, batch_of_rows, check_rows, token_rows
 
 ACTIVATIONS = {"silu": _lib.FST_SILU, "gelu": _lib.FST_GELU, "gelu_tanh": _lib.FST_GELU_TANH}
 
@@ -106,6 +106,12 @@ def flash_gated_feed_forward(
     chain of linears does; float16 hidden rows past 65504 are infinite). Results
     are bitwise reproducible.
     """
+    tensors = (x, w_gate, w_up, w_down, b_gate, b_up, b_down)
+    if x.is_cuda and activation in ACTIVATIONS and all(t is None or type(t) in PLAIN for t in (*tensors, seqlens)):
+        host = _lib.host()
+        out = None if host is None else host.feed_forward(*tensors, ACTIVATIONS[activation], seqlens)
+        if out is not None:
+            return out
     check_rows(x, w_gate, w_up, w_down, b_gate, b_up, b_down,
                seqlens if seqlens is not None and seqlens.is_cuda else None)
     if activation not in ACTIVATIONS:

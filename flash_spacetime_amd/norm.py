@@ -70,6 +70,12 @@ def check_rows(x: Tensor, *others: Optional[Tensor]) -> int:
     return BLOCK_DTYPES[x.dtype]
 
 
+# Tensors without methods of their own: calls of these go through the host
+# extension (csrc/fst_block_host.cpp), which gives back None for what it leaves to
+# the Python path.
+PLAIN = (Tensor, torch.nn.Parameter)
+
+
 class _LayerNorm(torch.autograd.Function):
     """Fused forward and deterministic backward; keeps the normalised rows
     (x, or the residual sum it returned) and two floats a row."""
@@ -152,6 +158,11 @@ def flash_layer_norm(
     Any strides are taken (rows a fixed stride apart in place, others copied).
     Statistics and sums are float32; results are bitwise reproducible.
     """
+    if x.is_cuda and all(t is None or type(t) in PLAIN for t in (x, residual, weight, bias, seqlens)):
+        host = _lib.host()
+        out = None if host is None else host.layer_norm(x, residual, weight, bias, eps, seqlens)
+        if out is not None:
+            return out
     check_rows(x, residual, weight, bias, seqlens if seqlens is not None and seqlens.is_cuda else None)
     n = x.shape[-1]
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):

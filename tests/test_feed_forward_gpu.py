@@ -266,3 +266,67 @@ def test_offsets_past_32_bits():
     got = _run(big, ws, bs, "silu", None, dy)
     want = ffn64(x, *ws, *bs, "silu", valid_rows(x.shape, None), dy[-last:])
     _compare([got[0][-last:], got[1][-last:], *got[2:]], want, torch.bfloat16)
+
+
+def test_double_backward_and_stale_inputs_are_refused():
+    x, ws, bs, dy = _make((5,), 16, 24, torch.float32, False, "twice")
+    x.requires_grad_(True)
+    g = torch.autograd.grad(flash_gated_feed_forward(x, *ws).sum(), x, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="twice"):
+        g.sum().backward()
+    for i in range(4):
+        args = [t.detach().clone() for t in (x, *ws)]
+        z = args[0].detach().requires_grad_(True) * 1.0
+        y = flash_gated_feed_forward(z, *args[1:])
+        with torch.no_grad():
+            (z if i == 0 else args[i]).add_(1.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward(dy)
+
+
+@pytest.mark.parametrize("biases", [False, True])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_host_extension_and_python_path_agree_bitwise(monkeypatch, dtype, biases):
+    from flash_spacetime_amd import _lib
+
+    assert _lib.host() is not None
+    lens = torch.tensor([5, 0, 12], device=DEV)
+    for key, lead, sl in (("rows", (33,), None), ("pad", (3, 12), lens), ("one", (), None)):
+        x, ws, bs, dy = _make(lead, 40, 72, TYPES[dtype], biases, (dtype, key))
+        a = _run(x, ws, bs, "gelu", sl, dy)
+        with monkeypatch.context() as m:
+            m.setattr(_lib, "host", lambda: None)
+            c = _run(x, ws, bs, "gelu", sl, dy)
+        for p, q in zip(a, c):
+            assert (p is None) == (q is None) and (p is None or torch.equal(p, q))
+
+
+def test_saved_tensor_hooks_see_what_the_backward_keeps():
+    x, ws, bs, dy = _make((10,), 64, 96, torch.float32, True, "hooks")
+    x.requires_grad_(True)
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(tuple(t.shape)) or t.cpu(), lambda t: t.to(DEV)):
+        y = flash_gated_feed_forward(x, *ws, *bs)
+    assert (10, 64) in seen and seen.count((10, 96)) == 3  # x; the hidden rows and, in float32, both projections
+    want = torch.autograd.grad(flash_gated_feed_forward(x, *ws, *bs), x, dy)[0]
+    assert torch.equal(torch.autograd.grad(y, x, dy)[0], want)
+
+
+def test_refusals():
+    x, ws, bs, _ = _make((2, 3), 16, 24, torch.float32, True, "refusals")
+    good = dict(x=x, w_gate=ws[0], w_up=ws[1], w_down=ws[2], b_gate=bs[0], b_up=bs[1], b_down=bs[2])
+    bad = [
+        (dict(x=x.double()), "bfloat16"), (dict(w_gate=ws[0].half()), "w_gate"), (dict(w_gate=ws[2]), "w_gate"),
+        (dict(w_up=ws[1][:8]), "w_up"), (dict(w_down=ws[0]), "w_down"), (dict(b_gate=bs[2]), "b_gate"),
+        (dict(b_up=bs[1].half()), "b_up"), (dict(b_down=bs[0]), "b_down"), (dict(activation="tanh"), "activation"),
+        (dict(seqlens=torch.tensor([1], device=DEV)), "seqlens"), (dict(seqlens=torch.tensor([True, False], device=DEV)), "integer"),
+        (dict(x=x[0], seqlens=torch.tensor([1, 2], device=DEV)), "padded"),
+    ]
+    for kwargs, what in bad:
+        with pytest.raises(ValueError, match=what):
+            flash_gated_feed_forward(**{**good, **kwargs})
+    odd = torch.randn(4, 12, device=DEV)
+    with pytest.raises(ValueError, match="multiples of 8"):
+        flash_gated_feed_forward(odd, torch.randn(24, 12, device=DEV), torch.randn(24, 12, device=DEV), torch.randn(12, 24, device=DEV))
+    with pytest.raises(RuntimeError, match="GPU"):
+        flash_gated_feed_forward(**{**good, "w_up": ws[1].cpu()})

@@ -292,3 +292,67 @@ def test_replays_in_a_graph():
         torch.cuda.synchronize()
         for a, c in zip(static, want):
             assert torch.equal(a, c), f"replay {i}"
+
+
+def test_double_backward_and_stale_inputs_are_refused():
+    """Only first derivatives are offered, and an input modified in place after
+    the forward is noticed, through the host extension and without it."""
+    x = torch.randn(4, 32, device=DEV, requires_grad=True)
+    g = torch.autograd.grad(flash_layer_norm(x).square().sum(), x, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="twice"):
+        g.sum().backward()
+    z = x.detach().clone().requires_grad_(True) * 1.0
+    y = flash_layer_norm(z)
+    z.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_host_extension_and_python_path_agree_bitwise(monkeypatch, dtype, residual):
+    from flash_spacetime_amd import _lib
+
+    assert _lib.host() is not None
+    lens = torch.tensor([5, 0, 12], device=DEV)
+    for key, shape, sl in (("rows", (33, 72), None), ("pad", (3, 12, 391), lens), ("one", (384,), None)):
+        x, r, w, b, dy, ds = _make(shape, TYPES[dtype], torch.float32, residual, (dtype, key))
+        a = _run(x, r, w, b, sl, dy, ds)
+        with monkeypatch.context() as m:
+            m.setattr(_lib, "host", lambda: None)
+            c = _run(x.detach(), None if r is None else r.detach(), w.detach(), b.detach(), sl, dy, ds)
+        for p, q in zip((*a[0], *a[1]), (*c[0], *c[1])):
+            assert (p is None) == (q is None) and (p is None or torch.equal(p, q))
+
+
+def test_saved_tensor_hooks_see_what_the_backward_keeps():
+    x = torch.randn(6, 64, device=DEV, requires_grad=True)
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(tuple(t.shape)) or t.cpu(), lambda t: t.to(DEV)):
+        y = flash_layer_norm(x)
+    assert (6, 64) in seen and (6, 2) in seen
+    dy = torch.randn_like(y)
+    want = torch.autograd.grad(flash_layer_norm(x), x, dy)[0]
+    assert torch.equal(torch.autograd.grad(y, x, dy)[0], want)
+
+
+def test_refusals():
+    x = torch.randn(2, 3, 16, device=DEV)
+    w = torch.randn(16, device=DEV)
+    bad = [
+        (dict(x=x.double()), "bfloat16"), (dict(weight=w[:8]), "weight"), (dict(weight=w.double()), "float32"),
+        (dict(weight=w, bias=w.half()), "bias"), (dict(x=x.half(), weight=w, bias=w.half()), "share"),
+        (dict(residual=x[:1]), "residual"), (dict(residual=x.half()), "residual"), (dict(eps=-1.0), "eps"),
+        (dict(seqlens=torch.tensor([1, 2, 3], device=DEV)), "seqlens"), (dict(seqlens=torch.tensor([1.0, 2.0], device=DEV)), "integer"),
+        (dict(x=x[0], seqlens=torch.tensor([1, 2], device=DEV)), "padded"), (dict(x=torch.zeros(2, 0, device=DEV)), "features"),
+        (dict(x=torch.zeros(1, 16385, device=DEV)), "16384"),
+    ]
+    for kwargs, what in bad:
+        call = {"x": x, **kwargs}
+        with pytest.raises(ValueError, match=what):
+            flash_layer_norm(**call)
+    with pytest.raises(RuntimeError, match="GPU"):
+        flash_layer_norm(x, w.cpu())
+    # lengths on the host are moved; the defaults are those of the docstring
+    y = flash_layer_norm(x, seqlens=torch.tensor([1, 2]))
+    assert bool((y[0, 1:] == 0).all()) and bool((y[1, :2] != 0).any())
