@@ -66,5 +66,7 @@ def __getattr__(name: str) -> object:
     if name in _OPS:
         import importlib
 
-        return getattr(importlib.import_module(f".{_OPS[name]}", __name__), name)
+        value = getattr(importlib.import_module(f".{_OPS[name]}", __name__), name)
+        globals()[name] = value  # found without this function from now on
+        return value
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

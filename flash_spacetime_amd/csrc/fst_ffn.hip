@@ -62,26 +62,35 @@ struct Transposes {
   int R[3], C[3], first[3];  // workgroups before the next matrix
 };
 
+// A workgroup turns a 64 x 64 tile through LDS, 16 bytes at a time in memory (by
+// elements it took 9.6 us at 3 x 384 x 1024, 20 at 3 x 1024 x 2752). R and C are
+// multiples of 8.
 template <typename E>
 __global__ __launch_bounds__(256) void ffn_transpose(Transposes p) {
-  __shared__ E tile[64][65];
+  constexpr int V = 16 / sizeof(E), PER = 64 / V;  // elements of a piece; pieces of a tile's row
+  typedef E Part __attribute__((ext_vector_type(V)));
+  __shared__ __attribute__((aligned(16))) E tile[64][64 + V];
   const int k = (int)blockIdx.x >= p.first[0] ? ((int)blockIdx.x >= p.first[1] ? 2 : 1) : 0;
   const int wg = (int)blockIdx.x - (k ? p.first[k - 1] : 0);
   const int R = p.R[k], C = p.C[k], nc = (C + 63) / 64;
   const int r0 = wg / nc * 64, c0 = wg % nc * 64;
   const E* in = static_cast<const E*>(p.in[k]);
   E* out = static_cast<E*>(p.out[k]);
-  const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int r = r0 + y + 4 * i;
-    if (r < R && c0 + x < C) tile[y + 4 * i][x] = in[(long)r * C + c0 + x];
+  for (int i = threadIdx.x; i < 64 * PER; i += 256) {
+    const int r = i / PER, c = i % PER * V;
+    if (r0 + r < R && c0 + c < C) {
+      const Part v = *reinterpret_cast<const Part*>(in + (long)(r0 + r) * C + c0 + c);
+#pragma unroll
+      for (int j = 0; j < V; ++j) tile[c + j][r] = v[j];
+    }
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int c = c0 + y + 4 * i;
-    if (c < C && r0 + x < R) out[c * p.ldo[k] + r0 + x] = tile[x][y + 4 * i];
+  for (int i = threadIdx.x; i < 64 * PER; i += 256) {
+    const int c = i / PER, r = i % PER * V;
+    if (c0 + c < C && r0 + r < R)
+      *reinterpret_cast<Part*>(out + (c0 + c) * p.ldo[k] + r0 + r) = *reinterpret_cast<const Part*>(&tile[c][r]);
   }
 }
 

@@ -514,23 +514,26 @@ void launch(const FfnProduct& p, hipStream_t st) {
   ffn_product<MODE, WF, WT, NI, NJ, OCC><<<(unsigned)((tiles + 7) / 8 * 8), 64 * WF * WT, 0, st>>>(p);
 }
 
-// Whether tiles of `f` features by `t` tokens, one workgroup a CU, beat tiles of a
-// quarter of the area, two a CU: their rounds over the chip. A full chip of small
-// tiles takes 1.05 to 1.2 times as long as one of large ones in 16-bit types
-// (65536 tokens, D = 1024, F = 2752 bf16: gate 761 against 706 us, output 365 / 308;
-// 100500 tokens, D = 384, F = 1024: gate 250 / 236, output 107 / 128 us, where
-// three large tiles take two rounds' time); float32, bound by the matrix cores, is
-// as fast in small ones and runs only those.
-bool large_tiles(const FfnProduct& p, int f, int t) {
-  auto tiles = [&](int ff, int tt) { return (long)((p.F + ff - 1) / ff) * ((p.tokens + tt - 1) / tt); };
-  const double large = (double)((tiles(f, t) + 255) / 256) * f * t;
-  const double small = (double)((tiles(f / 2, t / 2) + 511) / 512) * (f / 2) * (t / 2) * 2 * 1.15;
-  return large <= small;
-}
+// The three tiles of a product: 256 x 256 features (of all weights) by tokens, one
+// workgroup of eight waves a CU; 128 x 128, four waves, two a CU; 64 x 64, four
+// waves, four a CU. A k step (64 elements of 16 bits) of n workgroups on every CU takes
+// about 1.65 n, 0.54 n (one alone 0.64) and 0.22 n (alone 0.30) us, measured on
+// [tokens, F, K] = [65536, 2752, 1024], [7640, 768, 2048], [1024, 384, 2048] (bf16: large
+// 362 / 58 / 48 us, middle 405 / 33 / 21, small - / 42 / 9.5). float32 is bound by the
+// matrix cores four times as long in each: as fast in the middle tile as in the
+// large one, which it does without.
+enum Tile { kLarge, kMiddle, kSmall };
 
-template <int MODE>
-void launch_small(const FfnProduct& p, hipStream_t st) {
-  launch<MODE, 2, 2, 4, MODE == kFfnRedo ? 2 : 4, 2>(p, st);
+Tile pick(const FfnProduct& p, int mats, bool redo) {
+  const auto load = [&](int f, int t) {
+    const long tiles = (long)((p.F + f - 1) / f) * ((p.tokens + t - 1) / t);
+    return (double)((tiles + 255) / 256);
+  };
+  const double large = load(256 / mats, redo ? 192 : 256) * 1.65 * (redo ? 0.75 : 1.0);
+  const double nm = load(128 / mats, redo ? 64 : 128), ns = load(64 / mats, 64);
+  const double middle = (nm > 1 ? 0.54 * nm : 0.64) * (redo ? 0.55 : 1.0), small = ns > 1 ? 0.22 * ns : 0.30;
+  if (!F32 && large <= middle && large <= small) return kLarge;
+  return middle <= small ? kMiddle : kSmall;
 }
 
 template <int WM, int WN, int NI, int NJ, int OCC>
@@ -552,28 +555,35 @@ void launch_outer(const FfnOuter& p, hipStream_t st) {
 #define FST_CAT(a, b) FST_CAT2(a, b)
 
 int FST_CAT(ffn_product_, FST_NAME)(int mode, const FfnProduct& p, hipStream_t st) {
-  if constexpr (F32) {
+  const Tile tile = pick(p, mode == kFfnGate || mode == kFfnRedo ? 2 : 1, mode == kFfnRedo);
+  if constexpr (!F32) {
+    if (tile == kLarge) {
+      if (mode == kFfnGate)
+        launch<kFfnGate, 2, 4, 8, 4, 1>(p, st);
+      else if (mode == kFfnOut)
+        launch<kFfnOut, 2, 4, 8, 4, 1>(p, st);
+      else
+        launch<kFfnRedo, 2, 4, 8, 3, 1>(p, st);
+      return hipGetLastError() == hipSuccess ? FST_OK : FST_ELAUNCH;
+    }
+  }
+  constexpr int BACK = F32 ? kFfnGrad : kFfnRedo;
+  if (tile != kSmall) {
     if (mode == kFfnGate)
-      launch_small<kFfnGate>(p, st);
+      launch<kFfnGate, 2, 2, 4, 4, 2>(p, st);
     else if (mode == kFfnOut)
-      launch_small<kFfnOut>(p, st);
+      launch<kFfnOut, 2, 2, 4, 4, 2>(p, st);
     else
-      launch_small<kFfnGrad>(p, st);
-  } else if (mode == kFfnGate) {
-    if (large_tiles(p, 128, 256))
-      launch<kFfnGate, 2, 4, 8, 4, 1>(p, st);
-    else
-      launch_small<kFfnGate>(p, st);
-  } else if (mode == kFfnOut) {
-    if (large_tiles(p, 256, 256))
-      launch<kFfnOut, 2, 4, 8, 4, 1>(p, st);
-    else
-      launch_small<kFfnOut>(p, st);
+      launch<BACK, 2, 2, 4, F32 ? 4 : 2, 2>(p, st);
   } else {
-    if (large_tiles(p, 128, 192))
-      launch<kFfnRedo, 2, 4, 8, 3, 1>(p, st);
+    if (mode == kFfnGate)
+      launch<kFfnGate, 1, 4, 4, 1, 4>(p, st);
+    else if (mode == kFfnOut)
+      launch<kFfnOut, 2, 2, 2, 2, 4>(p, st);
+    else if constexpr (F32)
+      launch<kFfnGrad, 2, 2, 2, 2, 4>(p, st);
     else
-      launch_small<kFfnRedo>(p, st);
+      launch<kFfnRedo, 1, 4, 4, 1, 4>(p, st);
   }
   return hipGetLastError() == hipSuccess ? FST_OK : FST_ELAUNCH;
 }
