@@ -12,6 +12,8 @@
 // LDS layouts are the same bytes for every type.
 #include "fst_ffn.h"
 
+#include <type_traits>
+
 namespace fst {
 
 namespace {
@@ -136,12 +138,12 @@ __device__ __forceinline__ bool pick_tile(int wg, int nf, int nt, int& f, int& t
 // feature 4 GS a + 4 s + r, which the loads into LDS arrange. LDS rows are 128
 // bytes of k (whole lines of memory: 64-byte rows measured a fifth slower);
 // 16-byte part c of row r sits at c ^ ((r >> 1) & 7), so that the 16 rows of a
-// read pass cover the banks once. Two stages: the loads of a k step run while
-// the step before is multiplied, one barrier a step.
+// read pass cover the banks once. ST stages: the loads of ST - 1 k steps run while
+// a step is multiplied, one barrier a step.
 //
 // kFfnRedo runs two contractions after each other, a and u from x and then dh
 // from dy, and holds all three.
-template <int MODE, int WF, int WT, int NI, int NJ>
+template <int MODE, int WF, int WT, int NI, int NJ, int ST>
 struct Product {
   static constexpr int WAVES = WF * WT;
   // Weights whose rows share a stage's feature rows, side by side in each wave's NI.
@@ -153,17 +155,19 @@ struct Product {
   static constexpr int LW = BF / (8 * WAVES), LT = BT / (8 * WAVES), LD = FEATURES / (8 * WAVES);
   static constexpr int STAGE = (BF + BT) * 128;
   static constexpr int KE = 128 / ES;              // k of a step
+  // Loads of a wave that are newer than a step's (at least: dh's steps have fewer).
+  static constexpr int NEWER = (ST - 2) * (LT + (MODE == kFfnRedo && LD < LW ? LD : LW));
   static_assert(NF % 2 == 0 && BF % (8 * WAVES) == 0 && BT % (8 * WAVES) == 0 && FEATURES % (8 * WAVES) == 0, "tile");
 };
 
 __device__ __forceinline__ u32x4 read16(const unsigned char* p) { return *reinterpret_cast<const u32x4*>(p); }
 
-template <int MODE, int WF, int WT, int NI, int NJ, int OCC>
+template <int MODE, int WF, int WT, int NI, int NJ, int ST, int OCC>
 __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
-  typedef Product<MODE, WF, WT, NI, NJ> C;
+  typedef Product<MODE, WF, WT, NI, NJ, ST> C;
   constexpr int NF = C::NF, GS = C::GS, NE = 4 * GS, WAVES = C::WAVES;
   constexpr bool REDO = MODE == kFfnRedo;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[2][C::STAGE];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[ST][C::STAGE];
   const int tokens = p.count ? *p.count : p.tokens;
   const int nf = (p.F + C::FEATURES - 1) / C::FEATURES, nt = (tokens + C::BT - 1) / C::BT;
   int ft, tt;
@@ -207,26 +211,34 @@ __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
   const int steps = (p.K + C::KE - 1) / C::KE;
   const int tail = p.K % C::KE * ES;  // bytes of the last step, 0: all
 
-  // Loads of k step s into stage b; second: of dh's contraction.
-  auto issue = [&](int s, int b, bool second) __attribute__((always_inline)) {
-    unsigned char* base = lds[b] + wave * 1024;
-    // Parts past K are zeros in both operands.
-    const bool cut = tail != 0 && s == steps - 1 && part * 16 >= tail;
-    if (!REDO || !second) {
+  // Loads of k step s into stage b: x's contraction, and dh's. Parts past K are
+  // zeros in both operands.
+  const int total = REDO ? 2 * steps : steps;
+  auto cut_at = [&](int s) { return tail != 0 && s == steps - 1 && part * 16 >= tail; };
+  auto load_rows = [&](const char* const* rows, int s, unsigned char* base, bool cut) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < C::LW; ++i)
-        load_to_lds(C::MATS == 2 && mat[i] ? wr1 : wr0, base + i * WAVES * 1024, cut ? (int)0x80000000 : voff[i], s * 128);
-    } else {
+    for (int i = 0; i < C::LT; ++i) {
+      const char* q = cut ? reinterpret_cast<const char*>(&kZero16) : rows[i] + s * 128l;
+      __builtin_amdgcn_global_load_lds((glb_ptr)q, (lds_ptr)(base + C::BF * 128 + i * WAVES * 1024), 16, 0, 0);
+    }
+  };
+  auto issue = [&](int s, int b) __attribute__((always_inline)) {
+    unsigned char* base = lds[b] + wave * 1024;
+    const bool cut = cut_at(s);
+#pragma unroll
+    for (int i = 0; i < C::LW; ++i)
+      load_to_lds(C::MATS == 2 && mat[i] ? wr1 : wr0, base + i * WAVES * 1024, cut ? (int)0x80000000 : voff[i], s * 128);
+    load_rows(xp, s, base, cut);
+  };
+  auto issue_dh = [&](int s, int b) __attribute__((always_inline)) {
+    if constexpr (REDO) {
+      unsigned char* base = lds[b] + wave * 1024;
+      const bool cut = cut_at(s);
 #pragma unroll
       for (int i = 0; i < C::LD; ++i)
         load_to_lds(wr2, base + i * WAVES * 1024,
                     cut ? (int)0x80000000 : feature((i * WAVES + wave) >> 1) * row_bytes + part * 16, s * 128);
-    }
-#pragma unroll
-    for (int i = 0; i < C::LT; ++i) {
-      const char* from = (REDO && second ? yp[REDO ? i : 0] : xp[i]) + s * 128l;
-      const char* q = cut ? reinterpret_cast<const char*>(&kZero16) : from;
-      __builtin_amdgcn_global_load_lds((glb_ptr)q, (lds_ptr)(base + C::BF * 128 + i * WAVES * 1024), 16, 0, 0);
+      load_rows(yp, s, base, cut);
     }
   };
 
@@ -241,14 +253,28 @@ __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
     }
   }
   const int rd = n * 128, swz = (n >> 1) & 7;
-  issue(0, 0, false);
+#pragma unroll
+  for (int v = 0; v < ST - 1; ++v) {
+    if (v < steps)
+      issue(v, v);
+    else if (v < total)
+      issue_dh(v - steps, v);
+  }
+  int b = 0;
+  // Step v has landed and the stage before it is read: that one can be loaded anew.
+  auto wait = [&](int v) __attribute__((always_inline)) {
+    if (v + ST - 2 < total)
+      stage_wait<C::NEWER>();
+    else
+      stage_wait<0>();
+    return b == 0 ? ST - 1 : b - 1;
+  };
   for (int s = 0; s < steps; ++s) {
-    const int b = s & 1;
-    stage_wait<0>();
-    if (s + 1 < steps)
-      issue(s + 1, b ^ 1, false);
-    else if constexpr (REDO)
-      issue(0, b ^ 1, true);
+    const int free = wait(s), next = s + ST - 1;
+    if (next < steps)
+      issue(next, free);
+    else if (REDO && next < total)
+      issue_dh(next - steps, free);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const unsigned char* base = lds[b] + rd + (((4 * k + g) ^ swz) << 4);
@@ -262,12 +288,12 @@ __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
 #pragma unroll
         for (int i = 0; i < NI; ++i) acc[i][j] = Mma<T>::run(fw[i], fx[j], acc[i][j]);
     }
+    b = b == ST - 1 ? 0 : b + 1;
   }
   if constexpr (REDO) {
     for (int s = 0; s < steps; ++s) {
-      const int b = (steps + s) & 1;
-      stage_wait<0>();
-      if (s + 1 < steps) issue(s + 1, b ^ 1, true);
+      const int free = wait(steps + s), next = s + ST - 1;
+      if (next < steps) issue_dh(next, free);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const unsigned char* base = lds[b] + rd + (((4 * k + g) ^ swz) << 4);
@@ -281,6 +307,7 @@ __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
 #pragma unroll
           for (int i = 0; i < NF; ++i) dh[i][j] = Mma<T>::run(fw[i], fx[j], dh[i][j]);
       }
+      b = b == ST - 1 ? 0 : b + 1;
     }
   }
 
@@ -339,6 +366,121 @@ __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
         store_run<NE>(out + p.F, left, u);
       }
     }
+  }
+}
+
+// The same products for at most 16 NJ rows. Eight waves share 16 features (of each
+// weight) by the tokens and split k between them in contiguous runs, straight from memory
+// into registers: no stage waits for another, and the longest chain is an eighth
+// of k. The partial sums meet in LDS and are added in the waves' order.
+template <int MODE, int NJ>
+__global__ __launch_bounds__(512, MODE == kFfnRedo && NJ == 4 ? 2 : 4) void ffn_few(FfnProduct p) {
+  constexpr bool REDO = MODE == kFfnRedo;
+  constexpr int MATS = MODE == kFfnGate || REDO ? 2 : 1, ACCS = REDO ? 3 : MATS, KE = 64 / ES, AHEAD = NJ == 1 ? 4 : 2;
+  __shared__ f32x4 lds[8][ACCS * NJ][64];
+  const int tokens = p.count ? *p.count : p.tokens;
+  if (tokens <= 0) return;
+  const int f0 = blockIdx.x * 16, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, n = lane & 15;
+  const int row_bytes = (int)p.ldw * ES;
+  const int steps = (p.K + KE - 1) / KE, per = (steps + 7) / 8;
+  const int s0 = wave * per, s1 = min(s0 + per, steps);
+
+  f32x4 acc[ACCS][NJ];
+#pragma unroll
+  for (int a = 0; a < ACCS; ++a)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[a][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // acc[A0 .. A0 + MM) += the weights W0 .. against the tokens' rows of x.
+  auto contract = [&](auto first, auto count, int w0, const void* x, long ldx) __attribute__((always_inline)) {
+    constexpr int A0 = decltype(first)::value, MM = decltype(count)::value;
+    const char *wp[MM], *xp[NJ];
+#pragma unroll
+    for (int a = 0; a < MM; ++a)
+      wp[a] = static_cast<const char*>(p.w[w0 + a]) + (long)min(f0 + n, p.F - 1) * row_bytes + g * 16;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int t = min(16 * j + n, tokens - 1);  // past the last token: not stored
+      const long r = p.rows_in ? p.rows_in[t] : t;
+      xp[j] = static_cast<const char*>(x) + r * ldx * ES + g * 16;
+    }
+    for (int s = s0; s < s1; s += AHEAD) {
+      u32x4 fw[AHEAD][MM], fx[AHEAD][NJ];
+#pragma unroll
+      for (int q = 0; q < AHEAD; ++q) {
+        // Steps past the run and parts past K read zeros.
+        const bool in = s + q < s1 && (s + q) * KE + g * (16 / ES) < p.K;
+        const char* zero = reinterpret_cast<const char*>(&kZero16);
+#pragma unroll
+        for (int a = 0; a < MM; ++a) fw[q][a] = *reinterpret_cast<const u32x4*>(in ? wp[a] + (s + q) * 64 : zero);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) fx[q][j] = *reinterpret_cast<const u32x4*>(in ? xp[j] + (s + q) * 64 : zero);
+      }
+#pragma unroll
+      for (int q = 0; q < AHEAD; ++q)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int a = 0; a < MM; ++a) acc[A0 + a][j] = Mma<T>::run(fw[q][a], fx[q][j], acc[A0 + a][j]);
+    }
+  };
+  contract(std::integral_constant<int, 0>{}, std::integral_constant<int, MATS>{}, 0, p.x, p.ldx);
+  if constexpr (REDO) contract(std::integral_constant<int, 2>{}, std::integral_constant<int, 1>{}, 2, p.dy, p.lddy);
+#pragma unroll
+  for (int a = 0; a < ACCS; ++a)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) lds[wave][a * NJ + j][lane] = acc[a][j];
+  __syncthreads();
+  if (wave >= NJ) return;
+  // Wave j: features 4 g .. 4 g + 3 of token n of subtile j.
+  const int f = f0 + 4 * g, t = 16 * wave + n;
+  if (f >= p.F || t >= tokens) return;
+  float v[ACCS][4];
+#pragma unroll
+  for (int a = 0; a < ACCS; ++a) {
+    f32x4 sum = lds[0][a * NJ + wave][lane];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) sum += lds[w][a * NJ + wave][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[a][e] = sum[e];
+      if (MODE != kFfnGrad && a < MATS && p.bias[a < 2 ? a : 0])
+        v[a][e] += (float)static_cast<const T*>(p.bias[a < 2 ? a : 0])[f + e];
+    }
+  }
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  auto store = [&](void* out, long at, const float* q) {
+    T4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = (T)q[e];
+    *reinterpret_cast<T4*>(static_cast<T*>(out) + at) = o;
+  };
+  const long r = MODE == kFfnOut && p.rows_out ? p.rows_out[t] : t, at = r * p.ldo + f;
+  float unused;
+  if constexpr (MODE == kFfnGate) {
+    if (F32 && p.out[1]) {
+      store(p.out[1], at, v[0]);
+      store(p.out[2], at, v[1]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[0][e] = activate<false>(p.act, v[0][e], unused) * v[1][e];
+    store(p.out[0], at, v[0]);
+  } else if constexpr (MODE == kFfnOut) {
+    store(p.out[0], at, v[0]);
+  } else {
+    float da[4], du[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float a = REDO ? v[0][e] : (float)static_cast<const T*>(p.gate)[(long)t * p.F + f + e];
+      const float u = REDO ? v[MATS - 1][e] : (float)static_cast<const T*>(p.up)[(long)t * p.F + f + e];
+      const float dh = v[ACCS - 1][e];
+      float slope;
+      const float act = activate<true>(p.act, a, slope);
+      da[e] = dh * u * slope;
+      du[e] = dh * act;
+    }
+    store(p.out[0], at, da);
+    store(p.out[0], at + p.F, du);
   }
 }
 
@@ -507,31 +649,48 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void ffn_outer(FfnOuter p) {
   }
 }
 
-template <int MODE, int WF, int WT, int NI, int NJ, int OCC>
+template <int MODE, int WF, int WT, int NI, int NJ, int ST, int OCC>
 void launch(const FfnProduct& p, hipStream_t st) {
-  typedef Product<MODE, WF, WT, NI, NJ> C;
+  typedef Product<MODE, WF, WT, NI, NJ, ST> C;
   const long tiles = (long)((p.F + C::FEATURES - 1) / C::FEATURES) * ((p.tokens + C::BT - 1) / C::BT);
-  ffn_product<MODE, WF, WT, NI, NJ, OCC><<<(unsigned)((tiles + 7) / 8 * 8), 64 * WF * WT, 0, st>>>(p);
+  ffn_product<MODE, WF, WT, NI, NJ, ST, OCC><<<(unsigned)((tiles + 7) / 8 * 8), 64 * WF * WT, 0, st>>>(p);
 }
 
-// The three tiles of a product: 256 x 256 features (of all weights) by tokens, one
+constexpr int kFewTokens = 64;
+
+template <int MODE>
+void launch_few(const FfnProduct& p, hipStream_t st) {
+  const long nf = (p.F + 15) / 16;
+  if (p.tokens <= 16)
+    ffn_few<MODE, 1><<<(unsigned)nf, 512, 0, st>>>(p);
+  else
+    ffn_few<MODE, 4><<<(unsigned)nf, 512, 0, st>>>(p);
+}
+
+// The tiles of a product: 256 x 256 features (of all weights) by tokens, one
 // workgroup of eight waves a CU; 128 x 128, four waves, two a CU; 64 x 64, four
-// waves, four a CU. A k step (64 elements of 16 bits) of n workgroups on every CU takes
-// about 1.65 n, 0.54 n (one alone 0.64) and 0.22 n (alone 0.30) us, measured on
-// [tokens, F, K] = [65536, 2752, 1024], [7640, 768, 2048], [1024, 384, 2048] (bf16: large
-// 362 / 58 / 48 us, middle 405 / 33 / 21, small - / 42 / 9.5). float32 is bound by the
+// waves, two a CU with four stages (in calls this small the operands come from far:
+// with two stages 9.4 and 17.6 us where four take 7.3 and 12.8, [1024, 384] at K = 1024
+// and 2048). A k step (64 elements of 16 bits) of n workgroups on every CU takes about
+// 1.65 n, 0.54 n (one alone 0.64) and 0.24 n (alone 0.28) us, measured on [tokens, F,
+// K] = [65536, 2752, 1024], [7640, 768, 2048], [1024, 384, 2048] (bf16: large 362 / 58 / 48
+// us, middle 405 / 33 / 21, small - / 45 / 13). Up to 64 tokens the waves split k
+// instead (ffn_few: 4 tokens, D = 768, F = 2048 7.4 + 15.3 us in 64 x 64 tiles, 6.2 + 5.6;
+// 187 tokens, D = 384, F = 1024 5.7 + 7.0 against 6.4 + 7.2). float32 is bound by the
 // matrix cores four times as long in each: as fast in the middle tile as in the
 // large one, which it does without.
-enum Tile { kLarge, kMiddle, kSmall };
+enum Tile { kLarge, kMiddle, kSmall, kFew };
 
 Tile pick(const FfnProduct& p, int mats, bool redo) {
+  if (p.tokens <= kFewTokens) return kFew;
   const auto load = [&](int f, int t) {
     const long tiles = (long)((p.F + f - 1) / f) * ((p.tokens + t - 1) / t);
     return (double)((tiles + 255) / 256);
   };
-  const double large = load(256 / mats, redo ? 192 : 256) * 1.65 * (redo ? 0.75 : 1.0);
-  const double nm = load(128 / mats, redo ? 64 : 128), ns = load(64 / mats, 64);
-  const double middle = (nm > 1 ? 0.54 * nm : 0.64) * (redo ? 0.55 : 1.0), small = ns > 1 ? 0.22 * ns : 0.30;
+  const double nl = load(256 / mats, redo ? 192 : 256), nm = load(128 / mats, redo ? 64 : 128), ns = load(64 / mats, 64);
+  // Two weights' 64 x 64 tile has a quarter of each operand's rows reused less.
+  const double large = 1.65 * nl * (redo ? 0.75 : 1.0), middle = (nm > 1 ? 0.54 * nm : 0.64) * (redo ? 0.55 : 1.0),
+               small = (ns > 1 ? 0.24 * ns : 0.28) * (mats == 2 ? 1.3 : 1.0);
   if (!F32 && large <= middle && large <= small) return kLarge;
   return middle <= small ? kMiddle : kSmall;
 }
@@ -559,31 +718,38 @@ int FST_CAT(ffn_product_, FST_NAME)(int mode, const FfnProduct& p, hipStream_t s
   if constexpr (!F32) {
     if (tile == kLarge) {
       if (mode == kFfnGate)
-        launch<kFfnGate, 2, 4, 8, 4, 1>(p, st);
+        launch<kFfnGate, 2, 4, 8, 4, 2, 1>(p, st);
       else if (mode == kFfnOut)
-        launch<kFfnOut, 2, 4, 8, 4, 1>(p, st);
+        launch<kFfnOut, 2, 4, 8, 4, 2, 1>(p, st);
       else
-        launch<kFfnRedo, 2, 4, 8, 3, 1>(p, st);
+        launch<kFfnRedo, 2, 4, 8, 3, 2, 1>(p, st);
       return hipGetLastError() == hipSuccess ? FST_OK : FST_ELAUNCH;
     }
   }
   constexpr int BACK = F32 ? kFfnGrad : kFfnRedo;
-  if (tile != kSmall) {
+  if (tile == kFew) {
     if (mode == kFfnGate)
-      launch<kFfnGate, 2, 2, 4, 4, 2>(p, st);
+      launch_few<kFfnGate>(p, st);
     else if (mode == kFfnOut)
-      launch<kFfnOut, 2, 2, 4, 4, 2>(p, st);
+      launch_few<kFfnOut>(p, st);
     else
-      launch<BACK, 2, 2, 4, F32 ? 4 : 2, 2>(p, st);
+      launch_few<BACK>(p, st);
+  } else if (tile == kMiddle) {
+    if (mode == kFfnGate)
+      launch<kFfnGate, 2, 2, 4, 4, 2, 2>(p, st);
+    else if (mode == kFfnOut)
+      launch<kFfnOut, 2, 2, 4, 4, 2, 2>(p, st);
+    else
+      launch<BACK, 2, 2, 4, F32 ? 4 : 2, 2, 2>(p, st);
   } else {
     if (mode == kFfnGate)
-      launch<kFfnGate, 1, 4, 4, 1, 4>(p, st);
+      launch<kFfnGate, 1, 4, 4, 1, 4, 2>(p, st);
     else if (mode == kFfnOut)
-      launch<kFfnOut, 2, 2, 2, 2, 4>(p, st);
+      launch<kFfnOut, 2, 2, 2, 2, 4, 2>(p, st);
     else if constexpr (F32)
-      launch<kFfnGrad, 2, 2, 2, 2, 4>(p, st);
+      launch<kFfnGrad, 2, 2, 2, 2, 4, 2>(p, st);
     else
-      launch<kFfnRedo, 1, 4, 4, 1, 4>(p, st);
+      launch<kFfnRedo, 1, 4, 4, 1, 4, 2>(p, st);
   }
   return hipGetLastError() == hipSuccess ? FST_OK : FST_ELAUNCH;
 }
