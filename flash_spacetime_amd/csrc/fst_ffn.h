@@ -39,20 +39,28 @@ struct FfnProduct {
 // order afterwards.
 struct FfnOuter {
   const void *a, *b;
-  const int32_t *rows_a, *rows_b;  // rows of the tokens (one of them at most), or null
-  const int32_t* count;
   long lda, ldb;   // elements; in bytes below 2^32
-  int M, N, tokens, splits;
+  int M, N, splits;
   float* part;     // [splits][N][M]
   float* bias;     // [splits][N], or null
 };
 
+// The block's two: (x, [da | du]) and (h, dy), in one launch. Either may have no
+// splits: it is not asked for.
+struct FfnOuters {
+  FfnOuter p[2];
+  const int32_t* count;  // tokens, on the device (seqlens given); or null
+  const int32_t* rows;   // rows of x and dy of the tokens, or null
+  int tokens;
+  int first;             // workgroups of the first
+};
+
 typedef int (*ffn_product_fn)(int mode, const FfnProduct&, hipStream_t);
-typedef int (*ffn_outer_fn)(const FfnOuter&, bool large, hipStream_t);
+typedef int (*ffn_outer_fn)(FfnOuters&, bool large, hipStream_t);
 
 #define FST_FFN_DECL(name)                                      \
   int ffn_product_##name(int mode, const FfnProduct&, hipStream_t); \
-  int ffn_outer_##name(const FfnOuter&, bool large, hipStream_t);
+  int ffn_outer_##name(FfnOuters&, bool large, hipStream_t);
 FST_FFN_DECL(bf16)
 FST_FFN_DECL(f16)
 FST_FFN_DECL(f32)

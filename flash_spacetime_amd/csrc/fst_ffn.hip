@@ -21,45 +21,51 @@ namespace fst {
 
 namespace {
 
+// Zeros into the padding rows of event e, by thread `at` of `step`.
+__device__ __forceinline__ void zero_padding(unsigned char* out, long row_bytes, int e, int L, int len, long at, long step) {
+  u32x4* pad = reinterpret_cast<u32x4*>(out + ((long)e * L + len) * row_bytes);
+  const long parts = (L - len) * (row_bytes / 16);
+  for (long i = at; i < parts; i += step) pad[i] = u32x4{0, 0, 0, 0};
+}
+
 // Valid rows of a padded batch in order (map[0]: their number, map[1 ..]: the
-// rows; or map null), and zeros into the padding rows of out. Workgroup x takes
-// `per` consecutive events, its y-th slice of their rows.
+// rows), and zeros into the padding rows of out. Workgroup x takes `per`
+// consecutive events, its y-th slice of their rows.
 __global__ __launch_bounds__(256) void ffn_rows(const int32_t* seqlens, int B, int L, int per, int32_t* map,
                                                 unsigned char* out, long row_bytes) {
   __shared__ int red[256];
   const int e0 = blockIdx.x * per, e1 = min(e0 + per, B), tid = threadIdx.x;
-  int off = 0;
-  if (map) {
-    int sum = 0;
-    for (int e = tid; e < e0; e += 256) sum += event_len(seqlens, e, L);
-    red[tid] = sum;
+  int sum = 0;
+  for (int e = tid; e < e0; e += 256) sum += event_len(seqlens, e, L);
+  red[tid] = sum;
+  __syncthreads();
+  for (int h = 128; h > 0; h >>= 1) {
+    if (tid < h) red[tid] += red[tid + h];
     __syncthreads();
-    for (int h = 128; h > 0; h >>= 1) {
-      if (tid < h) red[tid] += red[tid + h];
-      __syncthreads();
-    }
-    off = red[0];
   }
+  int off = red[0];
   const long at = (long)blockIdx.y * 256 + tid, step = (long)gridDim.y * 256;
   for (int e = e0; e < e1; ++e) {
     const int len = event_len(seqlens, e, L);
-    const long row = (long)e * L;
-    if (map)
-      for (long l = at; l < len; l += step) map[1 + off + l] = (int32_t)(row + l);
-    u32x4* pad = reinterpret_cast<u32x4*>(out + (row + len) * row_bytes);
-    const long parts = (L - len) * (row_bytes / 16);
-    for (long i = at; i < parts; i += step) pad[i] = u32x4{0, 0, 0, 0};
+    for (long l = at; l < len; l += step) map[1 + off + l] = (int32_t)((long)e * L + l);
+    zero_padding(out, row_bytes, e, L, len, at, step);
     off += len;
   }
-  if (map && e1 == B && e0 < B && at == 0) map[0] = off;
+  if (e1 == B && e0 < B && at == 0) map[0] = off;
 }
 
-// out[c * ldo + r] = in[r * C + c] for up to three matrices [R, C] of E-byte elements.
+// out[c * ldo + r] = in[r * C + c] for up to three matrices [R, C]; the workgroups
+// after theirs write zeros into the padding rows of `pad`, slices of an event
+// each (seqlens given).
 struct Transposes {
   const void* in[3];
   void* out[3];
   long ldo[3];
   int R[3], C[3], first[3];  // workgroups before the next matrix
+  const int32_t* seqlens;
+  unsigned char* pad;
+  long row_bytes;
+  int L, slices;
 };
 
 // A workgroup turns a 64 x 64 tile through LDS, 16 bytes at a time in memory (by
@@ -70,6 +76,12 @@ __global__ __launch_bounds__(256) void ffn_transpose(Transposes p) {
   constexpr int V = 16 / sizeof(E), PER = 64 / V;  // elements of a piece; pieces of a tile's row
   typedef E Part __attribute__((ext_vector_type(V)));
   __shared__ __attribute__((aligned(16))) E tile[64][64 + V];
+  if ((int)blockIdx.x >= p.first[2]) {
+    const int at = (int)blockIdx.x - p.first[2], e = at / p.slices, slice = at - e * p.slices;
+    zero_padding(p.pad, p.row_bytes, e, p.L, event_len(p.seqlens, e, p.L), (long)slice * 256 + threadIdx.x,
+                 (long)p.slices * 256);
+    return;
+  }
   const int k = (int)blockIdx.x >= p.first[0] ? ((int)blockIdx.x >= p.first[1] ? 2 : 1) : 0;
   const int wg = (int)blockIdx.x - (k ? p.first[k - 1] : 0);
   const int R = p.R[k], C = p.C[k], nc = (C + 63) / 64;
@@ -150,37 +162,40 @@ ffn_outer_fn outer_of(int dtype) {
   return dtype == FST_BF16 ? ffn_outer_bf16 : dtype == FST_F16 ? ffn_outer_f16 : ffn_outer_f32;
 }
 
-// rows: valid rows listed in map (null: only the zeros of out's padding rows).
-void launch_rows(const int32_t* seqlens, int B, int L, int32_t* map, void* out, int D, size_t es, hipStream_t st) {
-  const int wgs = B < 1024 ? B : 1024, per = (B + wgs - 1) / wgs;
-  int slices = 1024 / wgs;
-  const int most = (L + 31) / 32;
-  slices = slices > most ? most : slices;
-  ffn_rows<<<dim3((B + per - 1) / per, slices), 256, 0, st>>>(seqlens, B, L, per, map,
-                                                             static_cast<unsigned char*>(out), (long)D * es);
+// Slices of an event's padding rows: about 1024 workgroups in all.
+int slices_of(int events, int L) {
+  const int most = (L + 31) / 32, want = events < 1024 ? 1024 / events : 1;
+  return want < most ? want : most;
 }
 
-// Tile and token runs of a weight's gradient [N, M]: the least of the rounds of
-// workgroups over the chip, at the rates of large and small tiles (a full chip in
-// bf16: 65536 tokens, M = 1024, N = 5504 920 against 1003 us; M = 2752, N = 1024
-// 474 / 538), plus the runs' partials written and read. float32 is as fast in
-// small tiles and has only those.
+void launch_rows(const int32_t* seqlens, int B, int L, int32_t* map, void* out, int D, size_t es, hipStream_t st) {
+  const int wgs = B < 1024 ? B : 1024, per = (B + wgs - 1) / wgs;
+  ffn_rows<<<dim3((B + per - 1) / per, slices_of(wgs, L)), 256, 0, st>>>(seqlens, B, L, per, map,
+                                                                        static_cast<unsigned char*>(out), (long)D * es);
+}
+
+// Tile and token runs of the weights' gradients [2 F, D] and [D, F]: the least of
+// the rounds of workgroups over the chip, at the rates of large and small tiles (a
+// full chip in bf16: 65536 tokens, M = 1024, N = 5504 920 against 1003 us; M = 2752, N =
+// 1024 474 / 538), plus the runs' partials written and read. float32 is as fast
+// in small tiles and has only those.
 struct OuterPlan {
   bool large;
   int splits;
 };
 
-OuterPlan plan_outer(int dtype, long tokens, int M, int N) {
+OuterPlan plan_outer(int dtype, long tokens, int D, int F) {
   OuterPlan best{false, 1};
   double least = -1;
   for (const bool large : {false, true}) {
     if (large && dtype == FST_F32) continue;
     const int e = large ? kOuterLarge : kOuterSmall;
-    const long tiles = (long)((M + e - 1) / e) * ((N + e - 1) / e), slots = large ? 256 : 512;
+    const auto tiles_of = [e](int m, int n) { return (long)((m + e - 1) / e) * ((n + e - 1) / e); };
+    const long tiles = tiles_of(D, 2 * F) + tiles_of(F, D), slots = large ? 256 : 512;
     const double rate = (dtype == FST_F32 ? 0.12e15 : large ? 0.8e15 : 0.72e15) / slots;
     for (int s = 1; s <= 64 && (s == 1 || s * 256l <= tokens); ++s) {
       const double work = (double)tokens / s * 2 * e * e / rate;
-      const double t = (double)((tiles * s + slots - 1) / slots) * work + s * 8.0 * M * N / 4e12;
+      const double t = (double)((tiles * s + slots - 1) / slots) * work + s * 24.0 * D * F / 4e12;
       if (least < 0 || t < least) best = OuterPlan{large, s}, least = t;
     }
   }
@@ -189,14 +204,13 @@ OuterPlan plan_outer(int dtype, long tokens, int M, int N) {
 
 struct GradLayout {
   size_t wdt, w2t, dadu, part0, part1, bias0, bias1, total;
-  OuterPlan first, second;
+  OuterPlan outer;
 };
 
 GradLayout grad_layout(int dtype, long rows, int D, int F) {
   GradLayout l;
   const size_t es = elem_size(dtype), df = (size_t)D * F;
-  l.first = plan_outer(dtype, rows, D, 2 * F);
-  l.second = plan_outer(dtype, rows, F, D);
+  l.outer = plan_outer(dtype, rows, D, F);
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const size_t at = off;
@@ -206,10 +220,10 @@ GradLayout grad_layout(int dtype, long rows, int D, int F) {
   l.wdt = take(df * es);
   l.w2t = take(2 * df * es);
   l.dadu = take((size_t)rows * 2 * F * es);
-  l.part0 = take(l.first.splits * 2 * df * 4);
-  l.part1 = take(l.second.splits * df * 4);
-  l.bias0 = take((size_t)l.first.splits * 2 * F * 4);
-  l.bias1 = take((size_t)l.second.splits * D * 4);
+  l.part0 = take(l.outer.splits * 2 * df * 4);
+  l.part1 = take(l.outer.splits * df * 4);
+  l.bias0 = take((size_t)l.outer.splits * 2 * F * 4);
+  l.bias1 = take((size_t)l.outer.splits * D * 4);
   l.total = off;
   return l;
 }
@@ -322,6 +336,14 @@ int fst_ffn_backward(int dtype, int activation, int B, int L, int D, int F, cons
     add(0, w_down, l.wdt, D, F, D);
     add(1, dx ? w_gate : nullptr, l.w2t, F, D, 2l * F);
     add(2, dx ? w_up : nullptr, l.w2t + F * es, F, D, 2l * F);
+    if (seqlens && dx) {
+      t.seqlens = seqlens;
+      t.pad = static_cast<unsigned char*>(dx);
+      t.row_bytes = (long)D * es;
+      t.L = L;
+      t.slices = slices_of(B, L);
+      grid += B * t.slices;
+    }
     if (es == 2)
       ffn_transpose<uint16_t><<<grid, 256, 0, st>>>(t);
     else
@@ -354,7 +376,6 @@ int fst_ffn_backward(int dtype, int activation, int B, int L, int D, int F, cons
     p.F = F;
     rc = product_of(dtype)(ffn_redo(dtype) ? kFfnRedo : kFfnGrad, p, st);
     if (rc == FST_OK && dx) {
-      if (seqlens) launch_rows(seqlens, B, L, nullptr, dx, D, es, st);
       p.w[0] = ws + l.w2t;
       p.bias[0] = nullptr;
       p.x = ws + l.dadu;
@@ -369,39 +390,16 @@ int fst_ffn_backward(int dtype, int activation, int B, int L, int D, int F, cons
     if (rc != FST_OK) return fail(rc, "feed-forward backward launch failed");
   }
   if (first || second) {
-    FfnOuter o{};
+    FfnOuters o{};
     o.count = seqlens ? rowmap : nullptr;
+    o.rows = map;
     o.tokens = (int)rows;
     float *p0 = reinterpret_cast<float*>(ws + l.part0), *p1 = reinterpret_cast<float*>(ws + l.part1);
     float *b0 = reinterpret_cast<float*>(ws + l.bias0), *b1 = reinterpret_cast<float*>(ws + l.bias1);
-    rc = FST_OK;
-    if (first) {
-      o.a = x;
-      o.rows_a = map;
-      o.lda = x_stride;
-      o.b = ws + l.dadu;
-      o.ldb = 2l * F;
-      o.M = D;
-      o.N = 2 * F;
-      o.splits = l.first.splits;
-      o.part = p0;
-      o.bias = db_gate || db_up ? b0 : nullptr;
-      rc = outer_of(dtype)(o, l.first.large, st);
-    }
-    if (second && rc == FST_OK) {
-      o.a = hidden;
-      o.rows_a = nullptr;
-      o.lda = F;
-      o.b = dy;
-      o.rows_b = map;
-      o.ldb = dy_stride;
-      o.M = F;
-      o.N = D;
-      o.splits = l.second.splits;
-      o.part = p1;
-      o.bias = db_down ? b1 : nullptr;
-      rc = outer_of(dtype)(o, l.second.large, st);
-    }
+    o.p[0] = FfnOuter{x, ws + l.dadu, (long)x_stride, 2l * F, D, 2 * F, first ? l.outer.splits : 0, p0,
+                      db_gate || db_up ? b0 : nullptr};
+    o.p[1] = FfnOuter{hidden, dy, F, (long)dy_stride, F, D, second ? l.outer.splits : 0, p1, db_down ? b1 : nullptr};
+    rc = outer_of(dtype)(o, l.outer.large, st);
     if (rc != FST_OK) return fail(rc, "feed-forward weight gradient launch failed");
     const long df = (long)D * F;
     const float* part[6] = {p0, p0 + df, p1, b0, b0 + F, b1};
@@ -414,7 +412,7 @@ int fst_ffn_backward(int dtype, int activation, int B, int L, int D, int F, cons
       s.out[k] = out[k];
       s.stride[k] = stride[k];
       s.count[k] = count[k];
-      s.splits[k] = k == 2 || k == 5 ? l.second.splits : l.first.splits;
+      s.splits[k] = l.outer.splits;
       if (out[k]) grid += (int)((count[k] + 1023) / 1024);
       s.first[k] = grid;
     }

@@ -565,21 +565,20 @@ struct OuterSide {
   }
 };
 
-template <int WM, int WN, int NI, int NJ, bool MA, bool MB, int OCC>
-__global__ __launch_bounds__(64 * WM * WN, OCC) void ffn_outer(FfnOuter p) {
+template <int WM, int WN, int NI, int NJ, bool MA, bool MB>
+__device__ __forceinline__ void outer_tile(const FfnOuter& p, const FfnOuters& all, int wg, unsigned char* lds) {
   constexpr int TM = 16 * NI * WM, TN = 16 * NJ * WN, NT = 64 * WM * WN;
   typedef OuterSide<TM, NT, MA> SideA;
   typedef OuterSide<TN, NT, MB> SideB;
   constexpr int A_BYTES = KT * SideA::ROW, STAGE = A_BYTES + KT * SideB::ROW;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[2][STAGE];
   const int nm = (p.M + TM - 1) / TM, nn = (p.N + TN - 1) / TN;
   // Consecutive workgroups of an XCD take the tiles of one run of tokens.
   const int total = nm * nn * p.splits, per = (total + 7) >> 3;
-  const int i8 = blockIdx.x >> 3, at = (blockIdx.x & 7) * per + i8;
+  const int i8 = wg >> 3, at = (wg & 7) * per + i8;
   if (i8 >= per || at >= total) return;
   const int split = at / (nm * nn), tile = at - split * nm * nn;
   const int m0 = tile % nm * TM, n0 = tile / nm * TN;
-  const int tokens = p.count ? *p.count : p.tokens;
+  const int tokens = all.count ? *all.count : all.tokens;
   const int run = ((tokens + p.splits - 1) / p.splits + KT - 1) / KT * KT;
   const int t0 = (int)min((long)split * run, (long)tokens), t1 = (int)min((long)t0 + run, (long)tokens);
 
@@ -587,8 +586,8 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void ffn_outer(FfnOuter p) {
   const int wm = wave % WM, wn = wave / WM, g = lane >> 4, n = lane & 15;
   SideA a;
   SideB bb;
-  a.init(p.a, p.rows_a, p.lda, m0, p.M, tid);
-  bb.init(p.b, p.rows_b, p.ldb, n0, p.N, tid);
+  a.init(p.a, all.rows, p.lda, m0, p.M, tid);
+  bb.init(p.b, all.rows, p.ldb, n0, p.N, tid);
   // The bias' gradient: the columns of b against a row of ones, in the first
   // waves of the first tile of m.
   const bool sums = p.bias && m0 == 0 && wm == 0;
@@ -604,17 +603,17 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void ffn_outer(FfnOuter p) {
   if (t0 < t1) {
     a.prefetch(t0, t1);
     bb.prefetch(t0, t1);
-    a.issue(t0, t1, lds[0], wave);
-    bb.issue(t0, t1, lds[0] + A_BYTES, wave);
+    a.issue(t0, t1, lds, wave);
+    bb.issue(t0, t1, lds + A_BYTES, wave);
     a.prefetch(t0 + KT, t1);
     bb.prefetch(t0 + KT, t1);
   }
-  int b = 0;
-  for (int t = t0; t < t1; t += KT, b ^= 1) {
+  unsigned char *now = lds, *next = lds + STAGE;
+  for (int t = t0; t < t1; t += KT) {
     stage_wait<0>();
     if (t + KT < t1) {
-      a.issue(t + KT, t1, lds[b ^ 1], wave);
-      bb.issue(t + KT, t1, lds[b ^ 1] + A_BYTES, wave);
+      a.issue(t + KT, t1, next, wave);
+      bb.issue(t + KT, t1, next + A_BYTES, wave);
       a.prefetch(t + 2 * KT, t1);
       bb.prefetch(t + 2 * KT, t1);
     }
@@ -622,9 +621,9 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void ffn_outer(FfnOuter p) {
     for (int k = 0; k < 2; ++k) {
       u32x4 fa[NI], fb[NJ];
 #pragma unroll
-      for (int i = 0; i < NI; ++i) fa[i] = SideA::frag(lds[b], k, wm * NI + i, g, n);
+      for (int i = 0; i < NI; ++i) fa[i] = SideA::frag(now, k, wm * NI + i, g, n);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) fb[j] = SideB::frag(lds[b] + A_BYTES, k, wn * NJ + j, g, n);
+      for (int j = 0; j < NJ; ++j) fb[j] = SideB::frag(now + A_BYTES, k, wn * NJ + j, g, n);
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -634,6 +633,9 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void ffn_outer(FfnOuter p) {
         for (int j = 0; j < NJ; ++j) sum[j] = Mma<T>::run(ones, fb[j], sum[j]);
       }
     }
+    unsigned char* const swap = now;
+    now = next;
+    next = swap;
   }
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
@@ -646,6 +648,22 @@ __global__ __launch_bounds__(64 * WM * WN, OCC) void ffn_outer(FfnOuter p) {
       if (m < p.M) *reinterpret_cast<f32x4*>(out + m) = acc[i][j];
     }
     if (sums && g == 0) p.bias[(long)split * p.N + nr] = sum[j][0];
+  }
+}
+
+// PADDED: the tokens' rows of x (the first problem's a) and dy (the second's b)
+// come from the list.
+template <int WM, int WN, int NI, int NJ, bool PADDED, int OCC>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void ffn_outer(FfnOuters ps) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * KT * ES * 16 * (NI * WM + NJ * WN)];
+  const int wg = blockIdx.x;
+  if constexpr (PADDED) {
+    if (wg < ps.first)
+      outer_tile<WM, WN, NI, NJ, true, false>(ps.p[0], ps, wg, lds);
+    else
+      outer_tile<WM, WN, NI, NJ, false, true>(ps.p[1], ps, wg - ps.first, lds);
+  } else {
+    outer_tile<WM, WN, NI, NJ, false, false>(ps.p[wg >= ps.first], ps, wg >= ps.first ? wg - ps.first : wg, lds);
   }
 }
 
@@ -696,16 +714,17 @@ Tile pick(const FfnProduct& p, int mats, bool redo) {
 }
 
 template <int WM, int WN, int NI, int NJ, int OCC>
-void launch_outer(const FfnOuter& p, hipStream_t st) {
-  constexpr int TM = 16 * NI * WM, TN = 16 * NJ * WN;
-  const int total = p.splits * ((p.M + TM - 1) / TM) * ((p.N + TN - 1) / TN), grid = (total + 7) / 8 * 8;
-  constexpr int NT = 64 * WM * WN;
-  if (p.rows_a)
-    ffn_outer<WM, WN, NI, NJ, true, false, OCC><<<grid, NT, 0, st>>>(p);
-  else if (p.rows_b)
-    ffn_outer<WM, WN, NI, NJ, false, true, OCC><<<grid, NT, 0, st>>>(p);
+void launch_outer(FfnOuters& ps, hipStream_t st) {
+  constexpr int TM = 16 * NI * WM, TN = 16 * NJ * WN, NT = 64 * WM * WN;
+  int grid = 0;
+  for (const FfnOuter& p : ps.p) {
+    if (&p == &ps.p[1]) ps.first = grid;
+    grid += (p.splits * ((p.M + TM - 1) / TM) * ((p.N + TN - 1) / TN) + 7) / 8 * 8;
+  }
+  if (ps.rows)
+    ffn_outer<WM, WN, NI, NJ, true, OCC><<<grid, NT, 0, st>>>(ps);
   else
-    ffn_outer<WM, WN, NI, NJ, false, false, OCC><<<grid, NT, 0, st>>>(p);
+    ffn_outer<WM, WN, NI, NJ, false, OCC><<<grid, NT, 0, st>>>(ps);
 }
 
 }  // namespace
@@ -754,7 +773,7 @@ int FST_CAT(ffn_product_, FST_NAME)(int mode, const FfnProduct& p, hipStream_t s
   return hipGetLastError() == hipSuccess ? FST_OK : FST_ELAUNCH;
 }
 
-int FST_CAT(ffn_outer_, FST_NAME)(const FfnOuter& p, bool large, hipStream_t st) {
+int FST_CAT(ffn_outer_, FST_NAME)(FfnOuters& p, bool large, hipStream_t st) {
   if constexpr (!F32) {
     if (large) launch_outer<2, 4, 8, 4, 1>(p, st);
   }
