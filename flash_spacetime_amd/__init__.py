@@ -27,6 +27,7 @@ from .reference import (  # noqa: F401
 
 __all__ = [
     "SpacetimeAttention",
+    "SpacetimeBlock",
     "flash_spacetime_attention",
     "flash_spacetime_attention_varlen",
     "flash_spacetime_attention_qkv",
@@ -51,6 +52,7 @@ __all__ = [
 
 _OPS = {
     "SpacetimeAttention": "attention",
+    "SpacetimeBlock": "attention",
     "flash_spacetime_attention": "forward",
     "flash_spacetime_attention_varlen": "forward",
     "flash_spacetime_attention_qkv": "forward",

@@ -1,4 +1,6 @@
-"""Model-side caller: `Attention_rel`-shaped multi-head attention on the fused op.
+"""Model-side callers: `Attention_rel`-shaped multi-head attention on the fused
+op, and the transformer block around it (`Block_rel`-shaped, on the fused layer
+norm and gated feed-forward block).
 
 graphnet reaches the reference operator through `Block_rel.forward_flash`
 (reference README.md:105-116): the module projects q, k and v with
@@ -119,3 +121,87 @@ class SpacetimeAttention(nn.Module):
         out = flash_spacetime_attention(q, k, v, feats, self.rel_proj.weight, self.rel_proj.bias, seqlens,
                                         None, *flags, key_padding_mask=key_padding_mask)
         return self.proj(merge_heads(out))
+
+
+class SpacetimeBlock(nn.Module):
+    """Pre-norm transformer block: spacetime attention and a gated feed-forward.
+
+        x = x + attn(norm1(x));  x = x + ffn(norm2(x))
+
+    as graphnet's `Block_rel` runs around the reference's operator (reference
+    README.md:105-116), its two-layer MLP replaced by the gated block. `norm1`,
+    `norm2`, `attn` (`SpacetimeAttention`) carry Block_rel's names; `ffn_gate`,
+    `ffn_up`, `ffn_down` are the feed-forward's linears. `hidden` defaults to 8/3
+    dim, rounded up to a multiple of 64 (the parameters of an ungated block of 4
+    dim).
+
+    `forward(x, feats, seqlens | key_padding_mask)` takes padded events `x [B, L,
+    dim]`, or with `cu_seqlens` packed ones `[T, dim]`, and returns the same
+    shape; padding rows are neither normalised nor multiplied and come back as
+    zeros. A stack saves a pass over the rows per block by leaving the last sum
+    to the next block's norm: `defer=True` returns `(x, branch)`, whose sum is the
+    block's output, and `branch=` takes the one the block before deferred.
+    """
+
+    def __init__(self, dim: int, num_heads: int = 8, channels: int = 16, hidden: Optional[int] = None,
+                 qkv_bias: bool = False, head_dim: Optional[int] = None, activation: str = "silu",
+                 ffn_bias: bool = True, eps: float = 1e-5, use_attn_bias: bool = True,
+                 use_activation_bias: bool = True, device=None, dtype=None) -> None:
+        super().__init__()
+        fk = {"device": device, "dtype": dtype}
+        if hidden is None:
+            hidden = -(-8 * dim // (3 * 64)) * 64
+        self.norm1 = nn.LayerNorm(dim, eps=eps, **fk)
+        self.attn = SpacetimeAttention(dim, num_heads, channels, qkv_bias, head_dim, use_attn_bias,
+                                       use_activation_bias, **fk)
+        self.norm2 = nn.LayerNorm(dim, eps=eps, **fk)
+        self.ffn_gate = nn.Linear(dim, hidden, bias=ffn_bias, **fk)
+        self.ffn_up = nn.Linear(dim, hidden, bias=ffn_bias, **fk)
+        self.ffn_down = nn.Linear(hidden, dim, bias=ffn_bias, **fk)
+        self.activation = activation
+
+    def forward(self, x: Tensor, feats: Tensor, seqlens: Optional[Tensor] = None,
+                key_padding_mask: Optional[Tensor] = None, cu_seqlens: Optional[Tensor] = None,
+                branch: Optional[Tensor] = None, defer: bool = False):
+        from .forward import _is_front_packed, _valid_from_mask
+
+        if cu_seqlens is not None and (seqlens is not None or key_padding_mask is not None):
+            raise ValueError("packed input takes cu_seqlens only (no lengths or mask)")
+        if x.dim() != (2 if cu_seqlens is not None else 3):
+            raise ValueError(f"x must be [T, dim] with cu_seqlens, else [B, L, dim], got {tuple(x.shape)}")
+        if key_padding_mask is None and seqlens is not None and seqlens.dim() == 2:
+            key_padding_mask, seqlens = seqlens, None
+        if key_padding_mask is not None:
+            if seqlens is not None:
+                raise ValueError("pass either seqlens or key_padding_mask, not both")
+            valid = _valid_from_mask(key_padding_mask, x.shape[1])
+            if not _is_front_packed(valid):
+                return self._scattered(x, feats, valid, branch, defer)
+            seqlens = valid.sum(1, dtype=torch.int32)
+        if cu_seqlens is None and seqlens is None:
+            raise ValueError("seqlens, key_padding_mask or cu_seqlens is required")
+        return self._block(x, feats, seqlens, cu_seqlens, branch, defer)
+
+    def _block(self, x, feats, seqlens, cu_seqlens, branch, defer):
+        from .feed_forward import flash_gated_feed_forward
+        from .norm import flash_layer_norm
+
+        n1, n2 = self.norm1, self.norm2
+        if branch is None:
+            y = flash_layer_norm(x, n1.weight, n1.bias, n1.eps, seqlens=seqlens)
+        else:
+            y, x = flash_layer_norm(branch, n1.weight, n1.bias, n1.eps, residual=x, seqlens=seqlens)
+        a = self.attn(y, feats, seqlens, cu_seqlens=cu_seqlens)
+        y, x = flash_layer_norm(a, n2.weight, n2.bias, n2.eps, residual=x, seqlens=seqlens)
+        f = flash_gated_feed_forward(y, self.ffn_gate.weight, self.ffn_up.weight, self.ffn_down.weight,
+                                     self.ffn_gate.bias, self.ffn_up.bias, self.ffn_down.bias, self.activation,
+                                     seqlens=seqlens)
+        return (x, f) if defer else x + f
+
+    def _scattered(self, x, feats, valid, branch, defer):
+        """Masks with holes: the valid tokens as packed events, put back afterwards."""
+        cu = torch.zeros(x.shape[0] + 1, dtype=torch.int32, device=x.device)
+        cu[1:] = torch.cumsum(valid.sum(1, dtype=torch.int32), 0, dtype=torch.int32)
+        out = self._block(x[valid], feats[valid], None, cu, None if branch is None else branch[valid], defer)
+        back = lambda t: t.new_zeros(*x.shape[:2], t.shape[-1]).index_put((valid,), t)  # noqa: E731
+        return tuple(back(t) for t in out) if defer else back(out)

@@ -39,9 +39,10 @@ struct Library {
   decltype(&fst_last_error) last_error = nullptr;
 } lib;
 
+// The block operators' entry points may be left out: theirs stay as they were.
 void bind_library(size_t supported, size_t fwd_ws, size_t fwd, size_t bwd_ws, size_t bwd, size_t last_error,
                   size_t norm_fwd, size_t norm_ws, size_t norm_bwd, size_t ffn_fwd, size_t ffn_ws, size_t ffn_bwd) {
-  bind_block_library(norm_fwd, norm_ws, norm_bwd, ffn_fwd, ffn_ws, ffn_bwd, last_error);
+  if (norm_fwd) bind_block_library(norm_fwd, norm_ws, norm_bwd, ffn_fwd, ffn_ws, ffn_bwd, last_error);
   lib.supported = reinterpret_cast<decltype(lib.supported)>(supported);
   lib.forward_workspace_bytes = reinterpret_cast<decltype(lib.forward_workspace_bytes)>(fwd_ws);
   lib.forward = reinterpret_cast<decltype(lib.forward)>(fwd);
@@ -277,7 +278,11 @@ py::object backward(const Dims& dims, const Tensor& q, const std::optional<Tenso
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.attr("build_id") = FST_BUILD_ID;
   m.attr("torch_version") = FST_TORCH_VERSION;
-  m.def("bind_library", &bind_library);
+  m.def("bind_library", &bind_library, py::arg("supported"), py::arg("forward_workspace_bytes"), py::arg("forward"),
+        py::arg("backward_workspace_bytes"), py::arg("backward"), py::arg("last_error"),
+        py::arg("layer_norm_forward") = 0, py::arg("layer_norm_backward_workspace_bytes") = 0,
+        py::arg("layer_norm_backward") = 0, py::arg("ffn_forward") = 0, py::arg("ffn_backward_workspace_bytes") = 0,
+        py::arg("ffn_backward") = 0);
   m.def("forward", &forward);
   m.def("backward", &backward);
   define_block_operators(m);

@@ -1,0 +1,148 @@
+"""GPU tests of SpacetimeBlock: attention, layer norm and the gated feed-forward
+block run together, as a model runs them, against the block's definition in
+float64 on the CPU (the attention oracle, torch's layer norm, linears), output
+and every gradient.
+
+Tolerances as those of the attention module's test (2e-2 bf16; float32 2e-4 and,
+for gradients, 1e-3, the attention's own bounds): the norms and the
+feed-forward add relative errors of 2^-8 and 2^-24 each, well inside.
+"""
+
+import copy
+
+import pytest
+import torch
+from torch.nn import functional as F
+
+import oracle
+from tests._cases import rel_err, seed_of
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    from flash_spacetime_amd import SpacetimeBlock, attention_rel_oracle_inputs, merge_heads
+
+DEV = "cuda"
+
+
+def _weights(ref, gen):
+    with torch.no_grad():
+        for name, p in ref.named_parameters():
+            v = torch.randn(p.shape, generator=gen, dtype=torch.float64) * (p.shape[-1] ** -0.5)
+            p.copy_(1 + 0.1 * v if name in ("norm1.weight", "norm2.weight") else v)
+
+
+def _reference(ref, x, feats, valid):
+    mask = oracle.float_padding_mask(valid, torch.float64)
+    q, k, v = attention_rel_oracle_inputs(ref.attn, ref.norm1(x), None)
+    att = oracle.attention(q, k, v, feats, ref.attn.rel_proj.weight, ref.attn.rel_proj.bias, key_padding_mask=mask)
+    x = x + ref.attn.proj(merge_heads(att))
+    y = ref.norm2(x)
+    act = {"silu": F.silu, "gelu": F.gelu}[ref.activation]
+    return x + ref.ffn_down(act(ref.ffn_gate(y)) * ref.ffn_up(y))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("mask", ["lengths", "front_mask", "holes"])
+@pytest.mark.parametrize("activation,bias", [("silu", True), ("gelu", False)])
+def test_block_matches_its_definition(dtype, mask, activation, bias):
+    batch, length, dim = 4, 40, 128
+    gen = torch.Generator().manual_seed(seed_of("block", dtype, mask, activation))
+    ref = SpacetimeBlock(dim, 4, qkv_bias=True, activation=activation, ffn_bias=bias, dtype=torch.float64)
+    assert ref.ffn_gate.weight.shape == (384, 128)
+    _weights(ref, gen)
+    mod = copy.deepcopy(ref).to(DEV, dtype)
+    with torch.no_grad():
+        for p, r in zip(mod.parameters(), ref.parameters()):
+            r.copy_(p.double().cpu())
+    x64 = torch.randn(batch, length, dim, generator=gen, dtype=torch.float64).to(dtype).double()
+    feats = torch.randn(batch, length, 5, generator=gen, dtype=torch.float64)
+    if mask == "holes":
+        valid = torch.rand(batch, length, generator=gen) < 0.6
+        valid[:, 3] = True
+    else:
+        valid = torch.arange(length)[None, :] < torch.tensor([length, 17, 1, 30])[:, None]
+    kwargs = ({"seqlens": valid.sum(1).to(DEV)} if mask == "lengths" else {"key_padding_mask": (~valid).to(DEV)})
+    gw = torch.randn(batch, length, dim, generator=gen, dtype=torch.float64)
+
+    x = x64.to(DEV, dtype)
+    x[~valid.to(DEV)] = float("nan")  # what padding holds is nobody's business
+    x.requires_grad_(True)
+    # the attention is handed norm1's rows, whose padding is zeros
+    out = mod(x, feats.to(DEV), **kwargs)
+    out.backward(gw.to(DEV, dtype))
+    assert bool((out.detach()[~valid.to(DEV)] == 0).all()) and bool((x.grad[~valid.to(DEV)] == 0).all())
+
+    xr = x64.clone().requires_grad_(True)
+    want = _reference(ref, xr, feats, valid)
+    vm = valid[..., None].expand(want.shape)
+    (want * (gw.to(dtype).double() * vm)).sum().backward()
+    tol = 2e-2 if dtype == torch.bfloat16 else 2e-4
+    gtol = 2e-2 if dtype == torch.bfloat16 else 1e-3
+    assert rel_err(out.detach().double().cpu() * vm, want.detach() * vm) <= tol
+    assert rel_err(x.grad.double().cpu(), xr.grad) <= gtol
+    for (name, p), r in zip(mod.named_parameters(), ref.parameters()):
+        err = rel_err(p.grad.double().cpu(), r.grad)
+        assert err <= gtol, f"grad {name}: relative error {err:.3e}"
+
+
+@pytest.mark.parametrize("layout", ["padded", "packed"])
+def test_deferred_sums_and_packed_events_agree(layout):
+    """Two blocks, float32: the second one's norm adds the first one's branch
+    (the same sums, rounded once as torch's), and packed events give the valid
+    rows of the padded ones."""
+    dim, lens = 96, torch.tensor([23, 1, 11, 40])
+    gen = torch.Generator().manual_seed(7)
+    blocks = [SpacetimeBlock(dim, 3, device=DEV) for _ in range(2)]
+    x = torch.randn(4, 40, dim, generator=gen).to(DEV)
+    feats = torch.randn(4, 40, 4, generator=gen).to(DEV)
+    valid = torch.arange(40)[None, :].to(DEV) < lens[:, None].to(DEV)
+    sl = lens.to(DEV)
+
+    def plain():
+        h = blocks[0](x, feats, sl)
+        return blocks[1](h, feats, sl)
+
+    want = plain()
+    if layout == "padded":
+        h, branch = blocks[0](x, feats, sl, defer=True)
+        got = blocks[1](h, feats, sl, branch=branch)
+        assert torch.equal(got, want)
+        h, branch = blocks[1](h, feats, sl, branch=branch, defer=True)
+        assert torch.equal(h + branch, want)
+    else:
+        cu = torch.tensor([0, *lens.cumsum(0).tolist()], device=DEV, dtype=torch.int32)
+        h, branch = blocks[0](x[valid], feats[valid], cu_seqlens=cu, defer=True)
+        got = blocks[1](h, feats[valid], cu_seqlens=cu, branch=branch)
+        assert rel_err(got.detach().double().cpu(), want.detach()[valid].double().cpu()) <= 1e-5
+
+
+def test_training_step_reaches_every_parameter():
+    """A stack's gradients are finite and not all zero, an event of no tokens
+    among them. (Updated bf16 weights say nothing: a step below 2^-8 leaves a norm
+    weight of 1 as it was.)"""
+    blocks = torch.nn.ModuleList(SpacetimeBlock(128, 4, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    gen = torch.Generator().manual_seed(3)
+    x = torch.randn(6, 50, 128, generator=gen).to(DEV, torch.bfloat16)
+    feats = torch.randn(6, 50, 4, generator=gen).to(DEV)
+    sl = torch.tensor([50, 7, 0, 23, 1, 44], device=DEV)
+    h, branch = x, None
+    for blk in blocks:
+        h, branch = blk(h, feats, sl, branch=branch, defer=True)
+    ((h + branch).float() - 1).square().mean().backward()
+    for name, p in blocks.named_parameters():
+        assert bool(p.grad.isfinite().all()) and bool((p.grad != 0).any()), name
+
+
+def test_refusals():
+    blk = SpacetimeBlock(64, 2, device=DEV)
+    x, feats = torch.randn(2, 9, 64, device=DEV), torch.randn(2, 9, 4, device=DEV)
+    sl = torch.tensor([9, 4], device=DEV)
+    with pytest.raises(ValueError, match="required"):
+        blk(x, feats)
+    with pytest.raises(ValueError, match="not both"):
+        blk(x, feats, sl, torch.zeros(2, 9, dtype=torch.bool, device=DEV))
+    with pytest.raises(ValueError, match="cu_seqlens only"):
+        blk(x[0], feats[0], sl, cu_seqlens=torch.tensor([0, 9], device=DEV))
+    with pytest.raises(ValueError, match="x must be"):
+        blk(x[0], feats[0], sl)

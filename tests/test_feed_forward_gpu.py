@@ -330,3 +330,47 @@ def test_refusals():
         flash_gated_feed_forward(odd, torch.randn(24, 12, device=DEV), torch.randn(24, 12, device=DEV), torch.randn(12, 24, device=DEV))
     with pytest.raises(RuntimeError, match="GPU"):
         flash_gated_feed_forward(**{**good, "w_up": ws[1].cpu()})
+
+
+@pytest.mark.parametrize("name", ["fst_layer_norm_forward", "fst_layer_norm_backward", "fst_ffn_forward", "fst_ffn_backward"])
+@pytest.mark.parametrize("status", [-1, -2, -3, -4])
+def test_failed_calls_raise_and_refused_ones_take_the_python_path(name, status):
+    """The library's entry points replaced by host functions that return a status
+    (nothing is launched): a refused forward goes to the Python path, which runs
+    it; any other failure is raised, once."""
+    import ctypes
+
+    from flash_spacetime_amd import _lib, flash_layer_norm
+
+    base = ("fst_supported", "fst_forward_workspace_bytes", "fst_forward", "fst_backward_workspace_bytes", "fst_backward",
+            "fst_last_error")
+    block = ("fst_layer_norm_forward", "fst_layer_norm_backward_workspace_bytes", "fst_layer_norm_backward",
+             "fst_ffn_forward", "fst_ffn_backward_workspace_bytes", "fst_ffn_backward")
+    lib, calls = _lib.load(), []
+    res, args = _lib.SIGNATURES[name]
+    stub = ctypes.CFUNCTYPE(res, *args)(lambda *_: calls.append(name) or status)
+
+    def bind(**stubs):
+        _lib.host().bind_library(*(ctypes.cast(stubs.get(n, getattr(lib, n)), ctypes.c_void_p).value for n in base + block))
+
+    x, ws, bs, dy = _make((6,), 16, 24, torch.float32, True, "stubs")
+
+    def step():
+        if "norm" not in name:
+            return _run(x, ws, bs, "silu", None, dy)
+        leaf = x.clone().requires_grad_(True)
+        y = flash_layer_norm(leaf)
+        return [y, *torch.autograd.grad(y, leaf, dy)]
+
+    want = step()
+    try:
+        bind(**{name: stub})
+        if status in (-1, -2) and name.endswith("forward"):
+            assert all(torch.equal(a, b) for a, b in zip(step(), want))
+        else:
+            with pytest.raises(RuntimeError, match="flash_layer_norm" if "norm" in name else "flash_gated_feed_forward"):
+                step()
+    finally:
+        bind()
+    assert calls == [name]
+    assert all(torch.equal(a, b) for a, b in zip(step(), want))
