@@ -22,9 +22,6 @@ typedef FST_T T;
 constexpr int ES = sizeof(T);
 constexpr bool F32 = ES == 4;
 
-typedef __attribute__((address_space(3))) void* lds_ptr;
-typedef const __attribute__((address_space(1))) void* glb_ptr;
-
 // What loads past an operand's end read: 16 zero bytes.
 __device__ const u32x4 kZero16 = {0, 0, 0, 0};
 
@@ -63,9 +60,23 @@ __device__ __forceinline__ void stage_wait() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-// 16 bytes a lane from the buffer into LDS (wave-uniform base, lane l's at 16 l).
-__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, unsigned char* dst, int voff, int soff) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)dst, 16, voff, soff, 0, 0);
+// 16 bytes a lane into LDS, lane l's at dst + 16 l (dst is wave-uniform), from a
+// buffer (zeros past its range) or an address. Written out because the compiler
+// waits for every load into LDS in flight before the transposing LDS reads it
+// makes from their builtin, and for all LDS reads at once; these loads have no
+// output register, and stage_wait counts them. m0, which they take the LDS address
+// from, is reserved: nothing else of these kernels uses it.
+__device__ __forceinline__ unsigned lds_offset(const unsigned char* dst) {
+  return __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)dst);
+}
+__device__ __forceinline__ void load_to_lds(u32x4 buffer, const unsigned char* dst, int voff, int soff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds_offset(dst)),
+               "v"(voff), "s"(buffer), "s"(soff)
+               : "memory");
+}
+__device__ __forceinline__ void load_to_lds(const char* from, const unsigned char* dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds_offset(dst)), "v"(from)
+               : "memory");
 }
 
 // act(a), and with D its derivative. sigmoid from the hardware's exp2 and
@@ -195,10 +206,10 @@ __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
   // subtracts it from the buffer's size).
   const int range = (p.F - f0) * row_bytes;
   auto weight = [&](int k) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(p.w[k]) + (long)f0 * row_bytes),
-                                             (short)0, range, 0x00020000);
+    const uint64_t at = (uint64_t)p.w[k] + (uint64_t)f0 * row_bytes;  // a 48-bit address, stride 0
+    return u32x4{(unsigned)at, (unsigned)(at >> 32) & 0xffffu, (unsigned)range, 0x00020000u};
   };
-  const __amdgpu_buffer_rsrc_t wr0 = weight(0), wr1 = weight(C::MATS - 1), wr2 = weight(REDO ? 2 : 0);
+  const u32x4 wr0 = weight(0), wr1 = weight(C::MATS - 1), wr2 = weight(REDO ? 2 : 0);
   const char *xp[C::LT], *yp[REDO ? C::LT : 1];
 #pragma unroll
   for (int i = 0; i < C::LT; ++i) {
@@ -219,7 +230,7 @@ __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
 #pragma unroll
     for (int i = 0; i < C::LT; ++i) {
       const char* q = cut ? reinterpret_cast<const char*>(&kZero16) : rows[i] + s * 128l;
-      __builtin_amdgcn_global_load_lds((glb_ptr)q, (lds_ptr)(base + C::BF * 128 + i * WAVES * 1024), 16, 0, 0);
+      load_to_lds(q, base + C::BF * 128 + i * WAVES * 1024);
     }
   };
   auto issue = [&](int s, int b) __attribute__((always_inline)) {
@@ -487,14 +498,18 @@ __global__ __launch_bounds__(512, MODE == kFfnRedo && NJ == 4 ? 2 : 4) void ffn_
 // ---------------------------------------------------------------------------
 // Weights' gradients. LDS holds rows of tokens, features along them: 16-bit
 // types read them transposed (ds_read_tr16), float32 element by element. A
-// stage is 64 tokens (float32: 32) of the tile's M features of a and N of b. 32-byte
-// (float32: 64-byte) slices of 16 features are stored in an order that depends
-// on the row, so that the rows of a read pass cover the banks once.
+// stage is 32 tokens of the tile's M features of a and N of b, and all stages but
+// one are in flight: a token's row is a few lines far from the next row's, part of
+// which always comes from beyond L2 (two stages of 64 tokens took 1365 us, their
+// loads alone 876, the products alone 763: 65536 tokens, D = 1024, F = 2752 bf16; four
+// of 32 take 1092). float32, bound by the matrix cores, runs two. 32-byte (float32:
+// 64-byte) slices of 16 features are stored in an order that depends on the row, so
+// that the rows of a read pass cover the banks once.
 // ---------------------------------------------------------------------------
-constexpr int KT = 128 / ES;
+constexpr int KT = 32, OUTER_STAGES = F32 ? 2 : 4;
 
 // One operand's side: FEATS features, loaded by NT threads. MAP: the tokens' rows
-// come from a list, read a stage ahead so that no load waits for it.
+// come from a list, of which LDS holds the entries of a few steps (RowList).
 template <int FEATS, int NT, bool MAP>
 struct OuterSide {
   static constexpr int ROW = FEATS * ES;  // bytes of a token's row
@@ -505,15 +520,12 @@ struct OuterSide {
   const char* base[LOADS];  // this lane's part of row 0 in each load
   unsigned ld[LOADS];       // row stride in bytes; 0 where the features do not exist
   int r[LOADS];             // its row of the stage
-  int next[MAP ? LOADS : 1];
-  const int32_t* rows;
 
   // Order of the slices of row r, in 16-byte parts.
   static __device__ __forceinline__ int swizzle(int r) {
     return F32 ? (r & 3) << 2 : ROW % 256 ? ((r >> 1) & 3) << 1 : (r & 7) << 1;
   }
-  __device__ __forceinline__ void init(const void* p, const int32_t* map, long ld_elems, int f0, int count, int tid) {
-    rows = map;
+  __device__ __forceinline__ void init(const void* p, long ld_elems, int f0, int count, int tid) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int at = i * NT + tid;
@@ -524,31 +536,26 @@ struct OuterSide {
       ld[i] = in ? (unsigned)(ld_elems * ES) : 0;
     }
   }
-  __device__ __forceinline__ void prefetch(int t0, int t1) {
-    if constexpr (MAP) {
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) next[i] = rows[min(t0 + r[i], t1 - 1)];
-    }
-  }
-  __device__ __forceinline__ void issue(int t0, int t1, unsigned char* dst, int wave) const {
+  // rows: the step's entries of the list (MAP).
+  __device__ __forceinline__ void issue(int t0, int t1, const int32_t* rows, unsigned char* dst, int wave) const {
     const bool whole = t0 + KT <= t1;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const unsigned row = MAP ? next[MAP ? i : 0] : t0 + r[i];
+      const unsigned row = MAP ? rows[r[i]] : t0 + r[i];
       const char* q = base[i] + (uint64_t)row * ld[i];
       if (!whole) q = t0 + r[i] < t1 ? q : reinterpret_cast<const char*>(&kZero16);
-      __builtin_amdgcn_global_load_lds((glb_ptr)q, (lds_ptr)(dst + i * NT * 16 + wave * 1024), 16, 0, 0);
+      load_to_lds(q, dst + i * NT * 16 + wave * 1024);
     }
   }
-  // Subtile `sub` (16 features) of half k of the stage's tokens as a matrix-core
-  // operand. 16-bit: tokens 4 g + .., 16 + 4 g + .. of the half in the lane's
-  // eight slots; float32: step e (of four) holds token 4 e + g.
-  static __device__ __forceinline__ u32x4 frag(const unsigned char* tile, int k, int sub, int g, int n) {
+  // Subtile `sub` (16 features) of the stage's tokens as a matrix-core operand.
+  // 16-bit: tokens 4 g + .., 16 + 4 g + .. in the lane's eight slots; float32: step
+  // e (of four) holds token 4 e + g.
+  static __device__ __forceinline__ u32x4 frag(const unsigned char* tile, int sub, int g, int n) {
     if constexpr (F32) {
       u32x4 v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int r = 16 * k + 4 * e + g;
+        const int r = 4 * e + g;
         v[e] = *reinterpret_cast<const unsigned*>(tile + r * ROW + (((sub << 2) ^ swizzle(g)) << 4) + 4 * n);
       }
       return v;
@@ -556,7 +563,7 @@ struct OuterSide {
       typedef short s16x4 __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
       const int r = 4 * g + (n >> 2), at = (((sub << 1) ^ swizzle(r)) << 4) + 8 * (n & 3);
-      const unsigned char* p = tile + (32 * k + r) * ROW + at;
+      const unsigned char* p = tile + r * ROW + at;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)p);
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p + 16 * ROW));
       const u32x2 a = __builtin_bit_cast(u32x2, lo), c = __builtin_bit_cast(u32x2, hi);
@@ -566,7 +573,8 @@ struct OuterSide {
 };
 
 template <int WM, int WN, int NI, int NJ, bool MA, bool MB>
-__device__ __forceinline__ void outer_tile(const FfnOuter& p, const FfnOuters& all, int wg, unsigned char* lds) {
+__device__ __forceinline__ void outer_tile(const FfnOuter& p, const FfnOuters& all, int wg, unsigned char* lds,
+                                           int32_t* list) {
   constexpr int TM = 16 * NI * WM, TN = 16 * NJ * WN, NT = 64 * WM * WN;
   typedef OuterSide<TM, NT, MA> SideA;
   typedef OuterSide<TN, NT, MB> SideB;
@@ -586,8 +594,8 @@ __device__ __forceinline__ void outer_tile(const FfnOuter& p, const FfnOuters& a
   const int wm = wave % WM, wn = wave / WM, g = lane >> 4, n = lane & 15;
   SideA a;
   SideB bb;
-  a.init(p.a, all.rows, p.lda, m0, p.M, tid);
-  bb.init(p.b, all.rows, p.ldb, n0, p.N, tid);
+  a.init(p.a, p.lda, m0, p.M, tid);
+  bb.init(p.b, p.ldb, n0, p.N, tid);
   // The bias' gradient: the columns of b against a row of ones, in the first
   // waves of the first tile of m.
   const bool sums = p.bias && m0 == 0 && wm == 0;
@@ -600,30 +608,50 @@ __device__ __forceinline__ void outer_tile(const FfnOuter& p, const FfnOuters& a
 #pragma unroll
     for (int i = 0; i < NI; ++i) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  if (t0 < t1) {
-    a.prefetch(t0, t1);
-    bb.prefetch(t0, t1);
-    a.issue(t0, t1, lds, wave);
-    bb.issue(t0, t1, lds + A_BYTES, wave);
-    a.prefetch(t0 + KT, t1);
-    bb.prefetch(t0 + KT, t1);
-  }
-  unsigned char *now = lds, *next = lds + STAGE;
-  for (int t = t0; t < t1; t += KT) {
+  // The list's rows of the tokens, in LDS by chunks of NT, two at a time: loaded as
+  // the stages are, a chunk ahead of the steps that use it, so that no load waits
+  // for a load (rows read into registers a step ahead had the compiler wait for
+  // everything in flight: 585 against 335 us, 256 x 768 padded, D = 384, F = 1024).
+  constexpr bool MAP = MA || MB;
+  const auto load_rows = [&](int t) __attribute__((always_inline)) {
+    const int32_t* from = all.rows + min(t + tid, t1 - 1);
+    const int32_t* dst = list + ((t - t0) & (2 * NT - 1)) + 64 * wave;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(
+                     lds_offset(reinterpret_cast<const unsigned char*>(dst))),
+                 "v"(from)
+                 : "memory");
+  };
+  const auto issue = [&](int t, unsigned char* dst) __attribute__((always_inline)) {
+    const int32_t* rows = MAP ? list + ((t - t0) & (2 * NT - 1)) : nullptr;
+    a.issue(t, t1, rows, dst, wave);
+    bb.issue(t, t1, rows, dst + A_BYTES, wave);
+  };
+  if (MAP && t0 < t1) {
+    load_rows(t0);
     stage_wait<0>();
-    if (t + KT < t1) {
-      a.issue(t + KT, t1, next, wave);
-      bb.issue(t + KT, t1, next + A_BYTES, wave);
-      a.prefetch(t + 2 * KT, t1);
-      bb.prefetch(t + 2 * KT, t1);
-    }
+  }
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+  for (int q = 0; q < OUTER_STAGES - 1; ++q)
+    if (t0 + q * KT < t1) issue(t0 + q * KT, lds + q * STAGE);
+  constexpr int LOADS = SideA::LOADS + SideB::LOADS;  // a step's; those of the list only tighten the wait
+  static_assert(NT >= (2 * OUTER_STAGES - 1) * KT, "a chunk of the list has landed before its first step is loaded");
+  int b = 0;
+  for (int t = t0; t < t1; t += KT) {
+    // A wave has issued two steps' loads since this step's.
+    if (t + (OUTER_STAGES - 2) * KT < t1)
+      stage_wait<(OUTER_STAGES - 2) * LOADS>();
+    else
+      stage_wait<0>();
+    if (MAP && ((t - t0) & (NT - 1)) == 0 && t + NT < t1) load_rows(t + NT);
+    if (t + (OUTER_STAGES - 1) * KT < t1) issue(t + (OUTER_STAGES - 1) * KT, lds + (b == 0 ? OUTER_STAGES - 1 : b - 1) * STAGE);
+    const unsigned char* now = lds + b * STAGE;
+#pragma unroll
+    for (int k = 0; k < KT * ES / 64; ++k) {
       u32x4 fa[NI], fb[NJ];
 #pragma unroll
-      for (int i = 0; i < NI; ++i) fa[i] = SideA::frag(now, k, wm * NI + i, g, n);
+      for (int i = 0; i < NI; ++i) fa[i] = SideA::frag(now + k * (64 / ES) * SideA::ROW, wm * NI + i, g, n);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) fb[j] = SideB::frag(now + A_BYTES, k, wn * NJ + j, g, n);
+      for (int j = 0; j < NJ; ++j) fb[j] = SideB::frag(now + A_BYTES + k * (64 / ES) * SideB::ROW, wn * NJ + j, g, n);
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -633,9 +661,7 @@ __device__ __forceinline__ void outer_tile(const FfnOuter& p, const FfnOuters& a
         for (int j = 0; j < NJ; ++j) sum[j] = Mma<T>::run(ones, fb[j], sum[j]);
       }
     }
-    unsigned char* const swap = now;
-    now = next;
-    next = swap;
+    b = b == OUTER_STAGES - 1 ? 0 : b + 1;
   }
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
@@ -655,15 +681,16 @@ __device__ __forceinline__ void outer_tile(const FfnOuter& p, const FfnOuters& a
 // come from the list.
 template <int WM, int WN, int NI, int NJ, bool PADDED, int OCC>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void ffn_outer(FfnOuters ps) {
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * KT * ES * 16 * (NI * WM + NJ * WN)];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[OUTER_STAGES * KT * ES * 16 * (NI * WM + NJ * WN)];
   const int wg = blockIdx.x;
   if constexpr (PADDED) {
+    __shared__ __attribute__((aligned(256))) int32_t list[2 * 64 * WM * WN];
     if (wg < ps.first)
-      outer_tile<WM, WN, NI, NJ, true, false>(ps.p[0], ps, wg, lds);
+      outer_tile<WM, WN, NI, NJ, true, false>(ps.p[0], ps, wg, lds, list);
     else
-      outer_tile<WM, WN, NI, NJ, false, true>(ps.p[1], ps, wg - ps.first, lds);
+      outer_tile<WM, WN, NI, NJ, false, true>(ps.p[1], ps, wg - ps.first, lds, list);
   } else {
-    outer_tile<WM, WN, NI, NJ, false, false>(ps.p[wg >= ps.first], ps, wg >= ps.first ? wg - ps.first : wg, lds);
+    outer_tile<WM, WN, NI, NJ, false, false>(ps.p[wg >= ps.first], ps, wg >= ps.first ? wg - ps.first : wg, lds, nullptr);
   }
 }
 
