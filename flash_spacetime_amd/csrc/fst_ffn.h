@@ -56,18 +56,14 @@ struct FfnOuters {
 };
 
 typedef int (*ffn_product_fn)(int mode, const FfnProduct&, hipStream_t);
-typedef int (*ffn_outer_fn)(FfnOuters&, bool large, hipStream_t);
+typedef int (*ffn_outer_fn)(FfnOuters&, int tile, hipStream_t);
 
 #define FST_FFN_DECL(name)                                      \
   int ffn_product_##name(int mode, const FfnProduct&, hipStream_t); \
-  int ffn_outer_##name(FfnOuters&, bool large, hipStream_t);
+  int ffn_outer_##name(FfnOuters&, int tile, hipStream_t);
 FST_FFN_DECL(bf16)
 FST_FFN_DECL(f16)
 FST_FFN_DECL(f32)
 #undef FST_FFN_DECL
-
-// Tile of an outer product: features of M and of N a workgroup takes; two small
-// ones or one large one a CU.
-constexpr int kOuterSmall = 128, kOuterLarge = 256;
 
 }  // namespace fst

@@ -174,29 +174,28 @@ void launch_rows(const int32_t* seqlens, int B, int L, int32_t* map, void* out, 
                                                                         static_cast<unsigned char*>(out), (long)D * es);
 }
 
-// Tile and token runs of the weights' gradients [2 F, D] and [D, F]: the least of
-// the rounds of workgroups over the chip, at the rates of large and small tiles (a
-// full chip in bf16: 65536 tokens, M = 1024, N = 5504 920 against 1003 us; M = 2752, N =
-// 1024 474 / 538), plus the runs' partials written and read. float32 is as fast
-// in small tiles and has only those.
+// Tile (features a side) and token runs of the weights' gradients [2 F, D] and [D,
+// F]: the least of the rounds of workgroups over the chip, at the rates a full
+// chip reached (PFLOP/s, bf16: 1.1 in large tiles, one a CU: 65536 tokens, D = 1024,
+// F = 2752, 9 runs 1105 us; 0.72 in small ones, two a CU: 4 runs 1412; 100500 tokens, D
+// = 384, F = 1024, 7 runs 334 where large tiles leave a third empty and take 360),
+// plus the runs' partials written and read. float32 is as fast in small tiles and
+// has only those.
 struct OuterPlan {
-  bool large;
-  int splits;
+  int tile, splits;
 };
 
 OuterPlan plan_outer(int dtype, long tokens, int D, int F) {
-  OuterPlan best{false, 1};
+  OuterPlan best{128, 1};
   double least = -1;
-  for (const bool large : {false, true}) {
-    if (large && dtype == FST_F32) continue;
-    const int e = large ? kOuterLarge : kOuterSmall;
-    const auto tiles_of = [e](int m, int n) { return (long)((m + e - 1) / e) * ((n + e - 1) / e); };
-    const long tiles = tiles_of(D, 2 * F) + tiles_of(F, D), slots = large ? 256 : 512;
-    const double rate = (dtype == FST_F32 ? 0.12e15 : large ? 0.8e15 : 0.72e15) / slots;
+  for (const int e : {128, 256}) {
+    if (e == 256 && dtype == FST_F32) continue;
+    const long tiles = (long)((D + e - 1) / e) * ((2 * F + e - 1) / e + (F + e - 1) / e), slots = e == 256 ? 256 : 512;
+    const double rate = (dtype == FST_F32 ? 0.12e15 : e == 256 ? 1.1e15 : 0.72e15) / slots;
     for (int s = 1; s <= 64 && (s == 1 || s * 256l <= tokens); ++s) {
       const double work = (double)tokens / s * 2 * e * e / rate;
-      const double t = (double)((tiles * s + slots - 1) / slots) * work + s * 24.0 * D * F / 4e12;
-      if (least < 0 || t < least) best = OuterPlan{large, s}, least = t;
+      const double t = (double)((tiles * s + slots - 1) / slots) * work + s * 24.0 * D * F / 5e12;
+      if (least < 0 || t < least) best = OuterPlan{e, s}, least = t;
     }
   }
   return best;
@@ -399,7 +398,7 @@ int fst_ffn_backward(int dtype, int activation, int B, int L, int D, int F, cons
     o.p[0] = FfnOuter{x, ws + l.dadu, (long)x_stride, 2l * F, D, 2 * F, first ? l.outer.splits : 0, p0,
                       db_gate || db_up ? b0 : nullptr};
     o.p[1] = FfnOuter{hidden, dy, F, (long)dy_stride, F, D, second ? l.outer.splits : 0, p1, db_down ? b1 : nullptr};
-    rc = outer_of(dtype)(o, l.outer.large, st);
+    rc = outer_of(dtype)(o, l.outer.tile, st);
     if (rc != FST_OK) return fail(rc, "feed-forward weight gradient launch failed");
     const long df = (long)D * F;
     const float* part[6] = {p0, p0 + df, p1, b0, b0 + F, b1};

@@ -677,21 +677,19 @@ __device__ __forceinline__ void outer_tile(const FfnOuter& p, const FfnOuters& a
   }
 }
 
-// PADDED: the tokens' rows of x (the first problem's a) and dy (the second's b)
-// come from the list.
-template <int WM, int WN, int NI, int NJ, bool PADDED, int OCC>
-__global__ __launch_bounds__(64 * WM * WN, OCC) void ffn_outer(FfnOuters ps) {
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[OUTER_STAGES * KT * ES * 16 * (NI * WM + NJ * WN)];
+// A workgroup's tile is DT of D by FT of F (or 2 F) features: D is the first
+// problem's m and the second's n. PADDED: the tokens' rows of x (the first's a) and
+// dy (the second's b) come from the list.
+template <int DT, int FT, int WF, bool PADDED, int OCC>
+__global__ __launch_bounds__(128 * WF, OCC) void ffn_outer(FfnOuters ps) {
+  constexpr int ND = DT / 16, NF = FT / 16;
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[OUTER_STAGES * KT * ES * (DT + FT)];
+  __shared__ __attribute__((aligned(256))) int32_t list[PADDED ? 2 * 128 * WF : 1];
   const int wg = blockIdx.x;
-  if constexpr (PADDED) {
-    __shared__ __attribute__((aligned(256))) int32_t list[2 * 64 * WM * WN];
-    if (wg < ps.first)
-      outer_tile<WM, WN, NI, NJ, true, false>(ps.p[0], ps, wg, lds, list);
-    else
-      outer_tile<WM, WN, NI, NJ, false, true>(ps.p[1], ps, wg - ps.first, lds, list);
-  } else {
-    outer_tile<WM, WN, NI, NJ, false, false>(ps.p[wg >= ps.first], ps, wg >= ps.first ? wg - ps.first : wg, lds, nullptr);
-  }
+  if (wg < ps.first)
+    outer_tile<2, WF, ND / 2, NF / WF, PADDED, false>(ps.p[0], ps, wg, lds, list);
+  else
+    outer_tile<2, WF, NF / 2, ND / WF, false, PADDED>(ps.p[1], ps, wg - ps.first, lds, list);
 }
 
 template <int MODE, int WF, int WT, int NI, int NJ, int ST, int OCC>
@@ -740,18 +738,17 @@ Tile pick(const FfnProduct& p, int mats, bool redo) {
   return middle <= small ? kMiddle : kSmall;
 }
 
-template <int WM, int WN, int NI, int NJ, int OCC>
+template <int DT, int FT, int WF, int OCC>
 void launch_outer(FfnOuters& ps, hipStream_t st) {
-  constexpr int TM = 16 * NI * WM, TN = 16 * NJ * WN, NT = 64 * WM * WN;
-  int grid = 0;
-  for (const FfnOuter& p : ps.p) {
-    if (&p == &ps.p[1]) ps.first = grid;
-    grid += (p.splits * ((p.M + TM - 1) / TM) * ((p.N + TN - 1) / TN) + 7) / 8 * 8;
-  }
+  const auto tiles = [](const FfnOuter& p, int m, int n) {
+    return (p.splits * ((p.M + m - 1) / m) * ((p.N + n - 1) / n) + 7) / 8 * 8;
+  };
+  ps.first = tiles(ps.p[0], DT, FT);
+  const int grid = ps.first + tiles(ps.p[1], FT, DT);
   if (ps.rows)
-    ffn_outer<WM, WN, NI, NJ, true, OCC><<<grid, NT, 0, st>>>(ps);
+    ffn_outer<DT, FT, WF, true, OCC><<<grid, 128 * WF, 0, st>>>(ps);
   else
-    ffn_outer<WM, WN, NI, NJ, false, OCC><<<grid, NT, 0, st>>>(ps);
+    ffn_outer<DT, FT, WF, false, OCC><<<grid, 128 * WF, 0, st>>>(ps);
 }
 
 }  // namespace
@@ -800,11 +797,11 @@ int FST_CAT(ffn_product_, FST_NAME)(int mode, const FfnProduct& p, hipStream_t s
   return hipGetLastError() == hipSuccess ? FST_OK : FST_ELAUNCH;
 }
 
-int FST_CAT(ffn_outer_, FST_NAME)(FfnOuters& p, bool large, hipStream_t st) {
+int FST_CAT(ffn_outer_, FST_NAME)(FfnOuters& p, int tile, hipStream_t st) {
   if constexpr (!F32) {
-    if (large) launch_outer<2, 4, 8, 4, 1>(p, st);
+    if (tile == 256) launch_outer<256, 256, 4, 1>(p, st);
   }
-  if (F32 || !large) launch_outer<2, 2, 4, 4, 2>(p, st);
+  if (tile == 128) launch_outer<128, 128, 2, 2>(p, st);
   return hipGetLastError() == hipSuccess ? FST_OK : FST_ELAUNCH;
 }
 
