@@ -177,8 +177,8 @@ void launch_rows(const int32_t* seqlens, int B, int L, int32_t* map, void* out, 
 // Tile (features a side) and token runs of the weights' gradients [2 F, D] and [D,
 // F]: the least of the rounds of workgroups over the chip, at the rates a full
 // chip reached (PFLOP/s, bf16: 1.1 in large tiles, one a CU: 65536 tokens, D = 1024,
-// F = 2752, 9 runs 1105 us; 0.72 in small ones, two a CU: 4 runs 1412; 100500 tokens, D
-// = 384, F = 1024, 7 runs 334 where large tiles leave a third empty and take 360),
+// F = 2752, 9 runs 1105 us; 0.8 in small ones, two a CU: 4 runs 1412; 100500 tokens of
+// 196608, D = 384, F = 1024, 7 runs 334 where large tiles leave a third empty and take 360),
 // plus the runs' partials written and read. float32 is as fast in small tiles and
 // has only those.
 struct OuterPlan {
@@ -191,7 +191,7 @@ OuterPlan plan_outer(int dtype, long tokens, int D, int F) {
   for (const int e : {128, 256}) {
     if (e == 256 && dtype == FST_F32) continue;
     const long tiles = (long)((D + e - 1) / e) * ((2 * F + e - 1) / e + (F + e - 1) / e), slots = e == 256 ? 256 : 512;
-    const double rate = (dtype == FST_F32 ? 0.12e15 : e == 256 ? 1.1e15 : 0.72e15) / slots;
+    const double rate = (dtype == FST_F32 ? 0.12e15 : e == 256 ? 1.1e15 : 0.8e15) / slots;
     for (int s = 1; s <= 64 && (s == 1 || s * 256l <= tokens); ++s) {
       const double work = (double)tokens / s * 2 * e * e / rate;
       const double t = (double)((tiles * s + slots - 1) / slots) * work + s * 24.0 * D * F / 5e12;
