@@ -83,9 +83,9 @@ __device__ __forceinline__ void load_to_lds(const char* from, const unsigned cha
 // reciprocal (1 ulp each). Phi(a) = erfc(-a / sqrt 2) / 2 with Abramowitz and
 // Stegun's formula 7.1.26 for erfc (absolute error 1.5e-7), whose exp(-a^2 / 2)
 // is also the density in the derivative.
-template <bool D>
-__device__ __forceinline__ float activate(int kind, float a, float& slope) {
-  if (kind == FST_GELU) {
+template <int KIND, bool D>
+__device__ __forceinline__ float activate(float a, float& slope) {
+  if constexpr (KIND == FST_GELU) {
     const float x = fabsf(a) * 0.70710678118654752f;
     const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
     const float e = __expf(-x * x);
@@ -94,16 +94,35 @@ __device__ __forceinline__ float activate(int kind, float a, float& slope) {
     const float phi = a < 0.f ? q : 1.f - q;
     if constexpr (D) slope = fmaf(a * e, 0.39894228040143268f, phi);
     return a * phi;
+  } else {
+    float z = a, dz = 1.f;  // the sigmoid's argument and its derivative
+    if constexpr (KIND == FST_GELU_TANH) {
+      const float c = 1.59576912160573071f, s = a * a;  // 2 sqrt(2 / pi)
+      z = c * a * fmaf(0.044715f, s, 1.f);
+      if constexpr (D) dz = c * fmaf(3.f * 0.044715f, s, 1.f);
+    }
+    const float g = __builtin_amdgcn_rcpf(1.f + __expf(-z));
+    const float h = a * g;
+    if constexpr (D) slope = fmaf(h * (1.f - g), dz, g);  // 0 * dz, not 0 * inf, where a * dz overflows
+    return h;
   }
-  float z = a, dz = 1.f;  // the sigmoid's argument and its derivative
-  if (kind == FST_GELU_TANH) {
-    const float c = 1.59576912160573071f, s = a * a;  // 2 sqrt(2 / pi)
-    z = c * a * fmaf(0.044715f, s, 1.f);
-    if constexpr (D) dz = c * fmaf(3.f * 0.044715f, s, 1.f);
-  }
-  const float g = __builtin_amdgcn_rcpf(1.f + __expf(-z));
-  if constexpr (D) slope = g * fmaf(a * dz, 1.f - g, 1.f);
-  return a * g;
+}
+
+// The same for N elements in place: one choice of the kind for all of them.
+template <int KIND, bool D, int N>
+__device__ __forceinline__ void activate_each(float* v, float* slope) {
+  float unused;
+#pragma unroll
+  for (int e = 0; e < N; ++e) v[e] = activate<KIND, D>(v[e], D ? slope[e] : unused);
+}
+template <bool D, int N>
+__device__ __forceinline__ void activate_run(int kind, float* v, float* slope) {
+  if (kind == FST_SILU)
+    activate_each<FST_SILU, D, N>(v, slope);
+  else if (kind == FST_GELU)
+    activate_each<FST_GELU, D, N>(v, slope);
+  else
+    activate_each<FST_GELU_TANH, D, N>(v, slope);
 }
 
 // N consecutive elements: loads and stores of `n` of them (a multiple of 8).
@@ -323,7 +342,6 @@ __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
   }
 
   // Epilogue: NE features of one token at a time.
-  float unused;
 #pragma unroll
   for (int q = 0; q < NF / GS; ++q) {
     const int f = f0 + (wf * (NF / GS) + q) * 16 * GS + NE * g;
@@ -351,8 +369,9 @@ __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
           store_run<NE>(static_cast<T*>(p.out[1]) + at, left, v);
           store_run<NE>(static_cast<T*>(p.out[2]) + at, left, u);
         }
+        activate_run<false, NE>(p.act, v, nullptr);
 #pragma unroll
-        for (int e = 0; e < NE; ++e) v[e] = activate<false>(p.act, v[e], unused) * u[e];
+        for (int e = 0; e < NE; ++e) v[e] *= u[e];
         store_run<NE>(static_cast<T*>(p.out[0]) + at, left, v);
       } else if constexpr (MODE == kFfnOut) {
         const long r = p.rows_out ? p.rows_out[t] : t;
@@ -365,11 +384,12 @@ __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
           load_run<NE>(static_cast<const T*>(p.gate) + (long)t * p.F + f, left, v);
           load_run<NE>(static_cast<const T*>(p.up) + (long)t * p.F + f, left, u);
         }
+        float slope[NE];
+        activate_run<true, NE>(p.act, v, slope);
 #pragma unroll
         for (int e = 0; e < NE; ++e) {
-          float slope;
-          const float act = activate<true>(p.act, v[e], slope);
-          v[e] = d[e] * u[e] * slope;
+          const float act = v[e];
+          v[e] = d[e] * u[e] * slope[e];
           u[e] = d[e] * act;
         }
         T* out = static_cast<T*>(p.out[0]) + (long)t * p.ldo + f;
@@ -467,28 +487,28 @@ __global__ __launch_bounds__(512, MODE == kFfnRedo && NJ == 4 ? 2 : 4) void ffn_
     *reinterpret_cast<T4*>(static_cast<T*>(out) + at) = o;
   };
   const long r = MODE == kFfnOut && p.rows_out ? p.rows_out[t] : t, at = r * p.ldo + f;
-  float unused;
   if constexpr (MODE == kFfnGate) {
     if (F32 && p.out[1]) {
       store(p.out[1], at, v[0]);
       store(p.out[2], at, v[1]);
     }
+    activate_run<false, 4>(p.act, v[0], nullptr);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[0][e] = activate<false>(p.act, v[0][e], unused) * v[1][e];
+    for (int e = 0; e < 4; ++e) v[0][e] *= v[1][e];
     store(p.out[0], at, v[0]);
   } else if constexpr (MODE == kFfnOut) {
     store(p.out[0], at, v[0]);
   } else {
-    float da[4], du[4];
+    float act[4], slope[4], da[4], du[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) act[e] = REDO ? v[0][e] : (float)static_cast<const T*>(p.gate)[(long)t * p.F + f + e];
+    activate_run<true, 4>(p.act, act, slope);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float a = REDO ? v[0][e] : (float)static_cast<const T*>(p.gate)[(long)t * p.F + f + e];
       const float u = REDO ? v[MATS - 1][e] : (float)static_cast<const T*>(p.up)[(long)t * p.F + f + e];
       const float dh = v[ACCS - 1][e];
-      float slope;
-      const float act = activate<true>(p.act, a, slope);
-      da[e] = dh * u * slope;
-      du[e] = dh * act;
+      da[e] = dh * u * slope[e];
+      du[e] = dh * act[e];
     }
     store(p.out[0], at, da);
     store(p.out[0], at + p.F, du);
