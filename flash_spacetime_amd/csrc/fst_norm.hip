@@ -77,30 +77,50 @@ __device__ __forceinline__ float group_sum(float x, float* red) {
 
 // Lane l's pieces of a row: elements (l + LPR i) V .. + V - 1, i < NC, zeros past
 // its end. EDGE: the row's length is no whole number of pieces or rows start
-// off 16 bytes; pieces are then read at element alignment and the last one by
-// elements.
+// off 16 bytes; pieces are then read at element alignment, the one that the row
+// ends in as the row's last V elements. Those are moved to their places, and what is
+// past the end cleared, when the piece is used: a load under a lane's own condition
+// would have to land before the next is issued (16 x 500 rows of 1367 f16, backward
+// 22.9 us so, 20.0 as it is).
 template <typename T, int LPR, int NC, bool EDGE>
 struct Pieces {
   static constexpr int V = kVec<T>, E = NC * V;
+  static constexpr bool SHORT = EDGE && NC == 1 && LPR == 16;  // rows may have fewer than V elements
   typename Piece<T>::V p[NC];
 
   static __device__ __forceinline__ int at(int l, int i) { return (l + LPR * i) * V; }
   __device__ __forceinline__ void load(const T* row, int l, int n) {
+    if (SHORT && n < V) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) p[0][j] = l == 0 && j < n ? row[j] : (T)0.f;
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int c = at(l, i);
-      if (EDGE ? c + V <= n : c < n) {
-        p[i] = EDGE ? *reinterpret_cast<const typename Piece<T>::VU*>(row + c)
-                    : *reinterpret_cast<const typename Piece<T>::V*>(row + c);
+      if constexpr (EDGE) {
+        p[i] = *reinterpret_cast<const typename Piece<T>::VU*>(row + min(c, n - V));
+      } else if (c < n) {
+        p[i] = *reinterpret_cast<const typename Piece<T>::V*>(row + c);
       } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) p[i][j] = EDGE && c + j < n ? row[c + j] : (T)0.f;
+        for (int j = 0; j < V; ++j) p[i][j] = (T)0.f;
       }
     }
   }
-  __device__ __forceinline__ void get(float* v) const {
+  __device__ __forceinline__ void get(float* v, int l, int n) const {
 #pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = (float)p[i / V][i % V];
+    for (int i = 0; i < NC; ++i) {
+      typename Piece<T>::V q = p[i];
+      if (EDGE && at(LPR, i) > n && !(SHORT && n < V)) {
+        const int c = at(l, i);
+        const unsigned __int128 x = __builtin_bit_cast(unsigned __int128, q);
+        const int past = (V - n % V) % V;  // elements of the last piece past the row's end
+        q = __builtin_bit_cast(typename Piece<T>::V, c >= n ? 0 : c + V > n ? x >> (8 * (int)sizeof(T) * past) : x);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[i * V + j] = (float)q[j];
+    }
   }
   static __device__ __forceinline__ void store(T* row, int l, int n, const float* v) {
 #pragma unroll
@@ -112,10 +132,10 @@ struct Pieces {
           *reinterpret_cast<typename Piece<T>::VU*>(row + c) = q;
         else
           *reinterpret_cast<typename Piece<T>::V*>(row + c) = q;
-      } else if (EDGE) {
+      } else if (EDGE && c < n) {
 #pragma unroll
         for (int j = 0; j < V; ++j)
-          if (c + j < n) row[c + j] = q[j];
+          if (j < n % V) row[c + j] = q[j];
       }
     }
   }
@@ -188,10 +208,10 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_fwd(NormArgs a, in
     float v[E];
     float2 st = make_float2(0.f, 0.f);
     if (now) {
-      x0.get(v);
+      x0.get(v, l, n);
       if (a.r) {
         float q[E];
-        r0.get(q);
+        r0.get(q, l, n);
         // The norm is of the sum as it is returned, so that the backward, which
         // has only that, differentiates the same function.
 #pragma unroll
@@ -269,8 +289,8 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_bwd(NormGradArgs a
     float g[E];
     if (now) {
       float v[E];
-      r0.s.get(v);
-      r0.dy.get(g);
+      r0.s.get(v, l, n);
+      r0.dy.get(g, l, n);
       const float2 st = r0.st;
       float c1 = 0.f, c2 = 0.f;
 #pragma unroll
@@ -288,7 +308,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_bwd(NormGradArgs a
 #pragma unroll
         for (int i = 0; i < E; ++i) g[i] = st.y * (g[i] - c1 - v[i] * c2);
         if (a.ds) {
-          r0.ds.get(v);
+          r0.ds.get(v, l, n);
 #pragma unroll
           for (int i = 0; i < E; ++i) g[i] += v[i];
         }
@@ -402,11 +422,19 @@ bool plan_norm(int dtype, int n, NormPlan& p) {
   return false;
 }
 
-// Most workgroups. The forward's stay at work on rows of their own (one a row
-// group had taken 2 to 5 times as long: each loads the parameters). The
-// backward's each write one partial of dw and db; two a CU keep enough rows in
-// flight (768 or 1024 are slower by what the partials cost).
-constexpr int kNormForward = 2048, kNormBlocks = 512;
+// Most workgroups. The forward's are those that its registers let run at once:
+// each loads the parameters and then has a row ahead in flight, which is lost on those
+// that would start after others (8000 rows of 1367 f16 3 / 4 / 8 a CU 15.2 / 18.0 / 21.1
+// us; 4000 of 16384 bf16 2 / 8 a CU 54 / 72). The backward's each write one partial of
+// dw and db; two a CU keep enough rows in flight (768 or 1024 are slower by what
+// the partials cost).
+constexpr int kNormBlocks = 512;
+
+int norm_forward_blocks(const NormPlan& p, int dtype) {
+  if (p.lpr == 1024) return 512;
+  const int registers = 22 + p.nc * (dtype == FST_F32 ? 30 : 44);  // of a lane: 54 .. 154
+  return 256 * (512 / registers);
+}
 
 int norm_rows_per_block(const NormPlan& p) { return p.lpr > 256 ? 1 : 256 / p.lpr; }
 
@@ -418,8 +446,8 @@ int norm_blocks(const NormPlan& p, long rows, int most) {
 bool aligned16(const void* p, long ld, size_t es) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * es % 16 == 0; }
 
 template <typename T>
-void launch_fwd(const NormPlan& p, const NormArgs& a, int w_f32, hipStream_t st) {
-  const int blocks = norm_blocks(p, a.rows, kNormForward), threads = p.lpr > 256 ? p.lpr : 256;
+void launch_fwd(const NormPlan& p, const NormArgs& a, int blocks, int w_f32, hipStream_t st) {
+  const int threads = p.lpr > 256 ? p.lpr : 256;
 #define FST_CASE(L, C)                                                                   \
   if constexpr (planned<T>(L, C)) {                                                      \
     if (p.lpr == L && p.nc == C) {                                                        \
@@ -500,13 +528,13 @@ int fst_layer_norm_forward(int dtype, int param_dtype, int B, int L, int N, cons
   p.edge = !aligned16(x, x_stride, es) || !aligned16(y, N, es) ||
            (residual && (!aligned16(residual, residual_stride, es) || !aligned16(sum, N, es)));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const int w_f32 = param_dtype == FST_F32;
+  const int w_f32 = param_dtype == FST_F32, blocks = norm_blocks(p, rows, norm_forward_blocks(p, dtype));
   if (dtype == FST_BF16)
-    launch_fwd<bf16>(p, a, w_f32, st);
+    launch_fwd<bf16>(p, a, blocks, w_f32, st);
   else if (dtype == FST_F16)
-    launch_fwd<f16>(p, a, w_f32, st);
+    launch_fwd<f16>(p, a, blocks, w_f32, st);
   else
-    launch_fwd<float>(p, a, w_f32, st);
+    launch_fwd<float>(p, a, blocks, w_f32, st);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(FST_ELAUNCH, "layer norm launch failed (%s)", hipGetErrorString(e));
   return FST_OK;
