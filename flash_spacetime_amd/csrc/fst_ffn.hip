@@ -390,8 +390,10 @@ int fst_ffn_backward(int dtype, int activation, int B, int L, int D, int F, cons
   }
   if (first || second) {
     FfnOuters o{};
-    o.count = seqlens ? rowmap : nullptr;
-    o.rows = map;
+    if (rows > 0) {  // without rows the forward has written no map
+      o.count = seqlens ? rowmap : nullptr;
+      o.rows = map;
+    }
     o.tokens = (int)rows;
     float *p0 = reinterpret_cast<float*>(ws + l.part0), *p1 = reinterpret_cast<float*>(ws + l.part1);
     float *b0 = reinterpret_cast<float*>(ws + l.bias0), *b1 = reinterpret_cast<float*>(ws + l.bias1);

@@ -115,6 +115,18 @@ def test_all_events_empty_and_no_rows():
     assert all(bool((t == 0).all()) for t in got[2:])
 
 
+@pytest.mark.parametrize("lead", [(0, 7), (3, 0)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_padded_batch_without_rows(dtype, lead):
+    """No event, or none of any length: the gradients of the weights are zeros,
+    whatever the memory that would have held the list of rows holds."""
+    x, ws, bs, dy = _make(lead, 64, 128, TYPES[dtype], True, "rowless")
+    lens = torch.full((lead[0],), 5, dtype=torch.int32, device=DEV)
+    got = _run(x, ws, bs, "silu", lens, dy)
+    assert got[0].shape == got[1].shape == (*lead, 64)
+    assert all(bool((t == 0).all()) for t in got[2:])
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("view", ["row_stride", "odd_stride", "transposed", "offset", "expanded", "batch_first"])
 def test_strides_and_alignments(dtype, view):
