@@ -19,13 +19,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 
-// The value rounded to T (to nearest, ties to even) once; everything before
-// it is held in float32.
-template <typename T>
-__device__ __forceinline__ T to_type(float x) {
-  return (T)x;
-}
-
 // Elements of a 16-byte piece.
 template <typename T>
 constexpr int kVec = 16 / (int)sizeof(T);

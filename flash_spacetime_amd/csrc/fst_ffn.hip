@@ -55,8 +55,8 @@ __global__ __launch_bounds__(256) void ffn_rows(const int32_t* seqlens, int B, i
 }
 
 // out[c * ldo + r] = in[r * C + c] for up to three matrices [R, C]; the workgroups
-// after theirs write zeros into the padding rows of `pad`, slices of an event
-// each (seqlens given).
+// after theirs write zeros into the padding rows of `pad` (seqlens given), `slices`
+// of them for an event and every `groups`-th after it.
 struct Transposes {
   const void* in[3];
   void* out[3];
@@ -65,7 +65,7 @@ struct Transposes {
   const int32_t* seqlens;
   unsigned char* pad;
   long row_bytes;
-  int L, slices;
+  int B, L, groups, slices;
 };
 
 // A workgroup turns a 64 x 64 tile through LDS, 16 bytes at a time in memory (by
@@ -77,9 +77,10 @@ __global__ __launch_bounds__(256) void ffn_transpose(Transposes p) {
   typedef E Part __attribute__((ext_vector_type(V)));
   __shared__ __attribute__((aligned(16))) E tile[64][64 + V];
   if ((int)blockIdx.x >= p.first[2]) {
-    const int at = (int)blockIdx.x - p.first[2], e = at / p.slices, slice = at - e * p.slices;
-    zero_padding(p.pad, p.row_bytes, e, p.L, event_len(p.seqlens, e, p.L), (long)slice * 256 + threadIdx.x,
-                 (long)p.slices * 256);
+    const int at = (int)blockIdx.x - p.first[2], slice = at % p.slices;
+    for (long e = at / p.slices; e < p.B; e += p.groups)
+      zero_padding(p.pad, p.row_bytes, (int)e, p.L, event_len(p.seqlens, (int)e, p.L), (long)slice * 256 + threadIdx.x,
+                   (long)p.slices * 256);
     return;
   }
   const int k = (int)blockIdx.x >= p.first[0] ? ((int)blockIdx.x >= p.first[1] ? 2 : 1) : 0;
@@ -339,9 +340,11 @@ int fst_ffn_backward(int dtype, int activation, int B, int L, int D, int F, cons
       t.seqlens = seqlens;
       t.pad = static_cast<unsigned char*>(dx);
       t.row_bytes = (long)D * es;
+      t.B = B;
       t.L = L;
-      t.slices = slices_of(B, L);
-      grid += B * t.slices;
+      t.groups = B < 16384 ? B : 16384;
+      t.slices = slices_of(t.groups, L);
+      grid += t.groups * t.slices;
     }
     if (es == 2)
       ffn_transpose<uint16_t><<<grid, 256, 0, st>>>(t);

@@ -115,6 +115,19 @@ def test_all_events_empty_and_no_rows():
     assert all(bool((t == 0).all()) for t in got[2:])
 
 
+def test_more_events_than_a_grid_has_workgroups():
+    """2^24 events of one row: their padding is zeroed by fewer workgroups."""
+    b, t = (1 << 24) + 3, torch.float16
+    x, ws, bs, _ = _make((64,), 8, 8, t, True, "events")
+    x = x.repeat(b // 64 + 1, 1)[:b].contiguous()
+    lens = (torch.arange(b, device=DEV) % 3 != 1).int()
+    valid = lens.bool()
+    a = _run(x[:, None], ws, bs, "silu", lens, x[:, None])
+    p = _run(x[valid], ws, bs, "silu", None, x[valid])
+    for got, want in zip(a[:2], p[:2]):
+        assert torch.equal(got[:, 0][valid], want) and bool((got[:, 0][~valid] == 0).all())
+
+
 @pytest.mark.parametrize("lead", [(0, 7), (3, 0)])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_padded_batch_without_rows(dtype, lead):
