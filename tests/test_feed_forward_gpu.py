@@ -178,6 +178,17 @@ def test_subsets_of_gradients():
             assert torch.equal(g, full[1 + i]), NAMES[1 + i]
 
 
+def test_one_tensor_in_two_places_and_a_graph_run_twice():
+    """Gate and up projection share weight and bias; the graph is kept."""
+    x, ws, bs, dy = _make((50,), 64, 128, torch.bfloat16, True, "shared")
+    _, _, dg, du, _, dbg, dbu, _ = _run(x, [ws[0], ws[0], ws[2]], [bs[0], bs[0], bs[2]], "gelu", None, dy)
+    w, b = ws[0].detach().requires_grad_(True), bs[0].detach().requires_grad_(True)
+    y = flash_gated_feed_forward(x, w, w, ws[2], b, b, bs[2], "gelu")
+    for keep in (True, False):
+        gw, gb = torch.autograd.grad(y, (w, b), dy, retain_graph=keep)
+        assert torch.equal(gw, dg + du) and torch.equal(gb, dbg + dbu)
+
+
 def test_activation_extremes():
     """Gates far into both tails: the activation and its derivative stay finite
     and right (a silu of -100 is -0, of 100 is 100)."""

@@ -206,6 +206,18 @@ def test_optional_parameters_and_gradients():
     assert float((torch.autograd.grad(y, rl, dy)[0].double().cpu() - want).abs().max()) <= 1e-4
 
 
+def test_one_tensor_in_two_places_and_a_graph_run_twice():
+    """The residual is x itself, weight and bias are one; the graph is kept."""
+    x, _, w, _, dy, ds = _make((37, 391), torch.bfloat16, torch.float32, True, "shared")
+    outs, (dx, dr, dw, db) = _run(x, x.clone(), w, w.clone(), None, dy, ds)
+    a, p = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    y, s = flash_layer_norm(a, p, p, residual=a)
+    assert torch.equal(y, outs[0]) and torch.equal(s, outs[1])
+    for keep in (True, False):
+        ga, gp = torch.autograd.grad((y, s), (a, p), (dy, ds), retain_graph=keep)
+        assert torch.equal(ga, dx + dr) and torch.equal(gp, dw + db)
+
+
 def test_rows_do_not_touch_each_other():
     """A row of NaN, one of infinities and one of the type's lowest value leave
     the others' bits alone; a constant row comes back as the bias."""
