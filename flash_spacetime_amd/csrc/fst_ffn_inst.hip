@@ -12,6 +12,7 @@
 // LDS layouts are the same bytes for every type.
 #include "fst_ffn.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace fst {
@@ -169,10 +170,30 @@ __device__ __forceinline__ bool pick_tile(int wg, int nf, int nt, int& f, int& t
 // bytes of k (whole lines of memory: 64-byte rows measured a fifth slower);
 // 16-byte part c of row r sits at c ^ ((r >> 1) & 7), so that the 16 rows of a
 // read pass cover the banks once. ST stages: the loads of ST - 1 k steps run while
-// a step is multiplied, one barrier a step.
+// a step is multiplied, one barrier a step. ST = 5: LDS holds five halves of stages
+// (one operand's), and the rows of the step after the next are on their way beside the
+// next step's weights (256 x 768 padded, D = 384, F = 1024 bf16: step 1222 -> 1198 us,
+// forward 360 -> 349; 65536 tokens, D = 1024, F = 2752: 4.06 -> 4.03 ms).
 //
 // kFfnRedo runs two contractions after each other, a and u from x and then dh
 // from dy, and holds all three.
+//
+// Bound by the matrix cores and the way to them: with 65536 tokens, D = 1024, F = 2752
+// in bf16 gate and up take 690 us (1.07 PFLOP/s), the output product 320 (1.15), dx 610
+// (1.21), kFfnRedo 1170 (0.95), where a library product of 8192 a side reaches 1.35
+// and one of the gate's shape 1.10. The matrix cores are busy half of the cycles, as
+// the LDS is (reads and the loads into it); no bank conflicts; four of five lines
+// come from L2. At K = 384 (100500 tokens, F = 1024: 208, 112, 205 and 352 us) a
+// workgroup's six steps stand beside its first loads and its stores (147 of 238 us
+// without an epilogue, before activations were chosen once per run). Measured and
+// slower or no faster: four waves of 128 x 128 (690 -> 830 us, the output product as
+// fast, with its LDS reads written ahead by hand), stores as whole lines
+// through LDS (236 -> 253 at K = 384), a workgroup that goes from tile to tile with the
+// next tile's first loads in flight (gate 210 -> 201 at K = 384, 690 -> 710 wide, kFfnRedo
+// spills and takes 413 and 1290), a higher wave priority around the products.
+// float32 (128 x 128 tiles; 16384 tokens, D = 512, F = 1408: 390, 185, 365 and kFfnGrad 270
+// us): matrix cores busy 80 to 85 % of the cycles, 63 % in kFfnGrad, which reads a and u
+// in its epilogue.
 template <int MODE, int WF, int WT, int NI, int NJ, int ST>
 struct Product {
   static constexpr int WAVES = WF * WT;
@@ -183,10 +204,12 @@ struct Product {
   static constexpr int FEATURES = 16 * NF * WF;    // of the output, a workgroup
   static constexpr int BF = 16 * NI * WF, BT = 16 * NJ * WT;
   static constexpr int LW = BF / (8 * WAVES), LT = BT / (8 * WAVES), LD = FEATURES / (8 * WAVES);
-  static constexpr int STAGE = (BF + BT) * 128;
+  static constexpr bool HALVES = ST == 5;
+  // A unit of LDS: a stage, or either operand's half of one.
+  static constexpr int UNIT = (HALVES ? std::max(BF, BT) : BF + BT) * 128;
   static constexpr int KE = 128 / ES;              // k of a step
   // Loads of a wave that are newer than a step's (at least: dh's steps have fewer).
-  static constexpr int NEWER = (ST - 2) * (LT + (MODE == kFfnRedo && LD < LW ? LD : LW));
+  static constexpr int NEWER = HALVES ? LT : (ST - 2) * (LT + (MODE == kFfnRedo && LD < LW ? LD : LW));
   static_assert(NF % 2 == 0 && BF % (8 * WAVES) == 0 && BT % (8 * WAVES) == 0 && FEATURES % (8 * WAVES) == 0, "tile");
 };
 
@@ -197,7 +220,7 @@ __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
   typedef Product<MODE, WF, WT, NI, NJ, ST> C;
   constexpr int NF = C::NF, GS = C::GS, NE = 4 * GS, WAVES = C::WAVES;
   constexpr bool REDO = MODE == kFfnRedo;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[ST][C::STAGE];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[ST][C::UNIT];
   const int tokens = p.count ? *p.count : p.tokens;
   const int nf = (p.F + C::FEATURES - 1) / C::FEATURES, nt = (tokens + C::BT - 1) / C::BT;
   int ft, tt;
@@ -245,30 +268,31 @@ __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
   // zeros in both operands.
   const int total = REDO ? 2 * steps : steps;
   auto cut_at = [&](int s) { return tail != 0 && s == steps - 1 && part * 16 >= tail; };
-  auto load_rows = [&](const char* const* rows, int s, unsigned char* base, bool cut) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < C::LT; ++i) {
-      const char* q = cut ? reinterpret_cast<const char*>(&kZero16) : rows[i] + s * 128l;
-      load_to_lds(q, base + C::BF * 128 + i * WAVES * 1024);
-    }
-  };
-  auto issue = [&](int s, int b) __attribute__((always_inline)) {
-    unsigned char* base = lds[b] + wave * 1024;
+  // Step v's rows of x, or dy after x's steps, and the weights'.
+  auto issue_rows = [&](int v, unsigned char* dst) __attribute__((always_inline)) {
+    const bool second = REDO && v >= steps;
+    const int s = second ? v - steps : v;
     const bool cut = cut_at(s);
 #pragma unroll
-    for (int i = 0; i < C::LW; ++i)
-      load_to_lds(C::MATS == 2 && mat[i] ? wr1 : wr0, base + i * WAVES * 1024, cut ? (int)0x80000000 : voff[i], s * 128);
-    load_rows(xp, s, base, cut);
+    for (int i = 0; i < C::LT; ++i) {
+      const char* row = second ? yp[REDO ? i : 0] : xp[i];
+      load_to_lds(cut ? reinterpret_cast<const char*>(&kZero16) : row + s * 128l, dst + (i * WAVES + wave) * 1024);
+    }
   };
-  auto issue_dh = [&](int s, int b) __attribute__((always_inline)) {
-    if constexpr (REDO) {
-      unsigned char* base = lds[b] + wave * 1024;
+  auto issue_weights = [&](int v, unsigned char* dst) __attribute__((always_inline)) {
+    if (REDO && v >= steps) {
+      const int s = v - steps;
       const bool cut = cut_at(s);
 #pragma unroll
       for (int i = 0; i < C::LD; ++i)
-        load_to_lds(wr2, base + i * WAVES * 1024,
+        load_to_lds(wr2, dst + (i * WAVES + wave) * 1024,
                     cut ? (int)0x80000000 : feature((i * WAVES + wave) >> 1) * row_bytes + part * 16, s * 128);
-      load_rows(yp, s, base, cut);
+    } else {
+      const bool cut = cut_at(v);
+#pragma unroll
+      for (int i = 0; i < C::LW; ++i)
+        load_to_lds(C::MATS == 2 && mat[i] ? wr1 : wr0, dst + (i * WAVES + wave) * 1024, cut ? (int)0x80000000 : voff[i],
+                    v * 128);
     }
   };
 
@@ -283,61 +307,74 @@ __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
     }
   }
   const int rd = n * 128, swz = (n >> 1) & 7;
+  if constexpr (C::HALVES) {
+    issue_rows(0, lds[0]);
+    issue_weights(0, lds[1]);
+    if (total > 1) issue_rows(1, lds[2]);
+  } else {
 #pragma unroll
-  for (int v = 0; v < ST - 1; ++v) {
-    if (v < steps)
-      issue(v, v);
-    else if (v < total)
-      issue_dh(v - steps, v);
+    for (int v = 0; v < ST - 1; ++v) {
+      if (v < total) {
+        issue_weights(v, lds[v]);
+        issue_rows(v, lds[v] + C::BF * 128);
+      }
+    }
   }
+  // Step v: it has landed, what the step before it read is free and loaded anew.
+  const unsigned char *at_rows, *at_weights;
   int b = 0;
-  // Step v has landed and the stage before it is read: that one can be loaded anew.
-  auto wait = [&](int v) __attribute__((always_inline)) {
-    if (v + ST - 2 < total)
+  auto step = [&](int v) __attribute__((always_inline)) {
+    if (v + (C::HALVES ? 1 : ST - 2) < total)
       stage_wait<C::NEWER>();
     else
       stage_wait<0>();
-    return b == 0 ? ST - 1 : b - 1;
+    const auto unit = [&](int i) { return lds[b + i < ST ? b + i : b + i - ST]; };
+    at_rows = unit(0) + rd + (C::HALVES ? 0 : C::BF * 128);
+    at_weights = unit(C::HALVES ? 1 : 0) + rd;
+    if constexpr (C::HALVES) {
+      if (v + 1 < total) issue_weights(v + 1, unit(3));
+      if (v + 2 < total) issue_rows(v + 2, unit(4));
+      b = b + 2 < ST ? b + 2 : b + 2 - ST;
+    } else {
+      if (v + ST - 1 < total) {
+        issue_weights(v + ST - 1, unit(ST - 1));
+        issue_rows(v + ST - 1, unit(ST - 1) + C::BF * 128);
+      }
+      b = b == ST - 1 ? 0 : b + 1;
+    }
   };
-  for (int s = 0; s < steps; ++s) {
-    const int free = wait(s), next = s + ST - 1;
-    if (next < steps)
-      issue(next, free);
-    else if (REDO && next < total)
-      issue_dh(next - steps, free);
+  for (int v = 0; v < steps; ++v) {
+    step(v);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const unsigned char* base = lds[b] + rd + (((4 * k + g) ^ swz) << 4);
+      const int c = ((4 * k + g) ^ swz) << 4;
       u32x4 fw[NI], fx[NJ];
 #pragma unroll
-      for (int i = 0; i < NI; ++i) fw[i] = read16(base + (wf * NI + i) * 2048);
+      for (int i = 0; i < NI; ++i) fw[i] = read16(at_weights + c + (wf * NI + i) * 2048);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) fx[j] = read16(base + C::BF * 128 + (wt * NJ + j) * 2048);
+      for (int j = 0; j < NJ; ++j) fx[j] = read16(at_rows + c + (wt * NJ + j) * 2048);
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
 #pragma unroll
         for (int i = 0; i < NI; ++i) acc[i][j] = Mma<T>::run(fw[i], fx[j], acc[i][j]);
     }
-    b = b == ST - 1 ? 0 : b + 1;
   }
   if constexpr (REDO) {
-    for (int s = 0; s < steps; ++s) {
-      const int free = wait(steps + s), next = s + ST - 1;
-      if (next < steps) issue_dh(next, free);
+    for (int v = steps; v < total; ++v) {
+      step(v);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        const unsigned char* base = lds[b] + rd + (((4 * k + g) ^ swz) << 4);
+        const int c = ((4 * k + g) ^ swz) << 4;
         u32x4 fw[NF], fx[NJ];
 #pragma unroll
-        for (int i = 0; i < NF; ++i) fw[i] = read16(base + (wf * NF + i) * 2048);
+        for (int i = 0; i < NF; ++i) fw[i] = read16(at_weights + c + (wf * NF + i) * 2048);
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) fx[j] = read16(base + C::BF * 128 + (wt * NJ + j) * 2048);
+        for (int j = 0; j < NJ; ++j) fx[j] = read16(at_rows + c + (wt * NJ + j) * 2048);
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
           for (int i = 0; i < NF; ++i) dh[i][j] = Mma<T>::run(fw[i], fx[j], dh[i][j]);
       }
-      b = b == ST - 1 ? 0 : b + 1;
     }
   }
 
@@ -736,8 +773,8 @@ void launch_few(const FfnProduct& p, hipStream_t st) {
 // with two stages 9.4 and 17.6 us where four take 7.3 and 12.8, [1024, 384] at K = 1024
 // and 2048). A k step (64 elements of 16 bits) of n workgroups on every CU takes about
 // 1.65 n, 0.54 n (one alone 0.64) and 0.24 n (alone 0.28) us, measured on [tokens, F,
-// K] = [65536, 2752, 1024], [7640, 768, 2048], [1024, 384, 2048] (bf16: large 362 / 58 / 48
-// us, middle 405 / 33 / 21, small - / 45 / 13). Up to 64 tokens the waves split k
+// K] = [65536, 2752, 1024], [7640, 768, 2048], [1024, 384, 2048] (bf16, in one run: large 362 /
+// 58 / 48 us, middle 405 / 33 / 21, small - / 45 / 13). Up to 64 tokens the waves split k
 // instead (ffn_few: 4 tokens, D = 768, F = 2048 7.4 + 15.3 us in 64 x 64 tiles, 6.2 + 5.6;
 // 187 tokens, D = 384, F = 1024 5.7 + 7.0 against 6.4 + 7.2). float32 is bound by the
 // matrix cores four times as long in each: as fast in the middle tile as in the
@@ -781,11 +818,11 @@ int FST_CAT(ffn_product_, FST_NAME)(int mode, const FfnProduct& p, hipStream_t s
   if constexpr (!F32) {
     if (tile == kLarge) {
       if (mode == kFfnGate)
-        launch<kFfnGate, 2, 4, 8, 4, 2, 1>(p, st);
+        launch<kFfnGate, 2, 4, 8, 4, 5, 1>(p, st);
       else if (mode == kFfnOut)
-        launch<kFfnOut, 2, 4, 8, 4, 2, 1>(p, st);
+        launch<kFfnOut, 2, 4, 8, 4, 5, 1>(p, st);
       else
-        launch<kFfnRedo, 2, 4, 8, 3, 2, 1>(p, st);
+        launch<kFfnRedo, 2, 4, 8, 3, 5, 1>(p, st);
       return hipGetLastError() == hipSuccess ? FST_OK : FST_ELAUNCH;
     }
   }

@@ -101,10 +101,11 @@ def flash_gated_feed_forward(
     computed, come back as zeros in the output and x's gradient, and add
     nothing to the weights' gradients.
 
-    Products accumulate in float32 on the matrix cores (bfloat16 and float16
-    round the projections and hidden rows to their type between them, as a
-    chain of linears does; float16 hidden rows past 65504 are infinite). Results
-    are bitwise reproducible.
+    Products accumulate in float32 on the matrix cores. bfloat16 and float16
+    round the hidden rows to their type between the products (float16 ones past
+    65504 are infinite) and the projections' gradients in the backward, which
+    forms the projections again, unrounded; float32 keeps them. "gelu" takes the
+    distribution function to 1e-7. Results are bitwise reproducible.
     """
     tensors = (x, w_gate, w_up, w_down, b_gate, b_up, b_down)
     if x.is_cuda and activation in ACTIVATIONS and all(t is None or type(t) in PLAIN for t in (*tensors, seqlens)):
