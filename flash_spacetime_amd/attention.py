@@ -109,14 +109,14 @@ class SpacetimeAttention(nn.Module):
             qkv = F.linear(x, w, bias).view(x.shape[0], 3, self.num_heads, self.head_dim)
             out = flash_spacetime_attention_qkv(qkv, feats, self.rel_proj.weight, self.rel_proj.bias, None, None,
                                                 *flags, cu_seqlens=cu_seqlens)
-            return self.proj(out.reshape(x.shape[0], -1))
+            return self.proj(out.flatten(-2))
         b, length, _ = x.shape
         if kv is None:
             w, bias = self.qkv_weight()
             qkv = F.linear(x, w, bias).view(b, length, 3, self.num_heads, self.head_dim)
             out = flash_spacetime_attention_qkv(qkv, feats, self.rel_proj.weight, self.rel_proj.bias, seqlens,
                                                 None, *flags, key_padding_mask=key_padding_mask)
-            return self.proj(out.reshape(b, length, -1))
+            return self.proj(out.flatten(-2))
         q, k, v = self.project_qkv(x, kv)
         out = flash_spacetime_attention(q, k, v, feats, self.rel_proj.weight, self.rel_proj.bias, seqlens,
                                         None, *flags, key_padding_mask=key_padding_mask)

@@ -134,6 +134,23 @@ def test_training_step_reaches_every_parameter():
         assert bool(p.grad.isfinite().all()) and bool((p.grad != 0).any()), name
 
 
+@pytest.mark.parametrize("shape", [(0, 7), (2, 0), (3, 5), (0,)], ids=["no_event", "no_length", "no_token", "packed"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+def test_batches_without_tokens(dtype, shape):
+    """Outputs are zeros of x's shape, and so is every gradient."""
+    blk = SpacetimeBlock(64, 2, device=DEV, dtype=dtype)
+    x = torch.ones(*shape, 64, device=DEV, dtype=dtype, requires_grad=True)
+    feats = torch.ones(*shape, 4, device=DEV)
+    if len(shape) == 1:
+        y = blk(x, feats, cu_seqlens=torch.zeros(1, dtype=torch.int32, device=DEV))
+    else:
+        y = blk(x, feats, torch.zeros(shape[0], dtype=torch.int32, device=DEV))
+    assert y.shape == x.shape and bool((y == 0).all())
+    grads = torch.autograd.grad(y, [x, *blk.parameters()], torch.ones_like(y), allow_unused=True)
+    for name, g in zip(["x", *(n for n, _ in blk.named_parameters())], grads):
+        assert g is None or bool((g == 0).all()), name
+
+
 def test_refusals():
     blk = SpacetimeBlock(64, 2, device=DEV)
     x, feats = torch.randn(2, 9, 64, device=DEV), torch.randn(2, 9, 4, device=DEV)
