@@ -654,14 +654,17 @@ __device__ __forceinline__ void outer_tile(const FfnOuter& p, const FfnOuters& a
   a.init(p.a, p.lda, m0, p.M, tid);
   bb.init(p.b, p.ldb, n0, p.N, tid);
   // The bias' gradient: the columns of b against a row of ones, in the first
-  // waves of the first tile of m.
+  // waves of the first tile of m. Sums of 256 tokens are added up apart: one chain over
+  // a run had a float32 column's rounding grow with its length.
   const bool sums = p.bias && m0 == 0 && wm == 0;
   const unsigned one = F32 ? 0x3f800000u : (__is_same(T, bf16) ? 0x3f803f80u : 0x3c003c00u);
   const u32x4 ones = {one, one, one, one};
   f32x4 acc[NI][NJ], sum[NJ];
+  float whole[NJ];
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     sum[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    whole[j] = 0.f;
 #pragma unroll
     for (int i = 0; i < NI; ++i) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -718,6 +721,13 @@ __device__ __forceinline__ void outer_tile(const FfnOuter& p, const FfnOuters& a
         for (int j = 0; j < NJ; ++j) sum[j] = Mma<T>::run(ones, fb[j], sum[j]);
       }
     }
+    if (sums && ((t - t0) & 255) == 256 - KT) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        whole[j] += sum[j][0];
+        sum[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+    }
     b = b == OUTER_STAGES - 1 ? 0 : b + 1;
   }
 #pragma unroll
@@ -730,7 +740,7 @@ __device__ __forceinline__ void outer_tile(const FfnOuter& p, const FfnOuters& a
       const int m = m0 + (wm * NI + i) * 16 + 4 * g;
       if (m < p.M) *reinterpret_cast<f32x4*>(out + m) = acc[i][j];
     }
-    if (sums && g == 0) p.bias[(long)split * p.N + nr] = sum[j][0];
+    if (sums && g == 0) p.bias[(long)split * p.N + nr] = whole[j] + sum[j][0];
   }
 }
 

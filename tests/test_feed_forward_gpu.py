@@ -178,6 +178,22 @@ def test_subsets_of_gradients():
             assert torch.equal(g, full[1 + i]), NAMES[1 + i]
 
 
+def test_bias_gradients_of_many_rows_in_float32():
+    """60000 rows beside weights of many tiles, whose runs of rows are long. A column
+    goes through chains of 64 additions (256 rows, four at a time), at most 235 (the
+    sums of 256 rows of all runs together) and one; the rounding of the k-th of n is
+    at most k / n 2^-24 of the whole, over sqrt 3 in the mean square, so a chain's is
+    sqrt(n / 9) 2^-24 and all of them sqrt(300 / 9) = 5.8. (One chain over each run
+    gave 6.5.)"""
+    x, ws, bs, dy = _make((60000,), 32, 3848, torch.float32, True, "many")
+    b = bs[2].detach().requires_grad_(True)
+    dy = 1 + 0.25 * dy
+    got, = torch.autograd.grad(flash_gated_feed_forward(x, *ws, *bs[:2], b, "silu"), b, dy)
+    want = dy.double().sum(0)
+    err = float((got.double() - want).norm() / want.norm())
+    assert err <= 5.8 * 2 ** -24, err * 2 ** 24
+
+
 def test_one_tensor_in_two_places_and_a_graph_run_twice():
     """Gate and up projection share weight and bias; the graph is kept."""
     x, ws, bs, dy = _make((50,), 64, 128, torch.bfloat16, True, "shared")
