@@ -5,7 +5,7 @@
 //
 // Both functions return None for anything but that form (tensors of several
 // devices or dtypes, subclasses, lengths that are not integers on the device,
-// calls the library refuses): the caller then takes the Python path, which
+// calls that torch records, calls the library refuses): the caller then takes the Python path, which
 // handles or rejects it. The library refuses before it launches a kernel. A
 // launch error raises. Nothing is kept between calls but the library's entry
 // points.
@@ -15,6 +15,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <optional>
 #include <stdexcept>
@@ -46,6 +47,11 @@ void check(int rc, const char* what, bool may_refuse) {
   if (may_refuse && (rc == FST_EINVAL || rc == FST_EUNSUPPORTED)) throw Refused();
   throw std::runtime_error(std::string(what) + ": " + lib.last_error());
 }
+
+// Whether torch's tracer is recording: it would take this path's outputs for
+// what at::empty gives, as it does not see the launch that fills them. The Python
+// path is recorded as a call.
+bool recorded() { return torch::jit::tracer::isTracing(); }
 
 bool plain(const Tensor& t, const at::Device& dev) {
   return t.defined() && t.layout() == at::kStrided && t.device() == dev && !at::isTensorSubclassLike(t) &&
@@ -230,7 +236,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
 py::object norm_call(const Tensor& x, const Maybe& residual, const Maybe& weight, const Maybe& bias, double eps,
                      const Maybe& seqlens) {
   const at::Device dev = x.device();
-  if (!lib.norm_forward || !dev.is_cuda() || !plain(x, dev) || !plain(residual, dev) || !plain(weight, dev) ||
+  if (!lib.norm_forward || !dev.is_cuda() || recorded() || !plain(x, dev) || !plain(residual, dev) || !plain(weight, dev) ||
       !plain(bias, dev) || !plain(seqlens, dev))
     return py::none();
   NormCall c;
@@ -341,7 +347,7 @@ struct FfnFunction : torch::autograd::Function<FfnFunction> {
 py::object ffn_call(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, const Maybe& bg,
                     const Maybe& bu, const Maybe& bd, int act, const Maybe& seqlens) {
   const at::Device dev = x.device();
-  if (!lib.ffn_forward || !dev.is_cuda()) return py::none();
+  if (!lib.ffn_forward || !dev.is_cuda() || recorded()) return py::none();
   for (const Tensor* t : {&x, &wg, &wu, &wd})
     if (!plain(*t, dev) || t->scalar_type() != x.scalar_type()) return py::none();
   for (const Maybe* t : {&bg, &bu, &bd})

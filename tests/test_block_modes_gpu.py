@@ -1,0 +1,61 @@
+"""GPU tests of the layer norm, the feed-forward block and SpacetimeBlock under
+torch's other ways of running a call: recorded, with forward-mode derivatives,
+under autocast."""
+
+import pytest
+import torch
+
+from tests._cases import seed_of
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    from flash_spacetime_amd import SpacetimeBlock, flash_gated_feed_forward, flash_layer_norm
+
+DEV = "cuda"
+
+
+def _randn(key, *shapes):
+    gen = torch.Generator().manual_seed(seed_of("modes", key))
+    return [torch.randn(*s, generator=gen).to(DEV) for s in shapes]
+
+
+def _calls():
+    """Both operators' calls: a function of its tensors, and those."""
+    x, r, w, b = _randn("norm", (50, 64), (50, 64), (64,), (64,))
+    wg, wu, wd = _randn("ffn", (128, 64), (128, 64), (64, 128))
+    return {
+        "norm": (lambda x, w, b: flash_layer_norm(x, w, b), [x, w, b]),
+        "norm_residual": (lambda x, r, w: sum(flash_layer_norm(x, w, residual=r)), [x, r, w]),
+        "ffn": (lambda *t: flash_gated_feed_forward(*t), [x, wg / 8, wu / 8, wd / 11]),
+    }
+
+
+def _leave_nan(*shapes):
+    """Memory of these shapes, freed, that holds NaN: what an output left unwritten shows."""
+    for _ in range(2):
+        _ = [torch.full(s, float("nan"), device=DEV) for s in shapes for _ in range(4)]
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("name", ["norm", "norm_residual", "ffn"])
+def test_traced_calls_compute(name, grad):
+    """torch.jit.trace records the operator as a call, also beside the host extension:
+    the traced function gives the operator's bits for inputs it has not seen."""
+    f, tensors = _calls()[name]
+    traced = torch.jit.trace(f, tuple(t.clone().requires_grad_(grad) for t in tensors), check_trace=False)
+    other = [1.5 * t.flip(0) for t in tensors]
+    want = f(*other)
+    _leave_nan(want.shape)
+    assert torch.equal(traced(*other), want)
+
+
+def test_traced_block_computes():
+    blk = SpacetimeBlock(64, 4, device=DEV)
+    x, feats = _randn("block", (2, 20, 64), (2, 20, 4))
+    lens = torch.tensor([20, 7], device=DEV)
+    traced = torch.jit.trace(blk, (x, feats, lens), check_trace=False)
+    other = 1.5 * x.flip(1)
+    want = blk(other, feats, lens)
+    _leave_nan(want.shape, (2, 20, 192))
+    assert torch.equal(traced(other, feats, lens), want)
