@@ -5,10 +5,10 @@
 //
 // Both functions return None for anything but that form (tensors of several
 // devices or dtypes, subclasses, lengths that are not integers on the device,
-// calls that torch records, calls the library refuses): the caller then takes the Python path, which
-// handles or rejects it. The library refuses before it launches a kernel. A
-// launch error raises. Nothing is kept between calls but the library's entry
-// points.
+// calls that torch records, forward-mode derivatives, calls the library
+// refuses): the caller then takes the Python path, which handles or rejects it.
+// The library refuses before it launches a kernel. A launch error raises.
+// Nothing is kept between calls but the library's entry points.
 #include "fst_block_host.h"
 
 #include <ATen/TensorSubclassLikeUtils.h>
@@ -53,9 +53,11 @@ void check(int rc, const char* what, bool may_refuse) {
 // path is recorded as a call.
 bool recorded() { return torch::jit::tracer::isTracing(); }
 
+// A tensor with a forward-mode derivative is not plain: without a node here its
+// derivative would be lost, and the Python path refuses it.
 bool plain(const Tensor& t, const at::Device& dev) {
   return t.defined() && t.layout() == at::kStrided && t.device() == dev && !at::isTensorSubclassLike(t) &&
-         !t.is_neg() && !t.is_conj();
+         !t.is_neg() && !t.is_conj() && !t._fw_grad(/*level=*/0).defined();
 }
 bool plain(const Maybe& t, const at::Device& dev) { return !t.has_value() || plain(*t, dev); }
 

@@ -4,6 +4,7 @@ under autocast."""
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from tests._cases import seed_of
 
@@ -59,3 +60,17 @@ def test_traced_block_computes():
     want = blk(other, feats, lens)
     _leave_nan(want.shape, (2, 20, 192))
     assert torch.equal(traced(other, feats, lens), want)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("name", ["norm", "norm_residual", "ffn"])
+def test_forward_mode_derivatives_are_refused(name, grad):
+    """They are not offered: a dual tensor in any place raises, with the host
+    extension as without it, and is not taken for a constant."""
+    f, tensors = _calls()[name]
+    for i, t in enumerate(tensors):
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(t.clone().requires_grad_(grad), torch.ones_like(t))
+            with pytest.raises(NotImplementedError, match="jvp"):
+                f(*tensors[:i], dual, *tensors[i + 1:])
+    f(*tensors)
