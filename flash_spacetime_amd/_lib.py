@@ -214,6 +214,21 @@ def require_gpu(t: torch.Tensor) -> None:
         )
 
 
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
+
+
+def recorded_by_fx() -> bool:
+    """Whether torch.fx's make_fx is recording: it sees the outputs allocated and
+    not the launch that fills them."""
+    return torch._C._get_dispatch_mode(_PROXY) is not None
+
+
+def refuse_fx_recording() -> None:
+    if recorded_by_fx():
+        raise RuntimeError("make_fx cannot record flash-spacetime's operators: the graph would return memory "
+                           "that nothing fills (torch.compile runs them between its graphs)")
+
+
 def frequencies(c: int) -> torch.Tensor:
     """The fp32 ladder the kernels embed with (host-side, no GPU needed)."""
     buf = (ctypes.c_float * (c // 2))()

@@ -29,7 +29,7 @@ def _native_backward(dims, q, k, v, pos4, w32, b32, lens, lse, grad_out, scale, 
     interleaved q (k and v None) (dqkv, None, None, dw, db); None where the call is
     not in the form it takes, runs another than the static plan, or the extension
     is not usable, for `_run_backward` to run or reject."""
-    if not (q.is_cuda and tune.static_only()):
+    if not (q.is_cuda and tune.static_only() and not _lib.recorded_by_fx()):
         return None
     host = _lib.host()
     if host is None:
@@ -48,6 +48,7 @@ def _run_backward(dims, q, k, v, pos4, w32, b32, lens, lse, grad_out, scale, vec
     kernels where it has grad_out's final shape, dtype and layout (the bf16
     rows kernel takes its reference D from it); otherwise it is left out,
     which changes nothing but the kernel's schedule of D updates."""
+    _lib.refuse_fx_recording()
     if grad_out.shape != q.shape:
         raise ValueError(f"grad_out must have the shape of the output {tuple(q.shape)}")
     interleaved = bool(dims[1] & _lib.FST_QKV_INTERLEAVED)

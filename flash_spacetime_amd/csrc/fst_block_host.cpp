@@ -12,6 +12,7 @@
 #include "fst_block_host.h"
 
 #include <ATen/TensorSubclassLikeUtils.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -48,10 +49,13 @@ void check(int rc, const char* what, bool may_refuse) {
   throw std::runtime_error(std::string(what) + ": " + lib.last_error());
 }
 
-// Whether torch's tracer is recording: it would take this path's outputs for
-// what at::empty gives, as it does not see the launch that fills them. The Python
-// path is recorded as a call.
-bool recorded() { return torch::jit::tracer::isTracing(); }
+// Whether torch's tracer or make_fx is recording: they would take this path's
+// outputs for what at::empty gives, as they do not see the launch that fills them.
+// The tracer records the Python path as a call; make_fx it refuses.
+bool recorded_by_fx() {
+  return c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value();
+}
+bool recorded() { return torch::jit::tracer::isTracing() || recorded_by_fx(); }
 
 // A tensor with a forward-mode derivative is not plain: without a node here its
 // derivative would be lost, and the Python path refuses it.
@@ -195,6 +199,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!recorded_by_fx(), "flash_layer_norm backward: make_fx cannot record it");
     const variable_list saved = ctx->get_saved_variables();
     const auto call = ctx->saved_data["call"].toIntVector();
     variable_list out(5);
@@ -318,6 +323,7 @@ struct FfnFunction : torch::autograd::Function<FfnFunction> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!recorded_by_fx(), "flash_gated_feed_forward backward: make_fx cannot record it");
     const variable_list v = ctx->get_saved_variables();
     const auto call = ctx->saved_data["call"].toIntVector();
     variable_list out(8);

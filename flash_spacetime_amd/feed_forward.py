@@ -62,6 +62,7 @@ class _GatedFeedForward(torch.autograd.Function):
     def backward(ctx: Any, dy: Tensor):  # type: ignore[override]
         x, wg, wu, wd, bg, bu, lens, hidden, gate, up, rowmap = ctx.saved_tensors
         dtype, act, b, length, d, f, x_stride, shape = ctx.meta
+        _lib.refuse_fx_recording()
         need = ctx.needs_input_grad[:7]
         like = {"device": x.device, "dtype": x.dtype}
         dyr, dy_stride = token_rows(dy.to(x.dtype), 16)

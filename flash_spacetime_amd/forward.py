@@ -143,6 +143,7 @@ class _Prepared:
 
     def __init__(self, q, k, v, feats, weight, bias, seqlens, scale, use_attn_bias,
                  use_activation_bias, cu_seqlens, interleaved: bool = False):
+        _lib.refuse_fx_recording()
         for t in (q, k, v, feats, weight):
             _lib.require_gpu(t)
         if q.dtype not in _DTYPES:
@@ -267,7 +268,8 @@ def _native_forward(q, k, v, feats, weight, bias, lens, scale, use_attn_bias, us
     or rejects it. interleaved: q is one contiguous interleaved tensor, k and v
     are None. Returns (out, lse, q, k, v, pos4,
     weight, bias, lens, dims, scale) as `_Prepared` and `_run_forward` form them."""
-    if not (q.is_cuda and tune.static_only() and (scale is None or type(scale) in (float, int))
+    if not (q.is_cuda and tune.static_only() and not _lib.recorded_by_fx()
+            and (scale is None or type(scale) in (float, int))
             and (k is None) == interleaved and (v is None) == interleaved):
         return None
     # Tensor subclasses keep their own methods: the Python path calls them.

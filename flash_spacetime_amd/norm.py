@@ -58,6 +58,7 @@ def batch_of_rows(x: Tensor, seqlens: Optional[Tensor]) -> Tuple[int, int, Optio
 
 def check_rows(x: Tensor, *others: Optional[Tensor]) -> int:
     """The C dtype of x, once x and the others are tensors of one GPU."""
+    _lib.refuse_fx_recording()
     for t in (x, *others):
         if t is not None:
             _lib.require_gpu(t)
@@ -115,6 +116,7 @@ class _LayerNorm(torch.autograd.Function):
         dtype, param_dtype, b, length, n, s_stride, shape, w_dtype, b_dtype = ctx.meta
         if dy is None and ds is None:
             return (None,) * 6
+        _lib.refuse_fx_recording()
         need_x, need_r, need_w, need_b = ctx.needs_input_grad[:4]
         dev = s.device
         dyr, dy_stride = token_rows(torch.zeros(shape, device=dev, dtype=s.dtype) if dy is None else dy.to(s.dtype))

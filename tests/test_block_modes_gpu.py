@@ -5,13 +5,15 @@ under autocast."""
 import pytest
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from tests._cases import seed_of
 
 pytestmark = pytest.mark.gpu
 
 if torch.cuda.is_available():
-    from flash_spacetime_amd import SpacetimeBlock, flash_gated_feed_forward, flash_layer_norm
+    from flash_spacetime_amd import (SpacetimeBlock, flash_gated_feed_forward, flash_layer_norm,
+                                     flash_spacetime_attention, flash_spacetime_attention_qkv)
 
 DEV = "cuda"
 
@@ -74,3 +76,31 @@ def test_forward_mode_derivatives_are_refused(name, grad):
             with pytest.raises(NotImplementedError, match="jvp"):
                 f(*tensors[:i], dual, *tensors[i + 1:])
     f(*tensors)
+
+
+@pytest.mark.parametrize("name", ["norm", "norm_residual", "ffn", "attention", "attention_qkv"])
+def test_make_fx_is_refused(monkeypatch, name):
+    """make_fx would record the outputs' allocation and not the launch: it is
+    refused, forward and backward, with the host extension and without."""
+    from flash_spacetime_amd import _lib
+
+    if name.startswith("attention"):
+        q, feats, w = _randn("fx", (1, 50, 3, 2, 32), (1, 50, 4), (32, 16))
+        lens = torch.tensor([50], device=DEV)
+        heads = lambda x, i: x[:, :, i].transpose(1, 2)  # noqa: E731
+        f = ((lambda x: flash_spacetime_attention(heads(x, 0), heads(x, 1), heads(x, 2), feats, w, None, lens))
+             if name == "attention" else lambda x: flash_spacetime_attention_qkv(x, feats, w, None, lens))
+        tensors = [q]
+    else:
+        f, tensors = _calls()[name]
+    for host in (True, False):
+        with monkeypatch.context() as m:
+            if not host:
+                m.setattr(_lib, "host", lambda: None)
+            with pytest.raises(RuntimeError, match="make_fx"):
+                make_fx(f)(*tensors)
+            leaf = tensors[0].clone().requires_grad_(True)
+            y = f(leaf, *tensors[1:])
+            with pytest.raises(RuntimeError, match="make_fx"):
+                make_fx(lambda g: torch.autograd.grad(y, leaf, g, retain_graph=True))(torch.ones_like(y))
+            torch.autograd.grad(y, leaf, torch.ones_like(y))
