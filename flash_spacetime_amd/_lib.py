@@ -116,6 +116,7 @@ SIGNATURES = {
          _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp],
     ),
     "fst_max_event_len": (_i, [_i, _i, _i, _i, _i]),
+    "fst_zero_tail": (_i, [_i, _i, _vp, _vp, _sz, _vp]),
     "fst_frequencies": (None, [_i, ctypes.POINTER(ctypes.c_float)]),
     "fst_last_error": (ctypes.c_char_p, []),
     "fst_version": (ctypes.c_char_p, []),

@@ -43,7 +43,10 @@ class SpacetimeAttention(nn.Module):
     `forward(x, feats, seqlens | key_padding_mask)` takes `x [B, L, dim]`,
     detector features `feats [B, L, F >= 4]` and the event lengths, and
     returns `[B, L, dim]`; with `cu_seqlens` it takes packed events, `x
-    [T, dim]` and `feats [T, F]`, and returns `[T, dim]`.
+    [T, dim]` and `feats [T, F]`, and returns `[T, dim]`. Packed tokens past
+    `cu_seqlens[-1]` belong to no event: they attend to nothing and add
+    nothing to the gradients (where the loss leaves them out, and their x is
+    finite).
     """
 
     def __init__(self, dim: int, num_heads: int = 8, channels: int = 16, qkv_bias: bool = False,
@@ -97,7 +100,7 @@ class SpacetimeAttention(nn.Module):
     def forward(self, x: Tensor, feats: Tensor, seqlens: Optional[Tensor] = None,
                 key_padding_mask: Optional[Tensor] = None, kv: Optional[Tensor] = None,
                 cu_seqlens: Optional[Tensor] = None) -> Tensor:
-        from .forward import flash_spacetime_attention, flash_spacetime_attention_qkv
+        from .forward import attention_qkv_zero_tail, flash_spacetime_attention, flash_spacetime_attention_qkv
 
         flags = (self.use_attn_bias, self.use_activation_bias)
         if cu_seqlens is not None:
@@ -107,8 +110,7 @@ class SpacetimeAttention(nn.Module):
                 raise ValueError(f"packed x must be [T, dim], got {tuple(x.shape)}")
             w, bias = self.qkv_weight()
             qkv = F.linear(x, w, bias).view(x.shape[0], 3, self.num_heads, self.head_dim)
-            out = flash_spacetime_attention_qkv(qkv, feats, self.rel_proj.weight, self.rel_proj.bias, None, None,
-                                                *flags, cu_seqlens=cu_seqlens)
+            out = attention_qkv_zero_tail(qkv, feats, self.rel_proj.weight, self.rel_proj.bias, cu_seqlens, *flags)
             return self.proj(out.flatten(-2))
         b, length, _ = x.shape
         if kv is None:

@@ -558,6 +558,21 @@ __global__ __launch_bounds__(256) void fill_zero_kernel(float* p, int n) {
   for (int i = threadIdx.x; i < n; i += 256) p[i] = 0.f;
 }
 
+// Zeros into the rows past every offset (as sanitize_steps bounds them: their
+// maximum within [0, T]) of a packed tensor whose rows are `parts` 16-byte pieces.
+__global__ __launch_bounds__(256) void zero_tail_kernel(const int32_t* cu, int B, int T, uint4* rows, long parts) {
+  __shared__ int wave_max[4];
+  int n = 0;
+  for (int b = threadIdx.x; b <= B; b += 256) n = max(n, cu[b]);
+  for (int d = 32; d > 0; d >>= 1) n = max(n, __shfl_xor(n, d));
+  if ((threadIdx.x & 63) == 0) wave_max[threadIdx.x >> 6] = n;
+  __syncthreads();
+  n = min(max(max(wave_max[0], wave_max[1]), max(wave_max[2], wave_max[3])), T);
+  const long end = (long)T * parts;
+  for (long i = n * parts + (long)blockIdx.x * 256 + threadIdx.x; i < end; i += (long)gridDim.x * 256)
+    rows[i] = make_uint4(0, 0, 0, 0);
+}
+
 struct BwdLayout {
   int rows_r, rows_c;   // rows (keys) per workgroup of the rows / cols kernels
   long grid_r, grid_c;
@@ -636,6 +651,21 @@ void fst_frequencies(int C, float* out) {
 int fst_max_event_len(int dtype, int flags, int H, int D, int C) {
   if (check_common(dtype, flags & ~FST_PLAN_MASK, 0, H, 0, 0, D, C) != FST_OK) return 0;
   return max_event_len(dtype, flags, H, D, C);
+}
+
+int fst_zero_tail(int B, int T, const int32_t* cu_seqlens, void* rows, size_t row_bytes, void* stream) {
+  clear_error();
+  if (B < 0 || T < 0) return fail(FST_EINVAL, "negative size (B=%d, T=%d)", B, T);
+  if (T == 0 || row_bytes == 0) return FST_OK;
+  if (!cu_seqlens || !rows) return fail(FST_EINVAL, "null tensor pointer");
+  if (row_bytes % 16 || reinterpret_cast<uintptr_t>(rows) % 16)
+    return fail(FST_EINVAL, "rows must be whole multiples of 16 bytes at a multiple of 16");
+  if (row_bytes > SIZE_MAX / 2 / (size_t)T) return fail(FST_EINVAL, "T=%d rows of %zu bytes are past 2^63", T, row_bytes);
+  const long parts = (long)(row_bytes / 16), need = ((long)T * parts + 255) / 256;
+  hipLaunchKernelGGL(zero_tail_kernel, dim3((unsigned)(need < 256 ? need : 256)), dim3(256), 0,
+                     reinterpret_cast<hipStream_t>(stream), cu_seqlens, B, T, static_cast<uint4*>(rows), parts);
+  if (hipGetLastError() != hipSuccess) return fail(FST_ELAUNCH, "zero tail launch failed");
+  return FST_OK;
 }
 
 int fst_plans(int dtype, int H, int D, int C) {

@@ -625,9 +625,19 @@ def _qkv_views(qkv: Tensor, packed: bool) -> Tuple[Tensor, Tensor, Tensor]:
     return qkv[:, :, 0].transpose(1, 2), qkv[:, :, 1].transpose(1, 2), qkv[:, :, 2].transpose(1, 2)
 
 
+def _zero_tail(rows: Tensor, cu: Tensor) -> None:
+    """Zeros into the tokens of a dense packed `rows [T, ..]` past every offset of
+    `cu` (int32 on its device): the kernels leave them unwritten."""
+    with torch.cuda.device(rows.device):
+        rc = _lib.load().fst_zero_tail(cu.numel() - 1, rows.shape[0], _lib.ptr(cu), _lib.ptr(rows),
+                                       rows[:1].numel() * rows.element_size(), _lib.stream_handle(rows.device))
+    _lib.check(rc, "flash_spacetime_attention_qkv")
+
+
 class _FlashSpacetimeAttentionQKV(torch.autograd.Function):
     """The fused op on one interleaved q/k/v tensor; its gradient is one
-    tensor of the same layout, written by the kernels slot by slot."""
+    tensor of the same layout, written by the kernels slot by slot. zero_tail:
+    packed tokens past the last event are zeros in both."""
 
     @staticmethod
     def forward(  # type: ignore[override]
@@ -641,6 +651,7 @@ class _FlashSpacetimeAttentionQKV(torch.autograd.Function):
         use_attn_bias: bool,
         use_activation_bias: bool,
         cu_seqlens: Optional[Tensor],
+        zero_tail: bool = False,
     ) -> Tensor:
         if feats.requires_grad:
             raise ValueError("feats (detector data) must not require grad")
@@ -653,6 +664,9 @@ class _FlashSpacetimeAttentionQKV(torch.autograd.Function):
                                              use_activation_bias, cu_seqlens, interleaved=True))
         out, lse, _, _, _, pos4, w32, b32, lens, ctx.dims, ctx.scale = done
         ret = out if packed else out.transpose(1, 2)  # [T, H, D] / [B, L, H, D], dense
+        ctx.zero_tail = zero_tail
+        if zero_tail:
+            _zero_tail(out, lens)
         ctx.save_for_backward(qkv, pos4, lens, lse, *_keep_output(ctx, out, ret))
         ctx.prep_meta = (w32, b32, weight.dtype, None if bias is None else bias.dtype)
         ctx.packed = packed
@@ -682,6 +696,8 @@ class _FlashSpacetimeAttentionQKV(torch.autograd.Function):
                 ctx.dims, q, k, v, pos4, w32, b32, lens, lse, g, ctx.scale, vec_shape(ctx.dims),
                 out_like=like, grads=_qkv_views(dqkv, ctx.packed), out=out,
             )
+        if ctx.zero_tail:
+            _zero_tail(dqkv, lens)
         use_attn_bias, use_activation_bias = ctx.flags
         proj_used = use_attn_bias or use_activation_bias
         return (
@@ -689,8 +705,22 @@ class _FlashSpacetimeAttentionQKV(torch.autograd.Function):
             None,
             dw.to(w_dtype) if (ctx.needs_input_grad[2] and proj_used) else None,
             db.to(b_dtype) if (ctx.needs_input_grad[3] and proj_used and db is not None) else None,
-            None, None, None, None, None,
+            None, None, None, None, None, None,
         )
+
+
+def attention_qkv_zero_tail(qkv: Tensor, feats: Tensor, weight: Tensor, bias: Optional[Tensor], cu_seqlens: Tensor,
+                            use_attn_bias: bool, use_activation_bias: bool) -> Tensor:
+    """`flash_spacetime_attention_qkv` on packed tokens of which those past
+    `cu_seqlens[-1]` belong to no event: zeros in the output and in the gradient,
+    so that the linears around the op take nothing in from them."""
+    if qkv.dtype == _HALF:
+        with _output_is_temporary():
+            out = attention_qkv_zero_tail(qkv.to(torch.bfloat16), feats, weight, bias, cu_seqlens, use_attn_bias,
+                                          use_activation_bias)
+        return out.to(_HALF)
+    return _FlashSpacetimeAttentionQKV.apply(qkv.contiguous(), feats, weight, bias, None, None, use_attn_bias,
+                                             use_activation_bias, cu_seqlens, True)
 
 
 def flash_spacetime_attention_qkv(
@@ -713,7 +743,8 @@ def flash_spacetime_attention_qkv(
     the three slots in place and write the gradient as one tensor of the same
     layout, so neither the projection's output nor its gradient is copied,
     split or stacked. Returns `[B, L, H, D]` (padding rows zero) or
-    `[T, H, D]`: the layout the output projection consumes. Lengths and
+    `[T, H, D]`: the layout the output projection consumes. Offsets as in
+    `flash_spacetime_attention_varlen` (cu_seqlens[-1] = T), lengths and
     masks as in `flash_spacetime_attention` (a mask with holes runs the
     packed path on the gathered valid tokens). Same values as
     `flash_spacetime_attention(q, k, v, ...)` on the split heads. No

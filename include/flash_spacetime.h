@@ -274,6 +274,13 @@ int fst_backward_phases(int phases, int dtype, int flags, int B, int H, int L, i
  * (the reference's Triton kernels state no bound). */
 int fst_max_event_len(int dtype, int flags, int H, int D, int C);
 
+/* Zeros into the rows of a dense packed tensor [T, row_bytes] past every offset
+ * of cu_seqlens [B + 1]: the tokens that belong to no event, which the entry
+ * points above leave unwritten. row_bytes and the address are multiples of 16.
+ * For callers that go on to work on all T rows (a linear's gradient would take
+ * in whatever the memory held). */
+int fst_zero_tail(int B, int T, const int32_t* cu_seqlens, void* rows, size_t row_bytes, void* stream);
+
 /* ---------------------------------------------------------------------------
  * The transformer block beside its attention: layer norm and the gated
  * feed-forward block (graphnet's Block_rel runs both around the reference's
