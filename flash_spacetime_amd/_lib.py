@@ -168,7 +168,7 @@ def _load_host():
                 "fst_supported", "fst_forward_workspace_bytes", "fst_forward", "fst_backward_workspace_bytes",
                 "fst_backward", "fst_last_error", "fst_layer_norm_forward", "fst_layer_norm_backward_workspace_bytes",
                 "fst_layer_norm_backward", "fst_ffn_forward", "fst_ffn_backward_workspace_bytes",
-                "fst_ffn_backward")))
+                "fst_ffn_backward", "fst_zero_tail")))
             return _fst_host
         why = f"it is build {have[0]} for torch {have[1]}, the library is build {build} and torch is {torch.__version__}"
     warnings.warn(f"the host extension _fst_host is not used ({why}); the operators run through ctypes. "

@@ -139,8 +139,9 @@ class SpacetimeBlock(nn.Module):
 
     `forward(x, feats, seqlens | key_padding_mask)` takes padded events `x [B, L,
     dim]`, or with `cu_seqlens` packed ones `[T, dim]`, and returns the same
-    shape; padding rows are neither normalised nor multiplied and come back as
-    zeros. A stack saves a pass over the rows per block by leaving the last sum
+    shape; padding rows (packed: those past `cu_seqlens[-1]`) are neither
+    normalised nor multiplied by the feed-forward, whatever they hold, and come
+    back as zeros. A stack saves a pass over the rows per block by leaving the last sum
     to the next block's norm: `defer=True` returns `(x, branch)`, whose sum is the
     block's output, and `branch=` takes the one the block before deferred.
     """
@@ -169,6 +170,8 @@ class SpacetimeBlock(nn.Module):
 
         if cu_seqlens is not None and (seqlens is not None or key_padding_mask is not None):
             raise ValueError("packed input takes cu_seqlens only (no lengths or mask)")
+        if cu_seqlens is not None and (cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1):
+            raise ValueError(f"cu_seqlens must be [events + 1], got {tuple(cu_seqlens.shape)}")
         if x.dim() != (2 if cu_seqlens is not None else 3):
             raise ValueError(f"x must be [T, dim] with cu_seqlens, else [B, L, dim], got {tuple(x.shape)}")
         if key_padding_mask is None and seqlens is not None and seqlens.dim() == 2:
@@ -189,11 +192,13 @@ class SpacetimeBlock(nn.Module):
         from .norm import flash_layer_norm
 
         n1, n2 = self.norm1, self.norm2
+        if cu_seqlens is not None:  # packed tokens past the last offset are padding
+            seqlens = cu_seqlens[-1:]
         if branch is None:
             y = flash_layer_norm(x, n1.weight, n1.bias, n1.eps, seqlens=seqlens)
         else:
             y, x = flash_layer_norm(branch, n1.weight, n1.bias, n1.eps, residual=x, seqlens=seqlens)
-        a = self.attn(y, feats, seqlens, cu_seqlens=cu_seqlens)
+        a = self.attn(y, feats, seqlens if cu_seqlens is None else None, cu_seqlens=cu_seqlens)
         y, x = flash_layer_norm(a, n2.weight, n2.bias, n2.eps, residual=x, seqlens=seqlens)
         f = flash_gated_feed_forward(y, self.ffn_gate.weight, self.ffn_up.weight, self.ffn_down.weight,
                                      self.ffn_gate.bias, self.ffn_up.bias, self.ffn_down.bias, self.activation,

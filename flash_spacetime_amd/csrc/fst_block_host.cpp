@@ -113,7 +113,8 @@ Tensor dense16(const Maybe& t) {
   return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
 }
 
-// Events of padded x [B, L, n] with lengths, or one of all rows.
+// Events of padded x [B, L, n] with lengths, one of rows [L, n] with one length, or
+// one of all rows.
 struct Batch {
   int64_t B = 1, L = 0;
   Tensor lens;
@@ -124,10 +125,10 @@ bool batch_of(const Tensor& x, const Maybe& seqlens, Batch& b) {
     return b.L <= INT32_MAX;
   }
   const auto t = seqlens->scalar_type();
-  if (x.dim() != 3 || seqlens->dim() != 1 || seqlens->size(0) != x.size(0) || (t != at::kInt && t != at::kLong))
-    return false;
-  b.B = x.size(0);
-  b.L = x.size(1);
+  if ((x.dim() != 3 && x.dim() != 2) || seqlens->dim() != 1 || (t != at::kInt && t != at::kLong)) return false;
+  b.B = x.dim() == 2 ? 1 : x.size(0);
+  b.L = x.size(x.dim() - 2);
+  if (seqlens->size(0) != b.B) return false;
   b.lens = seqlens->to(at::kInt).contiguous();
   return b.B <= INT32_MAX && b.L <= INT32_MAX;
 }

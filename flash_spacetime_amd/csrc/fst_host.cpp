@@ -37,11 +37,14 @@ struct Library {
   decltype(&fst_backward_workspace_bytes) backward_workspace_bytes = nullptr;
   decltype(&fst_backward) backward = nullptr;
   decltype(&fst_last_error) last_error = nullptr;
+  decltype(&fst_zero_tail) zero_tail = nullptr;
 } lib;
 
-// The block operators' entry points may be left out: theirs stay as they were.
+// The entry points after last_error may be left out: they stay as they were.
 void bind_library(size_t supported, size_t fwd_ws, size_t fwd, size_t bwd_ws, size_t bwd, size_t last_error,
-                  size_t norm_fwd, size_t norm_ws, size_t norm_bwd, size_t ffn_fwd, size_t ffn_ws, size_t ffn_bwd) {
+                  size_t norm_fwd, size_t norm_ws, size_t norm_bwd, size_t ffn_fwd, size_t ffn_ws, size_t ffn_bwd,
+                  size_t zero_tail) {
+  if (zero_tail) lib.zero_tail = reinterpret_cast<decltype(lib.zero_tail)>(zero_tail);
   if (norm_fwd) bind_block_library(norm_fwd, norm_ws, norm_bwd, ffn_fwd, ffn_ws, ffn_bwd, last_error);
   lib.supported = reinterpret_cast<decltype(lib.supported)>(supported);
   lib.forward_workspace_bytes = reinterpret_cast<decltype(lib.forward_workspace_bytes)>(fwd_ws);
@@ -271,6 +274,18 @@ py::object backward(const Dims& dims, const Tensor& q, const std::optional<Tenso
   return or_none(backward_call, dims, q, k, v, pos4, w32, b32, lens, lse, grad_out, scale, out, stream);
 }
 
+// fst_zero_tail on dense packed rows of a few dimensions (the caller's own buffers);
+// false where it is not bound.
+bool zero_tail(const Tensor& rows, const Tensor& cu, int64_t stream) {
+  if (!lib.zero_tail) return false;
+  const c10::DeviceGuard on(rows.device());
+  const int64_t T = rows.size(0);
+  const int rc = lib.zero_tail((int)cu.numel() - 1, (int)T, static_cast<const int32_t*>(cu.data_ptr()), rows.data_ptr(),
+                               rows.nbytes() / std::max<int64_t>(T, 1), reinterpret_cast<void*>(stream));
+  if (rc != FST_OK) throw std::runtime_error(std::string("fst_zero_tail: ") + lib.last_error());
+  return true;
+}
+
 }  // namespace
 
 // build_id: the library this extension belongs to; torch_version: the torch it
@@ -282,7 +297,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("backward_workspace_bytes"), py::arg("backward"), py::arg("last_error"),
         py::arg("layer_norm_forward") = 0, py::arg("layer_norm_backward_workspace_bytes") = 0,
         py::arg("layer_norm_backward") = 0, py::arg("ffn_forward") = 0, py::arg("ffn_backward_workspace_bytes") = 0,
-        py::arg("ffn_backward") = 0);
+        py::arg("ffn_backward") = 0, py::arg("zero_tail") = 0);
+  m.def("zero_tail", &zero_tail);
   m.def("forward", &forward);
   m.def("backward", &backward);
   define_block_operators(m);

@@ -100,7 +100,8 @@ def flash_gated_feed_forward(
     (with the normal distribution function) or "gelu_tanh". With `seqlens` `[B]` x
     is a padded `[B, L, D]`: rows past an event's length are neither read nor
     computed, come back as zeros in the output and x's gradient, and add
-    nothing to the weights' gradients.
+    nothing to the weights' gradients (`seqlens` `[1]` also goes with packed rows `[T,
+    D]`, of which the first `seqlens[0]` are tokens).
 
     Products accumulate in float32 on the matrix cores. bfloat16 and float16
     round the hidden rows to their type between the products (float16 ones past

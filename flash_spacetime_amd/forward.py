@@ -628,9 +628,13 @@ def _qkv_views(qkv: Tensor, packed: bool) -> Tuple[Tensor, Tensor, Tensor]:
 def _zero_tail(rows: Tensor, cu: Tensor) -> None:
     """Zeros into the tokens of a dense packed `rows [T, ..]` past every offset of
     `cu` (int32 on its device): the kernels leave them unwritten."""
+    host = _lib.host()
+    if host is not None and host.zero_tail(rows, cu, _raw_stream(rows)):
+        return
+    tokens = rows.shape[0]
     with torch.cuda.device(rows.device):
-        rc = _lib.load().fst_zero_tail(cu.numel() - 1, rows.shape[0], _lib.ptr(cu), _lib.ptr(rows),
-                                       rows[:1].numel() * rows.element_size(), _lib.stream_handle(rows.device))
+        rc = _lib.load().fst_zero_tail(cu.numel() - 1, tokens, cu.data_ptr(), rows.data_ptr(),
+                                       rows.nbytes // max(tokens, 1), _raw_stream(rows))
     _lib.check(rc, "flash_spacetime_attention_qkv")
 
 

@@ -43,17 +43,20 @@ def token_rows(t: Tensor, align: int = 1) -> Tuple[Tensor, int]:
 
 
 def batch_of_rows(x: Tensor, seqlens: Optional[Tensor]) -> Tuple[int, int, Optional[Tensor]]:
-    """(B, L, int32 lengths on x's device) of a padded `x [B, L, N]`, or every row
-    of `x [.., N]` as one event without lengths."""
+    """(B, L, int32 lengths on x's device) of a padded `x [B, L, N]`, or of rows `x
+    [L, N]` with the one length [1]; or every row of `x [.., N]` as one event without
+    lengths."""
     if seqlens is None:
         return 1, x.numel() // x.shape[-1], None
-    if x.dim() != 3:
-        raise ValueError(f"seqlens needs padded x [B, L, features], got {tuple(x.shape)}")
-    if seqlens.dim() != 1 or seqlens.shape[0] != x.shape[0]:
-        raise ValueError(f"seqlens must be [B={x.shape[0]}], got {tuple(seqlens.shape)}")
+    if x.dim() != 3 and not (x.dim() == 2 and tuple(seqlens.shape) == (1,)):
+        raise ValueError(f"seqlens needs padded x [B, L, features], or [1] packed x [T, features], got "
+                         f"{tuple(x.shape)}, seqlens {tuple(seqlens.shape)}")
+    batch, length = (1, *x.shape[:1]) if x.dim() == 2 else x.shape[:2]
+    if seqlens.dim() != 1 or seqlens.shape[0] != batch:
+        raise ValueError(f"seqlens must be [B={batch}], got {tuple(seqlens.shape)}")
     if seqlens.dtype.is_floating_point or seqlens.dtype == torch.bool:
         raise ValueError(f"seqlens must be an integer tensor, got {seqlens.dtype}")
-    return x.shape[0], x.shape[1], seqlens.to(device=x.device, dtype=torch.int32).contiguous()
+    return batch, length, seqlens.to(device=x.device, dtype=torch.int32).contiguous()
 
 
 def check_rows(x: Tensor, *others: Optional[Tensor]) -> int:
@@ -155,7 +158,8 @@ def flash_layer_norm(
     output added to the stream, and the stream normalised for the next one, in
     one pass. With `seqlens` `[B]` x is a padded `[B, L, N]`: rows past an
     event's length are not read, come back as zeros in y, s and every
-    gradient, and add nothing to the parameters' gradients.
+    gradient, and add nothing to the parameters' gradients. `seqlens` `[1]` also
+    goes with packed rows `[T, N]`, of which the first `seqlens[0]` are tokens.
 
     Any strides are taken (rows a fixed stride apart in place, others copied).
     Statistics and sums are float32; results are bitwise reproducible.
