@@ -574,8 +574,8 @@ int fst_layer_norm_backward(int dtype, int param_dtype, int B, int L, int N, con
   if (rows > 0) {
     NormGradArgs a{s, dy, dsum, weight, seqlens, reinterpret_cast<const float2*>(stats), dx, part,
                    rows, (long)s_stride, (long)dy_stride, (long)dsum_stride, L, N};
-    p.edge = !aligned16(s, s_stride, es) || !aligned16(dy, dy_stride, es) || (dx && !aligned16(dx, N, es)) ||
-             (dsum && !aligned16(dsum, dsum_stride, es));
+    p.edge = N * es % 16 != 0 || !aligned16(s, s_stride, es) || !aligned16(dy, dy_stride, es) ||
+             (dx && !aligned16(dx, N, es)) || (dsum && !aligned16(dsum, dsum_stride, es));
     if (dtype == FST_BF16)
       launch_bwd<bf16>(p, a, blocks, w_f32, st);
     else if (dtype == FST_F16)
