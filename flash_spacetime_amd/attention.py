@@ -189,7 +189,7 @@ class SpacetimeBlock(nn.Module):
 
     def _block(self, x, feats, seqlens, cu_seqlens, branch, defer):
         from .feed_forward import flash_gated_feed_forward
-        from .norm import flash_layer_norm
+        from .norm import autocast_dtype, flash_layer_norm
 
         n1, n2 = self.norm1, self.norm2
         if cu_seqlens is not None:  # packed tokens past the last offset are padding
@@ -200,6 +200,9 @@ class SpacetimeBlock(nn.Module):
             y, x = flash_layer_norm(branch, n1.weight, n1.bias, n1.eps, residual=x, seqlens=seqlens)
         a = self.attn(y, feats, seqlens if cu_seqlens is None else None, cu_seqlens=cu_seqlens)
         y, x = flash_layer_norm(a, n2.weight, n2.bias, n2.eps, residual=x, seqlens=seqlens)
+        low = autocast_dtype()
+        if low is not None:  # as autocast has a linear's rows; the norms stay in the stream's type
+            y = y.to(low)
         f = flash_gated_feed_forward(y, self.ffn_gate.weight, self.ffn_up.weight, self.ffn_down.weight,
                                      self.ffn_gate.bias, self.ffn_up.bias, self.ffn_down.bias, self.activation,
                                      seqlens=seqlens)

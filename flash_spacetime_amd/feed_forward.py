@@ -16,7 +16,7 @@ from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .norm import BLOCK_DTYPES, PLAIN, batch_of_rows, check_rows, token_rows
+from .norm import BLOCK_DTYPES, PLAIN, autocast_dtype, batch_of_rows, check_rows, token_rows
 
 ACTIVATIONS = {"silu": _lib.FST_SILU, "gelu": _lib.FST_GELU, "gelu_tanh": _lib.FST_GELU_TANH}
 
@@ -103,6 +103,9 @@ def flash_gated_feed_forward(
     nothing to the weights' gradients (`seqlens` `[1]` also goes with packed rows `[T,
     D]`, of which the first `seqlens[0]` are tokens).
 
+    Under `torch.autocast` tensors of different types are taken in autocast's
+    (16-bit rows beside float32 weights); of one type they stay in it.
+
     Products accumulate in float32 on the matrix cores. bfloat16 and float16
     round the hidden rows to their type between the products (float16 ones past
     65504 are infinite) and the projections' gradients in the backward, which
@@ -117,6 +120,10 @@ def flash_gated_feed_forward(
             return out
     check_rows(x, w_gate, w_up, w_down, b_gate, b_up, b_down,
                seqlens if seqlens is not None and seqlens.is_cuda else None)
+    low, types = autocast_dtype(), {t.dtype for t in tensors if t is not None}
+    if low is not None and len(types) > 1 and types <= BLOCK_DTYPES.keys():
+        tensors = tuple(None if t is None else t.to(low) for t in tensors)
+        return flash_gated_feed_forward(*tensors, activation, seqlens=seqlens)
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
     d = x.shape[-1]

@@ -74,6 +74,11 @@ def check_rows(x: Tensor, *others: Optional[Tensor]) -> int:
     return BLOCK_DTYPES[x.dtype]
 
 
+def autocast_dtype() -> Optional[torch.dtype]:
+    """The type torch.autocast has the GPU's products in; None outside of it."""
+    return torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else None
+
+
 # Tensors without methods of their own: calls of these go through the host
 # extension (csrc/fst_block_host.cpp), which gives back None for what it leaves to
 # the Python path.
@@ -161,6 +166,10 @@ def flash_layer_norm(
     gradient, and add nothing to the parameters' gradients. `seqlens` `[1]` also
     goes with packed rows `[T, N]`, of which the first `seqlens[0]` are tokens.
 
+    Under `torch.autocast` x and residual of different types are taken in the
+    wider one (a float32 stream and a 16-bit branch: float32), and parameters of
+    another 16-bit type in float32.
+
     Any strides are taken (rows a fixed stride apart in place, others copied).
     Statistics and sums are float32; results are bitwise reproducible.
     """
@@ -170,6 +179,11 @@ def flash_layer_norm(
         if out is not None:
             return out
     check_rows(x, residual, weight, bias, seqlens if seqlens is not None and seqlens.is_cuda else None)
+    if autocast_dtype() is not None and all(t is None or t.dtype in BLOCK_DTYPES for t in (residual, weight, bias)):
+        wide = x.dtype if residual is None else torch.promote_types(x.dtype, residual.dtype)
+        x, residual = x.to(wide), None if residual is None else residual.to(wide)
+        if any(t is not None and t.dtype not in (wide, torch.float32) for t in (weight, bias)):
+            weight, bias = (None if t is None else t.float() for t in (weight, bias))
     n = x.shape[-1]
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError(f"residual must have x's shape and dtype ({tuple(x.shape)}, {x.dtype}), got "

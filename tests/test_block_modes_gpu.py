@@ -104,3 +104,72 @@ def test_make_fx_is_refused(monkeypatch, name):
             with pytest.raises(RuntimeError, match="make_fx"):
                 make_fx(lambda g: torch.autograd.grad(y, leaf, g, retain_graph=True))(torch.ones_like(y))
             torch.autograd.grad(y, leaf, torch.ones_like(y))
+
+
+def _block_run(blk, x, feats, dy, **kwargs):
+    leaf = x.clone().requires_grad_(True)
+    y = blk(leaf, feats, **kwargs)
+    return y.detach(), torch.autograd.grad(y, [leaf, *blk.parameters()], dy.to(y.dtype))
+
+
+@pytest.mark.parametrize("layout", ["lengths", "holes", "packed"])
+@pytest.mark.parametrize("low", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+def test_block_under_autocast(low, layout):
+    """float32 parameters and stream under autocast: output and gradients are float32
+    and those of the float32 block up to the roundings of a 16-bit block (2e-2, the
+    bound of the 16-bit attention module); so with the last sum deferred."""
+    x, feats, dy = _randn(("autocast", layout), (3, 24, 64), (3, 24, 4), (3, 24, 64))
+    blocks = [SpacetimeBlock(64, 4, device=DEV) for _ in range(2)]
+    lens = torch.tensor([24, 7, 15], device=DEV)
+    kwargs = {"seqlens": lens}
+    if layout == "holes":
+        kwargs = {"key_padding_mask": torch.arange(24, device=DEV)[None] % 5 >= 1 + torch.arange(3, device=DEV)[:, None]}
+    elif layout == "packed":
+        x, feats, dy = (t.flatten(0, 1) for t in (x, feats, dy))
+        kwargs = {"cu_seqlens": torch.tensor([0, 30, 72], dtype=torch.int32, device=DEV)}
+    near = lambda a, b: float((a - b).double().norm()) <= 2e-2 * float(b.double().norm())  # noqa: E731
+    want = _block_run(blocks[0], x, feats, dy, **kwargs)
+    with torch.autocast("cuda", dtype=low):
+        got = _block_run(blocks[0], x, feats, dy, **kwargs)
+        h, branch = blocks[0](x, feats, **kwargs, defer=True)
+        two = blocks[1](h, feats, **kwargs, branch=branch).detach()
+        again = blocks[1](got[0], feats, **kwargs).detach()
+    assert branch.dtype == low and h.dtype == two.dtype == torch.float32
+    assert got[0].dtype == torch.float32 and near(got[0], want[0]) and near(two, again)
+    for a, b in zip(got[1], want[1]):
+        assert a.dtype == torch.float32 and near(a, b)
+
+
+def test_operators_under_autocast():
+    """Tensors of one type keep their bits; of several they are what the casts
+    written out give, gradients in the types that came in. Without autocast, and
+    for float64, they are refused as before."""
+    calls = _calls()
+    for f, tensors in calls.values():
+        want = f(*tensors)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            assert torch.equal(f(*tensors), want)
+    low = torch.bfloat16
+    f, (x, r, w) = calls["norm_residual"]
+    g, ffn = calls["ffn"]
+    with torch.autocast("cuda", dtype=low):
+        for a, b, p in ((x.to(low), r, w), (x, r.to(low), w.to(low)), (x.half(), r.to(low), w.half()), (x, r, w.to(low)),
+                        (x.half(), r.half(), w.to(low))):
+            leaves = [t.detach().requires_grad_(True) for t in (a, b, p)]
+            y = f(*leaves)
+            wide = torch.promote_types(a.dtype, b.dtype)
+            assert y.dtype == wide and torch.equal(y, f(a.to(wide), b.to(wide), p.float()))
+            for t, d in zip(leaves, torch.autograd.grad(y, leaves, y.detach())):
+                assert d.dtype == t.dtype and bool(d.isfinite().all()) and bool((d != 0).any())
+        mixed = [ffn[0].half(), ffn[1], ffn[2].to(low), ffn[3]]
+        leaves = [t.detach().requires_grad_(True) for t in mixed]
+        y = g(*leaves)
+        assert y.dtype == low and torch.equal(y, g(*(t.to(low) for t in mixed)))
+        for t, d in zip(leaves, torch.autograd.grad(y, leaves, y.detach())):
+            assert d.dtype == t.dtype and bool(d.isfinite().all()) and bool((d != 0).any())
+        for bad in (lambda: f(x, r.double(), w), lambda: g(ffn[0].double(), *ffn[1:]), lambda: f(x[:1], r, w)):
+            with pytest.raises(ValueError):
+                bad()
+    for bad in (lambda: f(x.to(low), r, w), lambda: g(ffn[0].to(low), *ffn[1:])):
+        with pytest.raises(ValueError, match="dtype"):
+            bad()
