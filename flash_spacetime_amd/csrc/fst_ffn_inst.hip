@@ -580,7 +580,7 @@ struct OuterSide {
 
   // Order of the slices of row r, in 16-byte parts.
   static __device__ __forceinline__ int swizzle(int r) {
-    return F32 ? (r & 3) << 2 : ROW % 256 ? ((r >> 1) & 3) << 1 : (r & 7) << 1;
+    return F32 ? (r & 3) << 2 : (r & 7) << 1;
   }
   __device__ __forceinline__ void init(const void* p, long ld_elems, int f0, int count, int tid) {
 #pragma unroll
@@ -788,7 +788,8 @@ void launch_few(const FfnProduct& p, hipStream_t st) {
 // instead (ffn_few: 4 tokens, D = 768, F = 2048 7.4 + 15.3 us in 64 x 64 tiles, 6.2 + 5.6;
 // 187 tokens, D = 384, F = 1024 5.7 + 7.0 against 6.4 + 7.2). float32 is bound by the
 // matrix cores four times as long in each: as fast in the middle tile as in the
-// large one, which it does without.
+// large one, which it does without. kFfnRedo has no small tile: one round of the
+// middle one takes 0.35 us a step, of a small one 0.36, more rounds less by more.
 enum Tile { kLarge, kMiddle, kSmall, kFew };
 
 Tile pick(const FfnProduct& p, int mats, bool redo) {
@@ -801,8 +802,8 @@ Tile pick(const FfnProduct& p, int mats, bool redo) {
   // Two weights' 64 x 64 tile has a quarter of each operand's rows reused less.
   const double large = 1.65 * nl * (redo ? 0.75 : 1.0), middle = (nm > 1 ? 0.54 * nm : 0.64) * (redo ? 0.55 : 1.0),
                small = (ns > 1 ? 0.24 * ns : 0.28) * (mats == 2 ? 1.3 : 1.0);
-  if (!F32 && large <= middle && large <= small) return kLarge;
-  return middle <= small ? kMiddle : kSmall;
+  if (!F32 && large <= middle && (redo || large <= small)) return kLarge;
+  return redo || middle <= small ? kMiddle : kSmall;
 }
 
 template <int DT, int FT, int WF, int OCC>
@@ -858,8 +859,6 @@ int FST_CAT(ffn_product_, FST_NAME)(int mode, const FfnProduct& p, hipStream_t s
       launch<kFfnOut, 2, 2, 2, 2, 4, 2>(p, st);
     else if constexpr (F32)
       launch<kFfnGrad, 2, 2, 2, 2, 4, 2>(p, st);
-    else
-      launch<kFfnRedo, 1, 4, 4, 1, 4, 2>(p, st);
   }
   return hipGetLastError() == hipSuccess ? FST_OK : FST_ELAUNCH;
 }
