@@ -109,6 +109,7 @@ SIGNATURES = {
         _i,
         [_i, _i, _i, _i, _i, _i, _vp, _l, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
     ),
+    "fst_ffn_tiles": (_i, [_i, _i, _i, _i, _i, _vp]),
     "fst_ffn_backward_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "fst_ffn_backward": (
         _i,

@@ -57,10 +57,12 @@ struct FfnOuters {
 
 typedef int (*ffn_product_fn)(int mode, const FfnProduct&, hipStream_t);
 typedef int (*ffn_outer_fn)(FfnOuters&, int tile, hipStream_t);
+typedef int (*ffn_tile_fn)(int mode, const FfnProduct&);
 
 #define FST_FFN_DECL(name)                                      \
   int ffn_product_##name(int mode, const FfnProduct&, hipStream_t); \
-  int ffn_outer_##name(FfnOuters&, int tile, hipStream_t);
+  int ffn_outer_##name(FfnOuters&, int tile, hipStream_t);          \
+  int ffn_tile_##name(int mode, const FfnProduct&);
 FST_FFN_DECL(bf16)
 FST_FFN_DECL(f16)
 FST_FFN_DECL(f32)

@@ -288,6 +288,25 @@ int fst_ffn_forward(int dtype, int activation, int B, int L, int D, int F, const
   return FST_OK;
 }
 
+int fst_ffn_tiles(int dtype, int B, int L, int D, int F, int32_t* tiles) {
+  clear_error();
+  const int rc = check_ffn(dtype, FST_SILU, B, L, D, F);
+  if (rc != FST_OK) return rc;
+  if (!tiles) return fail(FST_EINVAL, "null pointer");
+  const ffn_tile_fn tile_of = dtype == FST_BF16 ? ffn_tile_bf16 : dtype == FST_F16 ? ffn_tile_f16 : ffn_tile_f32;
+  FfnProduct p{};
+  p.tokens = B * L;
+  p.F = F;
+  tiles[0] = tile_of(kFfnGate, p);
+  tiles[2] = tile_of(ffn_redo(dtype) ? kFfnRedo : kFfnGrad, p);
+  p.F = D;
+  tiles[1] = tiles[3] = tile_of(kFfnOut, p);
+  const OuterPlan outer = plan_outer(dtype, (long)B * L, D, F);
+  tiles[4] = outer.tile;
+  tiles[5] = outer.splits;
+  return FST_OK;
+}
+
 size_t fst_ffn_backward_workspace_bytes(int dtype, int B, int L, int D, int F) {
   if (check_ffn(dtype, FST_SILU, B, L, D, F) != FST_OK) return 0;
   return grad_layout(dtype, (long)B * L, D, F).total;

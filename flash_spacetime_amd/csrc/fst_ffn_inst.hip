@@ -824,8 +824,17 @@ void launch_outer(FfnOuters& ps, hipStream_t st) {
 #define FST_CAT2(a, b) a##b
 #define FST_CAT(a, b) FST_CAT2(a, b)
 
+static Tile tile_of(int mode, const FfnProduct& p) {
+  return pick(p, mode == kFfnGate || mode == kFfnRedo ? 2 : 1, mode == kFfnRedo);
+}
+
+int FST_CAT(ffn_tile_, FST_NAME)(int mode, const FfnProduct& p) {
+  constexpr int side[] = {256, 128, 64, 16};
+  return side[tile_of(mode, p)];
+}
+
 int FST_CAT(ffn_product_, FST_NAME)(int mode, const FfnProduct& p, hipStream_t st) {
-  const Tile tile = pick(p, mode == kFfnGate || mode == kFfnRedo ? 2 : 1, mode == kFfnRedo);
+  const Tile tile = tile_of(mode, p);
   if constexpr (!F32) {
     if (tile == kLarge) {
       if (mode == kFfnGate)

@@ -333,6 +333,13 @@ int fst_ffn_forward(int dtype, int activation, int B, int L, int D, int F, const
                     const void* b_down, const int32_t* seqlens, void* hidden, void* gate, void* up, int32_t* rowmap,
                     void* y, void* stream);
 
+/* The tiles a call of these sizes runs, by the features a side: tiles[0 .. 3] of the
+ * gate and up projections, the output projection, the projections' gradients
+ * and x's gradient (256, 128, 64, or 16 where few rows split the contraction over
+ * the waves), tiles[4] of the weights' gradients, tiles[5] the runs of rows these are
+ * summed over. With seqlens they are chosen by B * L. Host-only, no GPU call. */
+int fst_ffn_tiles(int dtype, int B, int L, int D, int F, int32_t* tiles);
+
 /* Scratch bytes fst_ffn_backward needs. */
 size_t fst_ffn_backward_workspace_bytes(int dtype, int B, int L, int D, int F);
 
