@@ -100,11 +100,12 @@ __device__ __forceinline__ float activate(float a, float& slope) {
     if constexpr (KIND == FST_GELU_TANH) {
       const float c = 1.59576912160573071f, s = a * a;  // 2 sqrt(2 / pi)
       z = c * a * fmaf(0.044715f, s, 1.f);
-      if constexpr (D) dz = c * fmaf(3.f * 0.044715f, s, 1.f);
+      // Finite, so that 0 * dz is 0: from |a| = 10 on the factor beside it is.
+      if constexpr (D) dz = c * fmaf(3.f * 0.044715f, fminf(s, 1e30f), 1.f);
     }
     const float g = __builtin_amdgcn_rcpf(1.f + __expf(-z));
     const float h = a * g;
-    if constexpr (D) slope = fmaf(h * (1.f - g), dz, g);  // 0 * dz, not 0 * inf, where a * dz overflows
+    if constexpr (D) slope = fmaf(h * (1.f - g), dz, g);  // in this order: a * dz may overflow
     return h;
   }
 }
