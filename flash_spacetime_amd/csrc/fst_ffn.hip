@@ -10,8 +10,8 @@
 // products after them are one each), dx, and the weights' gradients, summed over
 // runs of the tokens in order. h is kept from the forward; a and u are formed
 // again (4 T F D operations beside the backward's 12) except in float32, which
-// keeps them: rounded to 16 bits they had moved the gradients to twice the
-// distance from 64 bits (bf16 0.0031 of their norm against 0.0024), and at D =
+// keeps them: rounded to 16 bits they had moved the gradients to 1.3 times
+// the distance from 64 bits (bf16 0.0031 of their norm against 0.0024), and at D =
 // 384 writing and reading them took as long as the products do.
 // Padded batches are gathered on the way: a list of the valid rows is the
 // products' token axis, so padding costs nothing but its zeros.

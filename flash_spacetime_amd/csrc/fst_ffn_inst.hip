@@ -180,11 +180,11 @@ __device__ __forceinline__ bool pick_tile(int wg, int nf, int nt, int& f, int& t
 // from dy, and holds all three.
 //
 // Bound by the matrix cores and the way to them: with 65536 tokens, D = 1024, F = 2752
-// in bf16 gate and up take 690 us (1.07 PFLOP/s), the output product 320 (1.15), dx 610
-// (1.21), kFfnRedo 1170 (0.95), where a library product of 8192 a side reaches 1.35
+// in bf16 gate and up take 692 us (1.07 PFLOP/s), the output product 326 (1.13), dx 616
+// (1.20), kFfnRedo 1188 (0.93), where a library product of 8192 a side reaches 1.35
 // and one of the gate's shape 1.10. The matrix cores are busy half of the cycles, as
 // the LDS is (reads and the loads into it); no bank conflicts; four of five lines
-// come from L2. At K = 384 (100500 tokens, F = 1024: 208, 112, 205 and 352 us) a
+// come from L2. At K = 384 (100500 tokens, F = 1024: 208, 110, 204 and 353 us) a
 // workgroup's six steps stand beside its first loads and its stores (147 of 238 us
 // without an epilogue, before activations were chosen once per run). Measured and
 // slower or no faster: four waves of 128 x 128 (690 -> 830 us, the output product as

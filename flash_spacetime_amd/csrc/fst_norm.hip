@@ -7,8 +7,8 @@
 //
 // A row is held in registers by a group of LPR lanes, so memory is read once
 // and written once; the bound is HBM bandwidth (256 x 768 padded rows of 384 bf16 with a
-// residual, half of them tokens: forward 82 us, 5.6 TB/s of what it has to move, backward
-// 102, 3.7; 60001 rows of 512 f32 38 and 63 us, 6.4 and 5.8 TB/s, some of it from the
+// residual, half of them tokens: forward 78 us, 5.9 TB/s of what it has to move, backward
+// 105, 3.7; 60001 rows of 512 f32 40 and 64 us, 6.2 and 5.8 TB/s, some of it from the
 // last level cache) or, in calls of few rows, the launch. Statistics, sums and
 // gradients are float32; each output is rounded once.
 #include "fst_block.h"

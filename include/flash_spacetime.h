@@ -291,10 +291,10 @@ int fst_zero_tail(int B, int T, const int32_t* cu_seqlens, void* rows, size_t ro
  * other way round) gives padded events' lengths, taken within [0, L]: rows past
  * them are not read, are zeros in every row-shaped output, and add nothing
  * to the gradients of weights and biases. Row strides are in elements;
- * outputs are dense. B * L is at most 2^31 - 1. dtype is FST_BF16, FST_F16 or
- * FST_F32; sums and statistics are float32, every output is rounded once.
- * Results are bitwise deterministic. As above nothing is allocated or
- * synchronised. */
+ * outputs are dense. B * L is at most 2^31 - 1 (fst_ffn_*: 2^31 - 65537).
+ * dtype is FST_BF16, FST_F16 or FST_F32; sums and statistics are float32, every
+ * output is rounded once. Results are bitwise deterministic. As above nothing is
+ * allocated or synchronised. */
 
 /* y = (s - mean(s)) / sqrt(var(s) + eps) * weight + bias over the N features of
  * a row, s = x, or with residual (nullable) s = x + residual rounded to dtype

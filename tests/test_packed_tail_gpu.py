@@ -169,3 +169,15 @@ def test_operators_take_packed_rows_with_one_length(monkeypatch, dtype, tokens):
             flash_layer_norm(x, seqlens=bad)
         with pytest.raises(ValueError, match="padded"):
             flash_gated_feed_forward(x, *ws, seqlens=bad)
+
+
+@pytest.mark.parametrize("kind", ["int64", "host", "strided"])
+def test_block_takes_offsets_of_any_kind(kind):
+    dim, n, cu, x, feats, dy = _case("f32", 4, "kinds")
+    module = SpacetimeBlock(dim, 4, device=DEV)
+    other = {"int64": cu.long(), "host": cu.cpu(), "strided": torch.stack([cu, cu + 99], 1)[:, 0]}[kind]
+    y, want = _grads(module, x, feats, cu, dy)
+    z, got = _grads(module, x, feats, other, dy)
+    assert torch.equal(y, z) and bool((y[n:] == 0).all())
+    for name, w in want.items():
+        assert torch.equal(got[name], w), name
