@@ -35,6 +35,14 @@ __all__ = [
     "flash_spacetime_backward",
     "flash_layer_norm",
     "flash_gated_feed_forward",
+    "flash_rms_norm",
+    "flash_rms_norm_fp8",
+    "ExpertOrder",
+    "flash_expert_route",
+    "flash_expert_sort",
+    "flash_expert_dispatch",
+    "flash_expert_combine",
+    "flash_expert_feed_forward",
     "spacetime_attention_reference",
     "spacetime_pair_features",
     "sinusoidal_frequencies",
@@ -60,6 +68,14 @@ _OPS = {
     "flash_spacetime_backward": "backward",
     "flash_layer_norm": "norm",
     "flash_gated_feed_forward": "feed_forward",
+    "flash_rms_norm": "rms_norm",
+    "flash_rms_norm_fp8": "rms_norm",
+    "ExpertOrder": "experts",
+    "flash_expert_route": "experts",
+    "flash_expert_sort": "experts",
+    "flash_expert_dispatch": "experts",
+    "flash_expert_combine": "experts",
+    "flash_expert_feed_forward": "experts",
 }
 
 

@@ -116,6 +116,30 @@ SIGNATURES = {
         [_i, _i, _i, _i, _i, _i, _vp, _l, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _l,
          _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp],
     ),
+    "fst_rms_norm_forward": (_i, [_i, _i, _i, _i, _i, _vp, _l, _vp, _l, _vp, _vp, _f, _vp, _vp, _vp, _vp]),
+    "fst_rms_norm_fp8": (_i, [_i, _i, _i, _i, _i, _vp, _l, _vp, _l, _vp, _vp, _f, _vp, _vp, _vp, _vp]),
+    "fst_rms_norm_backward_workspace_bytes": (_sz, [_i, _i, _i, _i]),
+    "fst_rms_norm_backward": (
+        _i,
+        [_i, _i, _i, _i, _i, _vp, _l, _vp, _vp, _vp, _vp, _l, _vp, _l, _vp, _vp, _vp, _sz, _vp],
+    ),
+    "fst_expert_route": (_i, [_i, _i, _i, _i, _i, _i, _vp, _l, _vp, _vp, _vp, _vp]),
+    "fst_expert_route_backward": (_i, [_i, _i, _i, _i, _i, _i, _vp, _l, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "fst_expert_sort_workspace_bytes": (_sz, [_i, _i]),
+    "fst_expert_sort": (_i, [_i, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "fst_expert_spread": (_i, [_i, _i, _l, _i, _i, _l, _vp, _l, _vp, _vp, _vp, _vp, _l, _vp, _vp, _vp]),
+    "fst_expert_gather": (_i, [_i, _i, _l, _i, _i, _l, _vp, _l, _vp, _vp, _vp, _vp]),
+    "fst_expert_ffn_forward": (
+        _i,
+        [_i, _i, _i, _i, _i, _i, _vp, _l, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    ),
+    "fst_expert_ffn_tiles": (_i, [_i, _i, _i, _i, _i, _vp]),
+    "fst_expert_ffn_backward_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "fst_expert_ffn_backward": (
+        _i,
+        [_i, _i, _i, _i, _i, _i, _vp, _l, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _l,
+         _vp, _vp, _vp, _vp, _vp, _sz, _vp],
+    ),
     "fst_max_event_len": (_i, [_i, _i, _i, _i, _i]),
     "fst_zero_tail": (_i, [_i, _i, _vp, _vp, _sz, _vp]),
     "fst_frequencies": (None, [_i, ctypes.POINTER(ctypes.c_float)]),
@@ -169,7 +193,11 @@ def _load_host():
                 "fst_supported", "fst_forward_workspace_bytes", "fst_forward", "fst_backward_workspace_bytes",
                 "fst_backward", "fst_last_error", "fst_layer_norm_forward", "fst_layer_norm_backward_workspace_bytes",
                 "fst_layer_norm_backward", "fst_ffn_forward", "fst_ffn_backward_workspace_bytes",
-                "fst_ffn_backward", "fst_zero_tail")))
+                "fst_ffn_backward", "fst_zero_tail", "fst_rms_norm_forward", "fst_rms_norm_fp8",
+                "fst_rms_norm_backward_workspace_bytes", "fst_rms_norm_backward", "fst_expert_route",
+                "fst_expert_route_backward", "fst_expert_sort_workspace_bytes", "fst_expert_sort", "fst_expert_spread",
+                "fst_expert_gather", "fst_expert_ffn_forward", "fst_expert_ffn_backward_workspace_bytes",
+                "fst_expert_ffn_backward")))
             return _fst_host
         why = f"it is build {have[0]} for torch {have[1]}, the library is build {build} and torch is {torch.__version__}"
     warnings.warn(f"the host extension _fst_host is not used ({why}); the operators run through ctypes. "

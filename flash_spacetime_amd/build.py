@@ -65,9 +65,12 @@ def source_hash() -> str:
 
 def _units():
     units = [("capi", CSRC / "fst_capi.hip", [f'-DFST_BUILD_ID="{source_hash()}"']),
-             ("norm", CSRC / "fst_norm.hip", []), ("ffn", CSRC / "fst_ffn.hip", [])]
+             ("norm", CSRC / "fst_norm.hip", []), ("rms", CSRC / "fst_rms.hip", []),
+             ("ffn", CSRC / "fst_ffn.hip", []), ("experts", CSRC / "fst_experts.hip", [])]
     for tag, ctype in FFN_DTYPES.items():
         units.append((f"ffn_{tag}", CSRC / "fst_ffn_inst.hip", [f"-DFST_T={ctype}", f"-DFST_NAME={tag}"]))
+        units.append((f"ffn_experts_{tag}", CSRC / "fst_ffn_inst.hip",
+                      [f"-DFST_T={ctype}", f"-DFST_NAME=experts_{tag}", "-DFST_EXPERTS=1"]))
     for tag, ctype in DTYPES.items():
         for d in HEAD_DIMS:
             name = f"{tag}_{d}"

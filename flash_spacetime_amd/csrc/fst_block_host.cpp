@@ -1,9 +1,10 @@
-// Host path of layer norm and the feed-forward block in native code: checks,
-// allocations, the C ABI call and the autograd node, on operands in the form
-// nearly every call gives them (norm.py and feed_forward.py decide the same in
-// Python; there a forward of 187 rows took 35 us of host time, its kernel 4).
+// Host path of the norms, the feed-forward block and the mixture of experts in
+// native code: checks, allocations, the C ABI call and the autograd node, on operands in
+// the form nearly every call gives them (norm.py, rms_norm.py, feed_forward.py and
+// experts.py decide the same in Python; there a forward of 187 rows took 35 us of host
+// time, its kernel 4).
 //
-// Both functions return None for anything but that form (tensors of several
+// All functions return None for anything but that form (tensors of several
 // devices or dtypes, subclasses, lengths that are not integers on the device,
 // calls that torch records, forward-mode derivatives, calls the library
 // refuses): the caller then takes the Python path, which handles or rejects it.
@@ -37,6 +38,19 @@ struct Library {
   decltype(&fst_ffn_forward) ffn_forward = nullptr;
   decltype(&fst_ffn_backward_workspace_bytes) ffn_workspace = nullptr;
   decltype(&fst_ffn_backward) ffn_backward = nullptr;
+  decltype(&fst_rms_norm_forward) rms_forward = nullptr;
+  decltype(&fst_rms_norm_fp8) rms_fp8 = nullptr;
+  decltype(&fst_rms_norm_backward_workspace_bytes) rms_workspace = nullptr;
+  decltype(&fst_rms_norm_backward) rms_backward = nullptr;
+  decltype(&fst_expert_route) route = nullptr;
+  decltype(&fst_expert_route_backward) route_backward = nullptr;
+  decltype(&fst_expert_sort_workspace_bytes) sort_workspace = nullptr;
+  decltype(&fst_expert_sort) sort = nullptr;
+  decltype(&fst_expert_spread) spread = nullptr;
+  decltype(&fst_expert_gather) gather = nullptr;
+  decltype(&fst_expert_ffn_forward) experts_forward = nullptr;
+  decltype(&fst_expert_ffn_backward_workspace_bytes) experts_workspace = nullptr;
+  decltype(&fst_expert_ffn_backward) experts_backward = nullptr;
   decltype(&fst_last_error) last_error = nullptr;
 } lib;
 
@@ -381,6 +395,436 @@ py::object ffn_call(const Tensor& x, const Tensor& wg, const Tensor& wu, const T
   return py::cast(ffn_forward(c, x, wg, wu, wd, bg, bu, bd, false).y);
 }
 
+// --- root-mean-square norm ----------------------------------------------------
+
+struct RmsRows {
+  Tensor x, w, y, s, aside;  // aside: rstd, or the scales of 8 bits
+  int64_t xs = 0;
+};
+
+RmsRows rms_forward(const NormCall& c, const Tensor& x, const Maybe& residual, const Maybe& weight, bool keep, bool fp8) {
+  const int n = (int)x.size(-1), B = (int)c.batch.B, L = (int)c.batch.L;
+  OnDevice on(x);
+  RmsRows k;
+  int64_t rs = 0;
+  Tensor r;
+  k.x = token_rows(x, k.xs, 1);
+  if (residual.has_value()) r = token_rows(*residual, rs, 1);
+  if (weight.has_value()) k.w = weight->contiguous();
+  const auto opt = x.options().requires_grad(false);
+  k.y = at::empty(x.sizes(), fp8 ? opt.dtype(at::kFloat8_e4m3fn) : opt);
+  if (r.defined()) k.s = at::empty(x.sizes(), opt);
+  if (fp8)
+    k.aside = at::empty(x.sizes().slice(0, x.dim() - 1), opt.dtype(at::kFloat));
+  else if (keep)
+    k.aside = at::empty({c.batch.B * c.batch.L}, opt.dtype(at::kFloat));
+  float* aside = static_cast<float*>(data(k.aside));
+  if (fp8)
+    check(lib.rms_fp8(c.dtype, c.param_dtype, B, L, n, data(k.x), k.xs, data(r), rs, data(k.w), ints(c.batch.lens),
+                      (float)c.eps, data(k.y), aside, data(k.s), on.stream),
+          "flash_rms_norm_fp8", true);
+  else
+    check(lib.rms_forward(c.dtype, c.param_dtype, B, L, n, data(k.x), k.xs, data(r), rs, data(k.w), ints(c.batch.lens),
+                          (float)c.eps, data(k.y), data(k.s), aside, on.stream),
+          "flash_rms_norm", true);
+  return k;
+}
+
+struct RmsFunction : torch::autograd::Function<RmsFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Maybe& residual, const Maybe& weight,
+                               const NormCall& c) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const RmsRows k = rms_forward(c, x, residual, weight, true, false);
+    const bool sum = k.s.defined();
+    ctx->save_for_backward({sum ? k.s : k.x, k.w, c.batch.lens, k.aside});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["call"] = c10::List<int64_t>({c.dtype, c.param_dtype, c.batch.B, c.batch.L, sum ? x.size(-1) : k.xs,
+                                                  wants_grad(x), wants_grad(residual), wants_grad(weight), sum});
+    return sum ? variable_list{k.y, k.s} : variable_list{k.y};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!recorded_by_fx(), "flash_rms_norm backward: make_fx cannot record it");
+    const variable_list saved = ctx->get_saved_variables();
+    const auto call = ctx->saved_data["call"].toIntVector();
+    variable_list out(4);
+    const Tensor& s = saved[0];
+    const Tensor ds_in = call[8] ? grads[1] : Tensor();
+    if (!grads[0].defined() && !ds_in.defined()) return out;
+    {
+      at::AutoGradMode no_graph(false);
+      OnDevice on(s);
+      const auto opt = s.options().requires_grad(false);
+      const int64_t n = s.size(-1), B = call[2], L = call[3];
+      int64_t dys, dss = 0;
+      const Tensor dy = token_rows(grads[0].defined() ? grads[0].to(s.scalar_type()) : at::zeros(s.sizes(), opt), dys, 1);
+      const Tensor ds = ds_in.defined() ? token_rows(ds_in.to(s.scalar_type()), dss, 1) : Tensor();
+      TORCH_CHECK(dy.sizes() == s.sizes() && dy.device() == s.device() && (!ds.defined() || (ds.sizes() == s.sizes() && ds.device() == s.device())),
+                  "flash_rms_norm backward: gradients must have the outputs' shape and device");
+      Tensor dx, dw, ws;
+      if (call[5] || call[6]) dx = at::empty(s.sizes(), opt);
+      size_t bytes = 0;
+      if (call[7]) {
+        dw = at::empty({n}, opt.dtype(call[1] == FST_F32 ? at::kFloat : s.scalar_type()));
+        bytes = lib.rms_workspace((int)call[0], (int)B, (int)L, (int)n);
+        ws = at::empty({(int64_t)std::max<size_t>(bytes, 1)}, opt.dtype(at::kByte));
+      }
+      check(lib.rms_backward((int)call[0], (int)call[1], (int)B, (int)L, (int)n, data(s), call[4], data(saved[1]),
+                             ints(saved[2]), static_cast<const float*>(data(saved[3])), data(dy), dys, data(ds), dss,
+                             data(dx), data(dw), data(ws), bytes, on.stream),
+            "flash_rms_norm backward", false);
+      if (call[5]) out[0] = dx;
+      if (call[6]) out[1] = dx;
+      out[2] = dw;
+    }
+    return once(std::move(out), "flash_rms_norm");
+  }
+};
+
+py::object rms_call(const Tensor& x, const Maybe& residual, const Maybe& weight, double eps, const Maybe& seqlens, bool fp8) {
+  const at::Device dev = x.device();
+  if (!lib.rms_forward || !dev.is_cuda() || recorded() || !plain(x, dev) || !plain(residual, dev) || !plain(weight, dev) ||
+      !plain(seqlens, dev))
+    return py::none();
+  NormCall c;
+  c.dtype = c.param_dtype = dtype_of(x.scalar_type());
+  c.eps = eps;
+  if (c.dtype < 0 || x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > INT32_MAX || !(eps >= 0)) return py::none();
+  if (residual.has_value() && (residual->sizes() != x.sizes() || residual->scalar_type() != x.scalar_type()))
+    return py::none();
+  if (weight.has_value()) {
+    if (weight->dim() != 1 || weight->size(0) != x.size(-1)) return py::none();
+    if (weight->scalar_type() != x.scalar_type() && weight->scalar_type() != at::kFloat) return py::none();
+    c.param_dtype = dtype_of(weight->scalar_type());
+  }
+  if (!batch_of(x, seqlens, c.batch)) return py::none();
+  variable_list out;
+  if (!fp8 && at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(residual) || wants_grad(weight))) {
+    out = RmsFunction::apply(x, residual, weight, c);
+  } else {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const RmsRows k = rms_forward(c, x, residual, weight, false, fp8);
+    out = fp8 ? variable_list{k.y, k.aside} : variable_list{k.y};
+    if (k.s.defined()) out.push_back(k.s);
+  }
+  if (out.size() == 3) return py::make_tuple(out[0], out[1], out[2]);
+  if (out.size() == 2) return py::make_tuple(out[0], out[1]);
+  return py::cast(out[0]);
+}
+
+// --- mixture of experts: router and sort ---------------------------------------
+
+struct RouteCall {
+  int dtype, K;
+  bool normalize;
+  Batch batch;
+};
+
+struct RouteFunction : torch::autograd::Function<RouteFunction> {
+  static void choose(const RouteCall& c, const Tensor& logits, Tensor& rows, int64_t& stride, Tensor& weights, Tensor& experts) {
+    OnDevice on(logits);
+    rows = token_rows(logits, stride, 1);
+    auto shape = logits.sizes().vec();
+    shape.back() = c.K;
+    const auto opt = logits.options().requires_grad(false);
+    weights = at::empty(shape, opt.dtype(at::kFloat));
+    experts = at::empty(shape, opt.dtype(at::kInt));
+    check(lib.route(c.dtype, (int)c.batch.B, (int)c.batch.L, (int)logits.size(-1), c.K, c.normalize, data(rows), stride,
+                    ints(c.batch.lens), static_cast<float*>(data(weights)), static_cast<int32_t*>(data(experts)), on.stream),
+          "flash_expert_route", true);
+  }
+
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const RouteCall& c) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    Tensor rows, weights, experts;
+    int64_t stride;
+    choose(c, logits, rows, stride, weights, experts);
+    ctx->mark_non_differentiable({experts});
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({c.normalize ? Tensor() : rows, c.batch.lens, weights, experts});
+    ctx->saved_data["call"] = c10::List<int64_t>({c.dtype, c.batch.B, c.batch.L, c.K, c.normalize, stride, (int64_t)logits.scalar_type()});
+    ctx->saved_data["shape"] = c10::List<int64_t>(logits.sizes());
+    return {weights, experts};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!recorded_by_fx(), "flash_expert_route backward: make_fx cannot record it");
+    variable_list out(2);
+    if (!grads[0].defined()) return out;
+    const variable_list v = ctx->get_saved_variables();
+    const auto call = ctx->saved_data["call"].toIntVector();
+    const auto shape = ctx->saved_data["shape"].toIntVector();
+    {
+      at::AutoGradMode no_graph(false);
+      OnDevice on(v[2]);
+      const Tensor dw = grads[0].to(at::kFloat).contiguous();
+      TORCH_CHECK(dw.sizes() == v[2].sizes() && dw.device() == v[2].device(),
+                  "flash_expert_route backward: the gradient must have the weights' shape and device");
+      out[0] = at::empty(shape, v[2].options().requires_grad(false).dtype((at::ScalarType)call[6]));
+      check(lib.route_backward((int)call[0], (int)call[1], (int)call[2], (int)shape.back(), (int)call[3], (int)call[4], data(v[0]),
+                               call[5], ints(v[1]), static_cast<const float*>(data(v[2])), ints(v[3]),
+                               static_cast<const float*>(data(dw)), data(out[0]), on.stream),
+            "flash_expert_route backward", false);
+    }
+    return once(std::move(out), "flash_expert_route");
+  }
+};
+
+py::object route_call(const Tensor& logits, int64_t K, bool normalize, const Maybe& seqlens) {
+  const at::Device dev = logits.device();
+  if (!lib.route || !dev.is_cuda() || recorded() || !plain(logits, dev) || !plain(seqlens, dev)) return py::none();
+  RouteCall c;
+  c.dtype = dtype_of(logits.scalar_type());
+  c.normalize = normalize;
+  if (c.dtype < 0 || logits.dim() < 1 || logits.size(-1) > INT32_MAX || K < 1 || K > logits.size(-1)) return py::none();
+  c.K = (int)K;
+  if (!batch_of(logits, seqlens, c.batch)) return py::none();
+  if (at::GradMode::is_enabled() && wants_grad(logits)) {
+    const variable_list out = RouteFunction::apply(logits, c);
+    return py::make_tuple(out[0], out[1]);
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  Tensor rows, weights, experts;
+  int64_t stride;
+  RouteFunction::choose(c, logits, rows, stride, weights, experts);
+  return py::make_tuple(weights, experts);
+}
+
+py::object sort_call(const Tensor& experts, int64_t E) {
+  const at::Device dev = experts.device();
+  if (!lib.sort || !dev.is_cuda() || recorded() || !plain(experts, dev) || experts.scalar_type() != at::kInt || experts.dim() < 1 ||
+      E < 1 || E > INT32_MAX || experts.numel() > INT32_MAX)
+    return py::none();
+  at::AutoDispatchBelowADInplaceOrView below;
+  OnDevice on(experts);
+  const Tensor from = experts.contiguous();
+  const auto opt = from.options().requires_grad(false);
+  const int slots = (int)from.numel();
+  const Tensor order = at::empty({slots}, opt), place = at::empty(from.sizes(), opt);
+  const size_t bytes = lib.sort_workspace(slots, (int)E);
+  const Tensor offsets = at::empty({E + 1}, opt);
+  const Tensor ws = bytes ? at::empty({(int64_t)bytes}, opt.dtype(at::kByte)) : Tensor();
+  check(lib.sort(slots, (int)E, ints(from), static_cast<int32_t*>(data(order)), static_cast<int32_t*>(data(place)),
+                 static_cast<int32_t*>(data(offsets)), data(ws), bytes, on.stream),
+        "flash_expert_sort", true);
+  return py::make_tuple(order, place, offsets);
+}
+
+// --- mixture of experts: rows to the experts and back ----------------------------
+
+struct Place {
+  Tensor place, offsets;  // dense
+};
+
+bool place_of(const Tensor& place, const Tensor& offsets, const at::Device& dev, Place& p) {
+  if (!plain(place, dev) || !plain(offsets, dev) || place.scalar_type() != at::kInt || offsets.scalar_type() != at::kInt ||
+      place.dim() < 1 || place.size(-1) < 1 || place.size(-1) > INT32_MAX || offsets.dim() != 1 || offsets.size(0) < 2)
+    return false;
+  p.place = place.contiguous();
+  p.offsets = offsets.contiguous();
+  return true;
+}
+
+// (rows at their places, dots with back)
+std::pair<Tensor, Tensor> spread_rows(const Tensor& x, const Place& p, const Tensor& weights, const Tensor& back, int64_t rows,
+                                      bool want_rows, const char* what, bool may_refuse) {
+  OnDevice on(x);
+  int64_t xs, bs = 0;
+  const int64_t n = x.size(-1), K = p.place.size(-1);
+  const Tensor xr = token_rows(x, xs, 1);
+  Tensor br, out, dw;
+  const auto opt = x.options().requires_grad(false);
+  if (back.defined()) {
+    br = token_rows(back, bs, 1);
+    dw = at::empty(p.place.sizes(), weights.options().requires_grad(false));
+  }
+  if (want_rows) out = at::empty({rows, n}, opt);
+  const int dtype = dtype_of(x.scalar_type());
+  check(lib.spread(dtype, weights.defined() ? dtype_of(weights.scalar_type()) : dtype, p.place.numel() / K, (int)K, (int)n, rows,
+                   data(xr), xs, ints(p.place), ints(p.offsets) + p.offsets.size(0) - 1, data(weights), data(br), bs, data(out),
+                   data(dw), on.stream),
+        what, may_refuse);
+  return {out, dw};
+}
+
+Tensor gather_rows(const Tensor& x, const Place& p, const Tensor& weights, const char* what, bool may_refuse) {
+  OnDevice on(x);
+  int64_t xs;
+  const Tensor xr = token_rows(x, xs, 1);
+  auto shape = p.place.sizes().vec();
+  const int64_t K = shape.back();
+  shape.back() = x.size(-1);
+  const Tensor out = at::empty(shape, x.options().requires_grad(false));
+  const int dtype = dtype_of(x.scalar_type());
+  check(lib.gather(dtype, weights.defined() ? dtype_of(weights.scalar_type()) : dtype, p.place.numel() / K, (int)K, (int)x.size(-1),
+                   x.size(0), data(xr), xs, ints(p.place), data(weights), data(out), on.stream),
+        what, may_refuse);
+  return out;
+}
+
+struct DispatchFunction : torch::autograd::Function<DispatchFunction> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Place& p) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({p.place, p.offsets});
+    return spread_rows(x, p, Tensor(), Tensor(), p.place.numel(), true, "flash_expert_dispatch", true).first;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!recorded_by_fx(), "flash_expert_dispatch backward: make_fx cannot record it");
+    const variable_list v = ctx->get_saved_variables();
+    variable_list out(2);
+    {
+      at::AutoGradMode no_graph(false);
+      TORCH_CHECK(grads[0].dim() == 2 && grads[0].size(0) == v[0].numel() && grads[0].device() == v[0].device(),
+                  "flash_expert_dispatch backward: the gradient must have the output's shape and device");
+      out[0] = gather_rows(grads[0], Place{v[0], v[1]}, Tensor(), "flash_expert_dispatch backward", false);
+    }
+    return once(std::move(out), "flash_expert_dispatch");
+  }
+};
+
+py::object dispatch_call(const Tensor& x, const Tensor& place, const Tensor& offsets) {
+  const at::Device dev = x.device();
+  Place p;
+  if (!lib.spread || !dev.is_cuda() || recorded() || !plain(x, dev) || dtype_of(x.scalar_type()) < 0 || x.dim() < 1 ||
+      x.size(-1) < 1 || x.size(-1) > INT32_MAX || !place_of(place, offsets, dev, p) ||
+      x.sizes().slice(0, x.dim() - 1) != place.sizes().slice(0, place.dim() - 1))
+    return py::none();
+  if (at::GradMode::is_enabled() && wants_grad(x)) return py::cast(DispatchFunction::apply(x, p));
+  at::AutoDispatchBelowADInplaceOrView below;
+  return py::cast(spread_rows(x, p, Tensor(), Tensor(), p.place.numel(), true, "flash_expert_dispatch", true).first);
+}
+
+struct CombineFunction : torch::autograd::Function<CombineFunction> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& ys, const Tensor& weights, const Place& p) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor w = weights.contiguous();
+    ctx->save_for_backward({wants_grad(weights) ? ys : Tensor(), w, p.place, p.offsets});
+    ctx->saved_data["call"] = c10::List<int64_t>({ys.size(0), (int64_t)ys.scalar_type(), wants_grad(ys)});
+    return gather_rows(ys, p, w, "flash_expert_combine", true);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!recorded_by_fx(), "flash_expert_combine backward: make_fx cannot record it");
+    const variable_list v = ctx->get_saved_variables();
+    const auto call = ctx->saved_data["call"].toIntVector();
+    variable_list out(3);
+    {
+      at::AutoGradMode no_graph(false);
+      const Tensor dy = grads[0].to((at::ScalarType)call[1]);
+      TORCH_CHECK(dy.sizes().slice(0, dy.dim() - 1) == v[2].sizes().slice(0, v[2].dim() - 1) && dy.device() == v[2].device(),
+                  "flash_expert_combine backward: the gradient must have the output's shape and device");
+      auto [dys, dw] = spread_rows(dy, Place{v[2], v[3]}, v[1], v[0], call[0], call[2], "flash_expert_combine backward", false);
+      out[0] = dys;
+      out[1] = dw;
+    }
+    return once(std::move(out), "flash_expert_combine");
+  }
+};
+
+py::object combine_call(const Tensor& ys, const Tensor& weights, const Tensor& place, const Tensor& offsets) {
+  const at::Device dev = ys.device();
+  Place p;
+  if (!lib.gather || !dev.is_cuda() || recorded() || !plain(ys, dev) || dtype_of(ys.scalar_type()) < 0 || ys.dim() != 2 ||
+      ys.size(1) < 1 || ys.size(1) > INT32_MAX || !plain(weights, dev) || !place_of(place, offsets, dev, p) ||
+      weights.sizes() != place.sizes() || (weights.scalar_type() != ys.scalar_type() && weights.scalar_type() != at::kFloat))
+    return py::none();
+  if (at::GradMode::is_enabled() && (wants_grad(ys) || wants_grad(weights)))
+    return py::cast(CombineFunction::apply(ys, weights, p));
+  at::AutoDispatchBelowADInplaceOrView below;
+  return py::cast(gather_rows(ys, p, weights.contiguous(), "flash_expert_combine", true));
+}
+
+// --- mixture of experts: feed-forward --------------------------------------------
+
+struct ExpertsCall {
+  int dtype, act;
+  int64_t rows, E, D, F;
+};
+
+struct ExpertsKept {
+  Tensor x, offsets, wg, wu, wd, hidden, gate, up, y;
+  int64_t xs;
+};
+
+ExpertsKept experts_forward(const ExpertsCall& c, const Tensor& x, const Tensor& offsets, const Tensor& wg, const Tensor& wu,
+                            const Tensor& wd, bool keep) {
+  OnDevice on(x);
+  ExpertsKept k;
+  k.x = token_rows(x, k.xs, 16);
+  k.offsets = offsets.contiguous();
+  k.wg = dense16(wg), k.wu = dense16(wu), k.wd = dense16(wd);
+  const auto opt = x.options().requires_grad(false);
+  k.y = at::empty(x.sizes(), opt);
+  k.hidden = at::empty({c.rows, c.F}, opt);
+  if (keep && c.dtype == FST_F32) k.gate = at::empty({c.rows, c.F}, opt), k.up = at::empty({c.rows, c.F}, opt);
+  check(lib.experts_forward(c.dtype, c.act, (int)c.rows, (int)c.E, (int)c.D, (int)c.F, data(k.x), k.xs, ints(k.offsets),
+                            data(k.wg), data(k.wu), data(k.wd), data(k.hidden), data(k.gate), data(k.up), data(k.y), on.stream),
+        "flash_expert_feed_forward", true);
+  return k;
+}
+
+struct ExpertsFunction : torch::autograd::Function<ExpertsFunction> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& offsets, const Tensor& wg, const Tensor& wu,
+                        const Tensor& wd, const ExpertsCall& c) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const ExpertsKept k = experts_forward(c, x, offsets, wg, wu, wd, true);
+    ctx->save_for_backward({k.x, k.offsets, k.wg, k.wu, k.wd, k.hidden, k.gate, k.up});
+    ctx->saved_data["call"] = c10::List<int64_t>({c.dtype, c.act, c.rows, c.E, c.D, c.F, k.xs, wants_grad(x), wants_grad(wg),
+                                                  wants_grad(wu), wants_grad(wd)});
+    return k.y;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!recorded_by_fx(), "flash_expert_feed_forward backward: make_fx cannot record it");
+    const variable_list v = ctx->get_saved_variables();
+    const auto call = ctx->saved_data["call"].toIntVector();
+    variable_list out(6);
+    {
+      at::AutoGradMode no_graph(false);
+      const Tensor& x = v[0];
+      OnDevice on(x);
+      const auto opt = x.options().requires_grad(false);
+      const int64_t rows = call[2], E = call[3], D = call[4], F = call[5];
+      int64_t dys;
+      const Tensor dy = token_rows(grads[0].to(x.scalar_type()), dys, 16);
+      TORCH_CHECK(dy.sizes() == x.sizes() && dy.device() == x.device(),
+                  "flash_expert_feed_forward backward: the gradient must have the output's shape and device");
+      const std::vector<int64_t> shapes[4] = {{rows, D}, {E, F, D}, {E, F, D}, {E, D, F}};
+      Tensor g[4];
+      for (int i = 0; i < 4; ++i)
+        if (call[7 + i]) g[i] = at::empty(shapes[i], opt);
+      const size_t bytes = lib.experts_workspace((int)call[0], (int)rows, (int)E, (int)D, (int)F);
+      const Tensor ws = at::empty({(int64_t)std::max<size_t>(bytes, 1)}, opt.dtype(at::kByte));
+      check(lib.experts_backward((int)call[0], (int)call[1], (int)rows, (int)E, (int)D, (int)F, data(x), call[6], ints(v[1]),
+                                 data(v[2]), data(v[3]), data(v[4]), data(v[5]), data(v[6]), data(v[7]), data(dy), dys,
+                                 data(g[0]), data(g[1]), data(g[2]), data(g[3]), data(ws), bytes, on.stream),
+            "flash_expert_feed_forward backward", false);
+      out[0] = g[0];
+      for (int i = 1; i < 4; ++i) out[1 + i] = g[i];
+    }
+    return once(std::move(out), "flash_expert_feed_forward");
+  }
+};
+
+py::object experts_call(const Tensor& x, const Tensor& offsets, const Tensor& wg, const Tensor& wu, const Tensor& wd, int act) {
+  const at::Device dev = x.device();
+  if (!lib.experts_forward || !dev.is_cuda() || recorded()) return py::none();
+  for (const Tensor* t : {&x, &wg, &wu, &wd})
+    if (!plain(*t, dev) || t->scalar_type() != x.scalar_type()) return py::none();
+  ExpertsCall c;
+  c.dtype = dtype_of(x.scalar_type());
+  c.act = act;
+  if (c.dtype < 0 || x.dim() != 2 || wg.dim() != 3 || !plain(offsets, dev) || offsets.scalar_type() != at::kInt) return py::none();
+  c.rows = x.size(0), c.D = x.size(1), c.E = wg.size(0), c.F = wg.size(1);
+  if (c.rows > INT32_MAX || c.D < 1 || c.D > INT32_MAX || c.F > INT32_MAX || c.E > INT32_MAX || wg.size(2) != c.D ||
+      wu.sizes() != wg.sizes() || wd.sizes() != at::IntArrayRef({c.E, c.D, c.F}) || offsets.dim() != 1 || offsets.size(0) != c.E + 1)
+    return py::none();
+  bool graph = false;
+  for (const Tensor* t : {&x, &wg, &wu, &wd}) graph |= wants_grad(*t);
+  if (at::GradMode::is_enabled() && graph) return py::cast(ExpertsFunction::apply(x, offsets, wg, wu, wd, c));
+  at::AutoDispatchBelowADInplaceOrView below;
+  return py::cast(experts_forward(c, x, offsets, wg, wu, wd, false).y);
+}
+
 // A refused call and a failed allocation are the Python path's to report.
 template <typename F, typename... A>
 py::object or_none(F f, const A&... args) {
@@ -405,6 +849,27 @@ void bind_block_library(size_t norm_fwd, size_t norm_ws, size_t norm_bwd, size_t
   lib.last_error = reinterpret_cast<decltype(lib.last_error)>(last_error);
 }
 
+void bind_experts_library(const py::args& at) {
+  if (at.empty()) return;
+  size_t i = 0;
+  const auto bind = [&](auto& field) {
+    field = reinterpret_cast<std::remove_reference_t<decltype(field)>>(py::cast<size_t>(at[i++]));
+  };
+  bind(lib.rms_forward);
+  bind(lib.rms_fp8);
+  bind(lib.rms_workspace);
+  bind(lib.rms_backward);
+  bind(lib.route);
+  bind(lib.route_backward);
+  bind(lib.sort_workspace);
+  bind(lib.sort);
+  bind(lib.spread);
+  bind(lib.gather);
+  bind(lib.experts_forward);
+  bind(lib.experts_workspace);
+  bind(lib.experts_backward);
+}
+
 void define_block_operators(py::module_& m) {
   m.def("layer_norm", [](const Tensor& x, const Maybe& residual, const Maybe& weight, const Maybe& bias, double eps,
                          const Maybe& seqlens) { return or_none(norm_call, x, residual, weight, bias, eps, seqlens); });
@@ -412,4 +877,22 @@ void define_block_operators(py::module_& m) {
                            const Maybe& bu, const Maybe& bd, int act, const Maybe& seqlens) {
     return or_none(ffn_call, x, wg, wu, wd, bg, bu, bd, act, seqlens);
   });
+  m.def("rms_norm", [](const Tensor& x, const Maybe& residual, const Maybe& weight, double eps, const Maybe& seqlens) {
+    return or_none(rms_call, x, residual, weight, eps, seqlens, false);
+  });
+  m.def("rms_norm_fp8", [](const Tensor& x, const Maybe& residual, const Maybe& weight, double eps, const Maybe& seqlens) {
+    return or_none(rms_call, x, residual, weight, eps, seqlens, true);
+  });
+  m.def("expert_route", [](const Tensor& logits, int64_t top_k, bool normalize, const Maybe& seqlens) {
+    return or_none(route_call, logits, top_k, normalize, seqlens);
+  });
+  m.def("expert_sort", [](const Tensor& experts, int64_t num_experts) { return or_none(sort_call, experts, num_experts); });
+  m.def("expert_dispatch", [](const Tensor& x, const Tensor& place, const Tensor& offsets) {
+    return or_none(dispatch_call, x, place, offsets);
+  });
+  m.def("expert_combine", [](const Tensor& ys, const Tensor& weights, const Tensor& place, const Tensor& offsets) {
+    return or_none(combine_call, ys, weights, place, offsets);
+  });
+  m.def("expert_feed_forward", [](const Tensor& x, const Tensor& offsets, const Tensor& wg, const Tensor& wu, const Tensor& wd,
+                                  int act) { return or_none(experts_call, x, offsets, wg, wu, wd, act); });
 }

@@ -1,0 +1,632 @@
+// Mixture of experts around its feed-forward (fst_ffn*.hip): the router, the
+// tokens' slots sorted by expert, and rows moved to the experts' order and back.
+//
+//   route: of each token's E logits the K largest (ties: the lowest index), and
+//     their softmax, over the chosen or over all:  w_k = exp(l_k - m) / sum.
+//     Backward over the chosen: dl_k = w_k (dw_k - sum_j w_j dw_j), else 0; over all:
+//     dl_e = [e chosen] w_e dw_e - p_e sum_j w_j dw_j, with p the softmax.
+//   sort: a stable counting sort of the T K slots by expert.
+//   spread: out[place[t, k]] = w[t, k] x[t] (w: 1), dw[t, k] = x[t] . back[place[t, k]].
+//   gather: out[t] = sum_k w[t, k] rows[place[t, k]] (w: 1).
+//
+// All are bound by memory (or the launch, in calls of few tokens): the movers read each
+// row once, hold it in registers (fst_rows.h) and write it to its K places, or
+// read K rows and write their sum. Sums are float32 in a fixed order; every output is
+// rounded once. Places outside the rows are skipped, whoever wrote them.
+#include "fst_rows.h"
+
+namespace fst {
+
+namespace {
+
+constexpr int kMostExperts = 512, kMostChosen = 16;
+
+// --- router -----------------------------------------------------------------
+
+struct RouteArgs {
+  const void* logits;
+  const int32_t* lens;
+  float* weights;
+  int32_t* experts;
+  long rows, ld;
+  int L, E, K, chosen;
+};
+
+struct RouteGradArgs {
+  const void* logits;
+  const int32_t* lens;
+  const float *weights, *dw;
+  const int32_t* experts;
+  void* dlogits;
+  long rows, ld;
+  int L, E, K, chosen;
+};
+
+// A logit as an unsigned in its order: NaN above all, 0 for what cannot be chosen
+// (-inf, and what was). The two zeros are one.
+__device__ __forceinline__ unsigned order_key(float v) {
+  if (v != v) return 0xffffffffu;
+  const unsigned u = __float_as_uint(v + 0.f);
+  return v == -__builtin_inff() ? 0u : u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(unsigned k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+
+// Reductions of unsigneds over groups of G = 16 or 64 lanes.
+template <int G, typename F>
+__device__ __forceinline__ unsigned group_reduce(unsigned x, F f) {
+  x = f(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, false));
+  x = f(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, false));
+  x = f(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, false));
+  x = f(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, false));
+  if constexpr (G == 64) {
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = f(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x = f(b[0], b[1]);
+  }
+  return x;
+}
+
+// Lane l of a row's G holds its logits l + G i, i < NC; -inf past the last.
+template <typename T, int G, int NC>
+__device__ __forceinline__ void load_logits(const T* row, int l, int E, float* v) {
+#pragma unroll
+  for (int i = 0; i < NC; ++i) v[i] = l + G * i < E ? (float)row[l + G * i] : -__builtin_inff();
+}
+
+template <typename T, int G, int NC>
+__global__ __launch_bounds__(256) void expert_route(RouteArgs a) {
+  const int l = threadIdx.x % G;
+  const long row = (long)blockIdx.x * (256 / G) + threadIdx.x / G;
+  if (row >= a.rows) return;
+  float w = 0.f;
+  int expert = -1;  // lane k: the k-th largest
+  if (row_valid(a.lens, row, a.L)) {
+    float v[NC];
+    load_logits<T, G, NC>(static_cast<const T*>(a.logits) + row * a.ld, l, a.E, v);
+    unsigned key[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) key[i] = order_key(v[i]);
+    float top = 0.f, mine = 0.f;
+    for (int k = 0; k < a.K; ++k) {
+      unsigned best = key[0], at = l;
+#pragma unroll
+      for (int i = 1; i < NC; ++i)
+        if (key[i] > best) best = key[i], at = l + G * i;
+      const unsigned most = group_reduce<G>(best, [](unsigned x, unsigned y) { return max(x, y); });
+      if (most == 0) break;  // nothing left to choose: the same for all lanes of the row
+      at = group_reduce<G>(best == most ? at : 0xffffffffu, [](unsigned x, unsigned y) { return min(x, y); });
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if ((int)at == l + G * i) key[i] = 0;
+      const float value = key_value(most);
+      if (k == 0) top = value;
+      if (l == k) mine = value, expert = (int)at;
+    }
+    w = expert >= 0 ? expf(mine - top) : 0.f;
+    float sum = 0.f;
+    if (a.chosen) {
+      sum = w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < NC; ++i) sum += l + G * i < a.E && !(v[i] == -__builtin_inff()) ? expf(v[i] - top) : 0.f;
+    }
+    sum = group_sum<G>(sum, nullptr);
+    w = expert >= 0 ? w / sum : 0.f;
+  }
+  if (l < a.K) {
+    a.weights[row * a.K + l] = w;
+    a.experts[row * a.K + l] = expert;
+  }
+}
+
+template <typename T, int G, int NC>
+__global__ __launch_bounds__(256) void expert_route_grad(RouteGradArgs a) {
+  const int l = threadIdx.x % G;
+  const long row = (long)blockIdx.x * (256 / G) + threadIdx.x / G;
+  if (row >= a.rows) return;
+  float d[NC];
+#pragma unroll
+  for (int i = 0; i < NC; ++i) d[i] = 0.f;
+  if (row_valid(a.lens, row, a.L)) {
+    int expert = -1;
+    float w = 0.f, g = 0.f;
+    if (l < a.K) expert = a.experts[row * a.K + l];
+    if (expert >= 0) w = a.weights[row * a.K + l], g = a.dw[row * a.K + l];
+    const float mean = group_sum<G>(w * g, nullptr);
+    g = a.chosen ? w * (g - mean) : w * g;
+    if (!a.chosen) {
+      float v[NC], top = -__builtin_inff(), sum = 0.f;
+      load_logits<T, G, NC>(static_cast<const T*>(a.logits) + row * a.ld, l, a.E, v);
+#pragma unroll
+      for (int i = 0; i < NC; ++i) top = fmaxf(top, v[i]);
+      top = key_value(group_reduce<G>(order_key(top), [](unsigned x, unsigned y) { return max(x, y); }));
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        v[i] = v[i] == -__builtin_inff() ? 0.f : expf(v[i] - top);
+        sum += v[i];
+      }
+      sum = group_sum<G>(sum, nullptr);
+#pragma unroll
+      for (int i = 0; i < NC; ++i) d[i] = sum == 0.f ? 0.f : -mean * (v[i] / sum);
+    }
+    for (int k = 0; k < a.K; ++k) {
+      const int at = __shfl(expert, k, G);
+      const float add = __shfl(g, k, G);
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (at == l + G * i) d[i] += add;
+    }
+  }
+  T* out = static_cast<T*>(a.dlogits) + row * a.E;
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+    if (l + G * i < a.E) out[l + G * i] = (T)d[i];
+}
+
+// f(lanes, logits a lane): 16 lanes a row up to 64 experts, a wave above.
+template <typename F>
+void by_experts(int E, F f) {
+  if (E <= 16)
+    f(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
+  else if (E <= 64)
+    f(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
+  else if (E <= 128)
+    f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+  else
+    f(std::integral_constant<int, 64>{}, std::integral_constant<int, 8>{});
+}
+
+int check_route(int dtype, int B, int L, int E, int K) {
+  if (dtype != FST_BF16 && dtype != FST_F32 && dtype != FST_F16)
+    return fail(FST_EINVAL, "dtype must be FST_BF16, FST_F16 or FST_F32, got %d", dtype);
+  if (B < 0 || L < 0) return fail(FST_EINVAL, "negative size (B=%d, L=%d)", B, L);
+  if (E < 1 || K < 1 || K > E) return fail(FST_EINVAL, "top_k must be 1 .. experts, got %d of %d", K, E);
+  if (E > kMostExperts || K > kMostChosen)
+    return fail(FST_EUNSUPPORTED, "at most %d experts and %d of them a token, got %d, %d", kMostExperts, kMostChosen, E, K);
+  if ((long)B * L * K > 0x7fffffffL - 65536) return fail(FST_EUNSUPPORTED, "too many slots (B=%d, L=%d, top_k=%d)", B, L, K);
+  return FST_OK;
+}
+
+// --- sort -------------------------------------------------------------------
+
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64, kMostBins = kMostExperts + 1;
+
+struct SortArgs {
+  const int32_t* experts;
+  int32_t *order, *place, *offsets;
+  int32_t* counts;  // [blocks][E + 1], or null: one workgroup
+  int slots, E, chunk, bits;
+};
+
+// A slot's bin: its expert, or E where that is none.
+__device__ __forceinline__ int bin_of(int expert, int E) { return (unsigned)expert < (unsigned)E ? expert : E; }
+
+__global__ __launch_bounds__(kSortThreads) void expert_count(SortArgs a) {
+  __shared__ int count[kMostBins];
+  for (int i = threadIdx.x; i <= a.E; i += kSortThreads) count[i] = 0;
+  __syncthreads();
+  const int s0 = blockIdx.x * a.chunk, s1 = min(s0 + a.chunk, a.slots);
+  for (int s = s0 + threadIdx.x; s < s1; s += kSortThreads) atomicAdd(&count[bin_of(a.experts[s], a.E)], 1);
+  __syncthreads();
+  for (int i = threadIdx.x; i <= a.E; i += kSortThreads) a.counts[(long)blockIdx.x * (a.E + 1) + i] = count[i];
+}
+
+// Each wave of a workgroup takes a run of its chunk. A slot's row: those of smaller
+// bins, of its bin in the chunks before and in the waves before, and those before it in
+// its wave, which ballots over the bin's bits tell. All integers: the order of the
+// additions does not matter.
+__global__ __launch_bounds__(kSortThreads) void expert_place(SortArgs a) {
+  __shared__ int next[kSortWaves][kMostBins];  // counts, then the next row, of each wave and bin
+  __shared__ int total[kMostBins], before[kMostBins];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bins = a.E + 1;
+  for (int i = tid; i < kSortWaves * bins; i += kSortThreads) next[i / bins][i % bins] = 0;
+  for (int i = tid; i < bins; i += kSortThreads) total[i] = before[i] = 0;
+  __syncthreads();
+  const int c0 = blockIdx.x * a.chunk, c1 = min(c0 + a.chunk, a.slots);
+  const int run = ((c1 - c0 + kSortWaves - 1) / kSortWaves + 63) / 64 * 64;
+  const int s0 = min(c0 + wave * run, c1), s1 = min(s0 + run, c1);
+  for (int s = s0 + lane; s < s1; s += 64) atomicAdd(&next[wave][bin_of(a.experts[s], a.E)], 1);
+  if (a.counts) {
+    const int all = gridDim.x * bins;
+    for (int i = tid; i < all; i += kSortThreads) {
+      const int b = i / bins, e = i - b * bins, n = a.counts[i];
+      if (n) {
+        atomicAdd(&total[e], n);
+        if (b < (int)blockIdx.x) atomicAdd(&before[e], n);
+      }
+    }
+  }
+  __syncthreads();
+  if (!a.counts) {
+    for (int i = tid; i < bins; i += kSortThreads) {
+      int n = 0;
+      for (int w = 0; w < kSortWaves; ++w) n += next[w][i];
+      total[i] = n;
+    }
+    __syncthreads();
+  }
+  if (wave == 0) {  // total -> rows of smaller bins
+    int carry = 0;
+    for (int i = lane; i - lane < bins; i += 64) {
+      const int n = i < bins ? total[i] : 0;
+      int sum = n;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const int up = __shfl_up(sum, d);
+        if (lane >= d) sum += up;
+      }
+      if (i < bins) {
+        total[i] = carry + sum - n;
+        if (blockIdx.x == 0) a.offsets[i] = carry + sum - n;
+      }
+      carry += __shfl(sum, 63);
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < bins; i += kSortThreads) {
+    int at = total[i] + before[i];
+    for (int w = 0; w < kSortWaves; ++w) {
+      const int n = next[w][i];
+      next[w][i] = at;
+      at += n;
+    }
+  }
+  __syncthreads();
+  volatile int* mine = next[wave];
+  for (int s = s0 + lane; s - lane < s1; s += 64) {
+    const bool in = s < s1;
+    const int bin = in ? bin_of(a.experts[s], a.E) : 0;
+    unsigned long long same = __ballot(in);
+    for (int b = 0; b < a.bits; ++b) {
+      const unsigned long long set = __ballot((bin >> b) & 1);
+      same &= (bin >> b) & 1 ? set : ~set;
+    }
+    const int rank = __popcll(same & ((1ull << lane) - 1));
+    const int row = in ? mine[bin] + rank : 0;
+    if (in && rank == 0) mine[bin] = row + __popcll(same);  // after every lane's read: LDS keeps a wave's order
+    if (in) {
+      a.place[s] = bin < a.E ? row : -1;
+      a.order[row] = bin < a.E ? s : -1;
+    }
+  }
+}
+
+struct SortPlan {
+  int blocks, chunk;
+};
+
+// Up to 8192 slots one workgroup does all; more are counted first, by chunks of which
+// every workgroup then adds up all counts (16384 of them at most).
+SortPlan sort_plan(int slots, int E) {
+  if (slots <= 8192) return SortPlan{1, slots};
+  int blocks = 16384 / (E + 1);
+  blocks = blocks > 256 ? 256 : blocks;
+  const int need = (slots + 2047) / 2048;
+  blocks = blocks > need ? need : blocks;
+  const int chunk = ((slots + blocks - 1) / blocks + 1023) / 1024 * 1024;
+  return SortPlan{(slots + chunk - 1) / chunk, chunk};
+}
+
+// --- rows to the experts and back -------------------------------------------
+
+struct MoveArgs {
+  const void* in;       // spread: the tokens' rows; gather: the experts'
+  const void* back;     // spread: the experts' rows the dots are with, or null
+  const void* weights;  // [tokens, K], or null
+  const int32_t* place;
+  const int32_t* used;  // spread: rows of the experts (what is behind is zeros)
+  void *out, *dw;
+  long tokens, rows, ld, ldb;
+  int K, n;
+};
+
+// Lanes of a wave that work on one row.
+template <int LPR>
+constexpr int kRowLanes = LPR < 64 ? LPR : 64;
+
+// Lane k of the row's lanes in a wave: the k-th place of token t (-1: none, and past
+// the K).
+template <int LPR>
+__device__ __forceinline__ int load_place(const MoveArgs& a, long t) {
+  const int k = threadIdx.x % kRowLanes<LPR>;
+  if (t >= a.tokens || k >= a.K) return -1;
+  const int r = a.place[t * a.K + k];
+  return (unsigned)r < (unsigned)a.rows ? r : -1;
+}
+template <int LPR>
+__device__ __forceinline__ bool any_place(int place) {
+  const unsigned long long b = __ballot(place >= 0);
+  if constexpr (LPR >= 64) return b != 0;
+  return ((b >> (threadIdx.x & 63 & ~(LPR - 1))) & ((1ull << (LPR & 63)) - 1)) != 0;
+}
+template <int LPR>
+__device__ __forceinline__ int place_at(int place, int k) {
+  return __shfl(place, k, kRowLanes<LPR>);
+}
+template <typename T>
+__device__ __forceinline__ float weight_at(const MoveArgs& a, long t, int k, bool f32) {
+  const long i = t * a.K + k;
+  return f32 ? static_cast<const float*>(a.weights)[i] : (float)static_cast<const T*>(a.weights)[i];
+}
+
+// A group walks the tokens with the next one's row, and the places of the one after it,
+// in flight; a token without places is not read.
+template <typename T, int LPR, int NC, bool EDGE, bool DOT>
+__global__ __launch_bounds__(LPR > 256 ? LPR : 256) void expert_spread(MoveArgs a, int w_f32) {
+  typedef Pieces<T, LPR, NC, EDGE> P;
+  constexpr int E = P::E, NT = LPR > 256 ? LPR : 256, G = NT / LPR;
+  __shared__ float red[LPR > 64 ? LPR / 64 : 1];
+  const int l = threadIdx.x % LPR, n = a.n;
+  const long step = (long)gridDim.x * G;
+  const long first = (long)blockIdx.x * G + threadIdx.x / LPR;
+  P x0, x1;
+  long t = first;
+  int now = load_place<LPR>(a, t), next = load_place<LPR>(a, t + step);
+  if (any_place<LPR>(now)) x0.load(static_cast<const T*>(a.in) + t * a.ld, l, n);
+  for (; t < a.tokens; t += step) {
+    const int later = load_place<LPR>(a, t + 2 * step);
+    if (any_place<LPR>(next)) x1.load(static_cast<const T*>(a.in) + (t + step) * a.ld, l, n);
+    float v[E];
+    if (any_place<LPR>(now)) x0.get(v, l, n);
+    for (int k = 0; k < a.K; ++k) {
+      const int r = place_at<LPR>(now, k);
+      float dot = 0.f;
+      if (r >= 0) {
+        if constexpr (DOT) {
+          P y;
+          float q[E];
+          y.load(static_cast<const T*>(a.back) + r * a.ldb, l, n);
+          y.get(q, l, n);
+#pragma unroll
+          for (int i = 0; i < E; ++i) dot = fmaf(v[i], q[i], dot);
+          dot = group_sum<LPR>(dot, red);
+        }
+        if (a.out) {
+          T* out = static_cast<T*>(a.out) + (long)r * n;
+          if (a.weights) {
+            const float w = weight_at<T>(a, t, k, w_f32);
+            float q[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) q[i] = w * v[i];
+            P::store(out, l, n, q);
+          } else {
+            P::store(out, l, n, v);
+          }
+        }
+      }
+      if (DOT && l == 0) {
+        if (w_f32)
+          static_cast<float*>(a.dw)[t * a.K + k] = dot;
+        else
+          static_cast<T*>(a.dw)[t * a.K + k] = (T)dot;
+      }
+    }
+    x0 = x1;
+    now = next;
+    next = later;
+  }
+  if (!a.out) return;
+  float zero[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) zero[i] = 0.f;
+  for (long r = max(*a.used, 0) + first; r < a.rows; r += step) P::store(static_cast<T*>(a.out) + r * n, l, n, zero);
+}
+
+// Two of a token's rows are in flight at a time, the next token's places before
+// them. A token without places is zeros.
+template <typename T, int LPR, int NC, bool EDGE>
+__global__ __launch_bounds__(LPR > 256 ? LPR : 256) void expert_gather(MoveArgs a, int w_f32) {
+  typedef Pieces<T, LPR, NC, EDGE> P;
+  constexpr int E = P::E, NT = LPR > 256 ? LPR : 256, G = NT / LPR;
+  const int l = threadIdx.x % LPR, n = a.n;
+  const long step = (long)gridDim.x * G;
+  long t = (long)blockIdx.x * G + threadIdx.x / LPR;
+  int now = load_place<LPR>(a, t);
+  for (; t < a.tokens; t += step) {
+    const int next = load_place<LPR>(a, t + step);
+    float sum[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) sum[i] = 0.f;
+    for (int k = 0; k < a.K; k += 2) {
+      const int ra = place_at<LPR>(now, k), rb = k + 1 < a.K ? place_at<LPR>(now, k + 1) : -1;
+      P xa, xb;
+      if (ra >= 0) xa.load(static_cast<const T*>(a.in) + ra * a.ld, l, n);
+      if (rb >= 0) xb.load(static_cast<const T*>(a.in) + rb * a.ld, l, n);
+      auto add = [&](const P& x, int k) __attribute__((always_inline)) {
+        float q[E];
+        x.get(q, l, n);
+        const float w = a.weights ? weight_at<T>(a, t, k, w_f32) : 1.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) sum[i] = fmaf(w, q[i], sum[i]);
+      };
+      if (ra >= 0) add(xa, k);
+      if (rb >= 0) add(xb, k + 1);
+    }
+    P::store(static_cast<T*>(a.out) + t * n, l, n, sum);
+    now = next;
+  }
+}
+
+constexpr int kMoveBlocks = 2048;
+
+int check_move(int dtype, int weight_dtype, int64_t tokens, int K, int N, int64_t rows, RowPlan& p) {
+  if (dtype != FST_BF16 && dtype != FST_F32 && dtype != FST_F16)
+    return fail(FST_EINVAL, "dtype must be FST_BF16, FST_F16 or FST_F32, got %d", dtype);
+  if (weight_dtype != dtype && weight_dtype != FST_F32)
+    return fail(FST_EINVAL, "weight_dtype must be dtype or FST_F32, got %d", weight_dtype);
+  if (tokens < 0 || rows < 0) return fail(FST_EINVAL, "negative size (%ld tokens, %ld rows)", (long)tokens, (long)rows);
+  if (K < 1 || N < 1) return fail(FST_EINVAL, "need at least one slot and one feature, got %d, %d", K, N);
+  if (K > kMostChosen) return fail(FST_EUNSUPPORTED, "at most %d slots a token, got %d", kMostChosen, K);
+  if (rows > 0x7fffffffL - 65536 || tokens * K > 0x7fffffffL - 65536) return fail(FST_EUNSUPPORTED, "too many rows");
+  if (!plan_rows(dtype, N, p)) return fail(FST_EUNSUPPORTED, "rows of N=%d features: at most %d", N, kRowMax);
+  return FST_OK;
+}
+
+template <typename T>
+void launch_spread(const RowPlan& p, const MoveArgs& a, int w_f32, hipStream_t st) {
+  const long most = a.out && a.rows > a.tokens ? a.rows : a.tokens;
+  const int threads = p.lpr > 256 ? p.lpr : 256, blocks = row_blocks(p, most, kMoveBlocks);
+  by_plan<T>(p, [&](auto lanes, auto pieces, auto edge) {
+    if (a.back)
+      expert_spread<T, lanes(), pieces(), edge(), true><<<blocks, threads, 0, st>>>(a, w_f32);
+    else
+      expert_spread<T, lanes(), pieces(), edge(), false><<<blocks, threads, 0, st>>>(a, w_f32);
+  });
+}
+
+template <typename T>
+void launch_gather(const RowPlan& p, const MoveArgs& a, int w_f32, hipStream_t st) {
+  const int threads = p.lpr > 256 ? p.lpr : 256, blocks = row_blocks(p, a.tokens, kMoveBlocks);
+  by_plan<T>(p, [&](auto lanes, auto pieces, auto edge) {
+    expert_gather<T, lanes(), pieces(), edge()><<<blocks, threads, 0, st>>>(a, w_f32);
+  });
+}
+
+int launched(const char* what) {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(FST_ELAUNCH, "%s launch failed (%s)", what, hipGetErrorString(e));
+  return FST_OK;
+}
+
+}  // namespace
+
+}  // namespace fst
+
+using namespace fst;
+
+extern "C" {
+
+int fst_expert_route(int dtype, int B, int L, int E, int K, int normalize, const void* logits, int64_t logits_stride,
+                     const int32_t* seqlens, float* weights, int32_t* experts, void* stream) {
+  clear_error();
+  const int rc = check_route(dtype, B, L, E, K);
+  if (rc != FST_OK) return rc;
+  const long rows = (long)B * L;
+  if (rows == 0) return FST_OK;
+  if (!logits || !weights || !experts) return fail(FST_EINVAL, "null tensor pointer");
+  if (logits_stride < E) return fail(FST_EINVAL, "row stride below E=%d", E);
+  const RouteArgs a{logits, seqlens, weights, experts, rows, (long)logits_stride, L, E, K, normalize != 0};
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  by_experts(E, [&](auto lanes, auto count) {
+    const unsigned grid = (unsigned)((rows * lanes() + 255) / 256);
+    if (dtype == FST_BF16)
+      expert_route<bf16, lanes(), count()><<<grid, 256, 0, st>>>(a);
+    else if (dtype == FST_F16)
+      expert_route<f16, lanes(), count()><<<grid, 256, 0, st>>>(a);
+    else
+      expert_route<float, lanes(), count()><<<grid, 256, 0, st>>>(a);
+  });
+  return launched("expert route");
+}
+
+int fst_expert_route_backward(int dtype, int B, int L, int E, int K, int normalize, const void* logits,
+                              int64_t logits_stride, const int32_t* seqlens, const float* weights,
+                              const int32_t* experts, const float* dweights, void* dlogits, void* stream) {
+  clear_error();
+  const int rc = check_route(dtype, B, L, E, K);
+  if (rc != FST_OK) return rc;
+  const long rows = (long)B * L;
+  if (rows == 0) return FST_OK;
+  if ((!normalize && !logits) || !weights || !experts || !dweights || !dlogits) return fail(FST_EINVAL, "null tensor pointer");
+  if (!normalize && logits_stride < E) return fail(FST_EINVAL, "row stride below E=%d", E);
+  const RouteGradArgs a{logits, seqlens, weights, dweights, experts, dlogits, rows, (long)logits_stride, L, E, K, normalize != 0};
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  by_experts(E, [&](auto lanes, auto count) {
+    const unsigned grid = (unsigned)((rows * lanes() + 255) / 256);
+    if (dtype == FST_BF16)
+      expert_route_grad<bf16, lanes(), count()><<<grid, 256, 0, st>>>(a);
+    else if (dtype == FST_F16)
+      expert_route_grad<f16, lanes(), count()><<<grid, 256, 0, st>>>(a);
+    else
+      expert_route_grad<float, lanes(), count()><<<grid, 256, 0, st>>>(a);
+  });
+  return launched("expert route backward");
+}
+
+static int check_sort(int slots, int E) {
+  if (slots < 0) return fail(FST_EINVAL, "negative size (%d slots)", slots);
+  if (E < 1) return fail(FST_EINVAL, "need at least one expert, got %d", E);
+  if (E > kMostExperts) return fail(FST_EUNSUPPORTED, "at most %d experts, got %d", kMostExperts, E);
+  if (slots > 0x7fffffff - 65536) return fail(FST_EUNSUPPORTED, "too many slots (%d)", slots);
+  return FST_OK;
+}
+
+size_t fst_expert_sort_workspace_bytes(int slots, int E) {
+  if (check_sort(slots, E) != FST_OK) return 0;
+  const SortPlan p = sort_plan(slots, E);
+  return p.blocks > 1 ? align256((size_t)p.blocks * (E + 1) * sizeof(int32_t)) : 0;
+}
+
+int fst_expert_sort(int slots, int E, const int32_t* experts, int32_t* order, int32_t* place, int32_t* offsets,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+  clear_error();
+  const int rc = check_sort(slots, E);
+  if (rc != FST_OK) return rc;
+  if (!offsets || (slots > 0 && (!experts || !order || !place))) return fail(FST_EINVAL, "null tensor pointer");
+  const SortPlan p = sort_plan(slots, E);
+  const size_t need = fst_expert_sort_workspace_bytes(slots, E);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(FST_EWORKSPACE, "workspace of %zu bytes is smaller than the %zu required", workspace_bytes, need);
+  int bits = 0;
+  while (E >> bits) ++bits;
+  const SortArgs a{experts, order, place, offsets, p.blocks > 1 ? static_cast<int32_t*>(workspace) : nullptr,
+                   slots, E, p.chunk, bits};
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (p.blocks > 1) expert_count<<<p.blocks, kSortThreads, 0, st>>>(a);
+  expert_place<<<p.blocks, kSortThreads, 0, st>>>(a);
+  return launched("expert sort");
+}
+
+int fst_expert_spread(int dtype, int weight_dtype, int64_t tokens, int K, int N, int64_t rows, const void* x,
+                      int64_t x_stride, const int32_t* place, const int32_t* used, const void* weights,
+                      const void* back, int64_t back_stride, void* out, void* dweights, void* stream) {
+  clear_error();
+  RowPlan p;
+  const int rc = check_move(dtype, weight_dtype, tokens, K, N, rows, p);
+  if (rc != FST_OK) return rc;
+  if (!out && !dweights) return FST_OK;
+  if ((out && !used) || (tokens > 0 && (!x || !place)) || (rows > 0 && !back != !dweights))
+    return fail(FST_EINVAL, "null tensor pointer");
+  if (x_stride < N || (back && back_stride < N)) return fail(FST_EINVAL, "row stride below N=%d", N);
+  if (tokens == 0 && rows == 0) return FST_OK;
+  const size_t es = elem_size(dtype);
+  const MoveArgs a{x, dweights ? (back ? back : x) : nullptr, weights, place, used, out, dweights,
+                   (long)tokens, (long)rows, (long)x_stride, (long)back_stride, K, N};
+  p.edge = N * es % 16 != 0 || !aligned16(x, x_stride, es) || (back && !aligned16(back, back_stride, es)) ||
+           reinterpret_cast<uintptr_t>(out) % 16 != 0;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const int w_f32 = weight_dtype == FST_F32;
+  if (dtype == FST_BF16)
+    launch_spread<bf16>(p, a, w_f32, st);
+  else if (dtype == FST_F16)
+    launch_spread<f16>(p, a, w_f32, st);
+  else
+    launch_spread<float>(p, a, w_f32, st);
+  return launched("expert spread");
+}
+
+int fst_expert_gather(int dtype, int weight_dtype, int64_t tokens, int K, int N, int64_t rows, const void* x,
+                      int64_t x_stride, const int32_t* place, const void* weights, void* out, void* stream) {
+  clear_error();
+  RowPlan p;
+  const int rc = check_move(dtype, weight_dtype, tokens, K, N, rows, p);
+  if (rc != FST_OK) return rc;
+  if (tokens == 0) return FST_OK;
+  if (!out || !place || (rows > 0 && !x)) return fail(FST_EINVAL, "null tensor pointer");
+  if (x_stride < N) return fail(FST_EINVAL, "row stride below N=%d", N);
+  const size_t es = elem_size(dtype);
+  const MoveArgs a{x, nullptr, weights, place, nullptr, out, nullptr, (long)tokens, (long)rows, (long)x_stride, 0, K, N};
+  p.edge = N * es % 16 != 0 || !aligned16(x, x_stride, es) || reinterpret_cast<uintptr_t>(out) % 16 != 0;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const int w_f32 = weight_dtype == FST_F32;
+  if (dtype == FST_BF16)
+    launch_gather<bf16>(p, a, w_f32, st);
+  else if (dtype == FST_F16)
+    launch_gather<f16>(p, a, w_f32, st);
+  else
+    launch_gather<float>(p, a, w_f32, st);
+  return launched("expert gather");
+}
+
+}  // extern "C"

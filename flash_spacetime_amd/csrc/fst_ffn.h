@@ -31,6 +31,12 @@ struct FfnProduct {
   long ldx, lddy, ldo, ldw;  // elements
   int tokens;              // tokens, or the most there can be
   int F, K, act;
+  // Mixtures of experts: rows of expert e from offsets[e] to offsets[e + 1], its
+  // weights w_next elements behind the expert's before it.
+  const int32_t* offsets;
+  int experts;
+  bool tail;               // write zeros into the rows past the last expert's
+  long w_next;
 };
 
 // C[n, m] = sum_token b[token, n] a[token, m], and sum_token b[token, n]: the
@@ -43,6 +49,11 @@ struct FfnOuter {
   int M, N, splits;
   float* part;     // [splits][N][M]
   float* bias;     // [splits][N], or null
+  // Mixtures of experts: part is [experts][splits][N][M]; without it the one split's
+  // rows n < half of each expert go to direct[0], the others to direct[1] (null: not
+  // asked for).
+  void* direct[2];
+  int half;
 };
 
 // The block's two: (x, [da | du]) and (h, dy), in one launch. Either may have no
@@ -53,6 +64,8 @@ struct FfnOuters {
   const int32_t* rows;   // rows of x and dy of the tokens, or null
   int tokens;
   int first;             // workgroups of the first
+  const int32_t* offsets;  // mixtures of experts: rows of each, [experts + 1]
+  int experts;
 };
 
 typedef int (*ffn_product_fn)(int mode, const FfnProduct&, hipStream_t);
@@ -66,6 +79,10 @@ typedef int (*ffn_tile_fn)(int mode, const FfnProduct&);
 FST_FFN_DECL(bf16)
 FST_FFN_DECL(f16)
 FST_FFN_DECL(f32)
+// The same with the tokens in runs, each with an expert's weights of its own.
+FST_FFN_DECL(experts_bf16)
+FST_FFN_DECL(experts_f16)
+FST_FFN_DECL(experts_f32)
 #undef FST_FFN_DECL
 
 }  // namespace fst

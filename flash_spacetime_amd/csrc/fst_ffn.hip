@@ -14,7 +14,8 @@
 // the distance from 64 bits (bf16 0.0031 of their norm against 0.0024), and at D =
 // 384 writing and reading them took as long as the products do.
 // Padded batches are gathered on the way: a list of the valid rows is the
-// products' token axis, so padding costs nothing but its zeros.
+// products' token axis, so padding costs nothing but its zeros. Mixtures of experts
+// run the same products over rows that lie in runs, one for each expert.
 #include "fst_ffn.h"
 
 namespace fst {
@@ -56,7 +57,8 @@ __global__ __launch_bounds__(256) void ffn_rows(const int32_t* seqlens, int B, i
 
 // out[c * ldo + r] = in[r * C + c] for up to three matrices [R, C]; the workgroups
 // after theirs write zeros into the padding rows of `pad` (seqlens given), `slices`
-// of them for an event and every `groups`-th after it.
+// of them for an event and every `groups`-th after it. Mixtures of experts: row y of
+// the grid takes expert y's matrices, next_in and next_out elements behind the first's.
 struct Transposes {
   const void* in[3];
   void* out[3];
@@ -66,6 +68,7 @@ struct Transposes {
   unsigned char* pad;
   long row_bytes;
   int B, L, groups, slices;
+  long next_in, next_out[3];
 };
 
 // A workgroup turns a 64 x 64 tile through LDS, 16 bytes at a time in memory (by
@@ -87,8 +90,8 @@ __global__ __launch_bounds__(256) void ffn_transpose(Transposes p) {
   const int wg = (int)blockIdx.x - (k ? p.first[k - 1] : 0);
   const int R = p.R[k], C = p.C[k], nc = (C + 63) / 64;
   const int r0 = wg / nc * 64, c0 = wg % nc * 64;
-  const E* in = static_cast<const E*>(p.in[k]);
-  E* out = static_cast<E*>(p.out[k]);
+  const E* in = static_cast<const E*>(p.in[k]) + blockIdx.y * p.next_in;
+  E* out = static_cast<E*>(p.out[k]) + blockIdx.y * p.next_out[k];
 #pragma unroll
   for (int i = threadIdx.x; i < 64 * PER; i += 256) {
     const int r = i / PER, c = i % PER * V;
@@ -131,6 +134,31 @@ __global__ __launch_bounds__(256) void ffn_grad_sum(GradSums p) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = (T)sum[i];
   *reinterpret_cast<T4*>(static_cast<T*>(p.out[k]) + e) = o;
+}
+
+// Gradients of the experts' weights = the sums of their partials [experts][splits][N][M]
+// over the splits, in order: dw_gate and dw_up are the rows n of each expert's first
+// partial below and from F on. Row y of the grid: expert y.
+struct ExpertSums {
+  const float* part[3];
+  void* out[3];
+  long next[3], count[3];  // elements between the splits' partials; of an expert's gradient
+  int splits, first[3];
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void expert_grad_sum(ExpertSums p) {
+  const int k = (int)blockIdx.x >= p.first[0] ? ((int)blockIdx.x >= p.first[1] ? 2 : 1) : 0;
+  const long i = ((long)((int)blockIdx.x - (k ? p.first[k - 1] : 0)) * 256 + threadIdx.x) * 4;
+  if (i >= p.count[k]) return;
+  const float* in = p.part[k] + (long)blockIdx.y * p.splits * p.next[k] + i;
+  f32x4 sum = *reinterpret_cast<const f32x4*>(in);
+  for (int s = 1; s < p.splits; ++s) sum += *reinterpret_cast<const f32x4*>(in + s * p.next[k]);
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  T4 o;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o[j] = (T)sum[j];
+  *reinterpret_cast<T4*>(static_cast<T*>(p.out[k]) + blockIdx.y * p.count[k] + i) = o;
 }
 
 int check_ffn(int dtype, int activation, int B, int L, int D, int F) {
@@ -186,16 +214,19 @@ struct OuterPlan {
   int tile, splits;
 };
 
-OuterPlan plan_outer(int dtype, long tokens, int D, int F) {
+OuterPlan plan_outer(int dtype, long tokens, int D, int F, int experts = 0) {
   OuterPlan best{128, 1};
+  if (experts) tokens = (tokens + experts - 1) / experts;
   double least = -1;
   for (const int e : {128, 256}) {
     if (e == 256 && dtype == FST_F32) continue;
-    const long tiles = (long)((D + e - 1) / e) * ((2 * F + e - 1) / e + (F + e - 1) / e), slots = e == 256 ? 256 : 512;
+    const long tiles = (long)((D + e - 1) / e) * ((2 * F + e - 1) / e + (F + e - 1) / e) * (experts ? experts : 1), slots = e == 256 ? 256 : 512;
     const double rate = (dtype == FST_F32 ? 0.12e15 : e == 256 ? 1.1e15 : 0.8e15) / slots;
     for (int s = 1; s <= 64 && (s == 1 || s * 256l <= tokens); ++s) {
       const double work = (double)tokens / s * 2 * e * e / rate;
-      const double t = (double)((tiles * s + slots - 1) / slots) * work + s * 24.0 * D * F / 5e12;
+      // An expert's gradient of one run is written as it is.
+      const double sums = experts ? (s > 1 ? (double)s * experts : 0) : s;
+      const double t = (double)((tiles * s + slots - 1) / slots) * work + sums * 24.0 * D * F / 5e12;
       if (least < 0 || t < least) best = OuterPlan{e, s}, least = t;
     }
   }
@@ -224,6 +255,59 @@ GradLayout grad_layout(int dtype, long rows, int D, int F) {
   l.part1 = take(l.outer.splits * df * 4);
   l.bias0 = take((size_t)l.outer.splits * 2 * F * 4);
   l.bias1 = take((size_t)l.outer.splits * D * 4);
+  l.total = off;
+  return l;
+}
+
+// --- mixtures of experts ------------------------------------------------------
+
+constexpr int kMostExperts = 512;
+
+ffn_product_fn experts_product_of(int dtype) {
+  return dtype == FST_BF16 ? ffn_product_experts_bf16 : dtype == FST_F16 ? ffn_product_experts_f16 : ffn_product_experts_f32;
+}
+ffn_outer_fn experts_outer_of(int dtype) {
+  return dtype == FST_BF16 ? ffn_outer_experts_bf16 : dtype == FST_F16 ? ffn_outer_experts_f16 : ffn_outer_experts_f32;
+}
+
+int check_experts(int dtype, int activation, int rows, int E, int D, int F) {
+  const int rc = check_ffn(dtype, activation, 1, rows, D, F);
+  if (rc != FST_OK) return rc;
+  if (E < 1) return fail(FST_EINVAL, "need at least one expert, got %d", E);
+  if (E > kMostExperts) return fail(FST_EUNSUPPORTED, "at most %d experts, got %d", kMostExperts, E);
+  return FST_OK;
+}
+
+FfnProduct experts_product(const int32_t* offsets, int E, int rows, int activation) {
+  FfnProduct p{};
+  p.offsets = offsets;
+  p.experts = E;
+  p.tokens = rows;
+  p.act = activation;
+  return p;
+}
+
+struct ExpertLayout {
+  size_t wdt, w2t, dadu, part0, part1, total;
+  OuterPlan outer;
+};
+
+ExpertLayout expert_layout(int dtype, int rows, int E, int D, int F) {
+  ExpertLayout l;
+  const size_t es = elem_size(dtype), all = (size_t)E * D * F;
+  l.outer = plan_outer(dtype, rows, D, F, E);
+  const size_t parts = l.outer.splits > 1 ? l.outer.splits * all * 4 : 0;
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = off;
+    off += align256(bytes);
+    return at;
+  };
+  l.wdt = take(all * es);
+  l.w2t = take(2 * all * es);
+  l.dadu = take((size_t)rows * 2 * F * es);
+  l.part0 = take(2 * parts);
+  l.part1 = take(parts);
   l.total = off;
   return l;
 }
@@ -448,6 +532,188 @@ int fst_ffn_backward(int dtype, int activation, int B, int L, int D, int F, cons
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(FST_ELAUNCH, "feed-forward backward launch failed (%s)", hipGetErrorString(e));
+  return FST_OK;
+}
+
+int fst_expert_ffn_forward(int dtype, int activation, int rows, int E, int D, int F, const void* x, int64_t x_stride,
+                           const int32_t* offsets, const void* w_gate, const void* w_up, const void* w_down,
+                           void* hidden, void* gate, void* up, void* y, void* stream) {
+  clear_error();
+  int rc = check_experts(dtype, activation, rows, E, D, F);
+  if (rc != FST_OK) return rc;
+  if (rows == 0) return FST_OK;
+  if (!x || !offsets || !w_gate || !w_up || !w_down || !hidden || !y || !gate != !up)
+    return fail(FST_EINVAL, "null tensor pointer");
+  if (gate && ffn_redo(dtype)) return fail(FST_EINVAL, "gate and up are kept in float32 only");
+  if (bad_stride(x_stride, D, elem_size(dtype)))
+    return fail(FST_EINVAL, "x's row stride must be at least D, whole 16 bytes and below 2^32");
+  if (misaligned({x, w_gate, w_up, w_down, hidden, gate, up, y}))
+    return fail(FST_EINVAL, "pointers must be multiples of 16 bytes");
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  FfnProduct p = experts_product(offsets, E, rows, activation);
+  p.w_next = (long)D * F;
+  p.w[0] = w_gate;
+  p.w[1] = w_up;
+  p.x = x;
+  p.ldx = x_stride;
+  p.out[0] = hidden;
+  p.out[1] = gate;
+  p.out[2] = up;
+  p.ldo = F;
+  p.ldw = p.K = D;
+  p.F = F;
+  rc = experts_product_of(dtype)(kFfnGate, p, st);
+  if (rc == FST_OK) {
+    p.w[0] = w_down;
+    p.x = hidden;
+    p.out[0] = y;
+    p.ldo = D;
+    p.ldx = p.ldw = p.K = F;
+    p.F = D;
+    p.tail = true;
+    rc = experts_product_of(dtype)(kFfnOut, p, st);
+  }
+  if (rc != FST_OK) return fail(rc, "experts' feed-forward launch failed");
+  return FST_OK;
+}
+
+int fst_expert_ffn_tiles(int dtype, int rows, int E, int D, int F, int32_t* tiles) {
+  clear_error();
+  const int rc = check_experts(dtype, FST_SILU, rows, E, D, F);
+  if (rc != FST_OK) return rc;
+  if (!tiles) return fail(FST_EINVAL, "null pointer");
+  const ffn_tile_fn tile_of =
+      dtype == FST_BF16 ? ffn_tile_experts_bf16 : dtype == FST_F16 ? ffn_tile_experts_f16 : ffn_tile_experts_f32;
+  FfnProduct p = experts_product(nullptr, E, rows, FST_SILU);
+  p.F = F;
+  tiles[0] = tile_of(kFfnGate, p);
+  tiles[2] = tile_of(ffn_redo(dtype) ? kFfnRedo : kFfnGrad, p);
+  p.F = D;
+  tiles[1] = tiles[3] = tile_of(kFfnOut, p);
+  const OuterPlan outer = plan_outer(dtype, rows, D, F, E);
+  tiles[4] = outer.tile;
+  tiles[5] = outer.splits;
+  return FST_OK;
+}
+
+size_t fst_expert_ffn_backward_workspace_bytes(int dtype, int rows, int E, int D, int F) {
+  if (check_experts(dtype, FST_SILU, rows, E, D, F) != FST_OK) return 0;
+  return expert_layout(dtype, rows, E, D, F).total;
+}
+
+int fst_expert_ffn_backward(int dtype, int activation, int rows, int E, int D, int F, const void* x, int64_t x_stride,
+                            const int32_t* offsets, const void* w_gate, const void* w_up, const void* w_down,
+                            const void* hidden, const void* gate, const void* up, const void* dy, int64_t dy_stride,
+                            void* dx, void* dw_gate, void* dw_up, void* dw_down, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  clear_error();
+  int rc = check_experts(dtype, activation, rows, E, D, F);
+  if (rc != FST_OK) return rc;
+  const bool first = dw_gate || dw_up;
+  if (!first && !dw_down && !dx) return FST_OK;
+  const size_t es = elem_size(dtype);
+  if (!offsets) return fail(FST_EINVAL, "null tensor pointer");
+  if (rows > 0) {
+    if (!x || !w_gate || !w_up || !w_down || !hidden || !dy || (!ffn_redo(dtype) && !(gate && up)))
+      return fail(FST_EINVAL, "null tensor pointer");
+    if (bad_stride(x_stride, D, es) || bad_stride(dy_stride, D, es))
+      return fail(FST_EINVAL, "row strides of x and dy must be at least D, whole 16 bytes and below 2^32");
+  }
+  if (misaligned({x, w_gate, w_up, w_down, hidden, gate, up, dy, dx, dw_gate, dw_up, dw_down, workspace}))
+    return fail(FST_EINVAL, "pointers must be multiples of 16 bytes");
+  const ExpertLayout l = expert_layout(dtype, rows, E, D, F);
+  if (!workspace || workspace_bytes < l.total)
+    return fail(FST_EWORKSPACE, "workspace of %zu bytes is smaller than the %zu required", workspace_bytes, l.total);
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const long df = (long)D * F;
+
+  if (rows > 0 && (first || dx)) {
+    Transposes t{};
+    int grid = 0;
+    auto add = [&](int k, const void* in, size_t out, int R, int C, long ldo, long next) {
+      t.in[k] = in;
+      t.out[k] = ws + out;
+      t.R[k] = R;
+      t.C[k] = C;
+      t.ldo[k] = ldo;
+      t.next_out[k] = next;
+      if (in) grid += ((R + 63) / 64) * ((C + 63) / 64);
+      t.first[k] = grid;
+    };
+    t.next_in = df;
+    add(0, w_down, l.wdt, D, F, D, df);
+    add(1, dx ? w_gate : nullptr, l.w2t, F, D, 2l * F, 2 * df);
+    add(2, dx ? w_up : nullptr, l.w2t + F * es, F, D, 2l * F, 2 * df);
+    if (es == 2)
+      ffn_transpose<uint16_t><<<dim3(grid, E), 256, 0, st>>>(t);
+    else
+      ffn_transpose<uint32_t><<<dim3(grid, E), 256, 0, st>>>(t);
+    FfnProduct p = experts_product(offsets, E, rows, activation);
+    p.w_next = df;
+    if (ffn_redo(dtype)) {
+      p.w[0] = w_gate;
+      p.w[1] = w_up;
+      p.w[2] = ws + l.wdt;
+      p.x = x;
+      p.ldx = x_stride;
+      p.dy = dy;
+      p.lddy = dy_stride;
+    } else {
+      p.w[0] = ws + l.wdt;
+      p.x = dy;
+      p.ldx = dy_stride;
+      p.gate = gate;
+      p.up = up;
+    }
+    p.out[0] = ws + l.dadu;
+    p.ldo = 2l * F;
+    p.ldw = p.K = D;
+    p.F = F;
+    rc = experts_product_of(dtype)(ffn_redo(dtype) ? kFfnRedo : kFfnGrad, p, st);
+    if (rc == FST_OK && dx) {
+      p.w_next = 2 * df;
+      p.w[0] = ws + l.w2t;
+      p.x = ws + l.dadu;
+      p.out[0] = dx;
+      p.ldo = D;
+      p.ldx = p.ldw = p.K = 2 * F;
+      p.F = D;
+      p.tail = true;
+      rc = experts_product_of(dtype)(kFfnOut, p, st);
+    }
+    if (rc != FST_OK) return fail(rc, "experts' feed-forward backward launch failed");
+  }
+  if (first || dw_down) {
+    const int splits = l.outer.splits;
+    float *p0 = reinterpret_cast<float*>(ws + l.part0), *p1 = reinterpret_cast<float*>(ws + l.part1);
+    FfnOuters o{};
+    o.offsets = offsets;
+    o.experts = E;
+    o.tokens = rows;
+    o.p[0] = FfnOuter{x, ws + l.dadu, (long)x_stride, 2l * F, D, 2 * F, first ? splits : 0, splits > 1 ? p0 : nullptr,
+                      nullptr, {dw_gate, dw_up}, F};
+    o.p[1] = FfnOuter{hidden, dy, F, (long)dy_stride, F, D, dw_down ? splits : 0, splits > 1 ? p1 : nullptr,
+                      nullptr, {dw_down, nullptr}, D};
+    rc = experts_outer_of(dtype)(o, l.outer.tile, st);
+    if (rc != FST_OK) return fail(rc, "experts' weight gradient launch failed");
+    if (splits > 1) {
+      ExpertSums s{{p0, p0 + df, p1}, {dw_gate, dw_up, dw_down}, {2 * df, 2 * df, df}, {df, df, df}, splits, {}};
+      int grid = 0;
+      for (int k = 0; k < 3; ++k) {
+        if (s.out[k]) grid += (int)((df + 1023) / 1024);
+        s.first[k] = grid;
+      }
+      if (dtype == FST_BF16)
+        expert_grad_sum<bf16><<<dim3(grid, E), 256, 0, st>>>(s);
+      else if (dtype == FST_F16)
+        expert_grad_sum<f16><<<dim3(grid, E), 256, 0, st>>>(s);
+      else
+        expert_grad_sum<float><<<dim3(grid, E), 256, 0, st>>>(s);
+    }
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return fail(FST_ELAUNCH, "experts' feed-forward backward launch failed (%s)", hipGetErrorString(e));
   return FST_OK;
 }
 

@@ -1,5 +1,7 @@
 // The feed-forward block's matrix products for one element type, built with
-// -DFST_T=<bf16|f16|float> -DFST_NAME=<bf16|f16|f32>.
+// -DFST_T=<bf16|f16|float> -DFST_NAME=<bf16|f16|f32>, and with -DFST_EXPERTS=1
+// for mixtures of experts (names experts_<type>): the tokens then lie in runs, one for
+// each expert, and a tile of tokens is of one run.
 //
 // Two kernels carry it:
 //  * ffn_product: tokens times a weight, contraction along the rows of both
@@ -22,6 +24,10 @@ namespace {
 typedef FST_T T;
 constexpr int ES = sizeof(T);
 constexpr bool F32 = ES == 4;
+#ifndef FST_EXPERTS
+#define FST_EXPERTS 0
+#endif
+constexpr bool EXPERTS = FST_EXPERTS;
 
 // What loads past an operand's end read: 16 zero bytes.
 __device__ const u32x4 kZero16 = {0, 0, 0, 0};
@@ -164,6 +170,71 @@ __device__ __forceinline__ bool pick_tile(int wg, int nf, int nt, int& f, int& t
   return true;
 }
 
+// Experts: the workgroup's feature tile, expert, and the rows t0 .. end - 1 of its tile
+// of BT tokens; expert = p.experts: rows past the last run, where they are asked for.
+// Workgroup wg of a grid over all tiles, or token tile `at` of a row of the grid (at >=
+// 0). Offsets are taken within the rows and in order, so that no table makes a tile reach
+// outside. Each wave adds up the runs' tiles by itself, 64 experts at a time. The rows past
+// the last run come after all tiles, so that every XCD has its share of the products.
+struct ExpertTile {
+  int ft, expert, t0, end;
+};
+
+template <int BT>
+__device__ __forceinline__ bool expert_tile(const FfnProduct& p, int wg, int nf, int at, ExpertTile& tile) {
+  const int lane = threadIdx.x & 63;
+  int start, stop, count, upto;  // of expert e0 + lane: its rows, its tiles, and those up to its last
+  const auto bound = [&](int i) { return min(max(p.offsets[i], 0), p.tokens); };
+  const auto scan = [&](int e0) __attribute__((always_inline)) {
+    const int e = e0 + lane;
+    start = e < p.experts ? bound(e) : 0;
+    stop = e < p.experts ? max(start, bound(e + 1)) : 0;
+    count = upto = (stop - start + BT - 1) / BT;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int below = __shfl_up(upto, d);
+      if (lane >= d) upto += below;
+    }
+  };
+  scan(0);
+  int total = __builtin_amdgcn_readlane(upto, 63);
+  for (int e0 = 64; e0 < p.experts; e0 += 64) {
+    scan(e0);
+    total += __builtin_amdgcn_readlane(upto, 63);
+  }
+  int tt = at, behind = at - total;  // place among the tiles past the last run
+  bool run;
+  if (at < 0) {
+    run = pick_tile(wg, nf, total, tile.ft, tt);
+    behind = wg - (nf * total + 7) / 8 * 8;
+  } else {
+    run = tt < total;
+  }
+  if (!run) {
+    if (!p.tail || behind < 0) return false;
+    const int tail = bound(p.experts);
+    tile.ft = at < 0 ? behind % nf : 0;
+    tile.expert = p.experts;
+    tile.t0 = (int)min((long)p.tokens, tail + (long)(at < 0 ? behind / nf : behind) * BT);
+    tile.end = p.tokens;
+    return tile.t0 < tile.end;
+  }
+  if (p.experts > 64) scan(0);
+  for (int e0 = 0; e0 < p.experts; e0 += 64) {
+    if (e0) scan(e0);
+    const int sum = __builtin_amdgcn_readlane(upto, 63);
+    if (tt < sum) {
+      const int src = __builtin_ctzll(__ballot(upto > tt)), from = __builtin_amdgcn_readlane(start, src);
+      tile.expert = e0 + src;
+      tile.t0 = from + (tt - __builtin_amdgcn_readlane(upto - count, src)) * BT;
+      tile.end = __builtin_amdgcn_readlane(stop, src);
+      return tile.t0 >= from && tile.t0 < tile.end;
+    }
+    tt -= sum;
+  }
+  return false;
+}
+
 // WF x WT waves of NI x NJ subtiles of 16 features by 16 tokens. The weight is
 // the matrix core's row operand, so a lane ends up with 4 GS consecutive
 // features of its tokens: slot m = 4 a + r of subtile s of a group of GS holds
@@ -222,11 +293,28 @@ __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
   constexpr int NF = C::NF, GS = C::GS, NE = 4 * GS, WAVES = C::WAVES;
   constexpr bool REDO = MODE == kFfnRedo;
   __shared__ __attribute__((aligned(1024))) unsigned char lds[ST][C::UNIT];
+  const int nf = (p.F + C::FEATURES - 1) / C::FEATURES;
+#if FST_EXPERTS
+  ExpertTile tile;
+  if (!expert_tile<C::BT>(p, blockIdx.x, nf, -1, tile)) return;
+  const int f0 = tile.ft * C::FEATURES, t0 = tile.t0, tokens = tile.end;
+  if (MODE == kFfnOut && tile.expert == p.experts) {  // rows of no expert
+    constexpr int PARTS = C::FEATURES * ES / 16;
+    for (int i = threadIdx.x; i < PARTS * C::BT; i += 64 * WAVES) {
+      const int t = t0 + i / PARTS, f = f0 + i % PARTS * kVec<T>;
+      if (t < tokens && f < p.F) *reinterpret_cast<u32x4*>(static_cast<T*>(p.out[0]) + (long)t * p.ldo + f) = u32x4{0, 0, 0, 0};
+    }
+    return;
+  }
+  const long w_at = (long)tile.expert * p.w_next * ES;
+#else
   const int tokens = p.count ? *p.count : p.tokens;
-  const int nf = (p.F + C::FEATURES - 1) / C::FEATURES, nt = (tokens + C::BT - 1) / C::BT;
+  const int nt = (tokens + C::BT - 1) / C::BT;
   int ft, tt;
   if (!pick_tile(blockIdx.x, nf, nt, ft, tt)) return;
   const int f0 = ft * C::FEATURES, t0 = tt * C::BT;
+  constexpr long w_at = 0;
+#endif
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wf = wave % WF, wt = wave / WF, g = lane >> 4, n = lane & 15;
 
@@ -249,7 +337,7 @@ __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
   // subtracts it from the buffer's size).
   const int range = (p.F - f0) * row_bytes;
   auto weight = [&](int k) {
-    const uint64_t at = (uint64_t)p.w[k] + (uint64_t)f0 * row_bytes;  // a 48-bit address, stride 0
+    const uint64_t at = (uint64_t)p.w[k] + w_at + (uint64_t)f0 * row_bytes;  // a 48-bit address, stride 0
     return u32x4{(unsigned)at, (unsigned)(at >> 32) & 0xffffu, (unsigned)range, 0x00020000u};
   };
   const u32x4 wr0 = weight(0), wr1 = weight(C::MATS - 1), wr2 = weight(REDO ? 2 : 0);
@@ -447,8 +535,24 @@ __global__ __launch_bounds__(512, MODE == kFfnRedo && NJ == 4 ? 2 : 4) void ffn_
   constexpr bool REDO = MODE == kFfnRedo;
   constexpr int MATS = MODE == kFfnGate || REDO ? 2 : 1, ACCS = REDO ? 3 : MATS, KE = 64 / ES, AHEAD = NJ == 1 ? 4 : 2;
   __shared__ f32x4 lds[8][ACCS * NJ][64];
+#if FST_EXPERTS
+  ExpertTile tile;
+  if (!expert_tile<16 * NJ>(p, 0, 0, blockIdx.y, tile)) return;
+  const int t0 = tile.t0, tokens = tile.end;
+  if (MODE == kFfnOut && tile.expert == p.experts) {  // rows of no expert
+    constexpr int PARTS = 16 * ES / 16;
+    const int t = t0 + threadIdx.x / PARTS, f = blockIdx.x * 16 + threadIdx.x % PARTS * kVec<T>;
+    if ((int)threadIdx.x < PARTS * 16 * NJ && t < tokens && f < p.F)
+      *reinterpret_cast<u32x4*>(static_cast<T*>(p.out[0]) + (long)t * p.ldo + f) = u32x4{0, 0, 0, 0};
+    return;
+  }
+  const long w_at = (long)tile.expert * p.w_next * ES;
+#else
   const int tokens = p.count ? *p.count : p.tokens;
   if (tokens <= 0) return;
+  constexpr int t0 = 0;
+  constexpr long w_at = 0;
+#endif
   const int f0 = blockIdx.x * 16, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, n = lane & 15;
   const int row_bytes = (int)p.ldw * ES;
@@ -466,10 +570,10 @@ __global__ __launch_bounds__(512, MODE == kFfnRedo && NJ == 4 ? 2 : 4) void ffn_
     const char *wp[MM], *xp[NJ];
 #pragma unroll
     for (int a = 0; a < MM; ++a)
-      wp[a] = static_cast<const char*>(p.w[w0 + a]) + (long)min(f0 + n, p.F - 1) * row_bytes + g * 16;
+      wp[a] = static_cast<const char*>(p.w[w0 + a]) + w_at + (long)min(f0 + n, p.F - 1) * row_bytes + g * 16;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      const int t = min(16 * j + n, tokens - 1);  // past the last token: not stored
+      const int t = min(t0 + 16 * j + n, tokens - 1);  // past the last token: not stored
       const long r = p.rows_in ? p.rows_in[t] : t;
       xp[j] = static_cast<const char*>(x) + r * ldx * ES + g * 16;
     }
@@ -502,7 +606,7 @@ __global__ __launch_bounds__(512, MODE == kFfnRedo && NJ == 4 ? 2 : 4) void ffn_
   __syncthreads();
   if (wave >= NJ) return;
   // Wave j: features 4 g .. 4 g + 3 of token n of subtile j.
-  const int f = f0 + 4 * g, t = 16 * wave + n;
+  const int f = f0 + 4 * g, t = t0 + 16 * wave + n;
   if (f >= p.F || t >= tokens) return;
   float v[ACCS][4];
 #pragma unroll
@@ -639,14 +743,22 @@ __device__ __forceinline__ void outer_tile(const FfnOuter& p, const FfnOuters& a
   constexpr int A_BYTES = KT * SideA::ROW, STAGE = A_BYTES + KT * SideB::ROW;
   const int nm = (p.M + TM - 1) / TM, nn = (p.N + TN - 1) / TN;
   // Consecutive workgroups of an XCD take the tiles of one run of tokens.
-  const int total = nm * nn * p.splits, per = (total + 7) >> 3;
+  const int total = nm * nn * p.splits * (EXPERTS ? all.experts : 1), per = (total + 7) >> 3;
   const int i8 = wg >> 3, at = (wg & 7) * per + i8;
   if (i8 >= per || at >= total) return;
-  const int split = at / (nm * nn), tile = at - split * nm * nn;
+  const int split = at / (nm * nn), tile = at - split * nm * nn;  // experts: a split of an expert's run
   const int m0 = tile % nm * TM, n0 = tile / nm * TN;
+#if FST_EXPERTS
+  const int expert = split / p.splits, piece = split - expert * p.splits;
+  const int first = min(max(all.offsets[expert], 0), all.tokens);
+  const int end = max(min(all.offsets[expert + 1], all.tokens), first);
+  const int run = ((end - first + p.splits - 1) / p.splits + KT - 1) / KT * KT;
+  const int t0 = (int)min(first + (long)piece * run, (long)end), t1 = (int)min((long)t0 + run, (long)end);
+#else
   const int tokens = all.count ? *all.count : all.tokens;
   const int run = ((tokens + p.splits - 1) / p.splits + KT - 1) / KT * KT;
   const int t0 = (int)min((long)split * run, (long)tokens), t1 = (int)min((long)t0 + run, (long)tokens);
+#endif
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave % WM, wn = wave / WM, g = lane >> 4, n = lane & 15;
@@ -735,6 +847,22 @@ __device__ __forceinline__ void outer_tile(const FfnOuter& p, const FfnOuters& a
   for (int j = 0; j < NJ; ++j) {
     const int nr = n0 + (wn * NJ + j) * 16 + n;
     if (nr >= p.N) continue;
+    if (EXPERTS && !p.part) {
+      const bool low = nr < p.half;
+      T* out = static_cast<T*>(p.direct[low ? 0 : 1]);
+      if (!out) continue;
+      out += ((long)split * (low ? p.half : p.N - p.half) + (low ? nr : nr - p.half)) * p.M;
+      typedef T T4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int m = m0 + (wm * NI + i) * 16 + 4 * g;
+        T4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = (T)acc[i][j][e];
+        if (m < p.M) *reinterpret_cast<T4*>(out + m) = o;
+      }
+      continue;
+    }
     float* out = p.part + ((long)split * p.N + nr) * p.M;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
@@ -760,22 +888,33 @@ __global__ __launch_bounds__(128 * WF, OCC) void ffn_outer(FfnOuters ps) {
     outer_tile<2, WF, NF / 2, ND / WF, false, PADDED>(ps.p[1], ps, wg - ps.first, lds, list);
 }
 
+// Tiles of t tokens, at most: each run may end in a tile of its own.
+long token_tiles(const FfnProduct& p, int t) {
+  if (EXPERTS) return p.tokens / t + std::min(p.tokens, p.experts) + (p.tail ? 1 : 0);
+  return (p.tokens + t - 1) / t;
+}
+
 template <int MODE, int WF, int WT, int NI, int NJ, int ST, int OCC>
 void launch(const FfnProduct& p, hipStream_t st) {
   typedef Product<MODE, WF, WT, NI, NJ, ST> C;
-  const long tiles = (long)((p.F + C::FEATURES - 1) / C::FEATURES) * ((p.tokens + C::BT - 1) / C::BT);
-  ffn_product<MODE, WF, WT, NI, NJ, ST, OCC><<<(unsigned)((tiles + 7) / 8 * 8), 64 * WF * WT, 0, st>>>(p);
+  const long tiles = (long)((p.F + C::FEATURES - 1) / C::FEATURES) * token_tiles(p, C::BT);
+  // Experts: the tiles past the last run begin at a multiple of eight.
+  ffn_product<MODE, WF, WT, NI, NJ, ST, OCC><<<(unsigned)((tiles + 7) / 8 * 8 + (EXPERTS ? 8 : 0)), 64 * WF * WT, 0, st>>>(p);
 }
 
 constexpr int kFewTokens = 64;
 
+// Tokens that share weights: all, or an expert's if the loads are even.
+int tokens_of_run(const FfnProduct& p) { return EXPERTS ? (p.tokens + p.experts - 1) / p.experts : p.tokens; }
+
 template <int MODE>
 void launch_few(const FfnProduct& p, hipStream_t st) {
-  const long nf = (p.F + 15) / 16;
-  if (p.tokens <= 16)
-    ffn_few<MODE, 1><<<(unsigned)nf, 512, 0, st>>>(p);
+  const unsigned nf = (unsigned)((p.F + 15) / 16);
+  const auto grid = [&](int t) { return EXPERTS ? dim3(nf, (unsigned)token_tiles(p, t)) : dim3(nf); };
+  if (tokens_of_run(p) <= 16)
+    ffn_few<MODE, 1><<<grid(16), 512, 0, st>>>(p);
   else
-    ffn_few<MODE, 4><<<(unsigned)nf, 512, 0, st>>>(p);
+    ffn_few<MODE, 4><<<grid(64), 512, 0, st>>>(p);
 }
 
 // The tiles of a product: 256 x 256 features (of all weights) by tokens, one
@@ -796,7 +935,8 @@ enum Tile { kLarge, kMiddle, kSmall, kFew };
 Tile pick(const FfnProduct& p, int mats, bool redo) {
   if (p.tokens <= kFewTokens) return kFew;
   const auto load = [&](int f, int t) {
-    const long tiles = (long)((p.F + f - 1) / f) * ((p.tokens + t - 1) / t);
+    const int run = tokens_of_run(p);
+    const long tiles = (long)((p.F + f - 1) / f) * ((run + t - 1) / t) * (EXPERTS ? (p.tokens + run - 1) / run : 1);
     return (double)((tiles + 255) / 256);
   };
   const double nl = load(256 / mats, redo ? 192 : 256), nm = load(128 / mats, redo ? 64 : 128), ns = load(64 / mats, 64);
@@ -809,15 +949,18 @@ Tile pick(const FfnProduct& p, int mats, bool redo) {
 
 template <int DT, int FT, int WF, int OCC>
 void launch_outer(FfnOuters& ps, hipStream_t st) {
-  const auto tiles = [](const FfnOuter& p, int m, int n) {
-    return (p.splits * ((p.M + m - 1) / m) * ((p.N + n - 1) / n) + 7) / 8 * 8;
+  const auto tiles = [&](const FfnOuter& p, int m, int n) {
+    return (p.splits * (EXPERTS ? ps.experts : 1) * ((p.M + m - 1) / m) * ((p.N + n - 1) / n) + 7) / 8 * 8;
   };
   ps.first = tiles(ps.p[0], DT, FT);
   const int grid = ps.first + tiles(ps.p[1], FT, DT);
-  if (ps.rows)
-    ffn_outer<DT, FT, WF, true, OCC><<<grid, 128 * WF, 0, st>>>(ps);
-  else
-    ffn_outer<DT, FT, WF, false, OCC><<<grid, 128 * WF, 0, st>>>(ps);
+  if constexpr (!EXPERTS) {
+    if (ps.rows) {
+      ffn_outer<DT, FT, WF, true, OCC><<<grid, 128 * WF, 0, st>>>(ps);
+      return;
+    }
+  }
+  ffn_outer<DT, FT, WF, false, OCC><<<grid, 128 * WF, 0, st>>>(ps);
 }
 
 }  // namespace

@@ -43,7 +43,7 @@ struct Library {
 // The entry points after last_error may be left out: they stay as they were.
 void bind_library(size_t supported, size_t fwd_ws, size_t fwd, size_t bwd_ws, size_t bwd, size_t last_error,
                   size_t norm_fwd, size_t norm_ws, size_t norm_bwd, size_t ffn_fwd, size_t ffn_ws, size_t ffn_bwd,
-                  size_t zero_tail) {
+                  size_t zero_tail, const py::args& more) {
   if (zero_tail) lib.zero_tail = reinterpret_cast<decltype(lib.zero_tail)>(zero_tail);
   if (norm_fwd) bind_block_library(norm_fwd, norm_ws, norm_bwd, ffn_fwd, ffn_ws, ffn_bwd, last_error);
   lib.supported = reinterpret_cast<decltype(lib.supported)>(supported);
@@ -52,6 +52,7 @@ void bind_library(size_t supported, size_t fwd_ws, size_t fwd, size_t bwd_ws, si
   lib.backward_workspace_bytes = reinterpret_cast<decltype(lib.backward_workspace_bytes)>(bwd_ws);
   lib.backward = reinterpret_cast<decltype(lib.backward)>(bwd);
   lib.last_error = reinterpret_cast<decltype(lib.last_error)>(last_error);
+  bind_experts_library(more);
 }
 
 // Whether the library refused the call (a status it returns before any

@@ -11,13 +11,11 @@
 // 105, 3.7; 60001 rows of 512 f32 40 and 64 us, 6.2 and 5.8 TB/s, some of it from the
 // last level cache) or, in calls of few rows, the launch. Statistics, sums and
 // gradients are float32; each output is rounded once.
-#include "fst_block.h"
+#include "fst_rows.h"
 
 namespace fst {
 
 namespace {
-
-constexpr int kNormMax = 16384;  // features of a row
 
 struct NormArgs {
   const void *x, *r, *w, *b;  // r, w, b may be null
@@ -40,140 +38,6 @@ struct NormGradArgs {
   long lds_, lddy, ldds;
   int L, n;
 };
-
-// Sum over the LPR lanes of a row's group (16, 32, 64 lanes of a wave, or a
-// whole workgroup of LPR / 64 waves through LDS); every lane gets it. The
-// order of the additions is fixed.
-__device__ __forceinline__ float row16_sum(float x) {
-#define FST_ROR(x, n) __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + n, 0xf, 0xf, false))
-  x += FST_ROR(x, 8);
-  x += FST_ROR(x, 4);
-  x += FST_ROR(x, 2);
-  x += FST_ROR(x, 1);
-#undef FST_ROR
-  return x;
-}
-
-template <int LPR>
-__device__ __forceinline__ float group_sum(float x, float* red) {
-  x = row16_sum(x);
-  if constexpr (LPR >= 32) {
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  }
-  if constexpr (LPR >= 64) {
-    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-  }
-  if constexpr (LPR > 64) {
-    constexpr int W = LPR / 64;
-    __syncthreads();  // the sums before are read
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
-    __syncthreads();
-    x = red[0];
-#pragma unroll
-    for (int i = 1; i < W; ++i) x += red[i];
-  }
-  return x;
-}
-
-// Lane l's pieces of a row: elements (l + LPR i) V .. + V - 1, i < NC, zeros past
-// its end. EDGE: the row's length is no whole number of pieces or rows start
-// off 16 bytes; pieces are then read at element alignment, the one that the row
-// ends in as the row's last V elements. Those are moved to their places, and what is
-// past the end cleared, when the piece is used: a load under a lane's own condition
-// would have to land before the next is issued (16 x 500 rows of 1367 f16, backward
-// 22.9 us so, 20.0 as it is).
-template <typename T, int LPR, int NC, bool EDGE>
-struct Pieces {
-  static constexpr int V = kVec<T>, E = NC * V;
-  static constexpr bool SHORT = EDGE && NC == 1 && LPR == 16;  // rows may have fewer than V elements
-  typename Piece<T>::V p[NC];
-
-  static __device__ __forceinline__ int at(int l, int i) { return (l + LPR * i) * V; }
-  __device__ __forceinline__ void load(const T* row, int l, int n) {
-    if (SHORT && n < V) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) p[0][j] = l == 0 && j < n ? row[j] : (T)0.f;
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int c = at(l, i);
-      if constexpr (EDGE) {
-        p[i] = *reinterpret_cast<const typename Piece<T>::VU*>(row + min(c, n - V));
-      } else if (c < n) {
-        p[i] = *reinterpret_cast<const typename Piece<T>::V*>(row + c);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) p[i][j] = (T)0.f;
-      }
-    }
-  }
-  __device__ __forceinline__ void get(float* v, int l, int n) const {
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      typename Piece<T>::V q = p[i];
-      if (EDGE && at(LPR, i) > n && !(SHORT && n < V)) {
-        const int c = at(l, i);
-        const unsigned __int128 x = __builtin_bit_cast(unsigned __int128, q);
-        const int past = (V - n % V) % V;  // elements of the last piece past the row's end
-        q = __builtin_bit_cast(typename Piece<T>::V, c >= n ? 0 : c + V > n ? x >> (8 * (int)sizeof(T) * past) : x);
-      }
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[i * V + j] = (float)q[j];
-    }
-  }
-  static __device__ __forceinline__ void store(T* row, int l, int n, const float* v) {
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int c = at(l, i);
-      const typename Piece<T>::V q = pack_piece<T>(v + i * V);
-      if (EDGE ? c + V <= n : c < n) {
-        if constexpr (EDGE)
-          *reinterpret_cast<typename Piece<T>::VU*>(row + c) = q;
-        else
-          *reinterpret_cast<typename Piece<T>::V*>(row + c) = q;
-      } else if (EDGE && c < n) {
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (j < n % V) row[c + j] = q[j];
-      }
-    }
-  }
-};
-
-// Parameters may be float32 or of the rows' type; null stands for `fill`.
-// Elements past the row's end are 0. Whole pieces come in 16-byte loads (by
-// elements, a workgroup's first microseconds were these loads: one event of 187
-// rows of 384 took 8.0 us).
-template <typename T>
-__device__ __forceinline__ void load_param(const void* p, bool f32, int c, int n, float fill, float* v) {
-  constexpr int V = kVec<T>;
-  typedef f32x4 f32x4u __attribute__((aligned(4)));
-  if (!p || c + V > n) {
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      v[i] = c + i >= n ? 0.f : !p ? fill : f32 ? static_cast<const float*>(p)[c + i] : (float)static_cast<const T*>(p)[c + i];
-  } else if (f32) {
-#pragma unroll
-    for (int i = 0; i < V; i += 4) {
-      const f32x4 q = *reinterpret_cast<const f32x4u*>(static_cast<const float*>(p) + c + i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[i + j] = q[j];
-    }
-  } else {
-    const typename Piece<T>::V q = *reinterpret_cast<const typename Piece<T>::VU*>(static_cast<const T*>(p) + c);
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = (float)q[i];
-  }
-}
-
-__device__ __forceinline__ bool row_valid(const int32_t* lens, long row, int L) {
-  if (!lens) return true;
-  const unsigned b = (unsigned)row / (unsigned)L;  // rows < 2^31
-  return (int)((unsigned)row - b * (unsigned)L) < event_len(lens, (int)b, L);
-}
 
 // Both kernels walk the rows a group at a time, with the next row's pieces in
 // flight while a row is worked on, and the length that says whether the row after
@@ -352,78 +216,6 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void norm_bwd(NormGradArgs a
   }
 }
 
-// dw | db = the column sums of part [blocks][2 n], in a fixed order: 32 columns a
-// workgroup, 32 threads a column, eight loads of each in flight.
-template <typename T>
-__global__ __launch_bounds__(1024) void norm_grad_sum(const float* part, int blocks, int n, void* dw, void* db,
-                                                      int w_f32) {
-  __shared__ float red[32][33];
-  const int c = threadIdx.x & 31, k = threadIdx.x >> 5;
-  const int col = blockIdx.x * 32 + c;
-  float sum = 0.f;
-  if (col < 2 * n) {
-    const float* in = part + col;
-    int i = k;
-    for (; i + 224 < blocks; i += 256) {
-      float v[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = in[(long)(i + 32 * j) * 2 * n];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sum += v[j];
-    }
-    for (; i < blocks; i += 32) sum += in[(long)i * 2 * n];
-  }
-  red[k][c] = sum;
-  __syncthreads();
-  if (k == 0 && col < 2 * n) {
-#pragma unroll
-    for (int i = 1; i < 32; ++i) sum += red[i][c];
-    void* out = col < n ? dw : db;
-    const int at = col < n ? col : col - n;
-    if (out) {
-      if (w_f32)
-        static_cast<float*>(out)[at] = sum;
-      else
-        static_cast<T*>(out)[at] = (T)sum;
-    }
-  }
-}
-
-// The lanes a row takes: the fewest whose share is at most three 16-byte
-// pieces a lane (four in float32: half as many elements), of which the backward
-// holds s, dy, w, dw, db and the next row's three without spilling (but for
-// float32 rows of more than 8192). Fewer lanes leave fewer idle: 256 x 768 rows
-// of 384 bf16, padded, by 16 / 32 / 64 lanes: forward 96 / 99 / 106 us, backward
-// 97 / 123 / 182.
-struct NormPlan {
-  int lpr, nc;
-  bool edge;
-};
-
-template <typename T>
-constexpr int kMostPieces = sizeof(T) == 4 ? 4 : 3;
-
-// Whether plan_norm gives some row L lanes of C pieces.
-template <typename T>
-constexpr bool planned(int L, int C) {
-  const int fewer = L == 16 ? 0 : L == 32 ? 16 : L == 64 ? 32 : L == 256 ? 64 : 256;
-  return C <= kMostPieces<T> && L * C > kMostPieces<T> * fewer && L * (C - 1) * kVec<T> < kNormMax;
-}
-
-bool plan_norm(int dtype, int n, NormPlan& p) {
-  const int v = 16 / (int)elem_size(dtype), most = dtype == FST_F32 ? kMostPieces<float> : kMostPieces<bf16>;
-  if (n > kNormMax) return false;
-  const int pieces = (n + v - 1) / v;
-  for (int lpr : {16, 32, 64, 256, 1024}) {
-    if (pieces <= most * lpr) {
-      p.lpr = lpr;
-      p.nc = (pieces + lpr - 1) / lpr;
-      return true;
-    }
-  }
-  return false;
-}
-
 // Most workgroups. The forward's are those that its registers let run at once:
 // each loads the parameters and then has a row ahead in flight, which is lost on those
 // that would start after others (8000 rows of 1367 f16 3 / 4 / 8 a CU 15.2 / 18.0 / 21.1
@@ -432,23 +224,14 @@ bool plan_norm(int dtype, int n, NormPlan& p) {
 // the partials cost).
 constexpr int kNormBlocks = 512;
 
-int norm_forward_blocks(const NormPlan& p, int dtype) {
+int norm_forward_blocks(const RowPlan& p, int dtype) {
   if (p.lpr == 1024) return 512;
   const int registers = 22 + p.nc * (dtype == FST_F32 ? 30 : 44);  // of a lane: 54 .. 154
   return 256 * (512 / registers);
 }
 
-int norm_rows_per_block(const NormPlan& p) { return p.lpr > 256 ? 1 : 256 / p.lpr; }
-
-int norm_blocks(const NormPlan& p, long rows, int most) {
-  const long need = (rows + norm_rows_per_block(p) - 1) / norm_rows_per_block(p);
-  return (int)(need < most ? need : most);
-}
-
-bool aligned16(const void* p, long ld, size_t es) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * es % 16 == 0; }
-
 template <typename T>
-void launch_fwd(const NormPlan& p, const NormArgs& a, int blocks, int w_f32, hipStream_t st) {
+void launch_fwd(const RowPlan& p, const NormArgs& a, int blocks, int w_f32, hipStream_t st) {
   const int threads = p.lpr > 256 ? p.lpr : 256;
 #define FST_CASE(L, C)                                                                   \
   if constexpr (planned<T>(L, C)) {                                                      \
@@ -470,7 +253,7 @@ void launch_fwd(const NormPlan& p, const NormArgs& a, int blocks, int w_f32, hip
 }
 
 template <typename T>
-void launch_bwd(const NormPlan& p, const NormGradArgs& a, int blocks, int w_f32, hipStream_t st) {
+void launch_bwd(const RowPlan& p, const NormGradArgs& a, int blocks, int w_f32, hipStream_t st) {
   const int threads = p.lpr > 256 ? p.lpr : 256;
 #define FST_CASE(L, C)                                                                   \
   if constexpr (planned<T>(L, C)) {                                                      \
@@ -491,7 +274,7 @@ void launch_bwd(const NormPlan& p, const NormGradArgs& a, int blocks, int w_f32,
 #undef FST_CASE
 }
 
-int check_norm(int dtype, int param_dtype, int B, int L, int N, NormPlan& p) {
+int check_norm(int dtype, int param_dtype, int B, int L, int N, RowPlan& p) {
   if (dtype != FST_BF16 && dtype != FST_F32 && dtype != FST_F16)
     return fail(FST_EINVAL, "dtype must be FST_BF16, FST_F16 or FST_F32, got %d", dtype);
   if (param_dtype != dtype && param_dtype != FST_F32)
@@ -499,8 +282,8 @@ int check_norm(int dtype, int param_dtype, int B, int L, int N, NormPlan& p) {
   if (B < 0 || L < 0) return fail(FST_EINVAL, "negative size (B=%d, L=%d)", B, L);
   if (N < 1) return fail(FST_EINVAL, "need at least one feature, got N=%d", N);
   if ((long)B * L > 0x7fffffffL) return fail(FST_EUNSUPPORTED, "more than 2^31 - 1 rows");
-  if (!plan_norm(dtype, N, p))
-    return fail(FST_EUNSUPPORTED, "rows of N=%d features: at most %d", N, kNormMax);
+  if (!plan_rows(dtype, N, p))
+    return fail(FST_EUNSUPPORTED, "rows of N=%d features: at most %d", N, kRowMax);
   return FST_OK;
 }
 
@@ -516,7 +299,7 @@ int fst_layer_norm_forward(int dtype, int param_dtype, int B, int L, int N, cons
                            const void* residual, int64_t residual_stride, const void* weight, const void* bias,
                            const int32_t* seqlens, float eps, void* y, void* sum, float* stats, void* stream) {
   clear_error();
-  NormPlan p;
+  RowPlan p;
   const int rc = check_norm(dtype, param_dtype, B, L, N, p);
   if (rc != FST_OK) return rc;
   const long rows = (long)B * L;
@@ -530,7 +313,7 @@ int fst_layer_norm_forward(int dtype, int param_dtype, int B, int L, int N, cons
   p.edge = !aligned16(x, x_stride, es) || !aligned16(y, N, es) ||
            (residual && (!aligned16(residual, residual_stride, es) || !aligned16(sum, N, es)));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const int w_f32 = param_dtype == FST_F32, blocks = norm_blocks(p, rows, norm_forward_blocks(p, dtype));
+  const int w_f32 = param_dtype == FST_F32, blocks = row_blocks(p, rows, norm_forward_blocks(p, dtype));
   if (dtype == FST_BF16)
     launch_fwd<bf16>(p, a, blocks, w_f32, st);
   else if (dtype == FST_F16)
@@ -543,9 +326,9 @@ int fst_layer_norm_forward(int dtype, int param_dtype, int B, int L, int N, cons
 }
 
 size_t fst_layer_norm_backward_workspace_bytes(int dtype, int B, int L, int N) {
-  NormPlan p;
+  RowPlan p;
   if (check_norm(dtype, dtype, B, L, N, p) != FST_OK) return 0;
-  return align256((size_t)norm_blocks(p, (long)B * L, kNormBlocks) * 2 * N * sizeof(float));
+  return align256((size_t)row_blocks(p, (long)B * L, kNormBlocks) * 2 * N * sizeof(float));
 }
 
 int fst_layer_norm_backward(int dtype, int param_dtype, int B, int L, int N, const void* s, int64_t s_stride,
@@ -553,7 +336,7 @@ int fst_layer_norm_backward(int dtype, int param_dtype, int B, int L, int N, con
                             int64_t dy_stride, const void* dsum, int64_t dsum_stride, void* dx, void* dweight,
                             void* dbias, void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
-  NormPlan p;
+  RowPlan p;
   const int rc = check_norm(dtype, param_dtype, B, L, N, p);
   if (rc != FST_OK) return rc;
   const long rows = (long)B * L;
@@ -563,7 +346,7 @@ int fst_layer_norm_backward(int dtype, int param_dtype, int B, int L, int N, con
     if (!s || !dy || !stats) return fail(FST_EINVAL, "null tensor pointer");
     if (s_stride < N || dy_stride < N || (dsum && dsum_stride < N)) return fail(FST_EINVAL, "row stride below N=%d", N);
   }
-  const int blocks = norm_blocks(p, rows, kNormBlocks);
+  const int blocks = row_blocks(p, rows, kNormBlocks);
   const size_t need = align256((size_t)blocks * 2 * N * sizeof(float));
   if (sums && need > 0 && (!workspace || workspace_bytes < need))
     return fail(FST_EWORKSPACE, "workspace of %zu bytes is smaller than the %zu required", workspace_bytes, need);
@@ -586,11 +369,11 @@ int fst_layer_norm_backward(int dtype, int param_dtype, int B, int L, int N, con
   if (sums) {
     const int grid = (2 * N + 31) / 32;
     if (dtype == FST_BF16)
-      norm_grad_sum<bf16><<<grid, 1024, 0, st>>>(part, blocks, N, dweight, dbias, w_f32);
+      column_sums<bf16><<<grid, 1024, 0, st>>>(part, blocks, N, 2 * N, dweight, dbias, w_f32);
     else if (dtype == FST_F16)
-      norm_grad_sum<f16><<<grid, 1024, 0, st>>>(part, blocks, N, dweight, dbias, w_f32);
+      column_sums<f16><<<grid, 1024, 0, st>>>(part, blocks, N, 2 * N, dweight, dbias, w_f32);
     else
-      norm_grad_sum<float><<<grid, 1024, 0, st>>>(part, blocks, N, dweight, dbias, w_f32);
+      column_sums<float><<<grid, 1024, 0, st>>>(part, blocks, N, 2 * N, dweight, dbias, w_f32);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return fail(FST_ELAUNCH, "layer norm backward launch failed (%s)", hipGetErrorString(e));

@@ -352,6 +352,98 @@ int fst_ffn_backward(int dtype, int activation, int B, int L, int D, int F, cons
                      void* dw_down, void* db_gate, void* db_up, void* db_down, void* workspace,
                      size_t workspace_bytes, void* stream);
 
+/* y = s / sqrt(mean(s^2) + eps) * weight over the N features of a row, s = x, or
+ * with residual (nullable) s = x + residual rounded to dtype and written to sum:
+ * fst_layer_norm_forward's rows, types and limits, without a mean and a bias. rstd
+ * (nullable) receives 1 / sqrt(mean(s^2) + eps) of the rows, [B * L], for the backward;
+ * of padding rows 0. */
+int fst_rms_norm_forward(int dtype, int param_dtype, int B, int L, int N, const void* x, int64_t x_stride,
+                         const void* residual, int64_t residual_stride, const void* weight, const int32_t* seqlens,
+                         float eps, void* y, void* sum, float* rstd, void* stream);
+
+/* The same y as 8-bit values q [B * L, N] (e4m3) times one scale a row [B * L]:
+ * scale = max |y| / 448, at least 2^-126, and q = y / scale, from the float32 y.
+ * Padding rows are zeros with scale 0; NaN stays NaN. */
+int fst_rms_norm_fp8(int dtype, int param_dtype, int B, int L, int N, const void* x, int64_t x_stride,
+                     const void* residual, int64_t residual_stride, const void* weight, const int32_t* seqlens,
+                     float eps, void* q, float* scale, void* sum, void* stream);
+
+/* Scratch bytes fst_rms_norm_backward needs (when dweight is asked for). */
+size_t fst_rms_norm_backward_workspace_bytes(int dtype, int B, int L, int N);
+
+/* From s (x, or the forward's sum), rstd, and the gradients dy of y and dsum
+ * (nullable) of sum: dx, the gradient of x and of residual alike, and dweight in
+ * param_dtype. Either is nullable. */
+int fst_rms_norm_backward(int dtype, int param_dtype, int B, int L, int N, const void* s, int64_t s_stride,
+                          const void* weight, const int32_t* seqlens, const float* rstd, const void* dy,
+                          int64_t dy_stride, const void* dsum, int64_t dsum_stride, void* dx, void* dweight,
+                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * A mixture of experts in the feed-forward's place: the router, the tokens' slots
+ * sorted by expert, their rows brought into that order and back, and the experts'
+ * gated feed-forward on rows in that order. Up to 512 experts, up to 16 slots a
+ * token; tokens times slots below 2^31 - 65536. */
+
+/* The K largest of each token's E logits (ties: the lowest index; NaN ranks highest;
+ * -inf is never chosen) and their softmax, over the chosen (normalize) or over all
+ * E: weights float32 and experts [B * L, K], by falling logit. Slots that find no logit,
+ * and those of padding rows, are expert -1 with weight 0. Rows lie logits_stride
+ * elements apart. */
+int fst_expert_route(int dtype, int B, int L, int E, int K, int normalize, const void* logits, int64_t logits_stride,
+                     const int32_t* seqlens, float* weights, int32_t* experts, void* stream);
+
+/* dlogits [B * L, E] in dtype from the forward's operands and results and dweights
+ * [B * L, K]. logits may be null with normalize. */
+int fst_expert_route_backward(int dtype, int B, int L, int E, int K, int normalize, const void* logits,
+                              int64_t logits_stride, const int32_t* seqlens, const float* weights,
+                              const int32_t* experts, const float* dweights, void* dlogits, void* stream);
+
+/* Scratch bytes fst_expert_sort needs. */
+size_t fst_expert_sort_workspace_bytes(int slots, int E);
+
+/* A stable sort of the slots by expert: offsets [E + 1], the first row of each expert's
+ * run and behind the last, order [slots], the slot of each row (-1 past the last run),
+ * and place [slots], the row of each slot (-1 where its expert is outside 0 .. E - 1). */
+int fst_expert_sort(int slots, int E, const int32_t* experts, int32_t* order, int32_t* place, int32_t* offsets,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* The tokens' rows x (x_stride elements apart, N features) at their places:
+ * out[place[t, k]] = weights[t, k] x[t] (weights nullable: 1; float32 or of dtype), and
+ * zeros from row *used on (offsets + E), of `rows` dense ones; and with back (rows of N,
+ * back_stride apart) dweights[t, k] = x[t] . back[place[t, k]] in weight_dtype, 0 for
+ * places outside the rows. out and dweights are each nullable. No two slots may share
+ * a place. */
+int fst_expert_spread(int dtype, int weight_dtype, int64_t tokens, int K, int N, int64_t rows, const void* x,
+                      int64_t x_stride, const int32_t* place, const int32_t* used, const void* weights,
+                      const void* back, int64_t back_stride, void* out, void* dweights, void* stream);
+
+/* out[t] = sum_k weights[t, k] x[place[t, k]] (weights nullable: 1), in float32 and in
+ * order; places outside the `rows` rows of x add nothing. */
+int fst_expert_gather(int dtype, int weight_dtype, int64_t tokens, int K, int N, int64_t rows, const void* x,
+                      int64_t x_stride, const int32_t* place, const void* weights, void* out, void* stream);
+
+/* fst_ffn_forward for rows in runs: those from offsets[e] to offsets[e + 1] - 1 (taken
+ * within the rows) with w_gate, w_up [E, F, D] and w_down [E, D, F] at e. Rows past the last run are
+ * zeros in y and are neither read nor written elsewhere. No biases. */
+int fst_expert_ffn_forward(int dtype, int activation, int rows, int E, int D, int F, const void* x, int64_t x_stride,
+                           const int32_t* offsets, const void* w_gate, const void* w_up, const void* w_down,
+                           void* hidden, void* gate, void* up, void* y, void* stream);
+
+/* fst_ffn_tiles of such a call, chosen as if the runs were even. Host-only, no GPU call. */
+int fst_expert_ffn_tiles(int dtype, int rows, int E, int D, int F, int32_t* tiles);
+
+/* Scratch bytes fst_expert_ffn_backward needs. */
+size_t fst_expert_ffn_backward_workspace_bytes(int dtype, int rows, int E, int D, int F);
+
+/* The gradients, from the forward's operands, its hidden, gate and up, and dy; those of
+ * an expert without rows are zeros. Each gradient is nullable. */
+int fst_expert_ffn_backward(int dtype, int activation, int rows, int E, int D, int F, const void* x, int64_t x_stride,
+                            const int32_t* offsets, const void* w_gate, const void* w_up, const void* w_down,
+                            const void* hidden, const void* gate, const void* up, const void* dy, int64_t dy_stride,
+                            void* dx, void* dw_gate, void* dw_up, void* dw_down, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
 /* The fp32 frequency ladder exp(-i ln(1e4) / (C/2)), i < C/2, that the kernels
  * embed with, written to out[0 .. C/2). Counterpart of sinusoidal_frequencies
  * (reference.py:45-56); evaluated with the same fp32 steps. */
