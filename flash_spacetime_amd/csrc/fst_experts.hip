@@ -29,7 +29,7 @@ struct RouteArgs {
   float* weights;
   int32_t* experts;
   long rows, ld;
-  int L, E, K, chosen;
+  int L, E, K, chosen, wide;
 };
 
 struct RouteGradArgs {
@@ -39,25 +39,27 @@ struct RouteGradArgs {
   const int32_t* experts;
   void* dlogits;
   long rows, ld;
-  int L, E, K, chosen;
+  int L, E, K, chosen, wide, wide_out;
 };
 
-// A logit as an unsigned in its order: NaN above all, 0 for what cannot be chosen
-// (-inf, and what was). The two zeros are one.
+// A logit as an unsigned in its order, NaN above all. The two zeros are one. Keys up to
+// -inf's cannot be chosen; 0 stands for what was.
+constexpr unsigned kNotChosen = 0x007fffffu;
 __device__ __forceinline__ unsigned order_key(float v) {
-  if (v != v) return 0xffffffffu;
   const unsigned u = __float_as_uint(v + 0.f);
-  return v == -__builtin_inff() ? 0u : u & 0x80000000u ? ~u : u | 0x80000000u;
+  return v != v ? 0xffffffffu : u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(unsigned k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
-// Reductions of unsigneds over groups of G = 16 or 64 lanes.
+// x reduced with f over groups of G = 8, 16 or 64 lanes, pairs first: every lane gets it.
 template <int G, typename F>
 __device__ __forceinline__ unsigned group_reduce(unsigned x, F f) {
-  x = f(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, false));
-  x = f(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x124, 0xf, 0xf, false));
-  x = f(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x122, 0xf, 0xf, false));
-  x = f(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x121, 0xf, 0xf, false));
+#define FST_WITH(pattern) f(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, pattern, 0xf, 0xf, false))
+  x = FST_WITH(0xb1);   // the other of a pair
+  x = FST_WITH(0x4e);   // the other pair of four
+  x = FST_WITH(0x141);  // the other four of eight
+  if constexpr (G >= 16) x = FST_WITH(0x140);
+#undef FST_WITH
   if constexpr (G == 64) {
     const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
     x = f(a[0], a[1]);
@@ -66,12 +68,36 @@ __device__ __forceinline__ unsigned group_reduce(unsigned x, F f) {
   }
   return x;
 }
+template <int G>
+__device__ __forceinline__ float lanes_sum(float x) {
+  return __uint_as_float(group_reduce<G>(__float_as_uint(x), [](unsigned a, unsigned b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
 
-// Lane l of a row's G holds its logits l + G i, i < NC; -inf past the last.
-template <typename T, int G, int NC>
-__device__ __forceinline__ void load_logits(const T* row, int l, int E, float* v) {
+// Lane l of a row's G holds its logits l NC .. + NC - 1; -inf past the last. wide: rows and
+// their ends on multiples of 16 bytes.
+template <typename T, int NC>
+constexpr bool kWideLogits = NC * sizeof(T) >= 16;
+
+template <typename T, int NC>
+__device__ __forceinline__ void load_logits(const T* row, int l, int E, bool wide, float* v) {
+  constexpr int V = kVec<T>;
+  if constexpr (kWideLogits<T, NC>) {
+    if (wide) {
 #pragma unroll
-  for (int i = 0; i < NC; ++i) v[i] = l + G * i < E ? (float)row[l + G * i] : -__builtin_inff();
+      for (int i = 0; i < NC; i += V) {
+        const bool in = l * NC + i < E;
+        typename Piece<T>::V q;
+        if (in) q = *reinterpret_cast<const typename Piece<T>::V*>(row + l * NC + i);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[i + j] = in ? (float)q[j] : -__builtin_inff();
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NC; ++i) v[i] = l * NC + i < E ? (float)row[l * NC + i] : -__builtin_inff();
 }
 
 template <typename T, int G, int NC>
@@ -83,22 +109,22 @@ __global__ __launch_bounds__(256) void expert_route(RouteArgs a) {
   int expert = -1;  // lane k: the k-th largest
   if (row_valid(a.lens, row, a.L)) {
     float v[NC];
-    load_logits<T, G, NC>(static_cast<const T*>(a.logits) + row * a.ld, l, a.E, v);
+    load_logits<T, NC>(static_cast<const T*>(a.logits) + row * a.ld, l, a.E, a.wide, v);
     unsigned key[NC];
 #pragma unroll
     for (int i = 0; i < NC; ++i) key[i] = order_key(v[i]);
     float top = 0.f, mine = 0.f;
     for (int k = 0; k < a.K; ++k) {
-      unsigned best = key[0], at = l;
+      unsigned best = key[0], at = l * NC;
 #pragma unroll
       for (int i = 1; i < NC; ++i)
-        if (key[i] > best) best = key[i], at = l + G * i;
+        if (key[i] > best) best = key[i], at = l * NC + i;
       const unsigned most = group_reduce<G>(best, [](unsigned x, unsigned y) { return max(x, y); });
-      if (most == 0) break;  // nothing left to choose: the same for all lanes of the row
+      if (most <= kNotChosen) break;  // nothing left to choose: the same for all lanes of the row
       at = group_reduce<G>(best == most ? at : 0xffffffffu, [](unsigned x, unsigned y) { return min(x, y); });
 #pragma unroll
       for (int i = 0; i < NC; ++i)
-        if ((int)at == l + G * i) key[i] = 0;
+        if ((int)at == l * NC + i) key[i] = 0;
       const float value = key_value(most);
       if (k == 0) top = value;
       if (l == k) mine = value, expert = (int)at;
@@ -109,9 +135,9 @@ __global__ __launch_bounds__(256) void expert_route(RouteArgs a) {
       sum = w;
     } else {
 #pragma unroll
-      for (int i = 0; i < NC; ++i) sum += l + G * i < a.E && !(v[i] == -__builtin_inff()) ? expf(v[i] - top) : 0.f;
+      for (int i = 0; i < NC; ++i) sum += !(v[i] == -__builtin_inff()) ? expf(v[i] - top) : 0.f;
     }
-    sum = group_sum<G>(sum, nullptr);
+    sum = lanes_sum<G>(sum);
     w = expert >= 0 ? w / sum : 0.f;
   }
   if (l < a.K) {
@@ -133,11 +159,11 @@ __global__ __launch_bounds__(256) void expert_route_grad(RouteGradArgs a) {
     float w = 0.f, g = 0.f;
     if (l < a.K) expert = a.experts[row * a.K + l];
     if (expert >= 0) w = a.weights[row * a.K + l], g = a.dw[row * a.K + l];
-    const float mean = group_sum<G>(w * g, nullptr);
+    const float mean = lanes_sum<G>(w * g);
     g = a.chosen ? w * (g - mean) : w * g;
     if (!a.chosen) {
       float v[NC], top = -__builtin_inff(), sum = 0.f;
-      load_logits<T, G, NC>(static_cast<const T*>(a.logits) + row * a.ld, l, a.E, v);
+      load_logits<T, NC>(static_cast<const T*>(a.logits) + row * a.ld, l, a.E, a.wide, v);
 #pragma unroll
       for (int i = 0; i < NC; ++i) top = fmaxf(top, v[i]);
       top = key_value(group_reduce<G>(order_key(top), [](unsigned x, unsigned y) { return max(x, y); }));
@@ -146,7 +172,7 @@ __global__ __launch_bounds__(256) void expert_route_grad(RouteGradArgs a) {
         v[i] = v[i] == -__builtin_inff() ? 0.f : expf(v[i] - top);
         sum += v[i];
       }
-      sum = group_sum<G>(sum, nullptr);
+      sum = lanes_sum<G>(sum);
 #pragma unroll
       for (int i = 0; i < NC; ++i) d[i] = sum == 0.f ? 0.f : -mean * (v[i] / sum);
     }
@@ -155,26 +181,46 @@ __global__ __launch_bounds__(256) void expert_route_grad(RouteGradArgs a) {
       const float add = __shfl(g, k, G);
 #pragma unroll
       for (int i = 0; i < NC; ++i)
-        if (at == l + G * i) d[i] += add;
+        if (at == l * NC + i) d[i] += add;
     }
   }
-  T* out = static_cast<T*>(a.dlogits) + row * a.E;
+  T* out = static_cast<T*>(a.dlogits) + row * a.E + l * NC;
+  if constexpr (kWideLogits<T, NC>) {
+    if (a.wide_out) {
+#pragma unroll
+      for (int i = 0; i < NC; i += kVec<T>)
+        if (l * NC + i < a.E) *reinterpret_cast<typename Piece<T>::V*>(out + i) = pack_piece<T>(d + i);
+      return;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < NC; ++i)
-    if (l + G * i < a.E) out[l + G * i] = (T)d[i];
+    if (l * NC + i < a.E) out[i] = (T)d[i];
 }
 
-// f(lanes, logits a lane): 16 lanes a row up to 64 experts, a wave above.
+// f(lanes, logits a lane). A lane's own logits are compared at a few instructions each,
+// lanes with each other at as many a step for all of them: few lanes with eight logits
+// each (but one for each of the K). 256 x 768 padded tokens of 64 f32 logits, K = 4:
+// 16 lanes of four 18.7 us, eight of eight KROUTE.
 template <typename F>
-void by_experts(int E, F f) {
-  if (E <= 16)
-    f(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
-  else if (E <= 64)
-    f(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
-  else if (E <= 128)
-    f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
-  else
-    f(std::integral_constant<int, 64>{}, std::integral_constant<int, 8>{});
+void by_experts(int E, int K, F f) {
+  const auto with = [&](auto lanes, auto count) { f(lanes, count); };
+#define FST_LANES(l, c) with(std::integral_constant<int, l>{}, std::integral_constant<int, c>{})
+  if (E <= 64 && K <= 8) {
+    if (E <= 8)
+      FST_LANES(8, 1);
+    else if (E <= 16)
+      FST_LANES(8, 2);
+    else
+      FST_LANES(8, 8);
+  } else if (E <= 16) {
+    FST_LANES(16, 1);
+  } else if (E <= 128) {
+    FST_LANES(16, 8);
+  } else {
+    FST_LANES(64, 8);
+  }
+#undef FST_LANES
 }
 
 int check_route(int dtype, int B, int L, int E, int K) {
@@ -202,45 +248,97 @@ struct SortArgs {
 // A slot's bin: its expert, or E where that is none.
 __device__ __forceinline__ int bin_of(int expert, int E) { return (unsigned)expert < (unsigned)E ? expert : E; }
 
+// Four of a wave's slots from `at` on, a lane's 64 apart: their bins, -1 past the end.
+__device__ __forceinline__ void load_bins(const SortArgs& a, int at, int end, int* bin) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) bin[j] = at + 64 * j + lane < end ? a.experts[at + 64 * j + lane] : -1;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) bin[j] = at + 64 * j + lane < end ? bin_of(bin[j], a.E) : -1;
+}
+
+// Among the wave's 64 slots: how many of this one's bin come before it, and how many there
+// are. Ballots over the bin's bits tell; an atomic addition for each slot would run 64
+// deep where all are of one bin, as padding is.
+__device__ __forceinline__ void rank_of(int bin, int bits, int& rank, int& count) {
+  unsigned long long same = __ballot(bin >= 0);
+  for (int b = 0; b < bits; ++b) {
+    const bool set = (bin >> b) & 1;
+    const unsigned long long those = __ballot(set);
+    same &= set ? those : ~those;
+  }
+  rank = __builtin_amdgcn_mbcnt_hi((unsigned)(same >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)same, 0));
+  count = __popcll(same);
+}
+
 __global__ __launch_bounds__(kSortThreads) void expert_count(SortArgs a) {
   __shared__ int count[kMostBins];
   for (int i = threadIdx.x; i <= a.E; i += kSortThreads) count[i] = 0;
   __syncthreads();
   const int s0 = blockIdx.x * a.chunk, s1 = min(s0 + a.chunk, a.slots);
-  for (int s = s0 + threadIdx.x; s < s1; s += kSortThreads) atomicAdd(&count[bin_of(a.experts[s], a.E)], 1);
+  for (int s = s0 + (threadIdx.x >> 6) * 256; s < s1; s += kSortWaves * 256) {
+    int bin[4];
+    load_bins(a, s, s1, bin);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      int rank, n;
+      rank_of(bin[j], a.bits, rank, n);
+      if (bin[j] >= 0 && rank == 0) atomicAdd(&count[bin[j]], n);
+    }
+  }
   __syncthreads();
   for (int i = threadIdx.x; i <= a.E; i += kSortThreads) a.counts[(long)blockIdx.x * (a.E + 1) + i] = count[i];
 }
 
 // Each wave of a workgroup takes a run of its chunk. A slot's row: those of smaller
 // bins, of its bin in the chunks before and in the waves before, and those before it in
-// its wave, which ballots over the bin's bits tell. All integers: the order of the
-// additions does not matter.
+// its wave. All integers: the order of the additions does not matter.
 __global__ __launch_bounds__(kSortThreads) void expert_place(SortArgs a) {
   __shared__ int next[kSortWaves][kMostBins];  // counts, then the next row, of each wave and bin
   __shared__ int total[kMostBins], before[kMostBins];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bins = a.E + 1;
-  for (int i = tid; i < kSortWaves * bins; i += kSortThreads) next[i / bins][i % bins] = 0;
-  for (int i = tid; i < bins; i += kSortThreads) total[i] = before[i] = 0;
-  __syncthreads();
   const int c0 = blockIdx.x * a.chunk, c1 = min(c0 + a.chunk, a.slots);
   const int run = ((c1 - c0 + kSortWaves - 1) / kSortWaves + 63) / 64 * 64;
   const int s0 = min(c0 + wave * run, c1), s1 = min(s0 + run, c1);
-  for (int s = s0 + lane; s < s1; s += 64) atomicAdd(&next[wave][bin_of(a.experts[s], a.E)], 1);
+  int bin[4], rank[4], count[4];
+  load_bins(a, s0, s1, bin);
+  volatile int* mine = next[wave];
+  for (int i = lane; i < bins; i += 64) mine[i] = 0;
+  for (int i = tid; i < bins; i += kSortThreads) total[i] = before[i] = 0;
+  __syncthreads();
   if (a.counts) {
-    const int all = gridDim.x * bins;
-    for (int i = tid; i < all; i += kSortThreads) {
-      const int b = i / bins, e = i - b * bins, n = a.counts[i];
-      if (n) {
-        atomicAdd(&total[e], n);
-        if (b < (int)blockIdx.x) atomicAdd(&before[e], n);
+    // Thread (part, bin): every parts-th workgroup's count, all loads in flight (sort_plan:
+    // at most 32).
+    const int width = 1 << a.bits, parts = max(kSortThreads / width, 1), e = tid & (width - 1), blocks = gridDim.x;
+    if (e < bins && tid / width < parts) {
+      int n[32], all = 0, low = 0;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const int b = tid / width + j * parts;
+        n[j] = b < blocks ? a.counts[(long)b * bins + e] : 0;
       }
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        all += n[j];
+        low += tid / width + j * parts < (int)blockIdx.x ? n[j] : 0;
+      }
+      atomicAdd(&total[e], all);
+      atomicAdd(&before[e], low);
+    }
+  }
+  for (int s = s0; s < s1; s += 256) {
+    if (s > s0) load_bins(a, s, s1, bin);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      rank_of(bin[j], a.bits, rank[j], count[j]);
+      if (bin[j] >= 0 && rank[j] == 0) mine[bin[j]] = mine[bin[j]] + count[j];
     }
   }
   __syncthreads();
   if (!a.counts) {
     for (int i = tid; i < bins; i += kSortThreads) {
       int n = 0;
+#pragma unroll
       for (int w = 0; w < kSortWaves; ++w) n += next[w][i];
       total[i] = n;
     }
@@ -264,30 +362,32 @@ __global__ __launch_bounds__(kSortThreads) void expert_place(SortArgs a) {
     }
   }
   __syncthreads();
-  for (int i = tid; i < bins; i += kSortThreads) {
-    int at = total[i] + before[i];
-    for (int w = 0; w < kSortWaves; ++w) {
-      const int n = next[w][i];
-      next[w][i] = at;
-      at += n;
+  // Sixteen threads a bin, one for each wave.
+  static_assert(kSortWaves == 16, "a row of lanes");
+  for (int i = tid >> 4; i < bins; i += kSortThreads / 16) {
+    const int w = tid & 15, n = next[w][i];
+    int sum = n;
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) {
+      const int up = __shfl_up(sum, d, 16);
+      if (w >= d) sum += up;
     }
+    next[w][i] = total[i] + before[i] + sum - n;
   }
   __syncthreads();
-  volatile int* mine = next[wave];
-  for (int s = s0 + lane; s - lane < s1; s += 64) {
-    const bool in = s < s1;
-    const int bin = in ? bin_of(a.experts[s], a.E) : 0;
-    unsigned long long same = __ballot(in);
-    for (int b = 0; b < a.bits; ++b) {
-      const unsigned long long set = __ballot((bin >> b) & 1);
-      same &= (bin >> b) & 1 ? set : ~set;
+  for (int s = s0; s < s1; s += 256) {
+    if (run > 256) {
+      load_bins(a, s, s1, bin);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) rank_of(bin[j], a.bits, rank[j], count[j]);
     }
-    const int rank = __popcll(same & ((1ull << lane) - 1));
-    const int row = in ? mine[bin] + rank : 0;
-    if (in && rank == 0) mine[bin] = row + __popcll(same);  // after every lane's read: LDS keeps a wave's order
-    if (in) {
-      a.place[s] = bin < a.E ? row : -1;
-      a.order[row] = bin < a.E ? s : -1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (bin[j] < 0) continue;
+      const int row = mine[bin[j]] + rank[j], slot = s + 64 * j + lane;
+      if (rank[j] == 0) mine[bin[j]] = row + count[j];  // after every lane's read: LDS keeps a wave's order
+      a.place[slot] = bin[j] < a.E ? row : -1;
+      a.order[row] = bin[j] < a.E ? slot : -1;
     }
   }
 }
@@ -344,10 +444,16 @@ template <int LPR>
 __device__ __forceinline__ int place_at(int place, int k) {
   return __shfl(place, k, kRowLanes<LPR>);
 }
-template <typename T>
-__device__ __forceinline__ float weight_at(const MoveArgs& a, long t, int k, bool f32) {
-  const long i = t * a.K + k;
+// Lane k's weight beside its place (1 without weights).
+template <typename T, int LPR>
+__device__ __forceinline__ float load_weight(const MoveArgs& a, long t, int place, bool f32) {
+  if (!a.weights || place < 0) return 1.f;
+  const long i = t * a.K + threadIdx.x % kRowLanes<LPR>;
   return f32 ? static_cast<const float*>(a.weights)[i] : (float)static_cast<const T*>(a.weights)[i];
+}
+template <int LPR>
+__device__ __forceinline__ float weight_at(float weight, int k) {
+  return __shfl(weight, k, kRowLanes<LPR>);
 }
 
 // A group walks the tokens with the next one's row, and the places of the one after it,
@@ -367,6 +473,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void expert_spread(MoveArgs 
   for (; t < a.tokens; t += step) {
     const int later = load_place<LPR>(a, t + 2 * step);
     if (any_place<LPR>(next)) x1.load(static_cast<const T*>(a.in) + (t + step) * a.ld, l, n);
+    const float weight = load_weight<T, LPR>(a, t, now, w_f32);
     float v[E];
     if (any_place<LPR>(now)) x0.get(v, l, n);
     for (int k = 0; k < a.K; ++k) {
@@ -385,7 +492,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void expert_spread(MoveArgs 
         if (a.out) {
           T* out = static_cast<T*>(a.out) + (long)r * n;
           if (a.weights) {
-            const float w = weight_at<T>(a, t, k, w_f32);
+            const float w = weight_at<LPR>(weight, k);
             float q[E];
 #pragma unroll
             for (int i = 0; i < E; ++i) q[i] = w * v[i];
@@ -425,6 +532,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void expert_gather(MoveArgs 
   int now = load_place<LPR>(a, t);
   for (; t < a.tokens; t += step) {
     const int next = load_place<LPR>(a, t + step);
+    const float weight = load_weight<T, LPR>(a, t, now, w_f32);
     float sum[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) sum[i] = 0.f;
@@ -436,7 +544,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void expert_gather(MoveArgs 
       auto add = [&](const P& x, int k) __attribute__((always_inline)) {
         float q[E];
         x.get(q, l, n);
-        const float w = a.weights ? weight_at<T>(a, t, k, w_f32) : 1.f;
+        const float w = weight_at<LPR>(weight, k);
 #pragma unroll
         for (int i = 0; i < E; ++i) sum[i] = fmaf(w, q[i], sum[i]);
       };
@@ -448,7 +556,10 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void expert_gather(MoveArgs 
   }
 }
 
-constexpr int kMoveBlocks = 2048;
+// Most workgroups: a group then has one token or two, and a row's wait is covered by the
+// other groups (256 x 768 padded, 384 bf16, two slots a token, spread / weighted gather /
+// spread with dots / gather: 2048 workgroups 70 / 87 / 124 / 74 us, 16384 65 / 76 / 112 / 64).
+constexpr int kMoveBlocks = 16384;
 
 int check_move(int dtype, int weight_dtype, int64_t tokens, int K, int N, int64_t rows, RowPlan& p) {
   if (dtype != FST_BF16 && dtype != FST_F32 && dtype != FST_F16)
@@ -506,9 +617,11 @@ int fst_expert_route(int dtype, int B, int L, int E, int K, int normalize, const
   if (rows == 0) return FST_OK;
   if (!logits || !weights || !experts) return fail(FST_EINVAL, "null tensor pointer");
   if (logits_stride < E) return fail(FST_EINVAL, "row stride below E=%d", E);
-  const RouteArgs a{logits, seqlens, weights, experts, rows, (long)logits_stride, L, E, K, normalize != 0};
+  const size_t es = elem_size(dtype);
+  const bool wide = aligned16(logits, logits_stride, es) && E * es % 16 == 0;
+  const RouteArgs a{logits, seqlens, weights, experts, rows, (long)logits_stride, L, E, K, normalize != 0, wide};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  by_experts(E, [&](auto lanes, auto count) {
+  by_experts(E, K, [&](auto lanes, auto count) {
     const unsigned grid = (unsigned)((rows * lanes() + 255) / 256);
     if (dtype == FST_BF16)
       expert_route<bf16, lanes(), count()><<<grid, 256, 0, st>>>(a);
@@ -530,9 +643,12 @@ int fst_expert_route_backward(int dtype, int B, int L, int E, int K, int normali
   if (rows == 0) return FST_OK;
   if ((!normalize && !logits) || !weights || !experts || !dweights || !dlogits) return fail(FST_EINVAL, "null tensor pointer");
   if (!normalize && logits_stride < E) return fail(FST_EINVAL, "row stride below E=%d", E);
-  const RouteGradArgs a{logits, seqlens, weights, dweights, experts, dlogits, rows, (long)logits_stride, L, E, K, normalize != 0};
+  const size_t es = elem_size(dtype);
+  const bool whole = E * es % 16 == 0, wide = whole && aligned16(logits, logits_stride, es);
+  const RouteGradArgs a{logits, seqlens, weights, dweights, experts, dlogits, rows, (long)logits_stride, L, E, K, normalize != 0,
+                        wide, whole && aligned16(dlogits, E, es)};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  by_experts(E, [&](auto lanes, auto count) {
+  by_experts(E, K, [&](auto lanes, auto count) {
     const unsigned grid = (unsigned)((rows * lanes() + 255) / 256);
     if (dtype == FST_BF16)
       expert_route_grad<bf16, lanes(), count()><<<grid, 256, 0, st>>>(a);

@@ -73,9 +73,11 @@ __device__ __forceinline__ void store8(unsigned char* row, int l, int n, const f
   }
 }
 
-// Both kernels walk the rows a group at a time, with the next row's pieces in
-// flight while a row is worked on, and the length that says whether the row after
-// it is a token before those.
+// Both kernels walk the rows a group at a time, and ask for the length that says
+// whether the next row is a token before they need it. The forward also has the next
+// row's pieces in flight while a row is worked on; the backward holds so much of a row
+// that a third wave on a SIMD is worth more (256 x 768 padded rows of 384 bf16 with a
+// residual: two rows in flight and two waves 106 us, one and three 93).
 template <typename T, int LPR, int NC, bool EDGE, bool Q8>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rms_fwd(RmsArgs a, int w_f32) {
   typedef Pieces<T, LPR, NC, EDGE> P;
@@ -144,7 +146,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rms_fwd(RmsArgs a, int 
 }
 
 template <typename T, int LPR, int NC, bool EDGE>
-__global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rms_bwd(RmsGradArgs a, int w_f32) {
+__global__ __launch_bounds__(LPR > 256 ? LPR : 256, LPR > 256 ? 1 : 3) void rms_bwd(RmsGradArgs a, int w_f32) {
   typedef Pieces<T, LPR, NC, EDGE> P;
   constexpr int V = P::V, E = P::E, NT = LPR > 256 ? LPR : 256, G = NT / LPR;
   __shared__ float red[LPR > 64 ? LPR / 64 : 1];
@@ -156,35 +158,28 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rms_bwd(RmsGradArgs a, 
   const long step = (long)gridDim.x * G;
   long row = (long)blockIdx.x * G + grp;
   auto is_token = [&](long r) { return r < a.rows && row_valid(a.lens, r, a.L); };
-  struct Row {
-    P s, dy, ds;
-    float rstd;
-  } r0, r1;
-  auto fetch = [&](long r, Row& q) {
-    q.rstd = a.rstd[r];
-    q.s.load(static_cast<const T*>(a.s) + r * a.lds_, l, n);
-    q.dy.load(static_cast<const T*>(a.dy) + r * a.lddy, l, n);
-    if (a.ds) q.ds.load(static_cast<const T*>(a.ds) + r * a.ldds, l, n);
-  };
-  bool now = is_token(row), next = is_token(row + step);
-  if (now) fetch(row, r0);
+  bool now = is_token(row);
   float w[E], dw[E];
 #pragma unroll
   for (int i = 0; i < NC; ++i) load_param<T>(a.w, w_f32, P::at(l, i), n, 1.f, w + i * V);
 #pragma unroll
   for (int i = 0; i < E; ++i) dw[i] = 0.f;
   for (; row < a.rows; row += step) {
-    const bool later = is_token(row + 2 * step);
-    if (next) fetch(row + step, r1);
+    const bool next = is_token(row + step);
     float g[E];
     if (now) {
+      P s, dy, ds;
+      const float rstd = a.rstd[row];
+      s.load(static_cast<const T*>(a.s) + row * a.lds_, l, n);
+      dy.load(static_cast<const T*>(a.dy) + row * a.lddy, l, n);
+      if (a.ds) ds.load(static_cast<const T*>(a.ds) + row * a.ldds, l, n);
       float v[E];
-      r0.s.get(v, l, n);
-      r0.dy.get(g, l, n);
+      s.get(v, l, n);
+      dy.get(g, l, n);
       float c = 0.f;
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        v[i] *= r0.rstd;  // xhat; past the row's end 0, as dy
+        v[i] *= rstd;  // xhat; past the row's end 0, as dy
         dw[i] = fmaf(g[i], v[i], dw[i]);
         g[i] *= w[i];
         c = fmaf(g[i], v[i], c);
@@ -192,9 +187,9 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rms_bwd(RmsGradArgs a, 
       if (a.dx) {
         c = group_sum<LPR>(c, red) * inv_n;
 #pragma unroll
-        for (int i = 0; i < E; ++i) g[i] = r0.rstd * fmaf(-v[i], c, g[i]);
+        for (int i = 0; i < E; ++i) g[i] = rstd * fmaf(-v[i], c, g[i]);
         if (a.ds) {
-          r0.ds.get(v, l, n);
+          ds.get(v, l, n);
 #pragma unroll
           for (int i = 0; i < E; ++i) g[i] += v[i];
         }
@@ -204,9 +199,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rms_bwd(RmsGradArgs a, 
       for (int i = 0; i < E; ++i) g[i] = 0.f;
     }
     if (a.dx) P::store(static_cast<T*>(a.dx) + row * n, l, n, g);
-    r0 = r1;
     now = next;
-    next = later;
   }
   if (!a.part) return;
   float* out = a.part + (long)blockIdx.x * n;
@@ -232,10 +225,13 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rms_bwd(RmsGradArgs a, 
   }
 }
 
-// Most workgroups of the backward: each writes one partial of dw.
-constexpr int kRmsBlocks = 512;
+// Most workgroups of the backward, each of which writes one partial of dw: those that
+// run at once.
+constexpr int kRmsBlocks = 768;
 
-int rms_forward_blocks(const RowPlan& p) { return p.lpr == 1024 ? 512 : 1024; }
+// The forward's: a group has one row or two (a wide model's 65536 rows of 1024 f16 to 8
+// bits, 800 / 1024 / 16384 workgroups: 93 / 88 / 85 us).
+int rms_forward_blocks(const RowPlan& p) { return p.lpr == 1024 ? 512 : 16384; }
 
 int check_rms(int dtype, int param_dtype, int B, int L, int N, RowPlan& p) {
   if (dtype != FST_BF16 && dtype != FST_F32 && dtype != FST_F16)
