@@ -734,31 +734,37 @@ struct OuterSide {
   }
 };
 
+// Experts: a piece of an expert's run.
+struct OuterRun {
+  int expert, piece;
+};
+
 template <int WM, int WN, int NI, int NJ, bool MA, bool MB>
 __device__ __forceinline__ void outer_tile(const FfnOuter& p, const FfnOuters& all, int wg, unsigned char* lds,
-                                           int32_t* list) {
+                                           int32_t* list, OuterRun at_run = {}) {
   constexpr int TM = 16 * NI * WM, TN = 16 * NJ * WN, NT = 64 * WM * WN;
   typedef OuterSide<TM, NT, MA> SideA;
   typedef OuterSide<TN, NT, MB> SideB;
   constexpr int A_BYTES = KT * SideA::ROW, STAGE = A_BYTES + KT * SideB::ROW;
   const int nm = (p.M + TM - 1) / TM, nn = (p.N + TN - 1) / TN;
+#if FST_EXPERTS
+  // Tile wg of an expert's piece of its run.
+  const int split = at_run.expert * p.splits + at_run.piece, tile = wg;
+  const int first = min(max(all.offsets[at_run.expert], 0), all.tokens);
+  const int end = max(min(all.offsets[at_run.expert + 1], all.tokens), first);
+  const int run = ((end - first + p.splits - 1) / p.splits + KT - 1) / KT * KT;
+  const int t0 = (int)min(first + (long)at_run.piece * run, (long)end), t1 = (int)min((long)t0 + run, (long)end);
+#else
   // Consecutive workgroups of an XCD take the tiles of one run of tokens.
-  const int total = nm * nn * p.splits * (EXPERTS ? all.experts : 1), per = (total + 7) >> 3;
+  const int total = nm * nn * p.splits, per = (total + 7) >> 3;
   const int i8 = wg >> 3, at = (wg & 7) * per + i8;
   if (i8 >= per || at >= total) return;
-  const int split = at / (nm * nn), tile = at - split * nm * nn;  // experts: a split of an expert's run
-  const int m0 = tile % nm * TM, n0 = tile / nm * TN;
-#if FST_EXPERTS
-  const int expert = split / p.splits, piece = split - expert * p.splits;
-  const int first = min(max(all.offsets[expert], 0), all.tokens);
-  const int end = max(min(all.offsets[expert + 1], all.tokens), first);
-  const int run = ((end - first + p.splits - 1) / p.splits + KT - 1) / KT * KT;
-  const int t0 = (int)min(first + (long)piece * run, (long)end), t1 = (int)min((long)t0 + run, (long)end);
-#else
+  const int split = at / (nm * nn), tile = at - split * nm * nn;
   const int tokens = all.count ? *all.count : all.tokens;
   const int run = ((tokens + p.splits - 1) / p.splits + KT - 1) / KT * KT;
   const int t0 = (int)min((long)split * run, (long)tokens), t1 = (int)min((long)t0 + run, (long)tokens);
 #endif
+  const int m0 = tile % nm * TM, n0 = tile / nm * TN;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave % WM, wn = wave / WM, g = lane >> 4, n = lane & 15;
@@ -873,6 +879,52 @@ __device__ __forceinline__ void outer_tile(const FfnOuter& p, const FfnOuters& a
   }
 }
 
+// Experts: the weights' tiles are numbered expert by expert, `tiles` to each. XCD x takes
+// those whose work begins in the x-th eighth of all: a tile's is its expert's tokens, and
+// as much as kTileTokens of them for its start and its stores. As many tiles to each
+// left an XCD with the largest loads running alone (65536 rows over 32 experts of 0 to 1.5
+// times the mean, D = 1024, F = 1376 bf16: KOUTER).
+constexpr int kTileTokens = 128;
+
+__device__ __forceinline__ void tiles_of_xcd(const FfnOuters& ps, int tiles, int xcd, int& first, int& last) {
+  const int lane = threadIdx.x & 63;
+  int upto, work;  // of expert e0 + lane: the work of a column of tiles up to it, and its own
+  const auto scan = [&](int e0) __attribute__((always_inline)) {
+    const int e = e0 + lane;
+    const int from = e < ps.experts ? min(max(ps.offsets[e], 0), ps.tokens) : 0;
+    const int to = e < ps.experts ? min(max(ps.offsets[e + 1], 0), ps.tokens) : 0;
+    work = upto = e < ps.experts ? max(to - from, 0) + kTileTokens : 0;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int below = __shfl_up(upto, d);
+      if (lane >= d) upto += below;
+    }
+  };
+  long all = 0;
+  for (int e0 = 0; e0 < ps.experts; e0 += 64) {
+    scan(e0);
+    all += __builtin_amdgcn_readlane(upto, 63);
+  }
+  // The first tile whose work begins at `share` of all or later.
+  const auto tile_at = [&](long share) __attribute__((always_inline)) {
+    long before = 0;
+    for (int e0 = 0; e0 < ps.experts; e0 += 64) {
+      if (ps.experts > 64) scan(e0);
+      const long sum = __builtin_amdgcn_readlane(upto, 63);
+      if (share < tiles * (before + sum)) {
+        const int src = __builtin_ctzll(__ballot(share < tiles * (before + upto)));
+        const long own = __builtin_amdgcn_readlane(work, src);
+        const long left = share - tiles * (before + __builtin_amdgcn_readlane(upto - work, src));
+        return (e0 + src) * tiles + (int)min(max((left + own - 1) / own, 0l), (long)tiles);
+      }
+      before += sum;
+    }
+    return ps.experts * tiles;
+  };
+  first = tile_at(xcd * (tiles * all) / 8);
+  last = xcd == 7 ? ps.experts * tiles : tile_at((xcd + 1) * (tiles * all) / 8);
+}
+
 // A workgroup's tile is DT of D by FT of F (or 2 F) features: D is the first
 // problem's m and the second's n. PADDED: the tokens' rows of x (the first's a) and
 // dy (the second's b) come from the list.
@@ -882,10 +934,27 @@ __global__ __launch_bounds__(128 * WF, OCC) void ffn_outer(FfnOuters ps) {
   __shared__ __attribute__((aligned(1024))) unsigned char lds[OUTER_STAGES * KT * ES * (DT + FT)];
   __shared__ __attribute__((aligned(256))) int32_t list[PADDED ? 2 * 128 * WF : 1];
   const int wg = blockIdx.x;
+#if FST_EXPERTS
+  // Both problems' tiles of a piece of a run one after the other: they share its rows.
+  const auto tiles = [](const FfnOuter& p, int m, int n) { return p.splits ? ((p.M + m - 1) / m) * ((p.N + n - 1) / n) : 0; };
+  const int one = tiles(ps.p[0], DT, FT), piece = one + tiles(ps.p[1], FT, DT), splits = max(ps.p[0].splits, ps.p[1].splits);
+  int at, last;
+  tiles_of_xcd(ps, piece * splits, wg & 7, at, last);
+  for (at += wg >> 3; at < last; at += gridDim.x >> 3) {
+    const int run = at / piece, tile = at - run * piece;
+    const OuterRun r{run / splits, run % splits};
+    if (tile < one)
+      outer_tile<2, WF, ND / 2, NF / WF, false, false>(ps.p[0], ps, tile, lds, list, r);
+    else
+      outer_tile<2, WF, NF / 2, ND / WF, false, false>(ps.p[1], ps, tile - one, lds, list, r);
+    __syncthreads();  // before the next tile is loaded over what this one read
+  }
+#else
   if (wg < ps.first)
     outer_tile<2, WF, ND / 2, NF / WF, PADDED, false>(ps.p[0], ps, wg, lds, list);
   else
     outer_tile<2, WF, NF / 2, ND / WF, false, PADDED>(ps.p[1], ps, wg - ps.first, lds, list);
+#endif
 }
 
 // Tiles of t tokens, at most: each run may end in a tile of its own.
