@@ -1004,11 +1004,17 @@ enum Tile { kLarge, kMiddle, kSmall, kFew };
 Tile pick(const FfnProduct& p, int mats, bool redo) {
   if (p.tokens <= kFewTokens) return kFew;
   const auto load = [&](int f, int t) {
-    const int run = tokens_of_run(p);
-    const long tiles = (long)((p.F + f - 1) / f) * ((run + t - 1) / t) * (EXPERTS ? (p.tokens + run - 1) / run : 1);
+    // Experts: each run ends in half a tile.
+    const long down = EXPERTS ? p.tokens / t + (std::min(p.tokens, p.experts) + 1) / 2 : (p.tokens + t - 1) / t;
+    const long tiles = (long)((p.F + f - 1) / f) * down;
     return (double)((tiles + 255) / 256);
   };
   const double nl = load(256 / mats, redo ? 192 : 256), nm = load(128 / mats, redo ? 64 : 128), ns = load(64 / mats, 64);
+  // Many runs leave partly filled rounds, and float32's tiles cost what their products do:
+  // 2.3 n and 0.69 n us a step of middle and small ones (16384 tokens over 8 experts, D =
+  // 512, F = 704: output product 148 and 134 us, its gradient 181 and 154, dx 284 and 254,
+  // the gate 229 and 261).
+  if (EXPERTS && F32) return 2.3 * nm <= 0.69 * ns * (mats == 2 ? 1.03 : 1.0) ? kMiddle : kSmall;
   // Two weights' 64 x 64 tile has a quarter of each operand's rows reused less.
   const double large = 1.65 * nl * (redo ? 0.75 : 1.0), middle = (nm > 1 ? 0.54 * nm : 0.64) * (redo ? 0.55 : 1.0),
                small = (ns > 1 ? 0.24 * ns : 0.28) * (mats == 2 ? 1.3 : 1.0);
