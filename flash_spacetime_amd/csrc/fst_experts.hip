@@ -275,7 +275,7 @@ __global__ __launch_bounds__(kSortThreads) void expert_count(SortArgs a) {
   __shared__ int count[kMostBins];
   for (int i = threadIdx.x; i <= a.E; i += kSortThreads) count[i] = 0;
   __syncthreads();
-  const int s0 = blockIdx.x * a.chunk, s1 = min(s0 + a.chunk, a.slots);
+  const int s0 = blockIdx.x * a.chunk, s1 = s0 + min(a.chunk, a.slots - s0);
   for (int s = s0 + (threadIdx.x >> 6) * 256; s < s1; s += kSortWaves * 256) {
     int bin[4];
     load_bins(a, s, s1, bin);
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(kSortThreads) void expert_place(SortArgs a) {
   __shared__ int next[kSortWaves][kMostBins];  // counts, then the next row, of each wave and bin
   __shared__ int total[kMostBins], before[kMostBins];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bins = a.E + 1;
-  const int c0 = blockIdx.x * a.chunk, c1 = min(c0 + a.chunk, a.slots);
+  const int c0 = blockIdx.x * a.chunk, c1 = c0 + min(a.chunk, a.slots - c0);
   const int run = ((c1 - c0 + kSortWaves - 1) / kSortWaves + 63) / 64 * 64;
   const int s0 = min(c0 + wave * run, c1), s1 = min(s0 + run, c1);
   int bin[4], rank[4], count[4];
@@ -400,12 +400,12 @@ struct SortPlan {
 // every workgroup then adds up all counts (16384 of them at most).
 SortPlan sort_plan(int slots, int E) {
   if (slots <= 8192) return SortPlan{1, slots};
-  int blocks = 16384 / (E + 1);
+  long blocks = 16384 / (E + 1);
   blocks = blocks > 256 ? 256 : blocks;
-  const int need = (slots + 2047) / 2048;
+  const long need = (slots + 2047l) / 2048;
   blocks = blocks > need ? need : blocks;
-  const int chunk = ((slots + blocks - 1) / blocks + 1023) / 1024 * 1024;
-  return SortPlan{(slots + chunk - 1) / chunk, chunk};
+  const long chunk = ((slots + blocks - 1) / blocks + 1023) / 1024 * 1024;
+  return SortPlan{(int)((slots + chunk - 1) / chunk), (int)chunk};
 }
 
 // --- rows to the experts and back -------------------------------------------
