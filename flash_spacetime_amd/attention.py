@@ -137,6 +137,15 @@ class SpacetimeBlock(nn.Module):
     dim, rounded up to a multiple of 64 (the parameters of an ungated block of 4
     dim).
 
+    `norm="rms"` runs root-mean-square norms (`nn.RMSNorm` parameters) in layer norm's
+    place. With `experts=E` the feed-forward is a mixture: `router` (a linear without a
+    bias) gives each token its logits, the `top_k` largest choose its experts and
+    their softmax weighs them, and `experts_gate`, `experts_up` `[E, hidden, dim]` and
+    `experts_down` `[E, dim, hidden]` are the experts' weights, without biases (`ffn_bias` is
+    the one feed-forward's). Padding goes to no expert. Nothing keeps the loads
+    even but the router: a penalty for uneven ones is the training's to add, from
+    `router(..)`'s logits.
+
     `forward(x, feats, seqlens | key_padding_mask)` takes padded events `x [B, L,
     dim]`, or with `cu_seqlens` packed ones `[T, dim]`, and returns the same
     shape; padding rows (packed: those past `cu_seqlens[-1]`) are neither
@@ -149,18 +158,33 @@ class SpacetimeBlock(nn.Module):
     def __init__(self, dim: int, num_heads: int = 8, channels: int = 16, hidden: Optional[int] = None,
                  qkv_bias: bool = False, head_dim: Optional[int] = None, activation: str = "silu",
                  ffn_bias: bool = True, eps: float = 1e-5, use_attn_bias: bool = True,
-                 use_activation_bias: bool = True, device=None, dtype=None) -> None:
+                 use_activation_bias: bool = True, device=None, dtype=None, norm: str = "layer",
+                 experts: Optional[int] = None, top_k: int = 2) -> None:
         super().__init__()
         fk = {"device": device, "dtype": dtype}
+        if norm not in ("layer", "rms"):
+            raise ValueError(f"norm must be 'layer' or 'rms', got {norm!r}")
+        if experts is not None and not 1 <= top_k <= experts:
+            raise ValueError(f"top_k must be 1 .. {experts} experts, got {top_k}")
         if hidden is None:
             hidden = -(-8 * dim // (3 * 64)) * 64
-        self.norm1 = nn.LayerNorm(dim, eps=eps, **fk)
+        make_norm = nn.LayerNorm if norm == "layer" else nn.RMSNorm
+        self.norm1 = make_norm(dim, eps=eps, **fk)
         self.attn = SpacetimeAttention(dim, num_heads, channels, qkv_bias, head_dim, use_attn_bias,
                                        use_activation_bias, **fk)
-        self.norm2 = nn.LayerNorm(dim, eps=eps, **fk)
-        self.ffn_gate = nn.Linear(dim, hidden, bias=ffn_bias, **fk)
-        self.ffn_up = nn.Linear(dim, hidden, bias=ffn_bias, **fk)
-        self.ffn_down = nn.Linear(hidden, dim, bias=ffn_bias, **fk)
+        self.norm2 = make_norm(dim, eps=eps, **fk)
+        self.experts, self.top_k = experts, top_k
+        if experts is None:
+            self.ffn_gate = nn.Linear(dim, hidden, bias=ffn_bias, **fk)
+            self.ffn_up = nn.Linear(dim, hidden, bias=ffn_bias, **fk)
+            self.ffn_down = nn.Linear(hidden, dim, bias=ffn_bias, **fk)
+        else:
+            self.router = nn.Linear(dim, experts, bias=False, **fk)
+            self.experts_gate = nn.Parameter(torch.empty(experts, hidden, dim, **fk))
+            self.experts_up = nn.Parameter(torch.empty(experts, hidden, dim, **fk))
+            self.experts_down = nn.Parameter(torch.empty(experts, dim, hidden, **fk))
+            for w in (self.experts_gate, self.experts_up, self.experts_down):  # as nn.Linear's
+                nn.init.uniform_(w, -w.shape[-1] ** -0.5, w.shape[-1] ** -0.5)
         self.activation = activation
 
     def forward(self, x: Tensor, feats: Tensor, seqlens: Optional[Tensor] = None,
@@ -188,25 +212,46 @@ class SpacetimeBlock(nn.Module):
         return self._block(x, feats, seqlens, cu_seqlens, branch, defer)
 
     def _block(self, x, feats, seqlens, cu_seqlens, branch, defer):
-        from .feed_forward import flash_gated_feed_forward
-        from .norm import autocast_dtype, flash_layer_norm
+        from .norm import autocast_dtype
 
-        n1, n2 = self.norm1, self.norm2
         if cu_seqlens is not None:  # packed tokens past the last offset are padding
             seqlens = cu_seqlens[-1:]
         if branch is None:
-            y = flash_layer_norm(x, n1.weight, n1.bias, n1.eps, seqlens=seqlens)
+            y = self._norm(self.norm1, x, None, seqlens)
         else:
-            y, x = flash_layer_norm(branch, n1.weight, n1.bias, n1.eps, residual=x, seqlens=seqlens)
+            y, x = self._norm(self.norm1, branch, x, seqlens)
         a = self.attn(y, feats, seqlens if cu_seqlens is None else None, cu_seqlens=cu_seqlens)
-        y, x = flash_layer_norm(a, n2.weight, n2.bias, n2.eps, residual=x, seqlens=seqlens)
+        y, x = self._norm(self.norm2, a, x, seqlens)
         low = autocast_dtype()
         if low is not None:  # as autocast has a linear's rows; the norms stay in the stream's type
             y = y.to(low)
-        f = flash_gated_feed_forward(y, self.ffn_gate.weight, self.ffn_up.weight, self.ffn_down.weight,
-                                     self.ffn_gate.bias, self.ffn_up.bias, self.ffn_down.bias, self.activation,
-                                     seqlens=seqlens)
+        f = self._feed_forward(y, seqlens) if self.experts is None else self._mixture(y, seqlens)
         return (x, f) if defer else x + f
+
+    def _norm(self, n, x, residual, seqlens):
+        from .norm import flash_layer_norm
+        from .rms_norm import flash_rms_norm
+
+        if isinstance(n, nn.LayerNorm):
+            return flash_layer_norm(x, n.weight, n.bias, n.eps, residual=residual, seqlens=seqlens)
+        return flash_rms_norm(x, n.weight, n.eps, residual=residual, seqlens=seqlens)
+
+    def _feed_forward(self, y, seqlens):
+        from .feed_forward import flash_gated_feed_forward
+
+        return flash_gated_feed_forward(y, self.ffn_gate.weight, self.ffn_up.weight, self.ffn_down.weight,
+                                        self.ffn_gate.bias, self.ffn_up.bias, self.ffn_down.bias, self.activation,
+                                        seqlens=seqlens)
+
+    def _mixture(self, y, seqlens):
+        from .experts import (flash_expert_combine, flash_expert_dispatch, flash_expert_feed_forward, flash_expert_route,
+                              flash_expert_sort)
+
+        weights, chosen = flash_expert_route(self.router(y), self.top_k, seqlens=seqlens)
+        order = flash_expert_sort(chosen, self.experts)
+        rows = flash_expert_feed_forward(flash_expert_dispatch(y, order), order.offsets, self.experts_gate, self.experts_up,
+                                         self.experts_down, self.activation)
+        return flash_expert_combine(rows, weights, order)
 
     def _scattered(self, x, feats, valid, branch, defer):
         """Masks with holes: the valid tokens as packed events, put back afterwards."""

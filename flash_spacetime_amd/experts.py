@@ -173,7 +173,7 @@ def _spread(what, x, place, offsets, weights=None, back=None, rows=None, out=Tru
     with torch.cuda.device(x.device):
         rc = _lib.load().fst_expert_spread(
             dtype, dtype if weights is None else BLOCK_DTYPES[weights.dtype], place.numel() // k, k, n, rows, P(xr), x_stride,
-            P(place), offsets.data_ptr() + 4 * (offsets.numel() - 1), P(weights), P(br), b_stride, P(o), P(dw),
+            P(place), offsets.data_ptr() + 4 * (int(offsets.numel()) - 1), P(weights), P(br), b_stride, P(o), P(dw),
             _lib.stream_handle(x.device))
     _lib.check(rc, what)
     return o, dw
@@ -269,6 +269,8 @@ def flash_expert_combine(ys: Tensor, weights: Tensor, order: ExpertOrder) -> Ten
             return out
     check_rows(ys, weights)
     place, offsets = _check_order(order, ys)
+    if autocast_dtype() is not None and weights.dtype in BLOCK_DTYPES and weights.dtype != ys.dtype:
+        weights = weights.float()
     if ys.dim() != 2:
         raise ValueError(f"ys must be [slots, D], got {tuple(ys.shape)}")
     if weights.shape != place.shape or weights.dtype not in (ys.dtype, torch.float32):
