@@ -473,11 +473,11 @@ __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
     const int f = f0 + (wf * (NF / GS) + q) * 16 * GS + NE * g;
     const int left = min(NE, p.F - f);
     if (left <= 0) continue;
-    float b0[NE], b1[NE];
+    float b0[NE], b1[NE];  // zeros for experts, which have no biases
 #pragma unroll
     for (int e = 0; e < NE; ++e) b0[e] = b1[e] = 0.f;
-    if (MODE != kFfnGrad && p.bias[0]) load_run<NE>(static_cast<const T*>(p.bias[0]) + f, left, b0);
-    if (C::MATS == 2 && p.bias[1]) load_run<NE>(static_cast<const T*>(p.bias[1]) + f, left, b1);
+    if (!EXPERTS && MODE != kFfnGrad && p.bias[0]) load_run<NE>(static_cast<const T*>(p.bias[0]) + f, left, b0);
+    if (!EXPERTS && C::MATS == 2 && p.bias[1]) load_run<NE>(static_cast<const T*>(p.bias[1]) + f, left, b1);
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int t = t0 + (wt * NJ + j) * 16 + n;
@@ -486,8 +486,8 @@ __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
 #pragma unroll
       for (int e = 0; e < NE; ++e) {
         v[e] = acc[GS * q + (e >> 2)][j][e & 3];
-        if constexpr (MODE != kFfnGrad) v[e] += b0[e];
-        if constexpr (C::MATS == 2) u[e] = acc[NF + GS * q + (e >> 2)][j][e & 3] + b1[e];
+        if constexpr (MODE != kFfnGrad && !EXPERTS) v[e] += b0[e];
+        if constexpr (C::MATS == 2) u[e] = acc[NF + GS * q + (e >> 2)][j][e & 3] + (EXPERTS ? 0.f : b1[e]);
       }
       if constexpr (MODE == kFfnGate) {
         const long at = (long)t * p.ldo + f;
@@ -617,7 +617,7 @@ __global__ __launch_bounds__(512, MODE == kFfnRedo && NJ == 4 ? 2 : 4) void ffn_
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       v[a][e] = sum[e];
-      if (MODE != kFfnGrad && a < MATS && p.bias[a < 2 ? a : 0])
+      if (!EXPERTS && MODE != kFfnGrad && a < MATS && p.bias[a < 2 ? a : 0])
         v[a][e] += (float)static_cast<const T*>(p.bias[a < 2 ? a : 0])[f + e];
     }
   }
@@ -1011,10 +1011,10 @@ Tile pick(const FfnProduct& p, int mats, bool redo) {
   };
   const double nl = load(256 / mats, redo ? 192 : 256), nm = load(128 / mats, redo ? 64 : 128), ns = load(64 / mats, 64);
   // Many runs leave partly filled rounds, and float32's tiles cost what their products do:
-  // 2.3 n and 0.69 n us a step of middle and small ones (16384 tokens over 8 experts, D =
-  // 512, F = 704: output product 148 and 134 us, its gradient 181 and 154, dx 284 and 254,
-  // the gate 229 and 261).
-  if (EXPERTS && F32) return 2.3 * nm <= 0.69 * ns * (mats == 2 ? 1.03 : 1.0) ? kMiddle : kSmall;
+  // 2.3 n and 0.62 n us a step of middle and small ones (16384 tokens over 8 experts, D =
+  // 512, F = 704: output product 148 and 123 us, its gradient 181 and 138, dx 284 and 237,
+  // the gate 229 and 232).
+  if (EXPERTS && F32) return 2.3 * nm <= 0.62 * ns * (mats == 2 ? 1.03 : 1.0) ? kMiddle : kSmall;
   // Two weights' 64 x 64 tile has a quarter of each operand's rows reused less.
   const double large = 1.65 * nl * (redo ? 0.75 : 1.0), middle = (nm > 1 ? 0.54 * nm : 0.64) * (redo ? 0.55 : 1.0),
                small = (ns > 1 ? 0.24 * ns : 0.28) * (mats == 2 ? 1.3 : 1.0);
@@ -1081,12 +1081,16 @@ int FST_CAT(ffn_product_, FST_NAME)(int mode, const FfnProduct& p, hipStream_t s
     else
       launch<BACK, 2, 2, 4, F32 ? 4 : 2, 2, 2>(p, st);
   } else {
+    // float32 experts run them in large calls too, where two stages and four workgroups a CU
+    // keep the matrix cores busier than four and two (pick's example: output product 134
+    // -> 123 us, its gradient 154 -> 138, dx 254 -> 237).
+    constexpr int ST = EXPERTS && F32 ? 2 : 4, OCC = EXPERTS && F32 ? 4 : 2;
     if (mode == kFfnGate)
-      launch<kFfnGate, 1, 4, 4, 1, 4, 2>(p, st);
+      launch<kFfnGate, 1, 4, 4, 1, ST, OCC>(p, st);
     else if (mode == kFfnOut)
-      launch<kFfnOut, 2, 2, 2, 2, 4, 2>(p, st);
+      launch<kFfnOut, 2, 2, 2, 2, ST, OCC>(p, st);
     else if constexpr (F32)
-      launch<kFfnGrad, 2, 2, 2, 2, 4, 2>(p, st);
+      launch<kFfnGrad, 2, 2, 2, 2, ST, OCC>(p, st);
   }
   return hipGetLastError() == hipSuccess ? FST_OK : FST_ELAUNCH;
 }
