@@ -711,6 +711,7 @@ int fst_expert_spread(int dtype, int weight_dtype, int64_t tokens, int K, int N,
   RowPlan p;
   const int rc = check_move(dtype, weight_dtype, tokens, K, N, rows, p);
   if (rc != FST_OK) return rc;
+  if (tokens == 0) back = dweights = nullptr;  // no dots: an empty result has no address
   if (!out && !dweights) return FST_OK;
   if ((out && !used) || (tokens > 0 && (!x || !place)) || (rows > 0 && !back != !dweights))
     return fail(FST_EINVAL, "null tensor pointer");

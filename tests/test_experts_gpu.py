@@ -460,3 +460,74 @@ def test_results_repeat_bitwise():
     want = step()
     for _ in range(5):
         assert all(torch.equal(a, b) for a, b in zip(step(), want))
+
+
+# --- sizes past 32 bits, and nothing at all -----------------------------------
+
+
+def test_rows_past_32_bits():
+    """280000 rows of 8192: byte and element offsets of the last rows pass 2^32 and 2^31."""
+    tokens, d, n = 280_000, 8192, 3
+    experts = torch.randint(0, n, (tokens, 1), generator=torch.Generator().manual_seed(1), dtype=torch.int32)
+    order = flash_expert_sort(experts.to(DEV), n)
+    x = torch.empty(tokens, d, device=DEV, dtype=torch.bfloat16)
+    x.copy_((torch.arange(tokens, device=DEV) % 251)[:, None] + (torch.arange(d, device=DEV) % 4)[None, :])
+    w = torch.full((tokens, 1), 0.5, device=DEV)
+    leaves = [x.requires_grad_(True), w.requires_grad_(True)]
+    xs = flash_expert_dispatch(leaves[0], order)
+    y = flash_expert_combine(xs, leaves[1], order)
+    dx, dw = torch.autograd.grad(y, leaves, x.detach())
+    at = torch.tensor([0, 1, 131_071, 140_001, 262_143, 262_145, tokens - 1])
+    place = order.place[:, 0].long()[at]
+    assert torch.equal(xs.detach()[place], x.detach()[at])
+    assert torch.equal(y.detach()[at], 0.5 * x.detach()[at]) and torch.equal(dx[at], 0.5 * x.detach()[at])
+    want = x.detach()[at].double().square().sum(-1)
+    assert bool(((dw[at, 0].double() - want).abs() <= 64 * E * want).all())
+
+
+def test_feed_forward_past_32_bits():
+    """The gradients' rows of 2 F: 300000 x 8192. Rows near either end against 64 bits."""
+    loads, d, f = [150_000, 0, 150_000], 64, 4096
+    x, ws, offsets, dy = _ffn_case([5], d, f, torch.bfloat16, "wide")
+    rn = _gen("past 32 bits")
+    x, dy = (rn(sum(loads), d).to(DEV, torch.bfloat16) for _ in range(2))
+    ws = [(rn(3, *w.shape[1:]) / w.shape[2] ** 0.5).to(DEV, torch.bfloat16) for w in ws]
+    offsets = torch.tensor([0, *loads]).cumsum(0).int().to(DEV)
+    got = _ffn(x, offsets, ws, "silu", dy)
+    for lo, hi, e in ((0, 500, 0), (149_500, 150_000, 0), (299_500, 300_000, 2)):
+        one = expert_ffn64(x[lo:hi], torch.tensor([0, hi - lo]), *(w[e:e + 1] for w in ws), "silu", dy[lo:hi])
+        _near("y", got[0][lo:hi], one[0], _tol(torch.bfloat16))
+        _near("dx", got[1][lo:hi], one[1], _tol(torch.bfloat16))
+    # dw_down of an expert, formed by halves of its rows
+    half = [expert_ffn64(x[lo:lo + 75_000], torch.tensor([0, 75_000]), *(w[2:] for w in ws), "silu", dy[lo:lo + 75_000])
+            for lo in (150_000, 225_000)]
+    for i, name in enumerate(NAMES[2:]):
+        _near(name, got[2 + i][2], (half[0][2 + i] + half[1][2 + i])[0], _tol(torch.bfloat16))
+        assert bool((got[2 + i][1] == 0).all())
+
+
+def test_tokens_without_rows_and_rows_without_tokens():
+    none = torch.full((5, 2), -1, dtype=torch.int32, device=DEV)
+    order = ExpertOrder(none[:, 0], none, torch.zeros(4, dtype=torch.int32, device=DEV))
+    ys = torch.empty(0, 48, device=DEV, requires_grad=True)
+    w = torch.full((5, 2), float("nan"), device=DEV, requires_grad=True)
+    y = flash_expert_combine(ys, w, order)
+    assert bool((y == 0).all())
+    dys, dw = torch.autograd.grad(y, (ys, w), torch.ones_like(y))
+    assert dys.shape == (0, 48) and bool((dw == 0).all())
+    order = flash_expert_sort(torch.empty(0, 2, dtype=torch.int32, device=DEV), 3)
+    ys = torch.full((7, 48), float("nan"), device=DEV, requires_grad=True)
+    w = torch.empty(0, 2, device=DEV, requires_grad=True)
+    y = flash_expert_combine(ys, w, order)
+    dys, dw = torch.autograd.grad(y, (ys, w), torch.ones_like(y))
+    assert y.shape == (0, 48) and dw.shape == (0, 2) and bool((dys == 0).all())
+    assert flash_expert_dispatch(torch.empty(0, 48, device=DEV), order).shape == (0, 48)
+
+
+@pytest.mark.parametrize("n", [1, 64, 65, 130, 300, 512])
+def test_as_many_experts_as_there_may_be(n):
+    """Runs are looked up 64 experts at a time; some are empty, the last ones not."""
+    loads = [(e * 7) % 5 * (e % 3 != 0) for e in range(n)]
+    loads[-1] = 3
+    x, ws, offsets, dy = _ffn_case(loads, 32, 40, torch.bfloat16, ("many experts", n), tail=6)
+    _check_ffn(x, ws, offsets, dy, "silu")

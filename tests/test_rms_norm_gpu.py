@@ -271,3 +271,20 @@ def test_refusals():
         flash_rms_norm_fp8(x, w.requires_grad_(True))
     with torch.no_grad():
         flash_rms_norm_fp8(x, w)
+
+
+def test_rows_past_32_bits():
+    """280000 rows of 8192: element offsets of the last rows pass 2^31."""
+    rows, n = 280_000, 8192
+    x = torch.empty(rows, n, device=DEV, dtype=torch.bfloat16)
+    x.copy_((1 + torch.arange(rows, device=DEV) % 63)[:, None] * (1 + torch.arange(n, device=DEV) % 3)[None, :])
+    x.requires_grad_(True)
+    y = flash_rms_norm(x)
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    q, scale = flash_rms_norm_fp8(x.detach())
+    for at in (0, 131_071, 262_143, 262_145, rows - 1):
+        row = x.detach()[at:at + 1].clone()
+        want = _run(row, None, None, None, torch.ones_like(row), None)
+        assert torch.equal(y.detach()[at:at + 1], want[0][0].detach()) and torch.equal(dx[at:at + 1], want[1][0])
+        one = flash_rms_norm_fp8(row.detach())
+        assert torch.equal(q[at:at + 1].float(), one[0].float()) and torch.equal(scale[at:at + 1], one[1])
