@@ -487,7 +487,10 @@ __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
       for (int e = 0; e < NE; ++e) {
         v[e] = acc[GS * q + (e >> 2)][j][e & 3];
         if constexpr (MODE != kFfnGrad && !EXPERTS) v[e] += b0[e];
-        if constexpr (C::MATS == 2) u[e] = acc[NF + GS * q + (e >> 2)][j][e & 3] + (EXPERTS ? 0.f : b1[e]);
+        if constexpr (C::MATS == 2) {
+          u[e] = acc[NF + GS * q + (e >> 2)][j][e & 3];
+          if constexpr (!EXPERTS) u[e] += b1[e];
+        }
       }
       if constexpr (MODE == kFfnGate) {
         const long at = (long)t * p.ldo + f;
@@ -1002,7 +1005,10 @@ void launch_few(const FfnProduct& p, hipStream_t st) {
 enum Tile { kLarge, kMiddle, kSmall, kFew };
 
 Tile pick(const FfnProduct& p, int mats, bool redo) {
-  if (p.tokens <= kFewTokens) return kFew;
+  // float32 pays for all 64 rows of a tile, of which a few experts' runs fill an eighth (rows
+  // over 64 experts, D = 1024, F = 1376, forward, in small tiles / split over the waves: 256 rows
+  // 346 / 237 us, 512 336 / 257, 1024 331 / 356); 16-bit types do not (512 rows 115 / 135).
+  if (p.tokens <= kFewTokens || (EXPERTS && F32 && tokens_of_run(p) <= 12)) return kFew;
   const auto load = [&](int f, int t) {
     // Experts: each run ends in half a tile.
     const long down = EXPERTS ? p.tokens / t + (std::min(p.tokens, p.experts) + 1) / 2 : (p.tokens + t - 1) / t;
