@@ -35,7 +35,7 @@ struct FfnProduct {
   // weights w_next elements behind the expert's before it.
   const int32_t* offsets;
   int experts;
-  bool tail;               // write zeros into the rows past the last expert's
+  bool tail;               // write zeros into the rows of no expert
   long w_next;
 };
 

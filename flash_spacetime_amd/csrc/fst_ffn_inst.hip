@@ -171,11 +171,12 @@ __device__ __forceinline__ bool pick_tile(int wg, int nf, int nt, int& f, int& t
 }
 
 // Experts: the workgroup's feature tile, expert, and the rows t0 .. end - 1 of its tile
-// of BT tokens; expert = p.experts: rows past the last run, where they are asked for.
+// of BT tokens; expert = p.experts: rows outside every run (past the last one, or before
+// the first, where a table is part of a longer one), where they are asked for.
 // Workgroup wg of a grid over all tiles, or token tile `at` of a row of the grid (at >=
 // 0). Offsets are taken within the rows and in order, so that no table makes a tile reach
-// outside. Each wave adds up the runs' tiles by itself, 64 experts at a time. The rows past
-// the last run come after all tiles, so that every XCD has its share of the products.
+// outside. Each wave adds up the runs' tiles by itself, 64 experts at a time. The rows of
+// no run come after all tiles, so that every XCD has its share of the products.
 struct ExpertTile {
   int ft, expert, t0, end;
 };
@@ -202,7 +203,7 @@ __device__ __forceinline__ bool expert_tile(const FfnProduct& p, int wg, int nf,
     scan(e0);
     total += __builtin_amdgcn_readlane(upto, 63);
   }
-  int tt = at, behind = at - total;  // place among the tiles past the last run
+  int tt = at, behind = at - total;  // place among the tiles of no run
   bool run;
   if (at < 0) {
     run = pick_tile(wg, nf, total, tile.ft, tt);
@@ -212,11 +213,12 @@ __device__ __forceinline__ bool expert_tile(const FfnProduct& p, int wg, int nf,
   }
   if (!run) {
     if (!p.tail || behind < 0) return false;
-    const int tail = bound(p.experts);
+    const int head = bound(0), heads = (head + BT - 1) / BT, row = at < 0 ? behind / nf : behind;
+    const bool before = row < heads;
     tile.ft = at < 0 ? behind % nf : 0;
     tile.expert = p.experts;
-    tile.t0 = (int)min((long)p.tokens, tail + (long)(at < 0 ? behind / nf : behind) * BT);
-    tile.end = p.tokens;
+    tile.end = before ? head : p.tokens;
+    tile.t0 = (int)min((long)tile.end, before ? (long)row * BT : max(head, bound(p.experts)) + (long)(row - heads) * BT);
     return tile.t0 < tile.end;
   }
   if (p.experts > 64) scan(0);
@@ -960,9 +962,10 @@ __global__ __launch_bounds__(128 * WF, OCC) void ffn_outer(FfnOuters ps) {
 #endif
 }
 
-// Tiles of t tokens, at most: each run may end in a tile of its own.
+// Tiles of t tokens, at most: each run, and the rows before and behind them, may end in a
+// tile of its own.
 long token_tiles(const FfnProduct& p, int t) {
-  if (EXPERTS) return p.tokens / t + std::min(p.tokens, p.experts) + (p.tail ? 1 : 0);
+  if (EXPERTS) return p.tokens / t + std::min(p.tokens, p.experts) + (p.tail ? 2 : 0);
   return (p.tokens + t - 1) / t;
 }
 
@@ -970,7 +973,7 @@ template <int MODE, int WF, int WT, int NI, int NJ, int ST, int OCC>
 void launch(const FfnProduct& p, hipStream_t st) {
   typedef Product<MODE, WF, WT, NI, NJ, ST> C;
   const long tiles = (long)((p.F + C::FEATURES - 1) / C::FEATURES) * token_tiles(p, C::BT);
-  // Experts: the tiles past the last run begin at a multiple of eight.
+  // Experts: the tiles of no run begin at a multiple of eight.
   ffn_product<MODE, WF, WT, NI, NJ, ST, OCC><<<(unsigned)((tiles + 7) / 8 * 8 + (EXPERTS ? 8 : 0)), 64 * WF * WT, 0, st>>>(p);
 }
 

@@ -345,8 +345,9 @@ def flash_expert_feed_forward(
     `x` is `[rows, D]` in bfloat16, float16 or float32 with the rows of expert e from
     `offsets[e]` to `offsets[e + 1] - 1` (`offsets [E + 1]` int32, from
     `flash_expert_sort`; E up to 512); `w_gate`, `w_up` `[E, F, D]` and `w_down` `[E, D, F]` share its
-    dtype. D and F are multiples of 8. Rows past the last expert's are neither read nor
-    computed and come back as zeros in the output and x's gradient; an expert without
+    dtype. D and F are multiples of 8. Offsets must not fall; they may be a part of a
+    longer table (with its experts' weights). Rows outside these experts' are neither read
+    nor computed and come back as zeros in the output and x's gradient; an expert without
     rows gets gradients of zeros. Types, activations, rounding and autocast are
     `flash_gated_feed_forward`'s; there are no biases.
 

@@ -424,8 +424,9 @@ int fst_expert_gather(int dtype, int weight_dtype, int64_t tokens, int K, int N,
                       int64_t x_stride, const int32_t* place, const void* weights, void* out, void* stream);
 
 /* fst_ffn_forward for rows in runs: those from offsets[e] to offsets[e + 1] - 1 (taken
- * within the rows) with w_gate, w_up [E, F, D] and w_down [E, D, F] at e. Rows past the last run are
- * zeros in y and are neither read nor written elsewhere. No biases. */
+ * within the rows; offsets must not fall) with w_gate, w_up [E, F, D] and w_down [E, D, F] at
+ * e. Rows before the first run and past the last are zeros in y and are neither read nor
+ * written elsewhere. No biases. */
 int fst_expert_ffn_forward(int dtype, int activation, int rows, int E, int D, int F, const void* x, int64_t x_stride,
                            const int32_t* offsets, const void* w_gate, const void* w_up, const void* w_down,
                            void* hidden, void* gate, void* up, void* y, void* stream);

@@ -343,6 +343,25 @@ def test_rows_past_the_last_expert(dtype, loads, tail):
     _check_ffn(x, ws, offsets, dy, "silu")
 
 
+@pytest.mark.parametrize("loads", [[3, 5, 0, 7], [40, 100, 0, 60, 33], [700, 300, 900, 400]])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_a_part_of_the_experts(dtype, loads):
+    """Offsets cut out of a longer table: rows before and behind are zeros, and what they
+    hold reaches nothing; the others have the whole call's bits."""
+    x, ws, offsets, dy = _ffn_case(loads, 64, 128, TYPES[dtype], (dtype, tuple(loads), "part"), tail=50)
+    want = _ffn(x, offsets, ws, "silu", dy)
+    lo, hi = int(offsets[1]), int(offsets[3])
+    x, dy = x.clone(), dy.clone()
+    for t, what in ((x, float("nan")), (dy, float("inf"))):
+        t[:lo], t[hi:] = what, what
+    got = _ffn(x, offsets[1:4], [w[1:3] for w in ws], "silu", dy)
+    for a, b in zip(got[:2], want[:2]):
+        assert bool((a[:lo] == 0).all()) and bool((a[hi:] == 0).all()) and torch.equal(a[lo:hi], b[lo:hi])
+    used = expert_ffn64(x[lo:hi], offsets[1:4] - offsets[1], *(w[1:3] for w in ws), "silu", dy[lo:hi])
+    for name, a, b in zip(NAMES[2:], got[2:], used[2:]):
+        _near(name, a, b, _tol(TYPES[dtype]))
+
+
 def test_no_rows():
     x, ws, offsets, dy = _ffn_case([0, 0, 0], 64, 128, torch.bfloat16, "none")
     got = _ffn(x, offsets, ws, "silu", dy)
