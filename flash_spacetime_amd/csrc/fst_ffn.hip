@@ -58,7 +58,8 @@ __global__ __launch_bounds__(256) void ffn_rows(const int32_t* seqlens, int B, i
 // out[c * ldo + r] = in[r * C + c] for up to three matrices [R, C]; the workgroups
 // after theirs write zeros into the padding rows of `pad` (seqlens given), `slices`
 // of them for an event and every `groups`-th after it. Mixtures of experts: row y of
-// the grid takes expert y's matrices, next_in and next_out elements behind the first's.
+// the grid takes expert y's matrices, next_in and next_out elements behind the first's, if
+// the expert has rows: nothing reads the others'.
 struct Transposes {
   const void* in[3];
   void* out[3];
@@ -69,6 +70,7 @@ struct Transposes {
   long row_bytes;
   int B, L, groups, slices;
   long next_in, next_out[3];
+  const int32_t* offsets;
 };
 
 // A workgroup turns a 64 x 64 tile through LDS, 16 bytes at a time in memory (by
@@ -79,6 +81,7 @@ __global__ __launch_bounds__(256) void ffn_transpose(Transposes p) {
   constexpr int V = 16 / sizeof(E), PER = 64 / V;  // elements of a piece; pieces of a tile's row
   typedef E Part __attribute__((ext_vector_type(V)));
   __shared__ __attribute__((aligned(16))) E tile[64][64 + V];
+  if (p.offsets && p.offsets[blockIdx.y + 1] <= p.offsets[blockIdx.y]) return;
   if ((int)blockIdx.x >= p.first[2]) {
     const int at = (int)blockIdx.x - p.first[2], slice = at % p.slices;
     for (long e = at / p.slices; e < p.B; e += p.groups)
@@ -647,6 +650,7 @@ int fst_expert_ffn_backward(int dtype, int activation, int rows, int E, int D, i
       t.first[k] = grid;
     };
     t.next_in = df;
+    t.offsets = offsets;
     add(0, w_down, l.wdt, D, F, D, df);
     add(1, dx ? w_gate : nullptr, l.w2t, F, D, 2l * F, 2 * df);
     add(2, dx ? w_up : nullptr, l.w2t + F * es, F, D, 2l * F, 2 * df);
