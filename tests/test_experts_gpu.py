@@ -153,6 +153,27 @@ def test_sorts(slots, k, n, kind):
         assert a.dtype == torch.int32 and torch.equal(a.cpu(), b), name
 
 
+def test_sorts_as_many_slots_as_there_may_be():
+    """2^31 - 65537 of them, expert by expert in turn: each one's row and slot by arithmetic."""
+    n, e, chunk = 0x7FFFFFFF - 65536, 5, 1 << 28
+    spans = [(a, min(n, a + chunk)) for a in range(0, n, chunk)]
+    ids = torch.empty(n, 1, dtype=torch.int32, device=DEV)
+    for a, b in spans:
+        ids[a:b, 0] = torch.arange(a, b, device=DEV) % (e + 1)  # the last: no expert
+    got = flash_expert_sort(ids, e)
+    del ids
+    counts = [(n + e - i) // (e + 1) for i in range(e)]
+    assert got.offsets.tolist() == [sum(counts[:i]) for i in range(e + 1)]
+    offsets = got.offsets.long()
+    for a, b in spans:
+        slot = torch.arange(a, b, device=DEV)
+        of = slot % (e + 1)
+        assert torch.equal(got.place[a:b, 0], torch.where(of == e, -1, offsets[of] + slot // (e + 1)).int())
+        of = torch.bucketize(slot, offsets[1:], right=True)
+        want = torch.where(of == e, -1, (slot - offsets[of]) * (e + 1) + of)
+        assert torch.equal(got.order[a:b], want.int())
+
+
 def test_sorts_other_integers_and_strides():
     experts = torch.tensor([[3, 1 << 32, -7], [0, 3, (1 << 40) + 1]])
     want = sorted64(torch.tensor([[3, -1, -1], [0, 3, -1]]), 4)
