@@ -44,10 +44,19 @@ struct RmsGradArgs {
 // zeros has one.
 constexpr float kTop8 = 448.f, kLeastScale = 0x1p-126f;
 
-// Bytes of a row from its values times `inv`, piece by piece. The row's largest value
-// comes out as 448 (1 + 2^-23) at most, which rounds to 448; NaN stays NaN.
+// Bytes of a row from its values over `scale`, piece by piece; inv: the rounded reciprocal
+// of scale, or both 0 (rows of zeros, and what is finite beside an infinite value). The
+// product with inv alone is a unit or two off, and values next to a border between two
+// bytes fell to its other side; the remainder v - q scale is exact in a multiply-add,
+// and q corrected by it is the quotient rounded to float32 (Markstein, IBM J. Res. Dev. 34,
+// 1990). The row's largest value comes out as 448 (1 + 2^-23) at most, which rounds to
+// 448; NaN stays NaN.
 template <typename P, bool EDGE>
-__device__ __forceinline__ void store8(unsigned char* row, int l, int n, const float* v, float inv) {
+__device__ __forceinline__ void store8(unsigned char* row, int l, int n, const float* v, float scale, float inv) {
+  const auto over = [&](float x) {
+    const float q = x * inv;
+    return fmaf(fmaf(-q, scale, x), inv, q);
+  };
   constexpr int V = P::V;
   typedef unsigned char Bytes __attribute__((ext_vector_type(V)));
   typedef Bytes BytesU __attribute__((aligned(1)));
@@ -58,8 +67,8 @@ __device__ __forceinline__ void store8(unsigned char* row, int l, int n, const f
 #pragma unroll
     for (int j = 0; j < V; j += 4) {
       const float* q = v + i * V + j;
-      int o = __builtin_amdgcn_cvt_pk_fp8_f32(q[0] * inv, q[1] * inv, 0, false);
-      o = __builtin_amdgcn_cvt_pk_fp8_f32(q[2] * inv, q[3] * inv, o, true);
+      int o = __builtin_amdgcn_cvt_pk_fp8_f32(over(q[0]), over(q[1]), 0, false);
+      o = __builtin_amdgcn_cvt_pk_fp8_f32(over(q[2]), over(q[3]), o, true);
       word[j / 4] = (unsigned)o;
     }
     const Bytes o = __builtin_bit_cast(Bytes, word);
@@ -105,7 +114,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rms_fwd(RmsArgs a, int 
   for (; row < a.rows; row += step) {
     const bool later = is_token(row + 2 * step);
     if (next) fetch(row + step, x1, r1);
-    float v[E], aside = 0.f, inv = 0.f;
+    float v[E], aside = 0.f, scale = 0.f, inv = 0.f;
     if (now) {
       x0.get(v, l, n);
       if (a.r) {
@@ -129,7 +138,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rms_fwd(RmsArgs a, int 
 #pragma unroll
         for (int i = 0; i < E; ++i) top = fmaxf(top, fabsf(v[i]));
         aside = fmaxf(group_max<LPR>(top, red) / kTop8, kLeastScale);
-        inv = 1.f / aside;
+        if (aside < __builtin_inff()) scale = aside, inv = 1.f / aside;
       }
     } else {
 #pragma unroll
@@ -137,7 +146,7 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void rms_fwd(RmsArgs a, int 
       if (a.r) P::store(static_cast<T*>(a.s) + row * n, l, n, v);
     }
     if constexpr (Q8)
-      store8<P, EDGE>(static_cast<unsigned char*>(a.y) + row * n, l, n, v, inv);
+      store8<P, EDGE>(static_cast<unsigned char*>(a.y) + row * n, l, n, v, scale, inv);
     else
       P::store(static_cast<T*>(a.y) + row * n, l, n, v);
     if (a.aside && l == 0) a.aside[row] = aside;
