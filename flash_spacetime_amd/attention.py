@@ -232,9 +232,9 @@ class SpacetimeBlock(nn.Module):
         from .norm import flash_layer_norm
         from .rms_norm import flash_rms_norm
 
-        if isinstance(n, nn.LayerNorm):
-            return flash_layer_norm(x, n.weight, n.bias, n.eps, residual=residual, seqlens=seqlens)
-        return flash_rms_norm(x, n.weight, n.eps, residual=residual, seqlens=seqlens)
+        if isinstance(n, nn.RMSNorm):
+            return flash_rms_norm(x, n.weight, n.eps, residual=residual, seqlens=seqlens)
+        return flash_layer_norm(x, n.weight, n.bias, n.eps, residual=residual, seqlens=seqlens)
 
     def _feed_forward(self, y, seqlens):
         from .feed_forward import flash_gated_feed_forward
