@@ -155,6 +155,10 @@ class SpacetimeBlock(nn.Module):
     block's output, and `branch=` takes the one the block before deferred.
     """
 
+    # Of blocks pickled before there were experts, which have no attributes for them.
+    experts: Optional[int] = None
+    top_k = 2
+
     def __init__(self, dim: int, num_heads: int = 8, channels: int = 16, hidden: Optional[int] = None,
                  qkv_bias: bool = False, head_dim: Optional[int] = None, activation: str = "silu",
                  ffn_bias: bool = True, eps: float = 1e-5, use_attn_bias: bool = True,

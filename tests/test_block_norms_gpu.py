@@ -1,4 +1,4 @@
-"""SpacetimeBlock with other modules in its norms' places."""
+"""SpacetimeBlock with other modules in its norms' places, and as an earlier version pickled it."""
 
 import copy
 
@@ -38,3 +38,12 @@ def test_a_layer_norm_of_another_class_stays_one():
     other = copy.deepcopy(block)
     other.norm1, other.norm2 = Norm(other.norm1), Norm(other.norm2)
     assert torch.equal(other(*args), want)
+
+
+def test_a_block_of_an_earlier_version_runs():
+    """Pickled before there were experts, it has no attributes for them."""
+    block, args = _block()
+    want = block(*args)
+    old = copy.deepcopy(block)
+    del old.__dict__["experts"], old.__dict__["top_k"]
+    assert torch.equal(old(*args), want)
