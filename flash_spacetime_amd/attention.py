@@ -138,9 +138,9 @@ class SpacetimeBlock(nn.Module):
     dim).
 
     `norm="rms"` runs root-mean-square norms (`nn.RMSNorm` parameters) in layer norm's
-    place. With `experts=E` the feed-forward is a mixture: `router` (a linear without a
-    bias) gives each token its logits, the `top_k` largest choose its experts and
-    their softmax weighs them, and `experts_gate`, `experts_up` `[E, hidden, dim]` and
+    place. With `experts=E` (up to 512) the feed-forward is a mixture: `router` (a linear
+    without a bias) gives each token its logits, the `top_k` (up to 16) largest choose its
+    experts and their softmax weighs them, and `experts_gate`, `experts_up` `[E, hidden, dim]` and
     `experts_down` `[E, dim, hidden]` are the experts' weights, without biases (`ffn_bias` is
     the one feed-forward's). Padding goes to no expert. Nothing keeps the loads
     even but the router: a penalty for uneven ones is the training's to add, from
@@ -170,6 +170,8 @@ class SpacetimeBlock(nn.Module):
             raise ValueError(f"norm must be 'layer' or 'rms', got {norm!r}")
         if experts is not None and not 1 <= top_k <= experts:
             raise ValueError(f"top_k must be 1 .. {experts} experts, got {top_k}")
+        if experts is not None and (experts > 512 or top_k > 16):  # flash_expert_route's most
+            raise ValueError(f"at most 512 experts and 16 of them a token, got {experts}, {top_k}")
         if hidden is None:
             hidden = -(-8 * dim // (3 * 64)) * 64
         make_norm = nn.LayerNorm if norm == "layer" else nn.RMSNorm
