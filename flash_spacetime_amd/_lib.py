@@ -128,7 +128,12 @@ SIGNATURES = {
     "fst_expert_sort_workspace_bytes": (_sz, [_i, _i]),
     "fst_expert_sort": (_i, [_i, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "fst_expert_spread": (_i, [_i, _i, _l, _i, _i, _l, _vp, _l, _vp, _vp, _vp, _vp, _l, _vp, _vp, _vp]),
+    "fst_expert_spread_order": (
+        _i,
+        [_i, _i, _l, _i, _i, _l, _vp, _l, _vp, _vp, _l, _vp, _vp, _vp, _l, _vp, _vp, _vp],
+    ),
     "fst_expert_gather": (_i, [_i, _i, _l, _i, _i, _l, _vp, _l, _vp, _vp, _vp, _vp]),
+    "fst_expert_gather_order": (_i, [_i, _i, _l, _i, _i, _l, _vp, _l, _vp, _vp, _vp, _vp, _vp]),
     "fst_expert_ffn_forward": (
         _i,
         [_i, _i, _i, _i, _i, _i, _vp, _l, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
@@ -195,8 +200,8 @@ def _load_host():
                 "fst_layer_norm_backward", "fst_ffn_forward", "fst_ffn_backward_workspace_bytes",
                 "fst_ffn_backward", "fst_zero_tail", "fst_rms_norm_forward", "fst_rms_norm_fp8",
                 "fst_rms_norm_backward_workspace_bytes", "fst_rms_norm_backward", "fst_expert_route",
-                "fst_expert_route_backward", "fst_expert_sort_workspace_bytes", "fst_expert_sort", "fst_expert_spread",
-                "fst_expert_gather", "fst_expert_ffn_forward", "fst_expert_ffn_backward_workspace_bytes",
+                "fst_expert_route_backward", "fst_expert_sort_workspace_bytes", "fst_expert_sort", "fst_expert_spread_order",
+                "fst_expert_gather_order", "fst_expert_ffn_forward", "fst_expert_ffn_backward_workspace_bytes",
                 "fst_expert_ffn_backward")))
             return _fst_host
         why = f"it is build {have[0]} for torch {have[1]}, the library is build {build} and torch is {torch.__version__}"

@@ -46,8 +46,8 @@ struct Library {
   decltype(&fst_expert_route_backward) route_backward = nullptr;
   decltype(&fst_expert_sort_workspace_bytes) sort_workspace = nullptr;
   decltype(&fst_expert_sort) sort = nullptr;
-  decltype(&fst_expert_spread) spread = nullptr;
-  decltype(&fst_expert_gather) gather = nullptr;
+  decltype(&fst_expert_spread_order) spread = nullptr;
+  decltype(&fst_expert_gather_order) gather = nullptr;
   decltype(&fst_expert_ffn_forward) experts_forward = nullptr;
   decltype(&fst_expert_ffn_backward_workspace_bytes) experts_workspace = nullptr;
   decltype(&fst_expert_ffn_backward) experts_backward = nullptr;
@@ -613,13 +613,16 @@ py::object sort_call(const Tensor& experts, int64_t E) {
 // --- mixture of experts: rows to the experts and back ----------------------------
 
 struct Place {
-  Tensor place, offsets;  // dense
+  Tensor order, place, offsets;  // dense
+  const int32_t* used() const { return ints(offsets) + offsets.size(0) - 1; }
 };
 
-bool place_of(const Tensor& place, const Tensor& offsets, const at::Device& dev, Place& p) {
-  if (!plain(place, dev) || !plain(offsets, dev) || place.scalar_type() != at::kInt || offsets.scalar_type() != at::kInt ||
-      place.dim() < 1 || place.size(-1) < 1 || place.size(-1) > INT32_MAX || offsets.dim() != 1 || offsets.size(0) < 2)
+bool place_of(const Tensor& order, const Tensor& place, const Tensor& offsets, const at::Device& dev, Place& p) {
+  for (const Tensor* t : {&order, &place, &offsets})
+    if (!plain(*t, dev) || t->scalar_type() != at::kInt) return false;
+  if (place.dim() < 1 || place.size(-1) < 1 || place.size(-1) > INT32_MAX || offsets.dim() != 1 || offsets.size(0) < 2)
     return false;
+  p.order = order.contiguous();
   p.place = place.contiguous();
   p.offsets = offsets.contiguous();
   return true;
@@ -641,7 +644,7 @@ std::pair<Tensor, Tensor> spread_rows(const Tensor& x, const Place& p, const Ten
   if (want_rows) out = at::empty({rows, n}, opt);
   const int dtype = dtype_of(x.scalar_type());
   check(lib.spread(dtype, weights.defined() ? dtype_of(weights.scalar_type()) : dtype, p.place.numel() / K, (int)K, (int)n, rows,
-                   data(xr), xs, ints(p.place), ints(p.offsets) + p.offsets.size(0) - 1, data(weights), data(br), bs, data(out),
+                   data(xr), xs, ints(p.place), ints(p.order), p.order.numel(), p.used(), data(weights), data(br), bs, data(out),
                    data(dw), on.stream),
         what, may_refuse);
   return {out, dw};
@@ -657,7 +660,7 @@ Tensor gather_rows(const Tensor& x, const Place& p, const Tensor& weights, const
   const Tensor out = at::empty(shape, x.options().requires_grad(false));
   const int dtype = dtype_of(x.scalar_type());
   check(lib.gather(dtype, weights.defined() ? dtype_of(weights.scalar_type()) : dtype, p.place.numel() / K, (int)K, (int)x.size(-1),
-                   x.size(0), data(xr), xs, ints(p.place), data(weights), data(out), on.stream),
+                   x.size(0), data(xr), xs, ints(p.place), p.used(), data(weights), data(out), on.stream),
         what, may_refuse);
   return out;
 }
@@ -665,7 +668,7 @@ Tensor gather_rows(const Tensor& x, const Place& p, const Tensor& weights, const
 struct DispatchFunction : torch::autograd::Function<DispatchFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Place& p) {
     at::AutoDispatchBelowADInplaceOrView below;
-    ctx->save_for_backward({p.place, p.offsets});
+    ctx->save_for_backward({p.order, p.place, p.offsets});
     return spread_rows(x, p, Tensor(), Tensor(), p.place.numel(), true, "flash_expert_dispatch", true).first;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -674,19 +677,19 @@ struct DispatchFunction : torch::autograd::Function<DispatchFunction> {
     variable_list out(2);
     {
       at::AutoGradMode no_graph(false);
-      TORCH_CHECK(grads[0].dim() == 2 && grads[0].size(0) == v[0].numel() && grads[0].device() == v[0].device(),
+      TORCH_CHECK(grads[0].dim() == 2 && grads[0].size(0) == v[1].numel() && grads[0].device() == v[1].device(),
                   "flash_expert_dispatch backward: the gradient must have the output's shape and device");
-      out[0] = gather_rows(grads[0], Place{v[0], v[1]}, Tensor(), "flash_expert_dispatch backward", false);
+      out[0] = gather_rows(grads[0], Place{v[0], v[1], v[2]}, Tensor(), "flash_expert_dispatch backward", false);
     }
     return once(std::move(out), "flash_expert_dispatch");
   }
 };
 
-py::object dispatch_call(const Tensor& x, const Tensor& place, const Tensor& offsets) {
+py::object dispatch_call(const Tensor& x, const Tensor& order, const Tensor& place, const Tensor& offsets) {
   const at::Device dev = x.device();
   Place p;
   if (!lib.spread || !dev.is_cuda() || recorded() || !plain(x, dev) || dtype_of(x.scalar_type()) < 0 || x.dim() < 1 ||
-      x.size(-1) < 1 || x.size(-1) > INT32_MAX || !place_of(place, offsets, dev, p) ||
+      x.size(-1) < 1 || x.size(-1) > INT32_MAX || !place_of(order, place, offsets, dev, p) ||
       x.sizes().slice(0, x.dim() - 1) != place.sizes().slice(0, place.dim() - 1))
     return py::none();
   if (at::GradMode::is_enabled() && wants_grad(x)) return py::cast(DispatchFunction::apply(x, p));
@@ -698,7 +701,7 @@ struct CombineFunction : torch::autograd::Function<CombineFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& ys, const Tensor& weights, const Place& p) {
     at::AutoDispatchBelowADInplaceOrView below;
     const Tensor w = weights.contiguous();
-    ctx->save_for_backward({wants_grad(weights) ? ys : Tensor(), w, p.place, p.offsets});
+    ctx->save_for_backward({wants_grad(weights) ? ys : Tensor(), w, p.order, p.place, p.offsets});
     ctx->saved_data["call"] = c10::List<int64_t>({ys.size(0), (int64_t)ys.scalar_type(), wants_grad(ys)});
     return gather_rows(ys, p, w, "flash_expert_combine", true);
   }
@@ -710,9 +713,10 @@ struct CombineFunction : torch::autograd::Function<CombineFunction> {
     {
       at::AutoGradMode no_graph(false);
       const Tensor dy = grads[0].to((at::ScalarType)call[1]);
-      TORCH_CHECK(dy.sizes().slice(0, dy.dim() - 1) == v[2].sizes().slice(0, v[2].dim() - 1) && dy.device() == v[2].device(),
+      const Place p{v[2], v[3], v[4]};
+      TORCH_CHECK(dy.sizes().slice(0, dy.dim() - 1) == p.place.sizes().slice(0, p.place.dim() - 1) && dy.device() == p.place.device(),
                   "flash_expert_combine backward: the gradient must have the output's shape and device");
-      auto [dys, dw] = spread_rows(dy, Place{v[2], v[3]}, v[1], v[0], call[0], call[2], "flash_expert_combine backward", false);
+      auto [dys, dw] = spread_rows(dy, p, v[1], v[0], call[0], call[2], "flash_expert_combine backward", false);
       out[0] = dys;
       out[1] = dw;
     }
@@ -720,11 +724,12 @@ struct CombineFunction : torch::autograd::Function<CombineFunction> {
   }
 };
 
-py::object combine_call(const Tensor& ys, const Tensor& weights, const Tensor& place, const Tensor& offsets) {
+py::object combine_call(const Tensor& ys, const Tensor& weights, const Tensor& order, const Tensor& place,
+                        const Tensor& offsets) {
   const at::Device dev = ys.device();
   Place p;
   if (!lib.gather || !dev.is_cuda() || recorded() || !plain(ys, dev) || dtype_of(ys.scalar_type()) < 0 || ys.dim() != 2 ||
-      ys.size(1) < 1 || ys.size(1) > INT32_MAX || !plain(weights, dev) || !place_of(place, offsets, dev, p) ||
+      ys.size(1) < 1 || ys.size(1) > INT32_MAX || !plain(weights, dev) || !place_of(order, place, offsets, dev, p) ||
       weights.sizes() != place.sizes() || (weights.scalar_type() != ys.scalar_type() && weights.scalar_type() != at::kFloat))
     return py::none();
   if (at::GradMode::is_enabled() && (wants_grad(ys) || wants_grad(weights)))
@@ -887,12 +892,11 @@ void define_block_operators(py::module_& m) {
     return or_none(route_call, logits, top_k, normalize, seqlens);
   });
   m.def("expert_sort", [](const Tensor& experts, int64_t num_experts) { return or_none(sort_call, experts, num_experts); });
-  m.def("expert_dispatch", [](const Tensor& x, const Tensor& place, const Tensor& offsets) {
-    return or_none(dispatch_call, x, place, offsets);
+  m.def("expert_dispatch", [](const Tensor& x, const Tensor& order, const Tensor& place, const Tensor& offsets) {
+    return or_none(dispatch_call, x, order, place, offsets);
   });
-  m.def("expert_combine", [](const Tensor& ys, const Tensor& weights, const Tensor& place, const Tensor& offsets) {
-    return or_none(combine_call, ys, weights, place, offsets);
-  });
+  m.def("expert_combine", [](const Tensor& ys, const Tensor& weights, const Tensor& order, const Tensor& place,
+                             const Tensor& offsets) { return or_none(combine_call, ys, weights, order, place, offsets); });
   m.def("expert_feed_forward", [](const Tensor& x, const Tensor& offsets, const Tensor& wg, const Tensor& wu, const Tensor& wd,
                                   int act) { return or_none(experts_call, x, offsets, wg, wu, wd, act); });
 }

@@ -419,11 +419,17 @@ struct MoveArgs {
   const void* back;     // spread: the experts' rows the dots are with, or null
   const void* weights;  // [tokens, K], or null
   const int32_t* place;
-  const int32_t* used;  // spread: rows of the experts (what is behind is zeros)
+  const int32_t* used;   // rows of the experts, on the device (null: all)
+  const int32_t* order;  // spread: the slot of each of the first order_rows rows, or null
   void *out, *dw;
   long tokens, rows, ld, ldb;
-  int K, n;
+  int K, n, order_rows;
 };
+
+// Rows that a place may name.
+__device__ __forceinline__ int place_end(const MoveArgs& a) {
+  return a.used ? min(max(*a.used, 0), (int)a.rows) : (int)a.rows;
+}
 
 // Lanes of a wave that work on one row.
 template <int LPR>
@@ -432,11 +438,38 @@ constexpr int kRowLanes = LPR < 64 ? LPR : 64;
 // Lane k of the row's lanes in a wave: the k-th place of token t (-1: none, and past
 // the K).
 template <int LPR>
-__device__ __forceinline__ int load_place(const MoveArgs& a, long t) {
+__device__ __forceinline__ int load_place(const MoveArgs& a, long t, int end) {
   const int k = threadIdx.x % kRowLanes<LPR>;
   if (t >= a.tokens || k >= a.K) return -1;
   const int r = a.place[t * a.K + k];
-  return (unsigned)r < (unsigned)a.rows ? r : -1;
+  return (unsigned)r < (unsigned)end ? r : -1;
+}
+// The same where the order gives that row to the slot, else -1: only such a slot writes it,
+// and rows that no slot writes are found by the rows (zero_free_rows). So every row has one
+// writer, whatever the tables hold: places may have been taken out since the sort.
+template <int LPR>
+__device__ __forceinline__ int own_place(const MoveArgs& a, int place, long t) {
+  if (!a.order || place < 0) return place;
+  return place < a.order_rows && a.order[place] == (int)(t * a.K) + (int)(threadIdx.x % kRowLanes<LPR>) ? place : -1;
+}
+// Zeros into the rows below `end` that own_place gives to no slot: a lane looks at one of
+// 64 rows, and the wave clears those found.
+template <typename T, int NT>
+__device__ __forceinline__ void zero_free_rows(const MoveArgs& a, int end) {
+  const int lane = threadIdx.x & 63;
+  const long slots = a.tokens * a.K;
+  for (long r0 = ((long)blockIdx.x * (NT / 64) + (threadIdx.x >> 6)) * 64; r0 < end; r0 += (long)gridDim.x * NT) {
+    const long r = r0 + lane;
+    bool none = r < end;
+    if (none && r < a.order_rows) {
+      const int slot = a.order[r];
+      none = slot < 0 || slot >= slots || a.place[slot] != r;
+    }
+    for (unsigned long long m = __ballot(none); m; m &= m - 1) {
+      T* row = static_cast<T*>(a.out) + (r0 + __builtin_ctzll(m)) * a.n;
+      for (int c = lane; c < a.n; c += 64) row[c] = (T)0.f;
+    }
+  }
 }
 template <int LPR>
 __device__ __forceinline__ bool any_place(int place) {
@@ -472,23 +505,28 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void expert_spread(MoveArgs 
   const int l = threadIdx.x % LPR, n = a.n;
   const long step = (long)gridDim.x * G;
   const long first = (long)blockIdx.x * G + threadIdx.x / LPR;
+  const int end = place_end(a);
   P x0, x1;
   long t = first;
-  int now = load_place<LPR>(a, t), next = load_place<LPR>(a, t + step);
+  int now = load_place<LPR>(a, t, end), next = load_place<LPR>(a, t + step, end);
   float weight_next = load_weight<T, LPR>(a, t, w_f32);
   if (any_place<LPR>(now)) x0.load(static_cast<const T*>(a.in) + t * a.ld, l, n);
+  int own_next = own_place<LPR>(a, now, t);
   for (; t < a.tokens; t += step) {
-    const int later = load_place<LPR>(a, t + 2 * step);
+    const int later = load_place<LPR>(a, t + 2 * step, end);
     if (any_place<LPR>(next)) x1.load(static_cast<const T*>(a.in) + (t + step) * a.ld, l, n);
+    const int own = own_next;
+    own_next = own_place<LPR>(a, next, t + step);
     const float weight = weight_next;
     weight_next = load_weight<T, LPR>(a, t + step, w_f32);
     float v[E];
     if (any_place<LPR>(now)) x0.get(v, l, n);
     for (int k = 0; k < a.K; ++k) {
-      const int r = place_at<LPR>(now, k);
+      const int to = place_at<LPR>(own, k);
       float dot = 0.f;
-      if (r >= 0) {
-        if constexpr (DOT) {
+      if constexpr (DOT) {
+        const int r = place_at<LPR>(now, k);
+        if (r >= 0) {
           P y;
           float q[E];
           y.load(static_cast<const T*>(a.back) + r * a.ldb, l, n);
@@ -497,17 +535,17 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void expert_spread(MoveArgs 
           for (int i = 0; i < E; ++i) dot = fmaf(v[i], q[i], dot);
           dot = group_sum<LPR>(dot, red);
         }
-        if (a.out) {
-          T* out = static_cast<T*>(a.out) + (long)r * n;
-          if (a.weights) {
-            const float w = weight_at<LPR>(weight, k);
-            float q[E];
+      }
+      if (a.out && to >= 0) {
+        T* out = static_cast<T*>(a.out) + (long)to * n;
+        if (a.weights) {
+          const float w = weight_at<LPR>(weight, k);
+          float q[E];
 #pragma unroll
-            for (int i = 0; i < E; ++i) q[i] = w * v[i];
-            P::store(out, l, n, q);
-          } else {
-            P::store(out, l, n, v);
-          }
+          for (int i = 0; i < E; ++i) q[i] = w * v[i];
+          P::store(out, l, n, q);
+        } else {
+          P::store(out, l, n, v);
         }
       }
       if (DOT && l == 0) {
@@ -525,7 +563,8 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void expert_spread(MoveArgs 
   float zero[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) zero[i] = 0.f;
-  for (long r = max(*a.used, 0) + first; r < a.rows; r += step) P::store(static_cast<T*>(a.out) + r * n, l, n, zero);
+  for (long r = end + first; r < a.rows; r += step) P::store(static_cast<T*>(a.out) + r * n, l, n, zero);
+  if (a.order) zero_free_rows<T, NT>(a, end);
 }
 
 // Two of a token's rows are in flight at a time, the next token's places before
@@ -537,10 +576,11 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void expert_gather(MoveArgs 
   const int l = threadIdx.x % LPR, n = a.n;
   const long step = (long)gridDim.x * G;
   long t = (long)blockIdx.x * G + threadIdx.x / LPR;
-  int now = load_place<LPR>(a, t);
+  const int end = place_end(a);
+  int now = load_place<LPR>(a, t, end);
   float weight_next = load_weight<T, LPR>(a, t, w_f32);
   for (; t < a.tokens; t += step) {
-    const int next = load_place<LPR>(a, t + step);
+    const int next = load_place<LPR>(a, t + step, end);
     const float weight = weight_next;
     weight_next = load_weight<T, LPR>(a, t + step, w_f32);
     float sum[E];
@@ -704,9 +744,10 @@ int fst_expert_sort(int slots, int E, const int32_t* experts, int32_t* order, in
   return launched("expert sort");
 }
 
-int fst_expert_spread(int dtype, int weight_dtype, int64_t tokens, int K, int N, int64_t rows, const void* x,
-                      int64_t x_stride, const int32_t* place, const int32_t* used, const void* weights,
-                      const void* back, int64_t back_stride, void* out, void* dweights, void* stream) {
+int fst_expert_spread_order(int dtype, int weight_dtype, int64_t tokens, int K, int N, int64_t rows, const void* x,
+                            int64_t x_stride, const int32_t* place, const int32_t* order, int64_t order_rows,
+                            const int32_t* used, const void* weights, const void* back, int64_t back_stride, void* out,
+                            void* dweights, void* stream) {
   clear_error();
   RowPlan p;
   const int rc = check_move(dtype, weight_dtype, tokens, K, N, rows, p);
@@ -716,10 +757,11 @@ int fst_expert_spread(int dtype, int weight_dtype, int64_t tokens, int K, int N,
   if ((out && !used) || (tokens > 0 && (!x || !place)) || (rows > 0 && !back != !dweights))
     return fail(FST_EINVAL, "null tensor pointer");
   if (x_stride < N || (back && back_stride < N)) return fail(FST_EINVAL, "row stride below N=%d", N);
+  if (order_rows < 0) return fail(FST_EINVAL, "negative size (%ld rows of the order)", (long)order_rows);
   if (tokens == 0 && rows == 0) return FST_OK;
   const size_t es = elem_size(dtype);
-  const MoveArgs a{x, dweights ? (back ? back : x) : nullptr, weights, place, used, out, dweights,
-                   (long)tokens, (long)rows, (long)x_stride, (long)back_stride, K, N};
+  const MoveArgs a{x, dweights ? (back ? back : x) : nullptr, weights, place, used, order, out, dweights,
+                   (long)tokens, (long)rows, (long)x_stride, (long)back_stride, K, N, (int)(order_rows < rows ? order_rows : rows)};
   p.edge = N * es % 16 != 0 || !aligned16(x, x_stride, es) || (back && !aligned16(back, back_stride, es)) ||
            reinterpret_cast<uintptr_t>(out) % 16 != 0;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
@@ -733,8 +775,16 @@ int fst_expert_spread(int dtype, int weight_dtype, int64_t tokens, int K, int N,
   return launched("expert spread");
 }
 
-int fst_expert_gather(int dtype, int weight_dtype, int64_t tokens, int K, int N, int64_t rows, const void* x,
-                      int64_t x_stride, const int32_t* place, const void* weights, void* out, void* stream) {
+int fst_expert_spread(int dtype, int weight_dtype, int64_t tokens, int K, int N, int64_t rows, const void* x,
+                      int64_t x_stride, const int32_t* place, const int32_t* used, const void* weights,
+                      const void* back, int64_t back_stride, void* out, void* dweights, void* stream) {
+  return fst_expert_spread_order(dtype, weight_dtype, tokens, K, N, rows, x, x_stride, place, nullptr, 0, used, weights, back,
+                                 back_stride, out, dweights, stream);
+}
+
+int fst_expert_gather_order(int dtype, int weight_dtype, int64_t tokens, int K, int N, int64_t rows, const void* x,
+                            int64_t x_stride, const int32_t* place, const int32_t* used, const void* weights, void* out,
+                            void* stream) {
   clear_error();
   RowPlan p;
   const int rc = check_move(dtype, weight_dtype, tokens, K, N, rows, p);
@@ -743,7 +793,7 @@ int fst_expert_gather(int dtype, int weight_dtype, int64_t tokens, int K, int N,
   if (!out || !place || (rows > 0 && !x)) return fail(FST_EINVAL, "null tensor pointer");
   if (x_stride < N) return fail(FST_EINVAL, "row stride below N=%d", N);
   const size_t es = elem_size(dtype);
-  const MoveArgs a{x, nullptr, weights, place, nullptr, out, nullptr, (long)tokens, (long)rows, (long)x_stride, 0, K, N};
+  const MoveArgs a{x, nullptr, weights, place, used, nullptr, out, nullptr, (long)tokens, (long)rows, (long)x_stride, 0, K, N, 0};
   p.edge = N * es % 16 != 0 || !aligned16(x, x_stride, es) || reinterpret_cast<uintptr_t>(out) % 16 != 0;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const int w_f32 = weight_dtype == FST_F32;
@@ -754,6 +804,11 @@ int fst_expert_gather(int dtype, int weight_dtype, int64_t tokens, int K, int N,
   else
     launch_gather<float>(p, a, w_f32, st);
   return launched("expert gather");
+}
+
+int fst_expert_gather(int dtype, int weight_dtype, int64_t tokens, int K, int N, int64_t rows, const void* x,
+                      int64_t x_stride, const int32_t* place, const void* weights, void* out, void* stream) {
+  return fst_expert_gather_order(dtype, weight_dtype, tokens, K, N, rows, x, x_stride, place, nullptr, weights, out, stream);
 }
 
 }  // extern "C"

@@ -27,7 +27,13 @@ class ExpertOrder(NamedTuple):
     """The tokens' slots sorted by expert (int32 tensors): `order [slots]`, the slot of
     each sorted row, -1 past the last expert's; `place [.., K]`, the row of each token's
     slots, -1 where they have no expert; `offsets [experts + 1]`, the first row of each
-    expert and behind the last."""
+    expert and behind the last.
+
+    `flash_expert_dispatch` and `flash_expert_combine` take a slot to have a row where its
+    place lies below `offsets[-1]`. Slots may be taken out after the sort (place -1, experts
+    cut off the end of `offsets`): they then read and write nothing, and the rows that they
+    had are zeros wherever rows are written. Otherwise order and place belong to each other,
+    `place[order[r]] = r`: no two slots share a row."""
 
     order: Tensor
     place: Tensor
@@ -166,7 +172,7 @@ def _spread(what, x, place, offsets, weights=None, back=None, rows=None, out=Tru
     xr, x_stride = token_rows(x)
     br, b_stride = (None, 0) if back is None else token_rows(back)
     rows = place.numel() if rows is None else rows
-    o = torch.empty(rows, n, device=x.device, dtype=x.dtype) if out else None
+    o = torch.zeros(rows, n, device=x.device, dtype=x.dtype) if out else None  # rows may be no slot's
     dw = None if back is None else torch.empty(place.shape, device=x.device, dtype=weights.dtype)
     dtype = BLOCK_DTYPES[x.dtype]
     P = _lib.ptr
@@ -227,26 +233,28 @@ class _Combine(torch.autograd.Function):
 
 
 def _check_order(order: ExpertOrder, x: Tensor) -> Tuple[Tensor, Tensor]:
-    """(place, offsets) of an order on x's device."""
+    """(place, offsets) of an order on x's device; places from offsets[-1] on are -1."""
     if not isinstance(order, ExpertOrder):
         raise ValueError(f"order must be an ExpertOrder (flash_expert_sort), got {type(order).__name__}")
-    for name, t in (("place", order.place), ("offsets", order.offsets)):
-        if t.dtype != torch.int32 or t.device != x.device:
-            raise ValueError(f"order.{name} must be int32 on {x.device}, got {t.dtype} on {t.device}")
+    for name, t in order._asdict().items():
+        if not isinstance(t, Tensor) or t.dtype != torch.int32 or t.device != x.device:
+            got = f"{t.dtype} on {t.device}" if isinstance(t, Tensor) else type(t).__name__
+            raise ValueError(f"order.{name} must be int32 on {x.device}, got {got}")
     if order.place.dim() < 1 or order.place.shape[-1] < 1 or order.offsets.dim() != 1 or order.offsets.numel() < 2:
         raise ValueError(f"order must have place [.., K] and offsets [experts + 1], got {tuple(order.place.shape)}, "
                          f"{tuple(order.offsets.shape)}")
-    return order.place.contiguous(), order.offsets.contiguous()
+    place, offsets = order.place.contiguous(), order.offsets.contiguous()
+    return place.masked_fill(place >= offsets[-1:], -1), offsets
 
 
 def flash_expert_dispatch(x: Tensor, order: ExpertOrder) -> Tensor:
     """The tokens' rows `x [.., D]` in the experts' order, `[slots, D]`: row
-    `order.place[t, k]` is x's row t. Rows past the last expert's are zeros, and a
-    token without experts is not read. x's gradient is the float32 sum over its slots,
+    `order.place[t, k]` is x's row t. Rows of no slot, those past the last expert's among
+    them, are zeros, and a token without experts is not read. x's gradient is the float32 sum over its slots,
     rounded once. Any strides are taken, D up to 16384."""
-    if x.is_cuda and type(x) in PLAIN and isinstance(order, ExpertOrder):
+    if x.is_cuda and isinstance(order, ExpertOrder) and all(type(t) in PLAIN for t in (x, *order)):
         host = _lib.host()
-        out = None if host is None else host.expert_dispatch(x, order.place, order.offsets)
+        out = None if host is None else host.expert_dispatch(x, *order)
         if out is not None:
             return out
     check_rows(x)
@@ -260,11 +268,11 @@ def flash_expert_combine(ys: Tensor, weights: Tensor, order: ExpertOrder) -> Ten
     """The experts' rows `ys [slots, D]` back at their tokens, weighted and summed:
     `y[t] = sum_k weights[t, k] ys[order.place[t, k]]`, `[.., D]`, summed in float32 and
     rounded once. `weights` is `order.place`'s shape in float32 or ys' dtype; slots without
-    an expert add nothing, whatever their weight. Gradients of ys (zeros past the last
-    expert's rows) and of the weights."""
-    if ys.is_cuda and type(ys) in PLAIN and type(weights) in PLAIN and isinstance(order, ExpertOrder):
+    an expert add nothing, whatever their weight. Gradients of ys (zeros in rows of no slot)
+    and of the weights."""
+    if ys.is_cuda and isinstance(order, ExpertOrder) and all(type(t) in PLAIN for t in (ys, weights, *order)):
         host = _lib.host()
-        out = None if host is None else host.expert_combine(ys, weights, order.place, order.offsets)
+        out = None if host is None else host.expert_combine(ys, weights, *order)
         if out is not None:
             return out
     check_rows(ys, weights)

@@ -411,17 +411,32 @@ int fst_expert_sort(int slots, int E, const int32_t* experts, int32_t* order, in
 /* The tokens' rows x (x_stride elements apart, N features) at their places:
  * out[place[t, k]] = weights[t, k] x[t] (weights nullable: 1; float32 or of dtype), and
  * zeros from row *used on (offsets + E), of `rows` dense ones; and with back (rows of N,
- * back_stride apart) dweights[t, k] = x[t] . back[place[t, k]] in weight_dtype, 0 for
- * places outside the rows. out and dweights are each nullable. No two slots may share
- * a place. */
+ * back_stride apart) dweights[t, k] = x[t] . back[place[t, k]] in weight_dtype. A place
+ * outside the rows, or from *used on, is none: its slot writes no row and has a dot of 0.
+ * out and dweights are each nullable. No two slots may share a place, and rows below
+ * *used that are no slot's place stay as they are. */
 int fst_expert_spread(int dtype, int weight_dtype, int64_t tokens, int K, int N, int64_t rows, const void* x,
                       int64_t x_stride, const int32_t* place, const int32_t* used, const void* weights,
                       const void* back, int64_t back_stride, void* out, void* dweights, void* stream);
+
+/* The same with the order the places came with, order[r] the slot of row r < order_rows
+ * (nullable: fst_expert_spread), which decides where they differ: row r is slot order[r]'s if
+ * that slot's place is r, and zeros if not. So every row is written, once, also where
+ * places have been taken out (-1) since the sort. */
+int fst_expert_spread_order(int dtype, int weight_dtype, int64_t tokens, int K, int N, int64_t rows, const void* x,
+                            int64_t x_stride, const int32_t* place, const int32_t* order, int64_t order_rows,
+                            const int32_t* used, const void* weights, const void* back, int64_t back_stride, void* out,
+                            void* dweights, void* stream);
 
 /* out[t] = sum_k weights[t, k] x[place[t, k]] (weights nullable: 1), in float32 and in
  * order; places outside the `rows` rows of x add nothing. */
 int fst_expert_gather(int dtype, int weight_dtype, int64_t tokens, int K, int N, int64_t rows, const void* x,
                       int64_t x_stride, const int32_t* place, const void* weights, void* out, void* stream);
+
+/* The same where places from *used on (nullable) add nothing either. */
+int fst_expert_gather_order(int dtype, int weight_dtype, int64_t tokens, int K, int N, int64_t rows, const void* x,
+                            int64_t x_stride, const int32_t* place, const int32_t* used, const void* weights, void* out,
+                            void* stream);
 
 /* fst_ffn_forward for rows in runs: those from offsets[e] to offsets[e + 1] - 1 (taken
  * within the rows; offsets must not fall) with w_gate, w_up [E, F, D] and w_down [E, D, F] at

@@ -3,7 +3,9 @@ or the module, that is asked for it, before any launch."""
 
 import pytest
 
-from flash_spacetime_amd import SpacetimeBlock
+from flash_spacetime_amd import SpacetimeBlock, _lib
+
+needs_lib = pytest.mark.skipif(not _lib.LIB_PATH.exists(), reason="libflash_spacetime.so not built")
 
 
 @pytest.mark.parametrize("experts,top_k,what", [(513, 2, "512"), (40, 17, "16"), (0, 1, "top_k"), (4, 0, "top_k")])
@@ -15,3 +17,24 @@ def test_block_refuses_what_its_router_does(experts, top_k, what):
 def test_block_takes_the_router_s_most():
     block = SpacetimeBlock(32, 4, hidden=8, experts=512, top_k=16)
     assert (block.experts, block.top_k, block.router.weight.shape[0]) == (512, 16, 512)
+
+
+@needs_lib
+def test_movers_of_an_order_refuse():
+    lib = _lib.load()
+
+    def spread(tokens=5, k=2, rows=10, xs=8, place=16, order=16, order_rows=10, used=16, out=16):
+        return lib.fst_expert_spread_order(0, 1, tokens, k, 8, rows, 16, xs, place, order, order_rows, used, None, None, 0, out,
+                                           None, None)
+
+    def gather(tokens=5, k=2, rows=10, xs=8, place=16, used=16, out=16):
+        return lib.fst_expert_gather_order(0, 1, tokens, k, 8, rows, 16, xs, place, used, None, out, None)
+
+    for f in (spread, gather):
+        assert f(tokens=-1) == _lib.FST_EINVAL and f(rows=-1) == _lib.FST_EINVAL and "negative" in _lib.last_error()
+        assert f(k=17) == _lib.FST_EUNSUPPORTED and f(rows=1 << 31) == _lib.FST_EUNSUPPORTED
+        assert f(xs=7) == _lib.FST_EINVAL and "stride" in _lib.last_error()
+        assert f(place=None) == _lib.FST_EINVAL and "null" in _lib.last_error()
+    assert spread(order_rows=-1) == _lib.FST_EINVAL and "order" in _lib.last_error()
+    assert spread(used=None) == _lib.FST_EINVAL and gather(out=None) == _lib.FST_EINVAL
+    assert spread(out=None) == _lib.FST_OK and spread(tokens=0, rows=0) == _lib.FST_OK and gather(tokens=0) == _lib.FST_OK
