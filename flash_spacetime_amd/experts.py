@@ -268,7 +268,8 @@ def flash_expert_combine(ys: Tensor, weights: Tensor, order: ExpertOrder) -> Ten
     """The experts' rows `ys [slots, D]` back at their tokens, weighted and summed:
     `y[t] = sum_k weights[t, k] ys[order.place[t, k]]`, `[.., D]`, summed in float32 and
     rounded once. `weights` is `order.place`'s shape in float32 or ys' dtype; slots without
-    an expert add nothing, whatever their weight. Gradients of ys (zeros in rows of no slot)
+    an expert add nothing, whatever their weight. ys may be cut behind the last expert's rows,
+    or go on behind the slots: a place past its end is none, as it is past `offsets[-1]`. Gradients of ys (zeros in rows of no slot)
     and of the weights."""
     if ys.is_cuda and isinstance(order, ExpertOrder) and all(type(t) in PLAIN for t in (ys, weights, *order)):
         host = _lib.host()
