@@ -24,6 +24,7 @@ namespace fst {
 namespace {
 
 constexpr int kMostExperts = 512, kMostChosen = 16;
+constexpr long kMostSlots = 0x7fffffffL - 65536;  // and rows
 
 // --- router -----------------------------------------------------------------
 
@@ -234,7 +235,7 @@ int check_route(int dtype, int B, int L, int E, int K) {
   if (E < 1 || K < 1 || K > E) return fail(FST_EINVAL, "top_k must be 1 .. experts, got %d of %d", K, E);
   if (E > kMostExperts || K > kMostChosen)
     return fail(FST_EUNSUPPORTED, "at most %d experts and %d of them a token, got %d, %d", kMostExperts, kMostChosen, E, K);
-  if ((long)B * L * K > 0x7fffffffL - 65536) return fail(FST_EUNSUPPORTED, "too many slots (B=%d, L=%d, top_k=%d)", B, L, K);
+  if ((long)B * L > kMostSlots / K) return fail(FST_EUNSUPPORTED, "too many slots (B=%d, L=%d, top_k=%d)", B, L, K);
   return FST_OK;
 }
 
@@ -619,7 +620,7 @@ int check_move(int dtype, int weight_dtype, int64_t tokens, int K, int N, int64_
   if (tokens < 0 || rows < 0) return fail(FST_EINVAL, "negative size (%ld tokens, %ld rows)", (long)tokens, (long)rows);
   if (K < 1 || N < 1) return fail(FST_EINVAL, "need at least one slot and one feature, got %d, %d", K, N);
   if (K > kMostChosen) return fail(FST_EUNSUPPORTED, "at most %d slots a token, got %d", kMostChosen, K);
-  if (rows > 0x7fffffffL - 65536 || tokens * K > 0x7fffffffL - 65536) return fail(FST_EUNSUPPORTED, "too many rows");
+  if (rows > kMostSlots || tokens > kMostSlots / K) return fail(FST_EUNSUPPORTED, "too many rows");
   if (!plan_rows(dtype, N, p)) return fail(FST_EUNSUPPORTED, "rows of N=%d features: at most %d", N, kRowMax);
   return FST_OK;
 }
@@ -714,7 +715,7 @@ static int check_sort(int slots, int E) {
   if (slots < 0) return fail(FST_EINVAL, "negative size (%d slots)", slots);
   if (E < 1) return fail(FST_EINVAL, "need at least one expert, got %d", E);
   if (E > kMostExperts) return fail(FST_EUNSUPPORTED, "at most %d experts, got %d", kMostExperts, E);
-  if (slots > 0x7fffffff - 65536) return fail(FST_EUNSUPPORTED, "too many slots (%d)", slots);
+  if (slots > kMostSlots) return fail(FST_EUNSUPPORTED, "too many slots (%d)", slots);
   return FST_OK;
 }
 

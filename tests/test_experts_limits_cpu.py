@@ -38,3 +38,18 @@ def test_movers_of_an_order_refuse():
     assert spread(order_rows=-1) == _lib.FST_EINVAL and "order" in _lib.last_error()
     assert spread(used=None) == _lib.FST_EINVAL and gather(out=None) == _lib.FST_EINVAL
     assert spread(out=None) == _lib.FST_OK and spread(tokens=0, rows=0) == _lib.FST_OK and gather(tokens=0) == _lib.FST_OK
+
+
+@needs_lib
+@pytest.mark.parametrize("k", [2, 4, 8, 16])
+def test_products_of_sizes_past_64_bits(k):
+    """Tokens times slots that come out small, or below 0, in 64 bits."""
+    lib = _lib.load()
+    for tokens in (2 ** 64 // k - 2 ** 33, 2 ** 62 // k, 2 ** 63 // k, 2 ** 63 - 1):
+        tokens = min(tokens, 2 ** 63 - 1)
+        assert lib.fst_expert_gather(0, 1, tokens, k, 8, 10, 16, 8, 16, None, 16, None) == _lib.FST_EUNSUPPORTED
+        assert lib.fst_expert_spread(0, 1, tokens, k, 8, 10, 16, 8, 16, 16, None, None, 0, 16, None, None) == _lib.FST_EUNSUPPORTED
+    most = 2 ** 31 - 1
+    for b, l in ((most, most), (most, 2 ** 30), (2 ** 30, most // k)):
+        assert lib.fst_expert_route(1, b, l, 16, k, 1, 16, 16, None, 16, 16, None) == _lib.FST_EUNSUPPORTED, (b, l)
+        assert lib.fst_expert_route_backward(1, b, l, 16, k, 1, None, 16, None, 16, 16, 16, 16, None) == _lib.FST_EUNSUPPORTED
