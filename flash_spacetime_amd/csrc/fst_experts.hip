@@ -19,6 +19,8 @@
 // rounded once. Places outside the rows are skipped, whoever wrote them.
 #include "fst_rows.h"
 
+#include <algorithm>
+
 namespace fst {
 
 namespace {
@@ -33,7 +35,7 @@ struct RouteArgs {
   const int32_t* lens;
   float* weights;
   int32_t* experts;
-  long rows, ld;
+  long first, rows, ld;  // first: of the launch
   int L, E, K, chosen, wide;
 };
 
@@ -43,7 +45,7 @@ struct RouteGradArgs {
   const float *weights, *dw;
   const int32_t* experts;
   void* dlogits;
-  long rows, ld;
+  long first, rows, ld;
   int L, E, K, chosen, wide, wide_out;
 };
 
@@ -108,7 +110,7 @@ __device__ __forceinline__ void load_logits(const T* row, int l, int E, bool wid
 template <typename T, int G, int NC>
 __global__ __launch_bounds__(256) void expert_route(RouteArgs a) {
   const int l = threadIdx.x % G;
-  const long row = (long)blockIdx.x * (256 / G) + threadIdx.x / G;
+  const long row = a.first + (long)blockIdx.x * (256 / G) + threadIdx.x / G;
   if (row >= a.rows) return;
   float w = 0.f;
   int expert = -1;  // lane k: the k-th largest
@@ -154,7 +156,7 @@ __global__ __launch_bounds__(256) void expert_route(RouteArgs a) {
 template <typename T, int G, int NC>
 __global__ __launch_bounds__(256) void expert_route_grad(RouteGradArgs a) {
   const int l = threadIdx.x % G;
-  const long row = (long)blockIdx.x * (256 / G) + threadIdx.x / G;
+  const long row = a.first + (long)blockIdx.x * (256 / G) + threadIdx.x / G;
   if (row >= a.rows) return;
   float d[NC];
 #pragma unroll
@@ -226,6 +228,15 @@ void by_experts(int E, int K, F f) {
     FST_LANES(64, 8);
   }
 #undef FST_LANES
+}
+
+// launch(grid) for every run of rows that one launch takes: the lanes of all of them have to
+// stay below 2^32, which 64 a row pass at 67 million rows.
+template <typename A, typename F>
+void by_runs(A& a, int lanes, F launch) {
+  constexpr long kLanes = 1l << 31;
+  for (a.first = 0; a.first < a.rows; a.first += kLanes / lanes)
+    launch((unsigned)((std::min(a.rows - a.first, kLanes / lanes) * lanes + 255) / 256));
 }
 
 int check_route(int dtype, int B, int L, int E, int K) {
@@ -670,16 +681,17 @@ int fst_expert_route(int dtype, int B, int L, int E, int K, int normalize, const
   if (logits_stride < E) return fail(FST_EINVAL, "row stride below E=%d", E);
   const size_t es = elem_size(dtype);
   const bool wide = aligned16(logits, logits_stride, es) && E * es % 16 == 0;
-  const RouteArgs a{logits, seqlens, weights, experts, rows, (long)logits_stride, L, E, K, normalize != 0, wide};
+  RouteArgs a{logits, seqlens, weights, experts, 0, rows, (long)logits_stride, L, E, K, normalize != 0, wide};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   by_experts(E, K, [&](auto lanes, auto count) {
-    const unsigned grid = (unsigned)((rows * lanes() + 255) / 256);
-    if (dtype == FST_BF16)
-      expert_route<bf16, lanes(), count()><<<grid, 256, 0, st>>>(a);
-    else if (dtype == FST_F16)
-      expert_route<f16, lanes(), count()><<<grid, 256, 0, st>>>(a);
-    else
-      expert_route<float, lanes(), count()><<<grid, 256, 0, st>>>(a);
+    by_runs(a, lanes(), [&](unsigned grid) {
+      if (dtype == FST_BF16)
+        expert_route<bf16, lanes(), count()><<<grid, 256, 0, st>>>(a);
+      else if (dtype == FST_F16)
+        expert_route<f16, lanes(), count()><<<grid, 256, 0, st>>>(a);
+      else
+        expert_route<float, lanes(), count()><<<grid, 256, 0, st>>>(a);
+    });
   });
   return launched("expert route");
 }
@@ -696,17 +708,18 @@ int fst_expert_route_backward(int dtype, int B, int L, int E, int K, int normali
   if (!normalize && logits_stride < E) return fail(FST_EINVAL, "row stride below E=%d", E);
   const size_t es = elem_size(dtype);
   const bool whole = E * es % 16 == 0, wide = whole && aligned16(logits, logits_stride, es);
-  const RouteGradArgs a{logits, seqlens, weights, dweights, experts, dlogits, rows, (long)logits_stride, L, E, K, normalize != 0,
-                        wide, whole && aligned16(dlogits, E, es)};
+  RouteGradArgs a{logits, seqlens, weights, dweights, experts, dlogits, 0, rows, (long)logits_stride, L, E, K, normalize != 0,
+                  wide, whole && aligned16(dlogits, E, es)};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   by_experts(E, K, [&](auto lanes, auto count) {
-    const unsigned grid = (unsigned)((rows * lanes() + 255) / 256);
-    if (dtype == FST_BF16)
-      expert_route_grad<bf16, lanes(), count()><<<grid, 256, 0, st>>>(a);
-    else if (dtype == FST_F16)
-      expert_route_grad<f16, lanes(), count()><<<grid, 256, 0, st>>>(a);
-    else
-      expert_route_grad<float, lanes(), count()><<<grid, 256, 0, st>>>(a);
+    by_runs(a, lanes(), [&](unsigned grid) {
+      if (dtype == FST_BF16)
+        expert_route_grad<bf16, lanes(), count()><<<grid, 256, 0, st>>>(a);
+      else if (dtype == FST_F16)
+        expert_route_grad<f16, lanes(), count()><<<grid, 256, 0, st>>>(a);
+      else
+        expert_route_grad<float, lanes(), count()><<<grid, 256, 0, st>>>(a);
+    });
   });
   return launched("expert route backward");
 }
