@@ -31,6 +31,7 @@ struct FfnProduct {
   long ldx, lddy, ldo, ldw;  // elements
   int tokens;              // tokens, or the most there can be
   int F, K, act;
+  int first;               // workgroup of the product that the launch begins with
   // Mixtures of experts: rows of expert e from offsets[e] to offsets[e + 1], its
   // weights w_next elements behind the expert's before it.
   const int32_t* offsets;

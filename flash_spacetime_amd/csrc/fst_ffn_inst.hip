@@ -298,7 +298,7 @@ __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
   const int nf = (p.F + C::FEATURES - 1) / C::FEATURES;
 #if FST_EXPERTS
   ExpertTile tile;
-  if (!expert_tile<C::BT>(p, blockIdx.x, nf, -1, tile)) return;
+  if (!expert_tile<C::BT>(p, p.first + blockIdx.x, nf, -1, tile)) return;
   const int f0 = tile.ft * C::FEATURES, t0 = tile.t0, tokens = tile.end;
   if (MODE == kFfnOut && tile.expert == p.experts) {  // rows of no expert
     constexpr int PARTS = C::FEATURES * ES / 16;
@@ -313,7 +313,7 @@ __global__ __launch_bounds__(64 * WF * WT, OCC) void ffn_product(FfnProduct p) {
   const int tokens = p.count ? *p.count : p.tokens;
   const int nt = (tokens + C::BT - 1) / C::BT;
   int ft, tt;
-  if (!pick_tile(blockIdx.x, nf, nt, ft, tt)) return;
+  if (!pick_tile(p.first + blockIdx.x, nf, nt, ft, tt)) return;
   const int f0 = ft * C::FEATURES, t0 = tt * C::BT;
   constexpr long w_at = 0;
 #endif
@@ -969,12 +969,19 @@ long token_tiles(const FfnProduct& p, int t) {
   return (p.tokens + t - 1) / t;
 }
 
+// A launch takes fewer than 2^32 lanes, which narrow rows pass at 2^30 of them: as many
+// launches as that needs.
 template <int MODE, int WF, int WT, int NI, int NJ, int ST, int OCC>
-void launch(const FfnProduct& p, hipStream_t st) {
+void launch(FfnProduct p, hipStream_t st) {
   typedef Product<MODE, WF, WT, NI, NJ, ST> C;
+  constexpr long most = (1l << 31) / (64 * WF * WT);
   const long tiles = (long)((p.F + C::FEATURES - 1) / C::FEATURES) * token_tiles(p, C::BT);
   // Experts: the tiles of no run begin at a multiple of eight.
-  ffn_product<MODE, WF, WT, NI, NJ, ST, OCC><<<(unsigned)((tiles + 7) / 8 * 8 + (EXPERTS ? 8 : 0)), 64 * WF * WT, 0, st>>>(p);
+  const long grid = (tiles + 7) / 8 * 8 + (EXPERTS ? 8 : 0);
+  for (long first = 0; first < grid; first += most) {
+    p.first = (int)first;
+    ffn_product<MODE, WF, WT, NI, NJ, ST, OCC><<<(unsigned)std::min(grid - first, most), 64 * WF * WT, 0, st>>>(p);
+  }
 }
 
 constexpr int kFewTokens = 64;
