@@ -4,6 +4,7 @@ or the module, that is asked for it, before any launch."""
 import pytest
 
 from flash_spacetime_amd import SpacetimeBlock, _lib
+from tests.test_expert_tiles_gpu import CASES, tiles
 
 needs_lib = pytest.mark.skipif(not _lib.LIB_PATH.exists(), reason="libflash_spacetime.so not built")
 
@@ -53,3 +54,16 @@ def test_products_of_sizes_past_64_bits(k):
     for b, l in ((most, most), (most, 2 ** 30), (2 ** 30, most // k)):
         assert lib.fst_expert_route(1, b, l, 16, k, 1, 16, 16, None, 16, 16, None) == _lib.FST_EUNSUPPORTED, (b, l)
         assert lib.fst_expert_route_backward(1, b, l, 16, k, 1, None, 16, None, 16, 16, 16, 16, None) == _lib.FST_EUNSUPPORTED
+
+
+@needs_lib
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_every_tile_of_the_experts_products_is_a_tested_cases(dtype):
+    """Gate, output, the projections' gradients, x's gradient, the weights' gradients written
+    directly and in pieces: the cases of test_expert_tiles_gpu.py reach what is compiled."""
+    of = [tiles(dtype, *c[:4]) for c in CASES]
+    assert of == [c[5 if dtype == "f32" else 4] for c in CASES]
+    wide = set() if dtype == "f32" else {256}
+    back = {16, 64, 128} if dtype == "f32" else {16, 128, 256}
+    assert [{t[i] for t in of} for i in range(4)] == [{16, 64, 128} | wide, {16, 64, 128} | wide, back, {16, 64, 128} | wide]
+    assert {(t[4], t[5] > 1) for t in of} >= {(e, s) for e in {128} | wide for s in (False, True)}
