@@ -67,3 +67,14 @@ def test_every_tile_of_the_experts_products_is_a_tested_cases(dtype):
     back = {16, 64, 128} if dtype == "f32" else {16, 128, 256}
     assert [{t[i] for t in of} for i in range(4)] == [{16, 64, 128} | wide, {16, 64, 128} | wide, back, {16, 64, 128} | wide]
     assert {(t[4], t[5] > 1) for t in of} >= {(e, s) for e in {128} | wide for s in (False, True)}
+
+
+@needs_lib
+def test_every_sort_s_counts_are_all_added_up():
+    """A workgroup adds up the counts of all, at most 32 loads a thread; the workspace's
+    rounding to 256 bytes holds at most 63 // (e + 1) workgroups' counts more."""
+    lib = _lib.load()
+    for e in range(1, 513):
+        for slots in (8193, 20000, 524288, 524289, 10 ** 7, 0x7FFFFFFF - 65536):
+            blocks = lib.fst_expert_sort_workspace_bytes(slots, e) // (4 * (e + 1)) - 63 // (e + 1)
+            assert blocks <= 32 * max(1024 // (1 << e.bit_length()), 1), (e, slots, blocks)
