@@ -252,7 +252,7 @@ def flash_expert_dispatch(x: Tensor, order: ExpertOrder) -> Tensor:
     `order.place[t, k]` is x's row t. Rows of no slot, those past the last expert's among
     them, are zeros, and a token without experts is not read. x's gradient is the float32 sum over its slots,
     rounded once. Any strides are taken, D up to 16384."""
-    if x.is_cuda and isinstance(order, ExpertOrder) and all(type(t) in PLAIN for t in (x, *order)):
+    if x.is_cuda and type(x) in PLAIN and isinstance(order, ExpertOrder) and isinstance(order.order, Tensor):
         host = _lib.host()
         out = None if host is None else host.expert_dispatch(x, *order)
         if out is not None:
@@ -271,7 +271,8 @@ def flash_expert_combine(ys: Tensor, weights: Tensor, order: ExpertOrder) -> Ten
     an expert add nothing, whatever their weight. ys may be cut behind the last expert's rows,
     or go on behind the slots: a place past its end is none, as it is past `offsets[-1]`. Gradients of ys (zeros in rows of no slot)
     and of the weights."""
-    if ys.is_cuda and isinstance(order, ExpertOrder) and all(type(t) in PLAIN for t in (ys, weights, *order)):
+    if (ys.is_cuda and type(ys) in PLAIN and type(weights) in PLAIN and isinstance(order, ExpertOrder)
+            and isinstance(order.order, Tensor)):
         host = _lib.host()
         out = None if host is None else host.expert_combine(ys, weights, *order)
         if out is not None:
