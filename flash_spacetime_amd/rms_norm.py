@@ -138,7 +138,8 @@ def flash_rms_norm(
     with `residual` the norm is of `s = x + residual`, rounded to x's dtype, and
     `(y, s)` is returned; with `seqlens` rows past an event's length are not read and come
     back as zeros everywhere. A row whose squares overflow float32 (values past 1e19)
-    comes out as zeros.
+    comes out as zeros, and with eps = 0 one whose squares all vanish (below 1e-23) is not
+    finite.
 
     Statistics and sums are float32; results are bitwise reproducible.
     """
