@@ -238,7 +238,7 @@ class SpacetimeBlock(nn.Module):
         from .norm import flash_layer_norm
         from .rms_norm import flash_rms_norm
 
-        if isinstance(n, nn.RMSNorm):
+        if isinstance(n, nn.RMSNorm) or not hasattr(n, "bias"):
             return flash_rms_norm(x, n.weight, n.eps, residual=residual, seqlens=seqlens)
         return flash_layer_norm(x, n.weight, n.bias, n.eps, residual=residual, seqlens=seqlens)
 

@@ -22,21 +22,31 @@ class Norm(nn.Module):
         self.weight, self.bias, self.eps = like.weight, like.bias, like.eps
 
 
-def _block():
+class Rms(nn.Module):
+    """A root-mean-square norm of another class: it has no bias."""
+
+    def __init__(self, like):
+        super().__init__()
+        self.weight, self.eps = like.weight, like.eps
+
+
+def _block(norm="layer"):
     torch.manual_seed(3)
-    block = SpacetimeBlock(64, 4, hidden=128, device=DEV)
+    block = SpacetimeBlock(64, 4, hidden=128, device=DEV, norm=norm)
     with torch.no_grad():
         for n in (block.norm1, block.norm2):
             n.weight.uniform_(0.5, 1.5)
-            n.bias.normal_()
+            if norm == "layer":
+                n.bias.normal_()
     return block, (torch.randn(2, 9, 64, device=DEV), torch.randn(2, 9, 5, device=DEV), torch.tensor([9, 4], device=DEV))
 
 
-def test_a_layer_norm_of_another_class_stays_one():
-    block, args = _block()
+@pytest.mark.parametrize("norm,cls", [("layer", Norm), ("rms", Rms)])
+def test_norms_of_another_class_stay_what_they_are(norm, cls):
+    block, args = _block(norm)
     want = block(*args)
     other = copy.deepcopy(block)
-    other.norm1, other.norm2 = Norm(other.norm1), Norm(other.norm2)
+    other.norm1, other.norm2 = cls(other.norm1), cls(other.norm2)
     assert torch.equal(other(*args), want)
 
 
